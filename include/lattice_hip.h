@@ -738,6 +738,111 @@ int lattice_hip_global_pool(int mode, const float* feats, int channels,
                             const int64_t* batch_offsets, int batches,
                             float* out, void* stream);
 
+/* ------------------------------------------- transformer operators -- */
+/* Operators of a transformer block over feature rows; the reference has no
+ * counterpart.  dtype is a lattice_dtype; sums, statistics and softmax states
+ * are held in fp32, every result is rounded once. */
+
+/* Layer norm of rows: y = (x - mean) / sqrt(var + eps) * weight + bias over
+ * the `channels` of each row.  x [rows, channels] with x_stride elements
+ * between rows, y contiguous.  weight and bias (NULL: 1 and 0) have
+ * `channels` values of the row's type.  Rows at and past *active_rows
+ * (device int32, NULL: all rows are active) become zeros.  statistics
+ * (NULL: not kept) gets float2 (mean, 1 / sqrt(var + eps)) of every row. */
+int lattice_hip_layer_norm(int dtype, const void* x, long long x_stride,
+                           int rows, int channels, const void* weight,
+                           const void* bias, float eps,
+                           const int32_t* active_rows, void* y,
+                           float* statistics, void* stream);
+
+/* Its gradients: grad_x [rows, channels] (zero on inactive rows), and, unless
+ * NULL, grad_weight and grad_bias [channels] summed over the active rows in
+ * an order fixed by the shape.  statistics as kept by the forward call. */
+size_t lattice_hip_layer_norm_grad_workspace_bytes(int rows, int channels);
+int lattice_hip_layer_norm_grad(int dtype, const void* grad_y,
+                                long long grad_y_stride, const void* x,
+                                long long x_stride, int rows, int channels,
+                                const void* weight, const float* statistics,
+                                const int32_t* active_rows, void* grad_x,
+                                void* grad_weight, void* grad_bias,
+                                void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Dropout: y[e] = residual[e] + (kept(e) ? x[e] * scale : 0) over `count`
+ * contiguous values (residual NULL: 0).  Element e is kept when word e % 4 of
+ * Philox 4x32-10 (Salmon et al., SC 2011) over the counter (e / 4, offset)
+ * and the key `seed` (each 64 bits, low word first) is at least `threshold`
+ * (0 .. 2^32).  The mask is a function of (seed, offset, e) alone: the
+ * gradient is the same call on the cotangent without a residual. */
+int lattice_hip_dropout(int dtype, const void* x, const void* residual,
+                        long long count, uint64_t seed, uint64_t offset,
+                        uint64_t threshold, float scale, void* y,
+                        void* stream);
+
+/* Rotary positions of several axes.  x [rows, heads, dim] (row and head
+ * strides in elements, unit stride in dim), y contiguous.  The first
+ * sum(dims) channels of a head are cut into `axes` (1 .. 4) sections of
+ * dims[a] channels (host, even); pair i of section a is turned by
+ * positions[row, a] * frequencies[pair] radians (times -1 if `inverse`),
+ * frequencies holding sum(dims) / 2 float64 values in section order; the
+ * other channels are copied.  A pair is (i, i + dims[a] / 2) of its section,
+ * or (2 i, 2 i + 1) if `interleaved`.  positions: int32, or float32 if
+ * float_positions, position_stride elements between rows.  The angle is
+ * reduced in float64. */
+int lattice_hip_rotary_positions(int dtype, const void* x,
+                                 long long x_row_stride,
+                                 long long x_head_stride, int rows, int heads,
+                                 int dim, const void* positions,
+                                 int float_positions,
+                                 long long position_stride,
+                                 const double* frequencies, int axes,
+                                 const int32_t* dims, int interleaved,
+                                 int inverse, void* y, void* stream);
+
+/* Attention over a sliding window with first keys that stay visible.
+ * Sequence s holds the query rows offsets[s] .. offsets[s + 1] and the key
+ * rows key_offsets[s] .. + min(key_lengths[s], key_offsets[s + 1] -
+ * key_offsets[s]) (key_lengths NULL: the difference).  Query i of nq, of a
+ * sequence with nk keys, has position p = i + nk - nq and sees key j where
+ * j <= p + right and (j >= p - left or j < sinks).  out = softmax(scale q k')
+ * v over what is seen; rows that see nothing, or lie in no sequence, are
+ * zero.  What a row does not see never reaches it, whatever its value.
+ * q [queries, heads, dim], k and v [keys, kv_heads, dim]: strides in
+ * elements, unit stride in dim, rows in whole 16-byte pieces on 16-byte
+ * boundaries; dim up to 128.  Head h reads key head h * kv_heads / heads.
+ * Offsets are device int32 and clamped to the rows there are. */
+typedef struct lattice_attention {
+    int dtype, queries, keys, heads, kv_heads, dim, sequences;
+    int left, right, sinks;
+    float scale;
+    const void *q, *k, *v;
+    long long q_row_stride, q_head_stride;
+    long long k_row_stride, k_head_stride;
+    long long v_row_stride, v_head_stride;
+    const int32_t *offsets, *key_offsets, *key_lengths;
+} lattice_attention;
+
+/* out [queries, heads, dim] contiguous.  lse (NULL: not kept) gets the
+ * float32 [queries, heads] log2 of each row's softmax sum, for the gradient
+ * (+inf on empty rows). */
+size_t lattice_hip_window_attention_workspace_bytes(
+    const lattice_attention* args);
+int lattice_hip_window_attention(const lattice_attention* args, void* out,
+                                 float* lse, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* Its gradients for the cotangent grad_out (contiguous, like out): grad_q,
+ * grad_k, grad_v contiguous; every row is written, in an order of sums fixed
+ * by the shapes and offsets. */
+size_t lattice_hip_window_attention_grad_workspace_bytes(
+    const lattice_attention* args);
+int lattice_hip_window_attention_grad(const lattice_attention* args,
+                                      const void* out, const float* lse,
+                                      const void* grad_out, void* grad_q,
+                                      void* grad_k, void* grad_v,
+                                      void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

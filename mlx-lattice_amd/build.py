@@ -28,12 +28,14 @@ NATIVE = HERE / 'native'
 INCLUDE = REPO / 'include'
 ARCH = 'gfx950'
 
-HIP_SOURCES = ['scan.hip', 'sort.hip', 'coords.hip', 'conv.hip', 'conv_grad.hip', 'pool.hip', 'quantize.hip']
+HIP_SOURCES = ['scan.hip', 'sort.hip', 'coords.hip', 'conv.hip', 'conv_grad.hip', 'pool.hip', 'quantize.hip',
+               'norm.hip', 'dropout.hip', 'rotary.hip', 'attention.hip', 'attention_grad.hip']
 HOST_SOURCES = [
     'native/features/coordinates/relations.cpp',
     'native/features/convolution/api.cpp',
     'native/features/pooling/pooling.cpp',
     'native/features/quantization/quantization.cpp',
+    'native/features/transformer/transformer.cpp',
     'native/bindings/module.cpp',
 ]
 

@@ -1,0 +1,236 @@
+// Rotary positions of several axes.
+//
+// The first channels of a head are cut into a section per axis; pair i of
+// section a, (u, v), is turned by t = position_a * frequency_i:
+//   u' = u cos t - v sin t,  v' = u sin t + v cos t,
+// and by -t for the gradient, which is the transpose.
+//
+// Bound by memory: x is read and y written once.  A block takes some rows and
+// first makes the cosines and sines that all heads of a row share in LDS, each
+// once.  The angle is position * frequency / (2 pi) turns in float64, reduced
+// to half a turn there: in float32 a coordinate of 10^5 would leave it wrong by
+// a hundredth of a radian.  Then a lane moves a 16-byte piece of a head; its
+// partners, which lie at any channel distance (an axis has any even number of
+// channels), come from the wave's copy of the piece in LDS.
+
+#include "rows.h"
+
+namespace lattice {
+namespace {
+
+constexpr int kRotaryBlock = 256;
+constexpr int kRotaryWaves = kRotaryBlock / kWave;
+constexpr int kRotaryAxes = 4;
+constexpr int kRotaryMaxDim = 1024;
+constexpr int kRotaryUnroll = 4;
+
+struct RotaryAxes {
+    int axes, pairs, interleaved;
+    int dims[kRotaryAxes];
+};
+
+struct RotaryPositions {
+    const void* values;
+    long long stride;
+    int is_float;
+    __device__ double at(long long row, int axis) const {
+        return is_float ? static_cast<double>(static_cast<const float*>(values)[row * stride + axis])
+                        : static_cast<double>(static_cast<const int32_t*>(values)[row * stride + axis]);
+    }
+};
+
+// Channel c of a head: the pair it belongs to (-1: copied), its partner's
+// channel, and the sign of the partner's part.
+struct RotaryChannel {
+    int pair, partner;
+    float sign;
+};
+__device__ inline RotaryChannel rotary_channel(const RotaryAxes& axes, int c) {
+    int start = 0;
+    for (int a = 0; a < axes.axes; ++a) {
+        const int width = axes.dims[a];
+        if (c < start + width) {
+            const int i = c - start, half = width / 2;
+            if (axes.interleaved) return {start / 2 + i / 2, c ^ 1, i & 1 ? 1.0f : -1.0f};
+            return i < half ? RotaryChannel{start / 2 + i, c + half, -1.0f}
+                            : RotaryChannel{start / 2 + i - half, c - half, 1.0f};
+        }
+        start += width;
+    }
+    return {-1, c, 0.0f};
+}
+
+// (cos, sin) of every pair of `count` rows from `first`.
+__device__ inline void rotary_table(float2* table, const RotaryAxes& axes, const RotaryPositions& positions,
+                                    const double* frequencies, long long first, int count, float sign) {
+    constexpr double kPerTurn = 0.15915494309189533577;  // 1 / (2 pi)
+    for (int i = threadIdx.x; i < count * axes.pairs; i += kRotaryBlock) {
+        const int row = i / axes.pairs, pair = i - row * axes.pairs;
+        int axis = 0, end = axes.dims[0] / 2;
+        while (pair >= end && axis + 1 < axes.axes) end += axes.dims[++axis] / 2;
+        const double turns = positions.at(first + row, axis) * (frequencies[pair] * kPerTurn);
+        float s, c;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+        table[i] = float2{c, sign * s};
+    }
+}
+
+// x rows of dim = chunks * V channels, chunks <= 64.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRotaryBlock)
+rotary_rows(const T* __restrict__ x, long long x_row, long long x_head, int rows, int heads, int dim,
+            RotaryPositions positions, const double* __restrict__ frequencies, RotaryAxes axes, float sign,
+            int block_rows, T* __restrict__ y) {
+    typedef RowVec<T, V> Vec;
+    extern __shared__ float2 table[];
+    __shared__ __align__(16) T stage[kRotaryWaves][kRotaryUnroll][kWave * V];
+    const int wave = threadIdx.x / kWave, lane = lane_id();
+    const int chunks = dim / V;
+    const int wave_heads = kWave / chunks;
+    const int sub = lane / chunks, c0 = (lane - sub * chunks) * V;
+    const bool used = sub < wave_heads;
+    int pair[V], from[V];
+    float turn[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const RotaryChannel ch = rotary_channel(axes, c0 + j);
+        pair[j] = ch.pair;
+        from[j] = sub * dim + ch.partner;
+        turn[j] = ch.sign;
+    }
+    const int head_groups = (heads + wave_heads - 1) / wave_heads;
+    const long long first = static_cast<long long>(blockIdx.x) * block_rows;
+    const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
+    rotary_table(table, axes, positions, frequencies, first, count, sign);
+    __syncthreads();
+    const int items = count * head_groups;
+    for (int base = wave; base < items; base += kRotaryWaves * kRotaryUnroll) {
+        Vec in[kRotaryUnroll];
+        int row[kRotaryUnroll], head[kRotaryUnroll];
+        bool live[kRotaryUnroll];
+#pragma unroll
+        for (int u = 0; u < kRotaryUnroll; ++u) {
+            const int item = base + u * kRotaryWaves;
+            row[u] = item / head_groups;
+            head[u] = (item - row[u] * head_groups) * wave_heads + sub;
+            live[u] = item < items && used && head[u] < heads;
+            if (live[u]) in[u] = Vec::load(x + (first + row[u]) * x_row + head[u] * x_head + c0);
+        }
+#pragma unroll
+        for (int u = 0; u < kRotaryUnroll; ++u)
+            if (live[u]) in[u].store(&stage[wave][u][lane * V]);
+        // The wave alone reads what it wrote, in order.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < kRotaryUnroll; ++u) {
+            if (!live[u]) continue;
+            Vec out;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (pair[j] < 0) {
+                    out.e[j] = in[u].e[j];
+                } else {
+                    const float2 t = table[row[u] * axes.pairs + pair[j]];
+                    const float other = static_cast<float>(stage[wave][u][from[j]]);
+                    out.set(j, in[u].at(j) * t.x + turn[j] * (other * t.y));
+                }
+            }
+            out.store(y + ((first + row[u]) * heads + head[u]) * dim + c0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Any dim and alignment: a lane a channel, its partner read from x.
+template <typename T>
+__global__ void __launch_bounds__(kRotaryBlock)
+rotary_channels(const T* __restrict__ x, long long x_row, long long x_head, int rows, int heads, int dim,
+                RotaryPositions positions, const double* __restrict__ frequencies, RotaryAxes axes, float sign,
+                int block_rows, T* __restrict__ y) {
+    extern __shared__ float2 table[];
+    const long long first = static_cast<long long>(blockIdx.x) * block_rows;
+    const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
+    rotary_table(table, axes, positions, frequencies, first, count, sign);
+    __syncthreads();
+    const long long width = static_cast<long long>(heads) * dim;
+    for (long long i = threadIdx.x; i < count * width; i += kRotaryBlock) {
+        const int row = static_cast<int>(i / width);
+        const int at = static_cast<int>(i - row * width);
+        const int head = at / dim;
+        const RotaryChannel ch = rotary_channel(axes, at - head * dim);
+        const T* in = x + (first + row) * x_row + head * x_head;
+        T out = in[at - head * dim];
+        if (ch.pair >= 0) {
+            const float2 t = table[row * axes.pairs + ch.pair];
+            out = static_cast<T>(static_cast<float>(out) * t.x +
+                                 ch.sign * (static_cast<float>(in[ch.partner]) * t.y));
+        }
+        y[first * width + i] = out;
+    }
+}
+
+template <typename T>
+int rotary_of(const void* x, long long x_row, long long x_head, int rows, int heads, int dim,
+              const RotaryPositions& positions, const double* frequencies, const RotaryAxes& axes, float sign,
+              void* y, hipStream_t stream) {
+    constexpr int kMost = 16 / sizeof(T);
+    const T* in = static_cast<const T*>(x);
+    T* out = static_cast<T*>(y);
+    // A table of about 512 pairs a block, fewer where that leaves units idle.
+    const int block_rows = static_cast<int>(std::max<long long>(
+        1, std::min<long long>(std::max(1, 512 / std::max(1, axes.pairs)), (rows + 1023ll) / 1024)));
+    const unsigned grid = static_cast<unsigned>((static_cast<long long>(rows) + block_rows - 1) / block_rows);
+    const size_t lds = static_cast<size_t>(block_rows) * axes.pairs * sizeof(float2);
+    if (row_vector<T>(dim, {x, y}, {x_row, x_head}) == kMost && dim / kMost <= kWave) {
+        rotary_rows<T, kMost><<<grid, kRotaryBlock, lds, stream>>>(in, x_row, x_head, rows, heads, dim, positions,
+                                                                   frequencies, axes, sign, block_rows, out);
+    } else {
+        rotary_channels<T><<<grid, kRotaryBlock, lds, stream>>>(in, x_row, x_head, rows, heads, dim, positions,
+                                                                frequencies, axes, sign, block_rows, out);
+    }
+    LATTICE_LAUNCH_CHECK();
+    return LATTICE_OK;
+}
+
+}  // namespace
+}  // namespace lattice
+
+using namespace lattice;
+
+extern "C" int lattice_hip_rotary_positions(int dtype, const void* x, long long x_row_stride, long long x_head_stride,
+                                            int rows, int heads, int dim, const void* positions, int float_positions,
+                                            long long position_stride, const double* frequencies, int axes,
+                                            const int32_t* dims, int interleaved, int inverse, void* y,
+                                            void* stream_ptr) {
+    LATTICE_REQUIRE(dtype == LATTICE_F32 || dtype == LATTICE_F16 || dtype == LATTICE_BF16,
+                    "rotary positions support float32, float16 and bfloat16.");
+    LATTICE_REQUIRE(rows >= 0 && heads > 0 && dim > 0 && dim <= kRotaryMaxDim,
+                    "rotary heads must have between 1 and 1024 channels.");
+    LATTICE_REQUIRE(x_row_stride >= 0 && x_head_stride >= 0 && position_stride >= 0,
+                    "rotary strides must be non-negative.");
+    LATTICE_REQUIRE(axes >= 1 && axes <= kRotaryAxes && dims, "rotary positions need between 1 and 4 axes.");
+    RotaryAxes sections{axes, 0, interleaved != 0, {0, 0, 0, 0}};
+    for (int a = 0; a < axes; ++a) {
+        LATTICE_REQUIRE(dims[a] >= 0 && dims[a] % 2 == 0 && dims[a] <= kRotaryMaxDim,
+                        "rotary dims must be even and non-negative.");
+        sections.dims[a] = dims[a];
+        sections.pairs += dims[a] / 2;
+    }
+    LATTICE_REQUIRE(2 * sections.pairs <= dim, "rotary dims must fit the head.");
+    if (rows == 0) return LATTICE_OK;
+    LATTICE_REQUIRE(x && y && positions && (frequencies || sections.pairs == 0),
+                    "rotary pointers must be non-null.");
+    const RotaryPositions at{positions, position_stride, float_positions != 0};
+    const float sign = inverse ? -1.0f : 1.0f;
+    hipStream_t stream = as_stream(stream_ptr);
+    if (dtype == LATTICE_F32)
+        return rotary_of<float>(x, x_row_stride, x_head_stride, rows, heads, dim, at, frequencies, sections, sign, y,
+                                stream);
+    if (dtype == LATTICE_F16)
+        return rotary_of<_Float16>(x, x_row_stride, x_head_stride, rows, heads, dim, at, frequencies, sections, sign,
+                                   y, stream);
+    return rotary_of<__bf16>(x, x_row_stride, x_head_stride, rows, heads, dim, at, frequencies, sections, sign, y,
+                             stream);
+}

@@ -1,12 +1,15 @@
 from mlx_lattice_amd.core.coords.builders import (
     build_relation_implicit_gemm_view,
 )
+from mlx_lattice_amd.ops.attention import batch_offsets, window_attention
 from mlx_lattice_amd.ops.conv import (
     conv3d,
     conv_transpose3d,
     generative_conv_transpose3d,
     subm_conv3d,
 )
+from mlx_lattice_amd.ops.dropout import dropout
+from mlx_lattice_amd.ops.norm import layer_norm
 from mlx_lattice_amd.ops.pool import (
     avg_pool3d,
     global_avg_pool,
@@ -37,10 +40,12 @@ from mlx_lattice_amd.ops.relations import (
     target_kernel_relation,
     transposed_kernel_relation,
 )
+from mlx_lattice_amd.ops.rotary import rotary_frequencies, rotary_positions
 from mlx_lattice_amd.ops.tensor import sparse_collate
 
 __all__ = [
     'avg_pool3d',
+    'batch_offsets',
     'build_generative_relation',
     'build_point_voxel_map',
     'build_kernel_relation',
@@ -51,6 +56,7 @@ __all__ = [
     'conv3d',
     'conv_transpose3d',
     'devoxelize',
+    'dropout',
     'generative_conv_transpose3d',
     'generative_kernel_relation',
     'global_avg_pool',
@@ -59,8 +65,11 @@ __all__ = [
     'interpolate_point_features',
     'kernel_offsets',
     'kernel_relation',
+    'layer_norm',
     'max_pool3d',
     'pool3d',
+    'rotary_frequencies',
+    'rotary_positions',
     'sparse_collate',
     'sparse_quantize',
     'subm_conv3d',
@@ -70,4 +79,5 @@ __all__ = [
     'transposed_kernel_relation',
     'voxelize',
     'voxelize_with_quantization',
+    'window_attention',
 ]

@@ -1,0 +1,88 @@
+"""Attention over a sliding window of rows, with first rows that stay visible
+(no reference counterpart)."""
+
+from __future__ import annotations
+
+import torch
+
+from mlx_lattice_amd._native import ext
+from mlx_lattice_amd.core import SparseTensor
+
+__all__ = ['batch_offsets', 'window_attention']
+
+_ALL = 2 ** 31 - 1
+
+
+def batch_offsets(x: SparseTensor) -> torch.Tensor:
+    """Row offsets ``(B + 1,)`` of the scans of ``x``, int32 on its device,
+    from ``batch_counts``; without them the active rows are one sequence.
+    Rows of a scan are adjacent, as ``sparse_collate`` lays them."""
+    counts = x.batch_counts
+    if counts is None or len(counts) == 1:
+        return torch.cat([torch.zeros_like(x.active_rows), x.active_rows])
+    offsets = [0]
+    for count in counts:
+        offsets.append(offsets[-1] + count)
+    return torch.tensor(offsets, dtype=torch.int32, device=x.device)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                     offsets: torch.Tensor,
+                     key_offsets: torch.Tensor | None = None,
+                     key_lengths: torch.Tensor | None = None,
+                     left: int | None = None, right: int | None = None,
+                     sinks: int = 0, scale: float | None = None
+                     ) -> torch.Tensor:
+    """Softmax attention of packed sequences, ``(queries, heads, dim)``.
+
+    ``q`` has shape ``(queries, heads, dim)``, ``k`` and ``v`` ``(keys,
+    kv_heads, dim)`` with ``heads`` a multiple of ``kv_heads``; each may be a
+    slice of packed rows.  float32, float16 or bfloat16, ``dim`` up to 128;
+    ``scale`` is ``dim ** -0.5`` by default.
+
+    Sequence ``s`` holds the query rows ``offsets[s] : offsets[s + 1]`` and the
+    key rows of ``key_offsets`` (``offsets`` by default), of which
+    ``key_lengths[s]`` are filled (all by default): a cache of ``B`` sequences
+    of ``L`` rows has ``key_offsets = arange(B + 1) * L``.  All three are int32
+    on the device and are not read back.
+
+    Query ``i`` of ``nq``, in a sequence of ``nk`` keys, has position ``p = i +
+    nk - nq``: queries sit at the end of the keys.  It sees key ``j`` where
+    ``j <= p + right`` and either ``j >= p - left`` or ``j < sinks``; ``None``
+    is no bound, ``right=0`` is causal.  A query that sees nothing gives zeros
+    and no gradient, as do rows in no sequence; what a query does not see never
+    reaches it, be it infinite or NaN.
+
+    Differentiable in ``q``, ``k`` and ``v``; the gradients of a shared key
+    head are summed over its query heads, in a fixed order.
+    """
+    left, right = (_ALL if b is None else int(b) for b in (left, right))
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if key_offsets is None:
+        key_offsets = offsets
+    layout = (offsets, key_offsets, key_lengths)
+    window = (left, right, int(sinks), float(scale))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or v.requires_grad):
+        return _WindowAttention.apply(q, k, v, *layout, window)
+    return ext.window_attention(q, k, v, *layout, *window, False)[0]
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, key_offsets, key_lengths, window):
+        out, lse = ext.window_attention(q, k, v, offsets, key_offsets,
+                                        key_lengths, *window, True)
+        ctx.save_for_backward(q, k, v, out, lse, offsets, key_offsets,
+                              key_lengths)
+        ctx.window = window
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, *layout = ctx.saved_tensors
+        grads = ext.window_attention_grad(grad_out, out, lse, q, k, v, *layout,
+                                          *ctx.window)
+        return (*grads, None, None, None, None)

@@ -17,6 +17,7 @@
 #include "features/pooling/api.h"
 #include "features/quantization/api.h"
 #include "features/coordinates/relations.h"
+#include "features/transformer/api.h"
 #include "foundation/runtime.h"
 #include "lattice_hip.h"
 
@@ -407,4 +408,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("in_active_rows"), py::arg("reduce"));
     m.def("global_pool", &ln::global_pool, py::arg("feats"), py::arg("batch_counts"), py::arg("mode"),
           "Per-batch global pooling: (B, C).");
+
+    // Operators of a transformer block (no reference counterpart).
+    m.def("layer_norm", &ln::layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),
+          py::arg("active_rows"), py::arg("keep_statistics"),
+          "Layer norm of rows: (y, statistics); statistics (N, 2) are kept for the gradient.");
+    m.def("layer_norm_grad", &ln::layer_norm_grad, py::arg("cotangent"), py::arg("x"), py::arg("weight"),
+          py::arg("statistics"), py::arg("active_rows"), py::arg("grad_weight"), py::arg("grad_bias"),
+          "Gradients of layer norm: (grad_x, grad_weight, grad_bias).");
+    m.def("dropout", &ln::dropout, py::arg("x"), py::arg("residual"), py::arg("seed"), py::arg("offset"),
+          py::arg("threshold"), py::arg("scale"), "Counter-based dropout, added to a residual.");
+    m.def("rotary_positions", &ln::rotary_positions, py::arg("x"), py::arg("positions"), py::arg("frequencies"),
+          py::arg("dims"), py::arg("interleaved"), py::arg("inverse"), "Rotary positions of several axes.");
+    m.def("window_attention", &ln::window_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"),
+          py::arg("key_offsets"), py::arg("key_lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"),
+          py::arg("scale"), py::arg("keep_lse"), "Attention over a sliding window: (out, lse).");
+    m.def("window_attention_grad", &ln::window_attention_grad, py::arg("cotangent"), py::arg("out"), py::arg("lse"),
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("key_offsets"),
+          py::arg("key_lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"), py::arg("scale"),
+          "Gradients of the windowed attention: (grad_q, grad_k, grad_v).");
 }

@@ -1,0 +1,41 @@
+// Operators of a transformer block over feature rows: layer norm, dropout,
+// rotary positions and windowed attention, with their gradients.
+#pragma once
+
+#include <torch/extension.h>
+
+#include <cstdint>
+#include <tuple>
+#include <vector>
+
+namespace lattice_native {
+
+// (y, statistics); statistics is empty unless kept for the gradient.
+std::tuple<at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                                              const c10::optional<at::Tensor>& bias, double eps,
+                                              const c10::optional<at::Tensor>& active_rows, bool keep_statistics);
+// (grad_x, grad_weight, grad_bias); the last two are empty unless asked for.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor& grad_y, const at::Tensor& x,
+                                                               const c10::optional<at::Tensor>& weight,
+                                                               const at::Tensor& statistics,
+                                                               const c10::optional<at::Tensor>& active_rows,
+                                                               bool grad_weight, bool grad_bias);
+
+at::Tensor dropout(const at::Tensor& x, const c10::optional<at::Tensor>& residual, uint64_t seed, uint64_t offset,
+                   uint64_t threshold, double scale);
+
+at::Tensor rotary_positions(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies,
+                            const std::vector<int>& dims, bool interleaved, bool inverse);
+
+// (out, lse); lse is empty unless kept for the gradient.
+std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& offsets, const at::Tensor& key_offsets,
+                                                    const c10::optional<at::Tensor>& key_lengths, int64_t left,
+                                                    int64_t right, int64_t sinks, double scale, bool keep_lse);
+// (grad_q, grad_k, grad_v).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_grad(
+    const at::Tensor& grad_out, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& q,
+    const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& key_offsets,
+    const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right, int64_t sinks, double scale);
+
+}  // namespace lattice_native
