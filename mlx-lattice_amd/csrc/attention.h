@@ -27,7 +27,7 @@ struct RowPartition {
     // The last sequence whose first slot, slot_of(start) + sequence, is at
     // most `slot`; all lanes of the wave together, 64 probes a step.
     template <typename SlotOf>
-    __device__ int find(long long slot, SlotOf slot_of) const {
+    __device__ int find(uint32_t slot, SlotOf slot_of) const {
         int lo = 0, n = count + 2;
         while (n > 1) {
             const int step = (n + kWave - 1) / kWave;
@@ -309,6 +309,8 @@ inline const char* attn_fault(const lattice_attention* a) {
                                  a->k_head_stride, a->v_row_stride, a->v_head_stride};
     for (long long s : strides)
         if (s < 0 || s % piece != 0) return "attention strides must be whole 16-byte pieces.";
+    if (std::max({a->q_row_stride, a->k_row_stride, a->v_row_stride}) >= piece << 20)
+        return "attention row strides must be under 16 MiB.";
     if (a->dim % piece != 0) return "attention rows must be whole 16-byte pieces.";
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) %
         16 != 0)

@@ -4,8 +4,12 @@
 //   s_ij = scale q_i . k_j over the keys j that query i sees,
 //   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),
 // with the running maximum m and sum of one pass over the keys.
+//
+// The rows of a tile are (query, head) pairs of the heads that share a key
+// head, so that each key is staged once for all of them and the band of keys
+// that a tile sees is as narrow as may be.
 
-#include "attention.h"
+#include "attention_tiles.h"
 
 namespace lattice {
 namespace {
@@ -13,26 +17,446 @@ namespace {
 constexpr int kAttnBlock = 256;
 constexpr int kAttnWaves = kAttnBlock / kWave;
 
-// A wave a (query row, head).
+// The share of a softmax over some of a row's keys: sum over them of
+// exp2(x - top) and of that times v.
+struct AttnPart {
+    float* values;  // [splits][queries * heads][dim]
+    float2* states;  // [splits][queries * heads]: (top, sum)
+};
+
+// A row's running maximum starts far below every score but above -inf, so
+// that what is masked (-inf) keeps an exponent of zero.
+constexpr float kAttnFloor = -3.0e38f;
+// The maximum in use may lag behind the scores by this many powers of two
+// before the sums are scaled down to a new one; the shares stay below 2^8,
+// far inside every type.
+constexpr float kAttnLag = 8.0f;
+
+template <typename T, int DP>
+struct AttnState {
+    static constexpr int kBlocks = DP / 32;
+    f32x16_attn acc[kBlocks];
+    float top, sum;
+
+    __device__ void clear() {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[b] = f32x16_attn{};
+        top = kAttnFloor;
+        sum = 0.0f;
+    }
+    __device__ void rescale(float factor) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[b] *= factor;
+        sum *= factor;
+    }
+};
+
+// The keys j0 .. j0 + 32 BLOCKS of a tile for the wave's 32 rows; `masked`:
+// some of them are not seen by some row.
+template <typename T, int DP, int KT>
+__device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>& state, const AttnOperand<T, DP>& q,
+                                   const char* keys, const char* values, float scale, int nk, int p, int j0,
+                                   bool masked) {
+    typedef AttnTile<T, DP, KT> Tile;
+    constexpr int kParts = KT / 32;
+    f32x16_attn s[kParts];
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) s[part] = tile_product<Tile, T, DP>(keys, 32 * part, q);
+    if (masked) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = j0 + 32 * part + result_row(r);
+                if (!attn_visible(a, nk, p, j)) s[part][r] = -INFINITY;
+            }
+        }
+    }
+    float most = s[0][0];
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, s[part][r]);
+    }
+    most = fmaxf(most, other_half(most)) * scale;
+    if (__any(most > state.top + kAttnLag)) {
+        const float next = fmaxf(state.top, most);
+        state.rescale(__builtin_amdgcn_exp2f(state.top - next));
+        state.top = next;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[part][r] = __builtin_amdgcn_exp2f(s[part][r] * scale - state.top);
+            sum += s[part][r];
+        }
+    }
+    state.sum += sum;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) add_columns<Tile, T>(state.acc, values, 32 * part, s[part]);
+}
+
+// What a wave's 32 rows are: row L % 32 of the tile.
+struct AttnRows {
+    int i, head, p;      // query of the sequence, head, position
+    bool valid;
+    int p_low, p_high;   // of all 32 rows
+};
+__device__ inline AttnRows attn_rows(const AttnSequence& s, int kv, uint32_t group, uint32_t first) {
+    const uint32_t rows = s.nq * group;
+    const uint32_t r = first + (lane_id() & 31);
+    const uint32_t in = min(r, rows - 1);
+    AttnRows w;
+    w.i = in / group;
+    w.head = kv * group + in % group;
+    w.p = w.i + s.shift();
+    w.valid = r < rows;
+    w.p_low = __builtin_amdgcn_readfirstlane(w.i) + s.shift();
+    w.p_high = __builtin_amdgcn_readlane(w.i, 31) + s.shift();
+    return w;
+}
+
+// Writes the wave's rows: the result, or a part of it (splits > 1).  A result
+// that is not finite is made again row by row: products over a tile carry a
+// zero share of what a row does not see, which spoils the row if that is not
+// finite.
+template <typename T, int DP>
+__device__ inline void write_rows(const lattice_attention& a, const AttnSequence& s, const AttnRows& w,
+                                  AttnState<T, DP>& state, bool partial, int split, const AttnPart& part, T* out,
+                                  float* lse, AttnRowScratch* scratch) {
+    const int half = lane_id() >> 5;
+    const float sum = state.sum + other_half(state.sum);
+    const long long at = (static_cast<long long>(s.q0) + w.i) * a.heads + w.head;
+    if (partial) {
+        if (!w.valid) return;
+        const long long row = static_cast<long long>(split) * a.queries * a.heads + at;
+        if (half == 0) part.states[row] = float2{state.top, sum};
+#pragma unroll
+        for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * b + 8 * g + 4 * half;
+                if (d >= a.dim) continue;
+                RowVec<float, 4> v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v.e[i] = state.acc[b][4 * g + i];
+                v.store(part.values + row * a.dim + d);
+            }
+        }
+        return;
+    }
+    const bool sees = attn_seen(a, s.nk, w.p).total() > 0;
+    const float inv = 1.0f / sum;
+    bool finite = true;
+#pragma unroll
+    for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            state.acc[b][r] = sees ? state.acc[b][r] * inv : 0.0f;
+            const int d = 32 * b + result_row(r);
+            finite = finite && (d >= a.dim || fabsf(state.acc[b][r]) < INFINITY);
+        }
+    }
+    const uint64_t spoilt = ballot(w.valid && !finite);
+    uint32_t again = static_cast<uint32_t>(spoilt) | static_cast<uint32_t>(spoilt >> 32);
+    if (w.valid && !(again >> (lane_id() & 31) & 1)) {
+        if (lse && half == 0) lse[at] = sees ? state.top + __builtin_amdgcn_logf(sum) : INFINITY;
+#pragma unroll
+        for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * b + 8 * g + 4 * half;
+                if (d >= a.dim) continue;
+                RowVec<T, 4> v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v.set(i, state.acc[b][4 * g + i]);
+                v.store(out + at * a.dim + d);
+            }
+        }
+    }
+    while (again) {
+        const int n = __ffs(again) - 1;
+        again &= again - 1;
+        attend_row<T>(a, s, __shfl(w.i, n), __shfl(w.head, n), out, lse, scratch);
+    }
+}
+
+// Which sequence, tile of M rows and key head a block has.
+struct AttnSlot {
+    AttnSequence s;
+    uint32_t rows, first;  // (query, head) pairs: of the sequence, before the tile's
+};
+template <int M>
+__device__ inline AttnSlot attn_slot(const lattice_attention& a, uint32_t group, uint32_t slot) {
+    // Sequence e has the slots from start / M + e on: enough for its tiles.
+    const auto slot_of = [group](int start, int e) { return start * group / M + e; };
+    const int e = query_rows(a).find(slot, slot_of);
+    AttnSlot t;
+    t.s = attn_sequence(a, e);
+    t.rows = t.s.nq * group;
+    t.first = (slot - slot_of(t.s.q0, e)) * M;
+    return t;
+}
+
+// 128 rows a block, 32 a wave, over tiles of KT keys that the waves share.
+// Double-buffered: a tile is copied to LDS while the one before is used.
+template <typename T, int DP, int KT>
+__global__ void __launch_bounds__(kAttnBlock, 2)
+attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
+    typedef AttnTile<T, DP, KT> Tile;
+    extern __shared__ __align__(128) char shared[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t group = a.heads / a.kv_heads;
+    const int kv = blockIdx.y, split = blockIdx.z;
+    const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
+    const AttnSequence s = t.s;
+    if (t.first >= t.rows) return;
+    const bool negate = a.scale < 0.0f;
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const AttnRows w = attn_rows(s, kv, group, t.first + 32 * wave);
+    AttnOperand<T, DP> q;
+    q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
+               w.head * a.q_head_stride,
+           a.dim, w.valid, negate);
+    AttnState<T, DP> state;
+    state.clear();
+    const int p_low = static_cast<int>(t.first / group) + s.shift();
+    const int p_high = static_cast<int>((min(t.first + 32 * kAttnWaves, t.rows) - 1) / group) + s.shift();
+    const AttnTiles tiles = attn_tiles<KT>(a, s.nk, p_low, p_high);
+    const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
+    const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
+    const T* keys = static_cast<const T*>(a.k) + s.k0 * a.k_row_stride + kv * a.k_head_stride;
+    const T* values = static_cast<const T*>(a.v) + s.k0 * a.v_row_stride + kv * a.v_head_stride;
+    const int pieces = a.dim * static_cast<int>(sizeof(T)) / 16;
+    const auto copy = [&](int index) {
+        const int j0 = tiles.tile(index) * KT;
+        char* at = shared + (index & 1) * 2 * Tile::kBytes;
+        Tile::template load<kAttnBlock>(at, keys + j0 * a.k_row_stride, a.k_row_stride, s.nk - j0, pieces,
+                                        threadIdx.x);
+        Tile::template load<kAttnBlock>(at + Tile::kBytes, values + j0 * a.v_row_stride, a.v_row_stride, s.nk - j0,
+                                        pieces, threadIdx.x);
+    };
+    if (from < to) copy(from);
+    __syncthreads();
+    for (int index = from; index < to; ++index) {
+        if (index + 1 < to) copy(index + 1);
+        const int j0 = tiles.tile(index) * KT;
+        const char* at = shared + (index & 1) * 2 * Tile::kBytes;
+        const bool none = j0 > w.p_high + a.right || (j0 + KT - 1 < w.p_low - a.left && j0 >= a.sinks);
+        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
+                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
+        if (!none)
+            attend_tile<T, DP, KT>(a, state, q, at, at + Tile::kBytes, scale, s.nk, w.p, j0, !all);
+        __syncthreads();
+    }
+    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, lse,
+                      reinterpret_cast<AttnRowScratch*>(shared) + wave);
+}
+
+// 32 rows a block, for few queries: each wave takes every fourth tile, and the
+// waves' parts are joined in LDS.
+template <typename T, int DP, int KT>
+__global__ void __launch_bounds__(kAttnBlock)
+attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
+    typedef AttnTile<T, DP, KT> Tile;
+    constexpr int kBlocks = AttnState<T, DP>::kBlocks;
+    extern __shared__ __align__(128) char shared[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t group = a.heads / a.kv_heads;
+    const int kv = blockIdx.y, split = blockIdx.z;
+    const AttnSlot t = attn_slot<32>(a, group, blockIdx.x);
+    const AttnSequence s = t.s;
+    if (t.first >= t.rows) return;
+    const bool negate = a.scale < 0.0f;
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const AttnRows w = attn_rows(s, kv, group, t.first);
+    AttnOperand<T, DP> q;
+    q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
+               w.head * a.q_head_stride,
+           a.dim, w.valid, negate);
+    AttnState<T, DP> state;
+    state.clear();
+    const AttnTiles tiles = attn_tiles<KT>(a, s.nk, w.p_low, w.p_high);
+    const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
+    const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
+    const T* keys = static_cast<const T*>(a.k) + s.k0 * a.k_row_stride + kv * a.k_head_stride;
+    const T* values = static_cast<const T*>(a.v) + s.k0 * a.v_row_stride + kv * a.v_head_stride;
+    const int pieces = a.dim * static_cast<int>(sizeof(T)) / 16;
+    char* mine = shared + wave * 2 * Tile::kBytes;
+    const int steps = (to - from + kAttnWaves - 1) / kAttnWaves;
+    for (int step = 0; step < steps; ++step) {
+        const int index = from + step * kAttnWaves + wave;
+        const int j0 = index < to ? tiles.tile(index) * KT : 0;
+        __syncthreads();
+        if (index < to) {
+            Tile::template load<kWave>(mine, keys + j0 * a.k_row_stride, a.k_row_stride, s.nk - j0, pieces, lane_id());
+            Tile::template load<kWave>(mine + Tile::kBytes, values + j0 * a.v_row_stride, a.v_row_stride, s.nk - j0,
+                                       pieces, lane_id());
+        }
+        __syncthreads();
+        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
+                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
+        if (index < to)
+            attend_tile<T, DP, KT>(a, state, q, mine, mine + Tile::kBytes, scale, s.nk, w.p, j0, !all);
+    }
+    // The waves' sums meet in the first wave, in wave order.
+    const int lane = lane_id();
+    state.sum += other_half(state.sum);
+    __syncthreads();
+    float2* states = reinterpret_cast<float2*>(shared);
+    float* sums = reinterpret_cast<float*>(shared + kAttnWaves * 32 * sizeof(float2));
+    if (lane < 32) states[wave * 32 + lane] = float2{state.top, state.sum};
+    __syncthreads();
+    float top = kAttnFloor;
+    for (int v = 0; v < kAttnWaves; ++v) top = fmaxf(top, states[v * 32 + (lane & 31)].x);
+    float sum = 0.0f;
+    for (int v = 0; v < kAttnWaves; ++v) {
+        const float2 other = states[v * 32 + (lane & 31)];
+        sum += other.y * __builtin_amdgcn_exp2f(other.x - top);
+    }
+    const float factor = __builtin_amdgcn_exp2f(state.top - top);
+    for (int v = 1; v < kAttnWaves; ++v) {
+        __syncthreads();
+        if (wave == v) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[(b * 16 + r) * kWave + lane] = state.acc[b][r] * factor;
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {
+            if (v == 1) state.rescale(factor);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) state.acc[b][r] += sums[(b * 16 + r) * kWave + lane];
+            }
+        }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    state.top = top;
+    state.sum = lane < 32 ? sum : 0.0f;  // write_rows adds the halves
+    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, lse,
+                      reinterpret_cast<AttnRowScratch*>(shared));
+}
+
+// Joins the parts of a row: a wave a (query row, head).
 template <typename T>
 __global__ void __launch_bounds__(kAttnBlock)
-attend_rows(lattice_attention a, T* __restrict__ out, float* __restrict__ lse) {
+join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
     __shared__ AttnRowScratch scratch[kAttnWaves];
-    const int wave = threadIdx.x / kWave;
-    const long long item = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
-    if (item >= static_cast<long long>(a.queries) * a.heads) return;
-    const int row = static_cast<int>(item / a.heads), head = static_cast<int>(item % a.heads);
-    const int e = query_rows(a).find(row, [](int start, int) { return static_cast<long long>(start); });
+    const int wave = threadIdx.x / kWave, lane = lane_id();
+    const long long items = static_cast<long long>(a.queries) * a.heads;
+    const long long at = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
+    if (at >= items) return;
+    const int row = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
+    const int e = query_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
     const AttnSequence s = attn_sequence(a, e);
-    attend_row<T>(a, s, row - s.q0, head, out, lse, &scratch[wave]);
+    const int i = row - s.q0;
+    const bool sees = attn_seen(a, s.nk, i + s.shift()).total() > 0;
+    float acc[kAttnMaxDim / kWave] = {}, top = kAttnFloor, sum = 0.0f;
+    if (sees) {
+        for (int z = 0; z < splits; ++z) top = fmaxf(top, part.states[z * items + at].x);
+        for (int z = 0; z < splits; ++z) {
+            const float2 state = part.states[z * items + at];
+            const float factor = __builtin_amdgcn_exp2f(state.x - top);
+            sum += state.y * factor;
+#pragma unroll
+            for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
+                const int d = lane + c * kWave;
+                if (d < a.dim) acc[c] += part.values[(z * items + at) * a.dim + d] * factor;
+            }
+        }
+    }
+    bool finite = true;
+#pragma unroll
+    for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
+        if (sees) acc[c] = lane + c * kWave < a.dim ? acc[c] / sum : 0.0f;
+        finite = finite && fabsf(acc[c]) < INFINITY;
+    }
+    if (__any(!finite)) {
+        attend_row<T>(a, s, i, head, out, lse, &scratch[wave]);
+        return;
+    }
+    if (lse && lane == 0) lse[at] = sees ? top + log2f(sum) : INFINITY;
+#pragma unroll
+    for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
+        const int d = lane + c * kWave;
+        if (d < a.dim) out[at * a.dim + d] = static_cast<T>(acc[c]);
+    }
+}
+
+// How a call is laid out: rows a tile, tiles of rows at most, and into how
+// many blocks the keys of a tile of rows are split.
+struct AttnLayout {
+    bool few;
+    long long slots;
+    int splits;
+};
+inline AttnLayout attn_layout(const lattice_attention& a) {
+    const int group = a.heads / a.kv_heads;
+    const long long pairs = static_cast<long long>(a.queries) * group;
+    const int sequences = std::max(1, a.sequences);
+    AttnLayout l;
+    // Few rows a sequence leave three of four waves of a large tile idle.
+    l.few = pairs <= 32ll * sequences;
+    const int m = l.few ? 32 : 128;
+    l.slots = pairs / m + a.sequences + 2;
+    // Blocks that have rows, and the keys that one sees, were the rows spread
+    // evenly over the sequences.
+    const long long busy =
+        std::max<long long>((pairs + m - 1) / m, std::min<long long>(sequences, a.queries)) * a.kv_heads;
+    const long long span = static_cast<long long>(a.left) + a.right + std::min(m, a.queries) + a.sinks;
+    const long long seen = std::min<long long>(span, (static_cast<long long>(a.keys) + sequences - 1) / sequences);
+    // Two blocks a compute unit, each with at least 512 keys.
+    const long long wanted = std::min<long long>((512 + busy - 1) / busy, seen / 512);
+    l.splits = static_cast<int>(std::max<long long>(1, std::min<long long>(wanted, 64)));
+    return l;
+}
+
+template <typename T, int DP>
+int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, T* out, float* lse,
+                  hipStream_t stream) {
+    constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
+    typedef AttnTile<T, DP, kTile> Tile;
+    const dim3 grid(static_cast<unsigned>(l.slots), a.kv_heads, l.splits);
+    if (l.few) {
+        constexpr int kFew = 32;
+        constexpr size_t kLds = std::max<size_t>(kAttnWaves * 2 * AttnTile<T, DP, kFew>::kBytes,
+                                                 kAttnWaves * 32 * sizeof(float2) + DP / 32 * 16 * kWave * 4);
+        static_assert(kLds >= sizeof(AttnRowScratch) && kLds <= 160 * 1024);
+        const auto kernel = attend_few<T, DP, kFew>;
+        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, lse);
+    } else {
+        constexpr size_t kLds = std::max<size_t>(4 * Tile::kBytes, kAttnWaves * sizeof(AttnRowScratch));
+        static_assert(kLds <= 160 * 1024);
+        const auto kernel = attend_tiles<T, DP, kTile>;
+        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, lse);
+    }
+    LATTICE_LAUNCH_CHECK();
+    if (l.splits > 1) {
+        join_parts<T><<<grid_for(static_cast<long long>(a.queries) * a.heads, kAttnWaves, 1u << 30), kAttnBlock, 0,
+                        stream>>>(a, l.splits, part, out, lse);
+        LATTICE_LAUNCH_CHECK();
+    }
+    return LATTICE_OK;
 }
 
 template <typename T>
-int attend(const lattice_attention& a, void* out, float* lse, hipStream_t stream) {
-    attend_rows<T><<<grid_for(static_cast<long long>(a.queries) * a.heads, kAttnWaves, 1u << 30), kAttnBlock, 0,
-                     stream>>>(a, static_cast<T*>(out), lse);
-    LATTICE_LAUNCH_CHECK();
-    return LATTICE_OK;
+int attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, void* out, float* lse,
+           hipStream_t stream) {
+    T* o = static_cast<T*>(out);
+    if (a.dim <= 32) return launch_attend<T, 32>(a, l, part, o, lse, stream);
+    if (a.dim <= 64) return launch_attend<T, 64>(a, l, part, o, lse, stream);
+    return launch_attend<T, 128>(a, l, part, o, lse, stream);
 }
 
 }  // namespace
@@ -41,7 +465,12 @@ int attend(const lattice_attention& a, void* out, float* lse, hipStream_t stream
 using namespace lattice;
 
 extern "C" size_t lattice_hip_window_attention_workspace_bytes(const lattice_attention* args) {
-    return attn_fault(args) ? 0 : 0;
+    if (attn_fault(args) || args->queries == 0) return 0;
+    const lattice_attention a = attn_bounded(*args);
+    const AttnLayout l = attn_layout(a);
+    if (l.splits == 1) return 0;
+    const size_t rows = static_cast<size_t>(l.splits) * a.queries * a.heads;
+    return aligned_bytes(rows * a.dim * sizeof(float)) + aligned_bytes(rows * sizeof(float2));
 }
 
 extern "C" int lattice_hip_window_attention(const lattice_attention* args, void* out, float* lse, void* workspace,
@@ -49,11 +478,18 @@ extern "C" int lattice_hip_window_attention(const lattice_attention* args, void*
     LATTICE_REQUIRE_ATTENTION(args);
     if (args->queries == 0) return LATTICE_OK;
     LATTICE_REQUIRE(out, "attention pointers must be non-null.");
-    (void)workspace;
-    (void)workspace_bytes;
     const lattice_attention a = attn_bounded(*args);
+    const AttnLayout l = attn_layout(a);
+    AttnPart part{nullptr, nullptr};
+    if (l.splits > 1) {
+        Workspace ws{static_cast<char*>(workspace), workspace ? workspace_bytes : 0};
+        const size_t rows = static_cast<size_t>(l.splits) * a.queries * a.heads;
+        part.values = ws.take<float>(rows * a.dim);
+        part.states = ws.take<float2>(rows);
+        LATTICE_REQUIRE(part.values && part.states, "attention workspace is too small.");
+    }
     hipStream_t stream = as_stream(stream_ptr);
-    if (a.dtype == LATTICE_F32) return attend<float>(a, out, lse, stream);
-    if (a.dtype == LATTICE_F16) return attend<_Float16>(a, out, lse, stream);
-    return attend<__bf16>(a, out, lse, stream);
+    if (a.dtype == LATTICE_F32) return attend<float>(a, l, part, out, lse, stream);
+    if (a.dtype == LATTICE_F16) return attend<_Float16>(a, l, part, out, lse, stream);
+    return attend<__bf16>(a, l, part, out, lse, stream);
 }

@@ -25,7 +25,7 @@ grad_query_rows(lattice_attention a, const T* __restrict__ out, const float* __r
     const long long item = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
     if (item >= static_cast<long long>(a.queries) * a.heads) return;
     const int row = static_cast<int>(item / a.heads), head = static_cast<int>(item % a.heads);
-    const int e = query_rows(a).find(row, [](int start, int) { return static_cast<long long>(start); });
+    const int e = query_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
     const AttnSequence s = attn_sequence(a, e);
     const float d = attn_delta(a, row, head, out, grad_out);
     if (lane_id() == 0) delta[item] = d;
@@ -42,7 +42,7 @@ grad_key_rows(lattice_attention a, const float* __restrict__ lse, const float* _
     const long long item = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
     if (item >= static_cast<long long>(a.keys) * a.kv_heads) return;
     const int row = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item % a.kv_heads);
-    const int e = key_rows(a).find(row, [](int start, int) { return static_cast<long long>(start); });
+    const int e = key_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
     const AttnSequence s = attn_sequence(a, e);
     grad_key_row<T>(a, s, row - s.k0, kv, lse, delta, grad_out, grad_k, grad_v, &scratch[wave]);
 }

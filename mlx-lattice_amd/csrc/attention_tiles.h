@@ -1,0 +1,200 @@
+// Tiles of the windowed attention's matrix-core kernels: 32 x 32 products
+// (v_mfma_f32_32x32x16 for 16-bit types, 32x32x2 for fp32) over rows staged in
+// LDS.
+//
+// A product's result holds, in lane L = 32 h + n and register r, row
+// 8 (r / 4) + 4 h + r % 4 of column n.  The scores are made transposed (rows:
+// keys, columns: queries), so that a lane holds the scores of one query: the
+// softmax runs within a lane but for one exchange between the halves, and a
+// lane's registers are, in the order they lie, the right operand of the next
+// product, whose left operand is read in the same order of rows.
+#pragma once
+
+#include "attention.h"
+
+namespace lattice {
+
+typedef float f32x16_attn __attribute__((ext_vector_type(16)));
+typedef float f32x4_attn __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_attn __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_attn __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_attn __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_attn __attribute__((ext_vector_type(4)));
+typedef short i16x4_attn __attribute__((__vector_size__(4 * sizeof(short))));
+
+// Frag: the 16 bytes a lane gives to the products over KSTEP channels (or
+// rows); half h holds values 8 h .. 8 h + 7 of 16 (fp32: 4 h .. 4 h + 3 of 8,
+// one at a time).
+template <typename T> struct AttnMath;
+template <> struct AttnMath<_Float16> {
+    typedef f16x8_attn Frag;
+    static constexpr int kStep = 16;
+    __device__ static f32x16_attn product(Frag a, Frag b, f32x16_attn c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct AttnMath<__bf16> {
+    typedef bf16x8_attn Frag;
+    static constexpr int kStep = 16;
+    __device__ static f32x16_attn product(Frag a, Frag b, f32x16_attn c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct AttnMath<float> {
+    typedef f32x4_attn Frag;
+    static constexpr int kStep = 8;
+    __device__ static f32x16_attn product(Frag a, Frag b, f32x16_attn c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ROWS rows of DP channels (zeros past the channels and rows there are) in
+// LDS, in 16-byte pieces; a row's pieces are permuted by an exclusive or with
+// 2 (row % 8), so that both a piece of each of many rows and pairs of pieces
+// of four neighbouring rows spread over the banks.
+template <typename T, int DP, int ROWS>
+struct AttnTile {
+    typedef typename AttnMath<T>::Frag Frag;
+    static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+    static constexpr int kPieces = kRowBytes / 16;
+    static constexpr int kBytes = ROWS * kRowBytes;
+    static constexpr int kMask = kPieces >= 16 ? 14 : kPieces >= 8 ? 6 : 2;
+    static constexpr int kElems = 16 / static_cast<int>(sizeof(T));
+
+    __device__ static int mix(int row) { return kPieces >= 8 ? (2 * row) & kMask : row & kMask; }
+    __device__ static int place(int row, int piece) { return row * kRowBytes + ((piece ^ mix(row)) << 4); }
+
+    // Copies rows 0 .. ROWS of `from` (rows at and past `rows`, and pieces at
+    // and past `pieces`, become zeros) by the waves of THREADS threads; the
+    // copies are asynchronous.
+    template <int THREADS>
+    __device__ static void load(char* to, const T* from, long long row_stride, int rows, int pieces, int thread) {
+        constexpr int kRange = 1 << 30;
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, kRange, 0x00020000);
+        const int stride = static_cast<int>(row_stride * static_cast<long long>(sizeof(T)));
+        const int wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+#pragma unroll
+        for (int i = 0; i < kBytes / (THREADS * 16); ++i) {
+            const int first = (i * (THREADS / kWave) + wave) * kWave;
+            const int at = first + lane_id();
+            const int row = at / kPieces;
+            const int piece = (at % kPieces) ^ mix(row);
+            // Offsets outside the range read as zeros.
+            const int offset = row < rows && piece < pieces ? row * stride + piece * 16 : kRange;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (__attribute__((address_space(3))) void*)(to + first * 16), 16, offset, 0, 0, 0);
+        }
+    }
+
+    // Left (or right) operand of a product over channels: row `row`, channels
+    // step * kStep on, the half's share.
+    __device__ static Frag row_frag(const char* tile, int row, int step, int half) {
+        return *reinterpret_cast<const Frag*>(tile + place(row, step * 2 + half));
+    }
+};
+
+// Transposed operand of a product over rows: channel 32 block + L % 32 of the
+// tile's rows in the order in which a lane's registers 8 step .. 8 step + 7
+// hold them: rows 16 step + 4 h + 0 .. 3 and 16 step + 8 + 4 h + 0 .. 3.
+template <typename Tile, typename T>
+__device__ inline typename AttnMath<T>::Frag column_frag(const char* tile, int step, int block) {
+    static_assert(sizeof(T) == 2);
+    const int lane = lane_id();
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int piece = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const char* at = tile + Tile::place(row, piece) + ((lane & 1) << 3) + step * 16 * Tile::kRowBytes;
+    typedef __attribute__((address_space(3))) i16x4_attn* Local;
+    struct Pair {
+        i16x4_attn a, b;
+    };
+    const Pair both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at)),
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at + 8 * Tile::kRowBytes))};
+    return __builtin_bit_cast(typename AttnMath<T>::Frag, both);
+}
+
+// acc[block] += (columns 32 block + n of the tile's 32 rows from `row0`)
+// times x, the registers of a product's result over those rows.
+template <typename Tile, typename T, int BLOCKS>
+__device__ inline void add_columns(f32x16_attn (&acc)[BLOCKS], const char* tile, int row0, const f32x16_attn& x) {
+    if constexpr (sizeof(T) == 2) {
+        typedef typename AttnMath<T>::Frag Frag;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            Frag b;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = static_cast<T>(x[8 * half + i]);
+#pragma unroll
+            for (int block = 0; block < BLOCKS; ++block)
+                acc[block] = AttnMath<T>::product(column_frag<Tile, T>(tile, row0 / 16 + half, block), b, acc[block]);
+        }
+    } else {
+        const int lane = lane_id();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = row0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+#pragma unroll
+            for (int block = 0; block < BLOCKS; ++block) {
+                const float a = *reinterpret_cast<const float*>(
+                    tile + Tile::place(row, 8 * block + ((lane & 31) >> 2)) + ((lane & 3) << 2));
+                acc[block] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[r], acc[block], 0, 0, 0);
+            }
+        }
+    }
+}
+
+// The operand of a wave's 32 rows (row L % 32 at `row`), kept in registers;
+// zeros past `dim`.
+template <typename T, int DP>
+struct AttnOperand {
+    typedef typename AttnMath<T>::Frag Frag;
+    static constexpr int kSteps = DP / AttnMath<T>::kStep;
+    Frag f[kSteps];
+
+    __device__ void load(const T* row, int dim, bool valid, bool negate) {
+        const int half = lane_id() >> 5;
+        constexpr int kShare = AttnMath<T>::kStep / 2;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+            const int d = (2 * c + half) * kShare;
+            f[c] = Frag{};
+            if (valid && d < dim) f[c] = *reinterpret_cast<const Frag*>(row + d);
+            if (negate) f[c] = -f[c];
+        }
+    }
+};
+
+// Rows row0 .. row0 + 31 of the tile times the operand's rows.
+template <typename Tile, typename T, int DP>
+__device__ inline f32x16_attn tile_product(const char* tile, int row0, const AttnOperand<T, DP>& b) {
+    const int lane = lane_id();
+    f32x16_attn c = {};
+#pragma unroll
+    for (int step = 0; step < AttnOperand<T, DP>::kSteps; ++step)
+        c = AttnMath<T>::product(Tile::row_frag(tile, row0 + (lane & 31), step, lane >> 5), b.f[step], c);
+    return c;
+}
+
+__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
+
+// Row of a result's register r.
+__device__ inline int result_row(int r) { return 8 * (r / 4) + 4 * (lane_id() >> 5) + r % 4; }
+
+// The tiles of KT keys that a range of positions sees: first those of the
+// first keys that lie before the window's, then the window's.
+struct AttnTiles {
+    int first, from, count;
+    __device__ int tile(int t) const { return t < first ? t : from + (t - first); }
+};
+template <int KT>
+__device__ inline AttnTiles attn_tiles(const lattice_attention& a, int nk, int p_low, int p_high) {
+    const int hi = min(nk - 1, p_high + a.right);
+    if (hi < 0) return {0, 0, 0};
+    const int from = max(0, p_low - a.left) / KT;
+    const int first = min((min(a.sinks, hi + 1) + KT - 1) / KT, from);
+    return {first, from, first + max(0, hi / KT - from + 1)};
+}
+
+}  // namespace lattice

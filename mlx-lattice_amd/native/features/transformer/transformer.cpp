@@ -192,7 +192,7 @@ int64_t piece_of(const at::Tensor& t) { return 16 / t.element_size(); }
 
 bool in_pieces(const at::Tensor& t) {
     const int64_t piece = piece_of(t);
-    return t.stride(2) == 1 && (t.size(0) <= 1 || t.stride(0) % piece == 0) &&
+    return t.stride(2) == 1 && (t.size(0) <= 1 || (t.stride(0) % piece == 0 && t.stride(0) < piece << 20)) &&
            (t.size(1) <= 1 || t.stride(1) % piece == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
