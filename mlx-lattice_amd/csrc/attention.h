@@ -7,6 +7,8 @@
 
 namespace lattice {
 
+constexpr int kAttnBlock = 256;
+constexpr int kAttnWaves = kAttnBlock / kWave;
 constexpr int kAttnMaxDim = 128;
 constexpr float kAttnLog2e = 1.44269504088896340736f;
 

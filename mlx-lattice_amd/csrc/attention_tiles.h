@@ -197,4 +197,41 @@ __device__ inline AttnTiles attn_tiles(const lattice_attention& a, int nk, int p
     return {first, from, first + max(0, hi / KT - from + 1)};
 }
 
+// What a wave's 32 rows are: row L % 32 of the tile.
+struct AttnRows {
+    int i, head, p;      // query of the sequence, head, position
+    bool valid;
+    int p_low, p_high;   // of all 32 rows
+};
+__device__ inline AttnRows attn_rows(const AttnSequence& s, int kv, uint32_t group, uint32_t first) {
+    const uint32_t rows = s.nq * group;
+    const uint32_t r = first + (lane_id() & 31);
+    const uint32_t in = min(r, rows - 1);
+    AttnRows w;
+    w.i = in / group;
+    w.head = kv * group + in % group;
+    w.p = w.i + s.shift();
+    w.valid = r < rows;
+    w.p_low = __builtin_amdgcn_readfirstlane(w.i) + s.shift();
+    w.p_high = __builtin_amdgcn_readlane(w.i, 31) + s.shift();
+    return w;
+}
+
+// Which sequence, tile of M rows and key head a block has.
+struct AttnSlot {
+    AttnSequence s;
+    uint32_t rows, first;  // (query, head) pairs: of the sequence, before the tile's
+};
+template <int M>
+__device__ inline AttnSlot attn_slot(const lattice_attention& a, uint32_t group, uint32_t slot) {
+    // Sequence e has the slots from start / M + e on: enough for its tiles.
+    const auto slot_of = [group](int start, int e) { return start * group / M + e; };
+    const int e = query_rows(a).find(slot, slot_of);
+    AttnSlot t;
+    t.s = attn_sequence(a, e);
+    t.rows = t.s.nq * group;
+    t.first = (slot - slot_of(t.s.q0, e)) * M;
+    return t;
+}
+
 }  // namespace lattice
