@@ -29,7 +29,8 @@ INCLUDE = REPO / 'include'
 ARCH = 'gfx950'
 
 HIP_SOURCES = ['scan.hip', 'sort.hip', 'coords.hip', 'conv.hip', 'conv_grad.hip', 'pool.hip', 'quantize.hip',
-               'norm.hip', 'dropout.hip', 'rotary.hip', 'attention.hip', 'attention_grad.hip']
+               'norm.hip', 'dropout.hip', 'rotary.hip', 'attention.hip', 'attention_grad.hip',
+               'attention_grad_f32.hip', 'attention_grad_f16.hip', 'attention_grad_bf16.hip']
 HOST_SOURCES = [
     'native/features/coordinates/relations.cpp',
     'native/features/convolution/api.cpp',

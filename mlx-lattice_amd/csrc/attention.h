@@ -174,17 +174,6 @@ __device__ inline void attend_row(const lattice_attention& a, const AttnSequence
     }
 }
 
-// delta = sum_d grad_out out of one row and head.
-template <typename T>
-__device__ inline float attn_delta(const lattice_attention& a, long long row, int head, const T* out,
-                                   const T* grad_out) {
-    const long long at = (row * a.heads + head) * a.dim;
-    float sum = 0.0f;
-    for (int d = lane_id(); d < a.dim; d += kWave)
-        sum += static_cast<float>(out[at + d]) * static_cast<float>(grad_out[at + d]);
-    return wave_sum(sum);
-}
-
 // grad_q of one query row and head.
 template <typename T>
 __device__ inline void grad_query_row(const lattice_attention& a, const AttnSequence& s, int i, int head,
@@ -231,11 +220,12 @@ __device__ inline void grad_query_row(const lattice_attention& a, const AttnSequ
     }
 }
 
-// grad_k and grad_v of one key row and key head: over the queries that see it
+// grad_k and grad_v of one key row and key head: states holds (lse, delta) by
+// key head, row and head; over the queries that see it
 // and the heads that share it, (query, head) pairs 64 at a time, one a lane.
 template <typename T>
 __device__ inline void grad_key_row(const lattice_attention& a, const AttnSequence& s, int j, int kv,
-                                    const float* lse, const float* delta, const T* grad_out, T* grad_k, T* grad_v,
+                                    const float* lse, const float2* states, const T* grad_out, T* grad_k, T* grad_v,
                                     AttnRowScratch* scratch) {
     const int lane = lane_id();
     const int group = a.heads / a.kv_heads;
@@ -260,7 +250,8 @@ __device__ inline void grad_key_row(const lattice_attention& a, const AttnSequen
             const int h = static_cast<int>((base + lane) % group);
             const long long at = (s.q0 + i) * a.heads + kv * group + h;
             p = exp2f(row_dot(scratch->a, q + i * a.q_row_stride + h * a.q_head_stride, a.dim) * scale - lse[at]);
-            slope = p * (row_dot(scratch->b, grad_out + at * a.dim, a.dim) - delta[at]);
+            slope = p * (row_dot(scratch->b, grad_out + at * a.dim, a.dim) -
+                         states[(static_cast<long long>(kv) * a.queries + s.q0 + i) * group + h].y);
         }
         wave_fence();
         scratch->p[lane] = p;

@@ -126,17 +126,12 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
     }
     const bool sees = attn_seen(a, s.nk, w.p).total() > 0;
     const float inv = 1.0f / sum;
-    bool finite = true;
 #pragma unroll
     for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            state.acc[b][r] = sees ? state.acc[b][r] * inv : 0.0f;
-            const int d = 32 * b + result_row(r);
-            finite = finite && (d >= a.dim || fabsf(state.acc[b][r]) < INFINITY);
-        }
+        for (int r = 0; r < 16; ++r) state.acc[b][r] = sees ? state.acc[b][r] * inv : 0.0f;
     }
-    const uint64_t spoilt = ballot(w.valid && !finite);
+    const uint64_t spoilt = ballot(w.valid && !finite_columns(state.acc, 1.0f));
     uint32_t again = static_cast<uint32_t>(spoilt) | static_cast<uint32_t>(spoilt >> 32);
     if (w.valid && !(again >> (lane_id() & 31) & 1)) {
         if (lse && half == 0) lse[at] = sees ? state.top + __builtin_amdgcn_logf(sum) : INFINITY;
@@ -187,16 +182,9 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, p_low, p_high);
     const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
     const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
-    const T* keys = static_cast<const T*>(a.k) + s.k0 * a.k_row_stride + kv * a.k_head_stride;
-    const T* values = static_cast<const T*>(a.v) + s.k0 * a.v_row_stride + kv * a.v_head_stride;
-    const int pieces = a.dim * static_cast<int>(sizeof(T)) / 16;
+    const KeyTiles<T, DP, KT, kAttnBlock> source(a, s, kv, threadIdx.x);
     const auto copy = [&](int index) {
-        const int j0 = tiles.tile(index) * KT;
-        char* at = shared + (index & 1) * 2 * Tile::kBytes;
-        Tile::template load<kAttnBlock>(at, keys + j0 * a.k_row_stride, a.k_row_stride, s.nk - j0, pieces,
-                                        threadIdx.x);
-        Tile::template load<kAttnBlock>(at + Tile::kBytes, values + j0 * a.v_row_stride, a.v_row_stride, s.nk - j0,
-                                        pieces, threadIdx.x);
+        source.copy(shared + (index & 1) * 2 * Tile::kBytes, tiles.tile(index) * KT, s.nk);
     };
     if (from < to) copy(from);
     __syncthreads();
@@ -241,20 +229,14 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, w.p_low, w.p_high);
     const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
     const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
-    const T* keys = static_cast<const T*>(a.k) + s.k0 * a.k_row_stride + kv * a.k_head_stride;
-    const T* values = static_cast<const T*>(a.v) + s.k0 * a.v_row_stride + kv * a.v_head_stride;
-    const int pieces = a.dim * static_cast<int>(sizeof(T)) / 16;
+    const KeyTiles<T, DP, KT, kWave> source(a, s, kv, lane_id());
     char* mine = shared + wave * 2 * Tile::kBytes;
     const int steps = (to - from + kAttnWaves - 1) / kAttnWaves;
     for (int step = 0; step < steps; ++step) {
         const int index = from + step * kAttnWaves + wave;
         const int j0 = index < to ? tiles.tile(index) * KT : 0;
         __syncthreads();
-        if (index < to) {
-            Tile::template load<kWave>(mine, keys + j0 * a.k_row_stride, a.k_row_stride, s.nk - j0, pieces, lane_id());
-            Tile::template load<kWave>(mine + Tile::kBytes, values + j0 * a.v_row_stride, a.v_row_stride, s.nk - j0,
-                                       pieces, lane_id());
-        }
+        if (index < to) source.copy(mine, j0, s.nk);
         __syncthreads();
         const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
                          (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);

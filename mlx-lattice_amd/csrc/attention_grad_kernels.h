@@ -1,0 +1,605 @@
+// Kernels of the windowed attention's gradients and their launches.
+#pragma once
+
+#include "attention_grad.h"
+
+namespace lattice {
+namespace {
+
+// Slopes are rounded to the type before their products.  In half precision
+// they are first scaled by a power of two that follows their size, since the
+// gradients of a long row are far below the type's smallest normal number;
+// the sums carry the scale and drop it at the end.
+template <typename T>
+struct SlopeScale {
+    static constexpr bool kUsed = false;
+    __device__ float factor() const { return 1.0f; }
+};
+__device__ inline float power_of_two(int exponent) { return __int_as_float((max(exponent, -126) + 127) << 23); }
+template <>
+struct SlopeScale<_Float16> {
+    static constexpr bool kUsed = true;
+    static constexpr int kNone = 100, kMost = 40;
+    int exponent = kNone;
+    __device__ float factor() const { return exponent == kNone ? 1.0f : power_of_two(exponent); }
+    // Follows the wave's largest slope; the factor by which the sums so far
+    // have to be scaled.  A column with a slope that is not finite is made
+    // again by itself and has no say in the others' scale.
+    __device__ float follow(float largest) {
+        largest = largest < INFINITY ? largest : 0.0f;
+        if (!__any(largest * power_of_two(exponent) > 32768.0f)) return 1.0f;
+        largest = wave_max(largest);
+        // The largest becomes 2^11 .. 2^12.
+        const int next = min(kMost, 138 - (__float_as_int(largest) >> 23));
+        const float change = exponent == kNone ? 1.0f : power_of_two(next - exponent);
+        exponent = next;
+        return change;
+    }
+};
+
+// The power of two that scales the shares of half precision.
+template <typename T> constexpr float kShareLog2 = 0.0f;
+template <> constexpr float kShareLog2<_Float16> = 14.0f;
+
+template <int BLOCKS>
+__device__ inline void scale_sums(f32x16_attn (&acc)[BLOCKS], float factor) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) acc[b] *= factor;
+}
+
+// Rounds slopes into the scale's range and adds their products to acc.
+template <typename Tile, typename T, int BLOCKS>
+__device__ inline void add_slopes(f32x16_attn (&acc)[BLOCKS], SlopeScale<T>& scale, const char* tile, int row0,
+                                  f32x16_attn& ds) {
+    if constexpr (SlopeScale<T>::kUsed) {
+        float largest = fabsf(ds[0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) largest = fmaxf(largest, fabsf(ds[r]));
+        const float change = scale.follow(largest);
+        if (change != 1.0f) scale_sums(acc, change);
+        ds *= scale.factor();
+    }
+    add_columns<Tile, T>(acc, tile, row0, ds);
+}
+
+// Stores column n of acc times `factor` into row n's `to` (dim channels);
+// lanes without a row pass valid = false.
+template <typename T, int BLOCKS>
+__device__ inline void store_columns(const f32x16_attn (&acc)[BLOCKS], float factor, T* to, int dim, bool valid) {
+    const int half = lane_id() >> 5;
+    if (!valid) return;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * b + 8 * g + 4 * half;
+            if (d >= dim) continue;
+            RowVec<T, 4> v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v.set(i, acc[b][4 * g + i] * factor);
+            v.store(to + d);
+        }
+    }
+}
+
+// Lanes (0 .. 31) whose column is not finite in either half.
+__device__ inline uint32_t spoilt_columns(bool valid, bool finite) {
+    const uint64_t spoilt = ballot(valid && !finite);
+    return static_cast<uint32_t>(spoilt) | static_cast<uint32_t>(spoilt >> 32);
+}
+
+// (lse, delta) of a query row and head, where the keys' pass reads them: by key
+// head, row and head, so that a tile's lie side by side.
+__device__ inline long long query_state(const lattice_attention& a, uint32_t group, long long row, int head) {
+    const uint32_t kv = head / group;
+    return (static_cast<long long>(kv) * a.queries + row) * group + (head - kv * group);
+}
+
+// grad_q, laid out as the forward pass; keeps lse and delta for the keys' pass.
+template <typename T, int DP, int KT>
+__global__ void __launch_bounds__(kAttnBlock, DP <= 64 || sizeof(T) == 2 ? 2 : 1)
+grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __restrict__ lse,
+                 const T* __restrict__ grad_out, T* __restrict__ grad_q, float2* __restrict__ states) {
+    typedef AttnTile<T, DP, KT> Tile;
+    typedef AttnOperand<T, DP> Operand;
+    constexpr int kBlocks = DP / 32;
+    extern __shared__ __align__(128) char shared[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int half = lane_id() >> 5;
+    const uint32_t group = a.heads / a.kv_heads;
+    const int kv = blockIdx.y;
+    const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
+    const AttnSequence s = t.s;
+    if (t.first >= t.rows) return;
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const AttnRows w = attn_rows(s, kv, group, t.first + 32 * wave);
+    const long long row = static_cast<long long>(s.q0) + w.i;
+    const long long at = row * a.heads + w.head;
+    Operand q, d;
+    q.load(static_cast<const T*>(a.q) + row * a.q_row_stride + w.head * a.q_head_stride, a.dim, w.valid,
+           a.scale < 0.0f);
+    d.load(grad_out + at * a.dim, a.dim, w.valid, false);
+    float along = 0.0f;
+    {
+        Operand o;
+        o.load(out + at * a.dim, a.dim, w.valid, false);
+#pragma unroll
+        for (int c = 0; c < Operand::kSteps; ++c) {
+#pragma unroll
+            for (int i = 0; i < Tile::kElems; ++i)
+                along += static_cast<float>(o.f[c][i]) * static_cast<float>(d.f[c][i]);
+        }
+        along += other_half(along);
+    }
+    const float log_sum = w.valid ? lse[at] : INFINITY;
+    if (w.valid && half == 0) states[query_state(a, group, row, w.head)] = float2{log_sum, along};
+    f32x16_attn acc[kBlocks] = {};
+    SlopeScale<T> slopes;
+    const int p_low = static_cast<int>(t.first / group) + s.shift();
+    const int p_high = static_cast<int>((min(t.first + 32 * kAttnWaves, t.rows) - 1) / group) + s.shift();
+    const AttnTiles tiles = attn_tiles<KT>(a, s.nk, p_low, p_high);
+    const KeyTiles<T, DP, KT, kAttnBlock> source(a, s, kv, threadIdx.x);
+    const auto copy = [&](int index) {
+        source.copy(shared + (index & 1) * 2 * Tile::kBytes, tiles.tile(index) * KT, s.nk);
+    };
+    if (tiles.count) copy(0);
+    __syncthreads();
+    for (int index = 0; index < tiles.count; ++index) {
+        if (index + 1 < tiles.count) copy(index + 1);
+        const int j0 = tiles.tile(index) * KT;
+        const char* k_tile = shared + (index & 1) * 2 * Tile::kBytes;
+        const char* v_tile = k_tile + Tile::kBytes;
+        const bool none = j0 > w.p_high + a.right || (j0 + KT - 1 < w.p_low - a.left && j0 >= a.sinks);
+        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
+                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
+        if (!none) {
+#pragma unroll
+            for (int part = 0; part < KT / 32; ++part) {
+                f32x16_attn p = tile_product<Tile, T, DP>(k_tile, 32 * part, q);
+                f32x16_attn dp = tile_product<Tile, T, DP>(v_tile, 32 * part, d);
+                if (!all) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!attn_visible(a, s.nk, w.p, j0 + 32 * part + result_row(r))) p[r] = -INFINITY;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
+                add_slopes<Tile, T>(acc, slopes, k_tile, 32 * part, dp);
+            }
+        }
+        __syncthreads();
+    }
+    // A row that is not finite is made again from what it sees alone.
+    const float factor = a.scale / slopes.factor();
+    uint32_t again = spoilt_columns(w.valid, finite_columns(acc, factor));
+    store_columns(acc, factor, grad_q + at * a.dim, a.dim, w.valid && !(again >> (lane_id() & 31) & 1));
+    while (again) {
+        const int n = __ffs(again) - 1;
+        again &= again - 1;
+        grad_query_row<T>(a, s, __shfl(w.i, n), __shfl(w.head, n), lse, __shfl(along, n), grad_out, grad_q,
+                          reinterpret_cast<AttnRowScratch*>(shared) + wave);
+    }
+}
+
+// ROWS (query, head) pairs r0 .. of a sequence and key head in LDS: q and
+// grad_out rows, and of each its lse (+inf past the rows there are, so that
+// its shares are zero), delta and position.
+template <typename T, int DP, int ROWS>
+struct QueryTile {
+    typedef AttnTile<T, DP, ROWS> Tile;
+    static constexpr int kBytes = 2 * Tile::kBytes + (ROWS * 12 + 127) / 128 * 128;
+
+    __device__ static const float* states(const char* tile) {
+        return reinterpret_cast<const float*>(tile + 2 * Tile::kBytes);
+    }
+};
+
+// Copies them by THREADS threads.  A tile starts at a multiple of ROWS; where
+// the heads of a group divide that, each starts with a group's first head and
+// the places of its rows are the same but for the base.
+template <typename T, int DP, int ROWS, int THREADS>
+struct QueryTiles {
+    typedef QueryTile<T, DP, ROWS> Queries;
+    typedef typename Queries::Tile Tile;
+    static constexpr int kCopies = Tile::copies(THREADS);
+    const T *q, *grad_out;  // of the sequence's first query and the key head's first head
+    const float2* states;
+    long long q_stride, d_stride;
+    int thread, wave, q_row, q_head, d_row, d_head, shift;
+    uint32_t group;
+    bool aligned;
+    int own_query;
+    int q_offsets[kCopies], d_offsets[kCopies];
+
+    // What a thread holds of the states until it stores them.
+    struct State {
+        float lse, delta;
+        int position;
+    };
+
+    __device__ QueryTiles(const lattice_attention& a, const AttnSequence& s, int kv, uint32_t heads,
+                          const float2* all_states, const T* all_grad_out, int of_thread) {
+        constexpr int kSize = sizeof(T);
+        thread = of_thread;
+        wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+        group = heads;
+        shift = s.shift();
+        q_stride = a.q_row_stride;
+        d_stride = static_cast<long long>(a.heads) * a.dim;
+        q = static_cast<const T*>(a.q) + s.q0 * q_stride + static_cast<long long>(kv) * group * a.q_head_stride;
+        grad_out = all_grad_out + s.q0 * d_stride + static_cast<long long>(kv) * group * a.dim;
+        states = all_states + (static_cast<long long>(kv) * a.queries + s.q0) * group;
+        q_row = static_cast<int>(a.q_row_stride) * kSize;
+        q_head = static_cast<int>(a.q_head_stride) * kSize;
+        d_row = a.heads * a.dim * kSize;
+        d_head = a.dim * kSize;
+        aligned = ROWS % group == 0;
+        places(0);
+    }
+    __device__ void places(uint32_t h0) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const uint32_t n = h0 + Tile::template copy_row<THREADS>(i, thread);
+            const int query = n / group, head = n - query * group;
+            const int piece = Tile::template copy_piece<THREADS>(i, thread, d_head / 16);
+            q_offsets[i] = query * q_row + head * q_head + piece;
+            d_offsets[i] = query * d_row + head * d_head + piece;
+        }
+        own_query = (h0 + thread) / group;
+    }
+    // Starts the copies of pairs r0 .. of `rows`; rows past them hold other
+    // rows or zeros, whose shares are zero.
+    __device__ State copy(char* to, uint32_t r0, uint32_t rows) {
+        const uint32_t i0 = r0 / group, h0 = r0 - i0 * group;
+        if (!aligned) places(h0);
+        const uint32_t count = min(rows - r0, static_cast<uint32_t>(ROWS));
+        // The range ends with the last query's last head.
+        const int last = (h0 + count - 1) / group;
+        Tile::template copy<THREADS>(to, q + i0 * q_stride,
+                                     last * q_row + static_cast<int>(group - 1) * q_head + d_head, q_offsets, wave);
+        Tile::template copy<THREADS>(to + Tile::kBytes, grad_out + i0 * d_stride,
+                                     last * d_row + static_cast<int>(group) * d_head, d_offsets, wave);
+        State state{INFINITY, 0.0f, static_cast<int>(i0) + own_query + shift};
+        if (thread < count) {
+            const float2 kept = states[r0 + thread];
+            state.lse = kept.x;
+            state.delta = kept.y;
+        }
+        return state;
+    }
+    __device__ void store(char* to, const State& state) const {
+        if (thread >= ROWS) return;
+        float* at = reinterpret_cast<float*>(to + 2 * Tile::kBytes);
+        at[thread] = state.lse;
+        at[ROWS + thread] = state.delta;
+        reinterpret_cast<int*>(at)[2 * ROWS + thread] = state.position;
+    }
+};
+
+// Adds the queries of a tile to a wave's 32 keys; `masked`: a lane's key is
+// seen from the positions lo .. hi alone.
+template <typename T, int DP, int QT>
+__device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k, const AttnOperand<T, DP>& v,
+                                   float scale, int lo, int hi, bool masked, f32x16_attn (&acc_k)[DP / 32],
+                                   f32x16_attn (&acc_v)[DP / 32], SlopeScale<T>& slopes) {
+    typedef QueryTile<T, DP, QT> Queries;
+    typedef typename Queries::Tile Tile;
+    const int half = lane_id() >> 5;
+    const char* d_tile = tile + Tile::kBytes;
+    const float* states = Queries::states(tile);
+#pragma unroll
+    for (int part = 0; part < QT / 32; ++part) {
+        f32x16_attn p = tile_product<Tile, T, DP>(tile, 32 * part, k);
+        f32x16_attn ds = tile_product<Tile, T, DP>(d_tile, 32 * part, v);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int row = 32 * part + 8 * g + 4 * half;
+            if (masked) {
+                const int4 at = *reinterpret_cast<const int4*>(states + 2 * QT + row);
+                const int position[4] = {at.x, at.y, at.z, at.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (position[i] < lo || position[i] > hi) p[4 * g + i] = -INFINITY;
+            }
+            const float4 lse = *reinterpret_cast<const float4*>(states + row);
+            const float4 delta = *reinterpret_cast<const float4*>(states + QT + row);
+            const float log_sum[4] = {lse.x, lse.y, lse.z, lse.w};
+            const float along[4] = {delta.x, delta.y, delta.z, delta.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * g + i;
+                p[r] = __builtin_amdgcn_exp2f(p[r] * scale - (log_sum[i] - kShareLog2<T>));
+                ds[r] = p[r] * (ds[r] - along[i]);
+            }
+        }
+        add_columns<Tile, T>(acc_v, d_tile, 32 * part, p);
+        add_slopes<Tile, T>(acc_k, slopes, tile, 32 * part, ds);
+    }
+}
+
+template <int DP> constexpr int kFirstValues = 2 * DP * 32;
+
+template <int BLOCKS>
+__device__ inline void store_part(float* to, const f32x16_attn (&acc_k)[BLOCKS], const f32x16_attn (&acc_v)[BLOCKS]) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            to[(b * 16 + r) * kWave + lane] = acc_k[b][r];
+            to[((BLOCKS + b) * 16 + r) * kWave + lane] = acc_v[b][r];
+        }
+    }
+}
+
+// The part of a slot: each wave takes every fourth tile of 32 pairs.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttnBlock)
+grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T* __restrict__ grad_out,
+                FirstParts parts) {
+    constexpr int QT = 32;
+    constexpr int kBlocks = DP / 32;
+    typedef QueryTile<T, DP, QT> Queries;
+    extern __shared__ __align__(128) char shared[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+    const uint32_t group = a.heads / a.kv_heads;
+    const int kv = blockIdx.y, j0 = blockIdx.z * 32;
+    const AttnSlot t = attn_slot<kFirstRows>(a, group, blockIdx.x);
+    const AttnSequence s = t.s;
+    const int j = j0 + (lane & 31);
+    if (t.first >= t.rows || j0 >= min(a.sinks, s.nk)) return;
+    const bool valid = j < s.nk;
+    const long long row = static_cast<long long>(s.k0) + min(j, s.nk - 1);
+    AttnOperand<T, DP> k, v;
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, a.scale < 0.0f);
+    v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
+    SlopeScale<T> slopes;
+    QueryTiles<T, DP, QT, kWave> source(a, s, kv, group, states, grad_out, lane);
+    // From the first pair whose query lies past the window of key j0.
+    const int i_from = max(0, j0 + a.left + 1 - s.shift());
+    const uint32_t from = max(t.first, static_cast<uint32_t>(min(i_from, s.nq)) * group / QT * QT);
+    const uint32_t to = min(t.first + kFirstRows, t.rows);
+    char* tile = shared + wave * Queries::kBytes;
+    for (uint32_t base = from; base < to; base += QT * kAttnWaves) {
+        const uint32_t r0 = base + QT * wave;
+        __syncthreads();
+        if (r0 < to) source.store(tile, source.copy(tile, r0, to));
+        __syncthreads();
+        if (r0 < to) {
+            const int p_low = static_cast<int>(r0 / group) + s.shift();
+            add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, p_low <= j0 + 31 + a.left, acc_k,
+                                   acc_v, slopes);
+        }
+    }
+    scale_sums(acc_k, 1.0f / slopes.factor());
+    // The waves' sums are added in wave order.
+    float* sums = reinterpret_cast<float*>(shared);
+    for (int u = 1; u < kAttnWaves; ++u) {
+        __syncthreads();
+        if (wave == u) store_part(sums, acc_k, acc_v);
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    acc_k[b][r] += sums[(b * 16 + r) * kWave + lane];
+                    acc_v[b][r] += sums[((kBlocks + b) * 16 + r) * kWave + lane];
+                }
+            }
+        }
+    }
+    if (wave == 0) store_part(parts.past_of(a, blockIdx.x, kv, blockIdx.z, kFirstValues<DP>), acc_k, acc_v);
+}
+
+// Adds the parts of 32 first keys of a sequence and key head, the window's
+// first and the others in slot order.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttnBlock)
+join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
+                const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
+    constexpr int kHeld = kFirstValues<DP> / kAttnBlock;
+    __shared__ AttnRowScratch scratch[kAttnWaves];
+    __shared__ uint32_t spoilt;
+    const uint32_t group = a.heads / a.kv_heads;
+    const int e = blockIdx.x + 1, kv = blockIdx.y, j0 = blockIdx.z * 32;
+    const AttnSequence s = attn_sequence(a, e);
+    const int keys = min(a.sinks, s.nk);
+    if (j0 >= keys) return;
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    const int j = j0 + (lane & 31);
+    const uint32_t slot = s.q0 * group / kFirstRows + e, slots = (s.nq * group + kFirstRows - 1) / kFirstRows;
+    float sum[kHeld];
+    const float* window = parts.window_of(a, e, kv, blockIdx.z, kFirstValues<DP>);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) sum[i] = window[i * kAttnBlock + threadIdx.x];
+    for (uint32_t u = 0; u < slots; ++u) {
+        const float* past = parts.past_of(a, slot + u, kv, blockIdx.z, kFirstValues<DP>);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) sum[i] += past[i * kAttnBlock + threadIdx.x];
+    }
+    const float share = __builtin_amdgcn_exp2f(-kShareLog2<T>);
+    if (threadIdx.x == 0) spoilt = 0;
+    __syncthreads();
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        sum[i] *= i < kHeld / 2 ? a.scale * share : share;
+        finite = finite && fabsf(sum[i]) < INFINITY;
+    }
+    if (!finite && j < keys) atomicOr(&spoilt, 1u << (lane & 31));
+    __syncthreads();
+    const uint32_t again = spoilt;
+    if (j < keys && !(again >> (lane & 31) & 1)) {
+        const long long at = ((static_cast<long long>(s.k0) + j) * a.kv_heads + kv) * a.dim;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int value = (i % (kHeld / 2)) * kAttnWaves + wave;  // register of the part
+            const int d = value / 16 * 32 + result_row(value % 16);
+            if (d < a.dim) (i < kHeld / 2 ? grad_k : grad_v)[at + d] = static_cast<T>(sum[i]);
+        }
+    }
+    for (int n = wave; n < 32; n += kAttnWaves) {
+        if (again >> n & 1)
+            grad_key_row<T>(a, s, j0 + n, kv, lse, states, grad_out, grad_k, grad_v, &scratch[wave]);
+    }
+}
+
+// grad_k and grad_v: 128 keys a block, 32 a wave, over the tiles of (query,
+// head) pairs that see them.
+template <typename T, int DP, int QT>
+__global__ void __launch_bounds__(kAttnBlock, DP <= 64 ? 2 : 1)
+grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
+               const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
+    constexpr int kBlocks = DP / 32;
+    constexpr int kKeys = 32 * kAttnWaves;
+    typedef QueryTile<T, DP, QT> Queries;
+    extern __shared__ __align__(128) char shared[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+    const uint32_t group = a.heads / a.kv_heads;
+    const int kv = blockIdx.y;
+    const auto slot_of = [](int start, int e) { return static_cast<uint32_t>(start) / kKeys + e; };
+    const int e = key_rows(a).find(blockIdx.x, slot_of);
+    const AttnSequence s = attn_sequence(a, e);
+    const int owned = max(0, key_rows(a).start(e + 1) - s.k0);
+    const int j0 = static_cast<int>(blockIdx.x - slot_of(s.k0, e)) * kKeys;
+    if (j0 >= owned) return;
+    const int j_wave = j0 + 32 * wave, j = j_wave + (lane & 31);
+    const bool valid = j < s.nk;
+    const long long row = static_cast<long long>(s.k0) + min(j, owned - 1);
+    AttnOperand<T, DP> k, v;
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, a.scale < 0.0f);
+    v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
+    SlopeScale<T> slopes;
+    QueryTiles<T, DP, QT, kAttnBlock> source(a, s, kv, group, states, grad_out, threadIdx.x);
+    const uint32_t rows = s.nq * group;
+    // The pairs whose window holds a key of the block.
+    const int i_from = max(0, j0 - a.right - s.shift());
+    const int i_to = min(s.nq, min(j0 + kKeys, s.nk) + a.left - s.shift());
+    const bool any = j0 < s.nk && i_from < i_to;
+    const uint32_t from = any ? i_from * group / QT : 0;
+    const uint32_t window_to = any ? (i_to * group + QT - 1) / QT : 0;
+    // Without a pass of their own, the first keys' other pairs follow.
+    const int past_from = max(0, j0 + a.left + 1 - s.shift());
+    const bool rest = parts.tiles == 0 && j0 < min(a.sinks, s.nk) && past_from < s.nq;
+    const uint32_t past = rest ? past_from * group / QT : 0;
+    const uint32_t past_to = rest ? (rows + QT - 1) / QT : 0;
+    const int window_tiles = static_cast<int>(window_to - from);
+    const int count = window_tiles + static_cast<int>(past_to - past);
+    const auto first_row = [&](int index) {
+        return (index < window_tiles ? from + index : past + (index - window_tiles)) * QT;
+    };
+    if (count > 0) source.store(shared, source.copy(shared, first_row(0), rows));
+    __syncthreads();
+    for (int index = 0; index < count; ++index) {
+        char* next = shared + ((index + 1) & 1) * Queries::kBytes;
+        typename QueryTiles<T, DP, QT, kAttnBlock>::State state{};
+        if (index + 1 < count) state = source.copy(next, first_row(index + 1), rows);
+        const char* tile = shared + (index & 1) * Queries::kBytes;
+        const uint32_t r0 = first_row(index);
+        const int p_low = static_cast<int>(r0 / group) + s.shift();
+        const int p_high = static_cast<int>((min(r0 + QT, rows) - 1) / group) + s.shift();
+        // In the window, or past it: of the first keys alone.
+        const bool outside = index >= window_tiles;
+        const int lo = !outside ? j - a.right : j < a.sinks ? j + a.left + 1 : INT_MAX;
+        const int hi = outside ? INT_MAX : j + a.left;
+        const bool none = outside ? j_wave >= a.sinks || p_high <= j_wave + a.left
+                                  : p_high < j_wave - a.right || p_low > j_wave + 31 + a.left;
+        const bool all = !outside && j_wave + 31 <= p_low + a.right && j_wave >= p_high - a.left;
+        if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, !all, acc_k, acc_v, slopes);
+        if (index + 1 < count) source.store(next, state);
+        __syncthreads();
+    }
+    scale_sums(acc_k, 1.0f / slopes.factor());
+    const int first_keys = parts.tiles ? min(a.sinks, s.nk) : 0;
+    if (j_wave < first_keys) store_part(parts.window_of(a, e, kv, j_wave / 32, kFirstValues<DP>), acc_k, acc_v);
+    // Keys past the sequence's get zeros; a key whose sums are not finite is
+    // made again from the queries that see it alone.
+    const float share = __builtin_amdgcn_exp2f(-kShareLog2<T>);
+    const float slope = a.scale * share;
+    const bool finite = finite_columns(acc_k, slope) && finite_columns(acc_v, share);
+    uint32_t again = spoilt_columns(valid && j >= first_keys, finite);
+    const bool mine = j < owned && j >= first_keys && !(again >> (lane & 31) & 1);
+    const long long at = (row * a.kv_heads + kv) * a.dim;
+    if (!valid) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc_k[b] = acc_v[b] = f32x16_attn{};
+    }
+    store_columns(acc_k, slope, grad_k + at, a.dim, mine);
+    store_columns(acc_v, share, grad_v + at, a.dim, mine);
+    while (again) {
+        const int n = __ffs(again) - 1;
+        again &= again - 1;
+        grad_key_row<T>(a, s, j_wave + n, kv, lse, states, grad_out, grad_k, grad_v,
+                        reinterpret_cast<AttnRowScratch*>(shared) + wave);
+    }
+}
+
+template <typename T, int DP>
+int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, const float* lse, const T* grad_out,
+                T* grad_q, T* grad_k, T* grad_v, float2* states, const FirstParts& parts, hipStream_t stream) {
+    constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
+    const int group = a.heads / a.kv_heads;
+    if (a.queries) {
+        constexpr size_t kLds = std::max<size_t>(4 * AttnTile<T, DP, kTile>::kBytes,
+                                                 kAttnWaves * sizeof(AttnRowScratch));
+        const auto kernel = grad_query_tiles<T, DP, kTile>;
+        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        const long long slots = static_cast<long long>(a.queries) * group / (32 * kAttnWaves) + a.sequences + 2;
+        kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, lse, grad_out,
+                                                                                            grad_q, states);
+        LATTICE_LAUNCH_CHECK();
+    }
+    if (a.keys == 0) return LATTICE_OK;
+    if (l.first_tiles) {
+        constexpr size_t kLds = std::max<size_t>(kAttnWaves * QueryTile<T, DP, 32>::kBytes,
+                                                 kFirstValues<DP> * sizeof(float));
+        static_assert(kLds <= 160 * 1024);
+        const auto kernel = grad_first_keys<T, DP>;
+        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        kernel<<<dim3(l.first_slots, a.kv_heads, l.first_tiles), kAttnBlock, kLds, stream>>>(a, states, grad_out,
+                                                                                            parts);
+        LATTICE_LAUNCH_CHECK();
+    }
+    constexpr size_t kLds =
+        std::max<size_t>(2 * QueryTile<T, DP, kTile>::kBytes, kAttnWaves * sizeof(AttnRowScratch));
+    static_assert(kLds <= 160 * 1024);
+    const auto kernel = grad_key_tiles<T, DP, kTile>;
+    LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    const long long slots = a.keys / (32 * kAttnWaves) + a.sequences + 2;
+    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
+                                                                                        parts, grad_k, grad_v);
+    LATTICE_LAUNCH_CHECK();
+    if (l.first_tiles && a.sequences) {
+        join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles), kAttnBlock, 0, stream>>>(
+            a, lse, states, grad_out, parts, grad_k, grad_v);
+        LATTICE_LAUNCH_CHECK();
+    }
+    return LATTICE_OK;
+}
+
+}  // namespace
+
+template <typename T>
+int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out, const float* lse,
+                const void* grad_out, void* grad_q, void* grad_k, void* grad_v, float2* states,
+                const FirstParts& parts, hipStream_t stream) {
+    const T* o = static_cast<const T*>(out);
+    const T* dy = static_cast<const T*>(grad_out);
+    T* dq = static_cast<T*>(grad_q);
+    T* dk = static_cast<T*>(grad_k);
+    T* dv = static_cast<T*>(grad_v);
+    if (a.dim <= 32) return launch_grad<T, 32>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
+    if (a.dim <= 64) return launch_grad<T, 64>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
+    return launch_grad<T, 128>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
+}
+
+}  // namespace lattice

@@ -50,43 +50,50 @@ template <> struct AttnMath<float> {
     }
 };
 
-// ROWS rows of DP channels (zeros past the channels and rows there are) in
-// LDS, in 16-byte pieces; a row's pieces are permuted by an exclusive or with
-// 2 (row % 8), so that both a piece of each of many rows and pairs of pieces
-// of four neighbouring rows spread over the banks.
+// ROWS rows of DP channels (zeros past the channels there are) in LDS, in
+// 16-byte pieces.  LDS serves 256 bytes a cycle from 64 banks: 16 lanes that
+// read a piece each of 16 rows, or 32 that read 64 bytes of each of 4 rows
+// (four neighbours, for a transposed operand).  A row's pieces are permuted by
+// an exclusive or with bits of the row, so that either falls on all banks.
 template <typename T, int DP, int ROWS>
 struct AttnTile {
     typedef typename AttnMath<T>::Frag Frag;
     static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
     static constexpr int kPieces = kRowBytes / 16;
     static constexpr int kBytes = ROWS * kRowBytes;
-    static constexpr int kMask = kPieces >= 16 ? 14 : kPieces >= 8 ? 6 : 2;
     static constexpr int kElems = 16 / static_cast<int>(sizeof(T));
 
-    __device__ static int mix(int row) { return kPieces >= 8 ? (2 * row) & kMask : row & kMask; }
+    __device__ static int mix(int row) {
+        const int quad = row >> 2 & 3;
+        return kPieces >= 16 ? (row & 3) << 2 | quad : kPieces == 8 ? (row >> 1 & 1) << 2 | quad : quad;
+    }
     __device__ static int place(int row, int piece) { return row * kRowBytes + ((piece ^ mix(row)) << 4); }
 
-    // Copies rows 0 .. ROWS of `from` (rows at and past `rows`, and pieces at
-    // and past `pieces`, become zeros) by the waves of THREADS threads; the
-    // copies are asynchronous.
+    // Copies by the waves of THREADS threads: the row and piece of copy i.
+    static constexpr int kRange = 1 << 30;
+    static constexpr int copies(int threads) { return kBytes / (threads * 16); }
     template <int THREADS>
-    __device__ static void load(char* to, const T* from, long long row_stride, int rows, int pieces, int thread) {
-        constexpr int kRange = 1 << 30;
+    __device__ static int copy_row(int i, int thread) {
+        return ((i * (THREADS / kWave) + thread / kWave) * kWave + lane_id()) / kPieces;
+    }
+    // A piece past the head's lies outside every range and reads as zeros.
+    template <int THREADS>
+    __device__ static int copy_piece(int i, int thread, int pieces) {
+        const int at = (i * (THREADS / kWave) + thread / kWave) * kWave + lane_id();
+        const int piece = (at % kPieces) ^ mix(at / kPieces);
+        return piece < pieces ? piece * 16 : kRange;
+    }
+    // Starts the copies of offsets[i] of `from`; past `range` bytes they give
+    // zeros.  The memory counter tells when they are done.
+    template <int THREADS>
+    __device__ static void copy(char* to, const T* from, int range, const int* offsets, int wave) {
         const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, kRange, 0x00020000);
-        const int stride = static_cast<int>(row_stride * static_cast<long long>(sizeof(T)));
-        const int wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, range, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kBytes / (THREADS * 16); ++i) {
-            const int first = (i * (THREADS / kWave) + wave) * kWave;
-            const int at = first + lane_id();
-            const int row = at / kPieces;
-            const int piece = (at % kPieces) ^ mix(row);
-            // Offsets outside the range read as zeros.
-            const int offset = row < rows && piece < pieces ? row * stride + piece * 16 : kRange;
+        for (int i = 0; i < copies(THREADS); ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rsrc, (__attribute__((address_space(3))) void*)(to + first * 16), 16, offset, 0, 0, 0);
-        }
+                rsrc, (__attribute__((address_space(3))) void*)(to + (i * (THREADS / kWave) + wave) * kWave * 16), 16,
+                offsets[i], 0, 0, 0);
     }
 
     // Left (or right) operand of a product over channels: row `row`, channels
@@ -105,13 +112,13 @@ __device__ inline typename AttnMath<T>::Frag column_frag(const char* tile, int s
     const int lane = lane_id();
     const int row = 4 * (lane >> 5) + ((lane & 15) >> 2);
     const int piece = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const char* at = tile + Tile::place(row, piece) + ((lane & 1) << 3) + step * 16 * Tile::kRowBytes;
+    const char* at = tile + ((lane & 1) << 3) + step * 16 * Tile::kRowBytes;
     typedef __attribute__((address_space(3))) i16x4_attn* Local;
     struct Pair {
         i16x4_attn a, b;
     };
-    const Pair both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at)),
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at + 8 * Tile::kRowBytes))};
+    const Pair both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at + Tile::place(row, piece))),
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((Local)(at + Tile::place(row + 8, piece)))};
     return __builtin_bit_cast(typename AttnMath<T>::Frag, both);
 }
 
@@ -144,6 +151,44 @@ __device__ inline void add_columns(f32x16_attn (&acc)[BLOCKS], const char* tile,
         }
     }
 }
+
+// The keys and values of a sequence and key head, copied KT rows at a time
+// into two tiles one after the other.
+template <typename T, int DP, int KT, int THREADS>
+struct KeyTiles {
+    typedef AttnTile<T, DP, KT> Tile;
+    static constexpr int kCopies = Tile::copies(THREADS);
+    const T *keys, *values;
+    long long k_stride, v_stride;
+    int row_bytes, wave;
+    int k_offsets[kCopies], v_offsets[kCopies];
+
+    __device__ KeyTiles(const lattice_attention& a, const AttnSequence& s, int kv, int thread) {
+        keys = static_cast<const T*>(a.k) + s.k0 * a.k_row_stride + kv * a.k_head_stride;
+        values = static_cast<const T*>(a.v) + s.k0 * a.v_row_stride + kv * a.v_head_stride;
+        k_stride = a.k_row_stride;
+        v_stride = a.v_row_stride;
+        row_bytes = a.dim * static_cast<int>(sizeof(T));
+        wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+        constexpr int kSize = sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = Tile::template copy_row<THREADS>(i, thread);
+            const int piece = Tile::template copy_piece<THREADS>(i, thread, row_bytes / 16);
+            k_offsets[i] = row * static_cast<int>(k_stride) * kSize + piece;
+            v_offsets[i] = row * static_cast<int>(v_stride) * kSize + piece;
+        }
+    }
+    // Rows j0 .. of the sequence's nk; the range ends with the last of them.
+    __device__ void copy(char* to, int j0, int nk) const {
+        const int last = min(nk - j0, KT) - 1;
+        constexpr int kSize = sizeof(T);
+        Tile::template copy<THREADS>(to, keys + j0 * k_stride, last * static_cast<int>(k_stride) * kSize + row_bytes,
+                                     k_offsets, wave);
+        Tile::template copy<THREADS>(to + Tile::kBytes, values + j0 * v_stride,
+                                     last * static_cast<int>(v_stride) * kSize + row_bytes, v_offsets, wave);
+    }
+};
 
 // The operand of a wave's 32 rows (row L % 32 at `row`), kept in registers;
 // zeros past `dim`.
@@ -181,6 +226,23 @@ __device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
 
 // Row of a result's register r.
 __device__ inline int result_row(int r) { return 8 * (r / 4) + 4 * (lane_id() >> 5) + r % 4; }
+
+// Whether a column's sums times `factor` are finite (channels past a head's
+// are zeros, or as infinite as the others).
+template <int BLOCKS>
+__device__ inline bool finite_columns(const f32x16_attn (&acc)[BLOCKS], float factor) {
+    uint32_t largest = 0;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            // The bits of magnitudes are ordered, NaN above infinity.
+            const uint32_t bits = __float_as_uint(acc[b][r] * factor) & 0x7fffffffu;
+            largest = max(largest, bits);
+        }
+    }
+    return largest < 0x7f800000u;
+}
 
 // The tiles of KT keys that a range of positions sees: first those of the
 // first keys that lie before the window's, then the window's.
