@@ -10,14 +10,24 @@ from mlx_lattice_amd.nn.quantized_conv import (
     QuantizedGenerativeConvTranspose3d,
     QuantizedSubmConv3d,
 )
+from mlx_lattice_amd.nn.transformer import (
+    Dropout,
+    LayerNorm,
+    VoxelTransformerBlock,
+    WindowAttention,
+)
 
 __all__ = [
     'Conv3d',
     'ConvTranspose3d',
+    'Dropout',
     'GenerativeConvTranspose3d',
+    'LayerNorm',
     'QuantizedConv3d',
     'QuantizedConvTranspose3d',
     'QuantizedGenerativeConvTranspose3d',
     'QuantizedSubmConv3d',
     'SubmConv3d',
+    'VoxelTransformerBlock',
+    'WindowAttention',
 ]

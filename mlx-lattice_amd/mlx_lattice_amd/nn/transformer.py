@@ -1,0 +1,158 @@
+"""Modules of a transformer block over the rows of voxel scans (no reference
+counterpart): layer norm, counter-based dropout, windowed attention with rotary
+positions by voxel coordinates, and the block they make with pointwise convs.
+
+Rows of a scan are adjacent and in scan order, as a sorted cloud or
+``sparse_collate`` of sorted clouds lays them; the window is one of rows in
+that order."""
+
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from mlx_lattice_amd.core import SparseTensor
+from mlx_lattice_amd.nn.conv import SubmConv3d
+from mlx_lattice_amd.ops import (
+    batch_offsets,
+    dropout,
+    layer_norm,
+    rotary_frequencies,
+    rotary_positions,
+    window_attention,
+)
+
+__all__ = ['Dropout', 'LayerNorm', 'VoxelTransformerBlock', 'WindowAttention']
+
+
+class LayerNorm(nn.Module):
+    """Layer norm of feature rows delegating to :func:`layer_norm`."""
+
+    def __init__(self, channels: int, *, eps: float = 1e-5, bias: bool = True,
+                 device=None, dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(
+            torch.ones(channels, device=device, dtype=dtype),
+            requires_grad=False)
+        self.bias = nn.Parameter(
+            torch.zeros(channels, device=device, dtype=dtype),
+            requires_grad=False) if bias else None
+
+    def forward(self, x: SparseTensor) -> SparseTensor:
+        return layer_norm(x, self.weight, self.bias, eps=self.eps)
+
+
+class Dropout(nn.Module):
+    """Dropout delegating to :func:`dropout`, with a residual.
+
+    ``seed`` is the layer's own; ``calls`` counts its training passes and is
+    the generator's offset, so that each pass has a mask of its own and a run
+    repeats from the two numbers.
+    """
+
+    def __init__(self, p: float, *, seed: int) -> None:
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError('p must be between 0 and 1.')
+        self.p = p
+        self.seed = seed
+        self.calls = 0
+
+    def forward(self, x: SparseTensor, *,
+                residual: SparseTensor | None = None) -> SparseTensor:
+        if not self.training or self.p == 0.0:
+            if residual is None:
+                return x
+            if not x.same_coords(residual):
+                raise ValueError('sparse tensor coordinates must match.')
+            return x.replace(feats=x.feats + residual.feats)
+        self.calls += 1
+        return dropout(x, self.p, seed=self.seed, offset=self.calls - 1,
+                       residual=residual)
+
+
+class WindowAttention(nn.Module):
+    """Attention of each row over the rows ``left`` before to ``right`` after
+    it in its scan, and the scan's first ``sinks`` rows.
+
+    One pointwise conv makes the queries, keys and values; the heads of the
+    first two are turned by the voxel's x, y and z, a third of a head's
+    channels each.
+    """
+
+    def __init__(self, channels: int, heads: int, *,
+                 kv_heads: int | None = None, left: int | None = 128,
+                 right: int | None = 128, sinks: int = 0,
+                 rotary_base: float = 10000.0, bias: bool = True, device=None,
+                 dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        self.heads = heads
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or channels % heads or (channels // heads) % 2:
+            raise ValueError('channels must be an even number for each head.')
+        if self.kv_heads < 1 or heads % self.kv_heads:
+            raise ValueError(
+                'the number of heads must be a multiple of the number of key '
+                'heads.')
+        self.dim = channels // heads
+        self.left, self.right, self.sinks = left, right, sinks
+        third = self.dim // 6 * 2
+        self.dims = (self.dim - 2 * third, third, third)
+        # Not a buffer: its float64 is kept when the module changes dtype.
+        self._frequencies = rotary_frequencies(self.dims, rotary_base,
+                                               device=device)
+        self.project = SubmConv3d(
+            channels, (heads + 2 * self.kv_heads) * self.dim, kernel_size=1,
+            bias=bias, device=device, dtype=dtype)
+        self.out = SubmConv3d(channels, channels, kernel_size=1, bias=bias,
+                              device=device, dtype=dtype)
+
+    def forward(self, x: SparseTensor, *,
+                offsets: torch.Tensor | None = None) -> SparseTensor:
+        """``offsets``: the scans' row offsets, which the layers of a level
+        can share; ``batch_offsets(x)`` by default.  A tensor of several scans
+        that has lost its ``batch_counts``, as strided convs give it, needs
+        ``batch_offsets(x, batches)``."""
+        if offsets is None:
+            offsets = batch_offsets(x)
+        packed = self.project(x).feats.view(x.capacity, -1, self.dim)
+        turned = packed[:, :self.heads + self.kv_heads]
+        turned = rotary_positions(turned, x.coords[:, 1:],
+                                  self._on(x.device), dims=self.dims)
+        rows = window_attention(
+            turned[:, :self.heads], turned[:, self.heads:],
+            packed[:, self.heads + self.kv_heads:], left=self.left,
+            right=self.right, sinks=self.sinks, offsets=offsets)
+        return self.out(x.replace(feats=rows.view(x.capacity, -1)))
+
+    def _on(self, device: torch.device) -> torch.Tensor:
+        if self._frequencies.device != device:
+            self._frequencies = self._frequencies.to(device)
+        return self._frequencies
+
+
+class VoxelTransformerBlock(nn.Module):
+    """Pre-norm block: ``x + dropout(attention(norm(x)))``, then the same with
+    a ReLU layer of ``hidden`` channels (4 times the channels by default)."""
+
+    def __init__(self, channels: int, heads: int, *, hidden: int | None = None,
+                 p: float = 0.0, seed: int = 0, device=None,
+                 dtype: torch.dtype = torch.float32, **attention) -> None:
+        super().__init__()
+        hidden = 4 * channels if hidden is None else hidden
+        made = {'device': device, 'dtype': dtype}
+        self.norm1 = LayerNorm(channels, **made)
+        self.attention = WindowAttention(channels, heads, **attention, **made)
+        self.drop1 = Dropout(p, seed=2 * seed)
+        self.norm2 = LayerNorm(channels, **made)
+        self.expand = SubmConv3d(channels, hidden, kernel_size=1, **made)
+        self.contract = SubmConv3d(hidden, channels, kernel_size=1, **made)
+        self.drop2 = Dropout(p, seed=2 * seed + 1)
+
+    def forward(self, x: SparseTensor, *,
+                offsets: torch.Tensor | None = None) -> SparseTensor:
+        mixed = self.attention(self.norm1(x), offsets=offsets)
+        x = self.drop1(mixed, residual=x)
+        inner = self.expand(self.norm2(x), activation='relu')
+        return self.drop2(self.contract(inner), residual=x)

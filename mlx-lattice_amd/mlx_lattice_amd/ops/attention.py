@@ -13,17 +13,29 @@ __all__ = ['batch_offsets', 'window_attention']
 _ALL = 2 ** 31 - 1
 
 
-def batch_offsets(x: SparseTensor) -> torch.Tensor:
-    """Row offsets ``(B + 1,)`` of the scans of ``x``, int32 on its device,
-    from ``batch_counts``; without them the active rows are one sequence.
-    Rows of a scan are adjacent, as ``sparse_collate`` lays them."""
+def batch_offsets(x: SparseTensor, batches: int = 1) -> torch.Tensor:
+    """Row offsets ``(B + 1,)`` of the scans of ``x``, int32 on its device.
+
+    From ``batch_counts`` where ``x`` has them; else its active rows hold the
+    scans 0 to ``batches - 1`` (a strided conv's output has no counts).  Rows
+    of a scan are adjacent and scans in order, as ``sparse_collate`` lays them
+    and strided convs keep them.
+    """
     counts = x.batch_counts
-    if counts is None or len(counts) == 1:
+    if counts is not None and len(counts) > 1:
+        offsets = [0]
+        for count in counts:
+            offsets.append(offsets[-1] + count)
+        return torch.tensor(offsets, dtype=torch.int32, device=x.device)
+    if batches < 1:
+        raise ValueError('batches must be positive.')
+    if counts is not None or batches == 1:
         return torch.cat([torch.zeros_like(x.active_rows), x.active_rows])
-    offsets = [0]
-    for count in counts:
-        offsets.append(offsets[-1] + count)
-    return torch.tensor(offsets, dtype=torch.int32, device=x.device)
+    rows = torch.arange(x.capacity, device=x.device)
+    scan = torch.where(rows < x.active_rows, x.batch_indices, batches)
+    return torch.searchsorted(
+        scan, torch.arange(batches + 1, dtype=scan.dtype, device=x.device),
+        out_int32=True)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
