@@ -221,12 +221,13 @@ __device__ inline void grad_query_row(const lattice_attention& a, const AttnSequ
 }
 
 // grad_k and grad_v of one key row and key head: states holds (lse, delta) by
-// key head, row and head; over the queries that see it
+// key head, row and head, channels from_dim .. to_dim are written; over the
+// queries that see it
 // and the heads that share it, (query, head) pairs 64 at a time, one a lane.
 template <typename T>
 __device__ inline void grad_key_row(const lattice_attention& a, const AttnSequence& s, int j, int kv,
                                     const float* lse, const float2* states, const T* grad_out, T* grad_k, T* grad_v,
-                                    AttnRowScratch* scratch) {
+                                    AttnRowScratch* scratch, int from_dim = 0, int to_dim = kAttnMaxDim) {
     const int lane = lane_id();
     const int group = a.heads / a.kv_heads;
     const long long row = static_cast<long long>(s.k0) + j;
@@ -275,7 +276,7 @@ __device__ inline void grad_key_row(const lattice_attention& a, const AttnSequen
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
         const int d = lane + c * kWave;
-        if (d >= a.dim) continue;
+        if (d >= a.dim || d < from_dim || d >= to_dim) continue;
         grad_k[at + d] = static_cast<T>(acc_k[c] * a.scale);
         grad_v[at + d] = static_cast<T>(acc_v[c]);
     }
@@ -320,6 +321,12 @@ inline lattice_attention attn_bounded(const lattice_attention& a) {
     b.right = std::min(b.right, most);
     b.sinks = std::min(b.sinks, a.keys);
     return b;
+}
+
+// Dynamic LDS past the 64 KiB that every kernel may use has to be allowed.
+inline hipError_t allow_lds(const void* kernel, size_t bytes) {
+    if (bytes <= 64 * 1024) return hipSuccess;
+    return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
 #define LATTICE_REQUIRE_ATTENTION(args)                           \

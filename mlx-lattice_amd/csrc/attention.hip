@@ -48,30 +48,24 @@ struct AttnState {
     }
 };
 
-// The keys j0 .. j0 + 32 BLOCKS of a tile for the wave's 32 rows; `masked`:
-// some of them are not seen by some row.
-template <typename T, int DP, int KT>
-__device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>& state, const AttnOperand<T, DP>& q,
-                                   const char* keys, const char* values, float scale, int nk, int p, int j0,
+// Adds the keys j0 .. j0 + 32 PARTS, rows row0 .. of a tile, to the sums of the
+// wave's 32 rows; `masked`: some of them are not seen by some row.
+template <int PARTS, typename T, int DP, int KT>
+__device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T, DP>& q, const char* keys,
+                                   const char* values, int row0, float scale, const AttnMask& mask, int j0,
                                    bool masked) {
     typedef AttnTile<T, DP, KT> Tile;
-    constexpr int kParts = KT / 32;
-    f32x16_attn s[kParts];
+    f32x16_attn s[PARTS];
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) s[part] = tile_product<Tile, T, DP>(keys, 32 * part, q);
+    for (int part = 0; part < PARTS; ++part) 
+        s[part] = tile_product<Tile, T, DP>(keys, row0 + 32 * part, q, f32x16_attn{});
     if (masked) {
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = j0 + 32 * part + result_row(r);
-                if (!attn_visible(a, nk, p, j)) s[part][r] = -INFINITY;
-            }
-        }
+        for (int part = 0; part < PARTS; ++part) mask.apply(s[part], j0 + 32 * part, j0 < mask.sinks);
     }
     float most = s[0][0];
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
+    for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, s[part][r]);
     }
@@ -83,7 +77,7 @@ __device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>&
     }
     float sum = 0.0f;
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
+    for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[part][r] = __builtin_amdgcn_exp2f(s[part][r] * scale - state.top);
@@ -92,7 +86,30 @@ __device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>&
     }
     state.sum += sum;
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) add_columns<Tile, T>(state.acc, values, 32 * part, s[part]);
+    for (int part = 0; part < PARTS; ++part) add_columns<Tile, T>(state.acc, values, row0 + 32 * part, s[part]);
+}
+
+// A tile of KT keys: at once where every row sees every key, else 32 keys at a
+// time, those that some row sees.  Heads of 128 take every tile at once: a
+// second form of the loop costs them more registers than it saves products
+// (16k causal rows, window 4096: 612 us with it, 572 without; 120k rows of
+// heads of 32, window 257: 143 with it, 171 without).
+template <typename T, int DP, int KT>
+__device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>& state, const AttnOperand<T, DP>& q,
+                                   const char* keys, const char* values, float scale, int nk, const AttnRows& w,
+                                   const AttnMask& mask, int j0) {
+    const AttnView view = attn_view(a, nk, w.p_low, w.p_high, j0, KT);
+    if (view == kSeesNone) return;
+    if (KT > 32 && (DP >= 128 || view == kSeesAll)) {
+        attend_keys<KT / 32, T, DP, KT>(state, q, keys, values, 0, scale, mask, j0, view == kSeesSome);
+        return;
+    }
+    if (KT > 32 && DP >= 128) return;
+    for (int row0 = 0; row0 < KT; row0 += 32) {
+        const AttnView part = attn_view(a, nk, w.p_low, w.p_high, j0 + row0, 32);
+        if (part != kSeesNone)
+            attend_keys<1, T, DP, KT>(state, q, keys, values, row0, scale, mask, j0 + row0, part == kSeesSome);
+    }
 }
 
 // Writes the wave's rows: the result, or a part of it (splits > 1).  A result
@@ -175,6 +192,7 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
                w.head * a.q_head_stride,
            a.dim, w.valid, negate);
+    const AttnMask mask(a, s.nk, w.p);
     AttnState<T, DP> state;
     state.clear();
     const int p_low = static_cast<int>(t.first / group) + s.shift();
@@ -190,23 +208,22 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     __syncthreads();
     for (int index = from; index < to; ++index) {
         if (index + 1 < to) copy(index + 1);
-        const int j0 = tiles.tile(index) * KT;
         const char* at = shared + (index & 1) * 2 * Tile::kBytes;
-        const bool none = j0 > w.p_high + a.right || (j0 + KT - 1 < w.p_low - a.left && j0 >= a.sinks);
-        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
-                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
-        if (!none)
-            attend_tile<T, DP, KT>(a, state, q, at, at + Tile::kBytes, scale, s.nk, w.p, j0, !all);
+        attend_tile<T, DP, KT>(a, state, q, at, at + Tile::kBytes, scale, s.nk, w, mask, tiles.tile(index) * KT);
         __syncthreads();
     }
     write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, lse,
                       reinterpret_cast<AttnRowScratch*>(shared) + wave);
 }
 
-// 32 rows a block, for few queries: each wave takes every fourth tile, and the
-// waves' parts are joined in LDS.
-template <typename T, int DP, int KT>
-__global__ void __launch_bounds__(kAttnBlock)
+// Waves a block for few queries: two tiles a wave fit the LDS of a unit.
+template <typename T, int DP> constexpr int few_waves() { return DP * static_cast<int>(sizeof(T)) <= 256 ? 8 : 4; }
+
+// 32 rows a block, for few queries: each wave takes its own tiles
+// of KT keys, with no wait for the others, and the waves' parts are joined in
+// LDS.
+template <typename T, int DP, int KT, int kFewWaves>
+__global__ void __launch_bounds__(kFewWaves * kWave)
 attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
     typedef AttnTile<T, DP, KT> Tile;
     constexpr int kBlocks = AttnState<T, DP>::kBlocks;
@@ -224,6 +241,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
                w.head * a.q_head_stride,
            a.dim, w.valid, negate);
+    const AttnMask mask(a, s.nk, w.p);
     AttnState<T, DP> state;
     state.clear();
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, w.p_low, w.p_high);
@@ -231,50 +249,50 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
     const KeyTiles<T, DP, KT, kWave> source(a, s, kv, lane_id());
     char* mine = shared + wave * 2 * Tile::kBytes;
-    const int steps = (to - from + kAttnWaves - 1) / kAttnWaves;
-    for (int step = 0; step < steps; ++step) {
-        const int index = from + step * kAttnWaves + wave;
-        const int j0 = index < to ? tiles.tile(index) * KT : 0;
-        __syncthreads();
-        if (index < to) source.copy(mine, j0, s.nk);
-        __syncthreads();
-        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
-                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
-        if (index < to)
-            attend_tile<T, DP, KT>(a, state, q, mine, mine + Tile::kBytes, scale, s.nk, w.p, j0, !all);
+    for (int index = from + wave; index < to; index += kFewWaves) {
+        const int j0 = tiles.tile(index) * KT;
+        source.copy(mine, j0, s.nk);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wave_fence();
+        attend_tile<T, DP, KT>(a, state, q, mine, mine + Tile::kBytes, scale, s.nk, w, mask, j0);
+        wave_fence();
     }
-    // The waves' sums meet in the first wave, in wave order.
+    // Every wave's sums to the largest maximum, then pairwise into the first
+    // wave's.
     const int lane = lane_id();
     state.sum += other_half(state.sum);
     __syncthreads();
     float2* states = reinterpret_cast<float2*>(shared);
-    float* sums = reinterpret_cast<float*>(shared + kAttnWaves * 32 * sizeof(float2));
+    float* sums = reinterpret_cast<float*>(shared + kFewWaves * 32 * sizeof(float2));
     if (lane < 32) states[wave * 32 + lane] = float2{state.top, state.sum};
     __syncthreads();
-    float top = kAttnFloor;
-    for (int v = 0; v < kAttnWaves; ++v) top = fmaxf(top, states[v * 32 + (lane & 31)].x);
-    float sum = 0.0f;
-    for (int v = 0; v < kAttnWaves; ++v) {
+    float top = kAttnFloor, sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) top = fmaxf(top, states[v * 32 + (lane & 31)].x);
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) {
         const float2 other = states[v * 32 + (lane & 31)];
         sum += other.y * __builtin_amdgcn_exp2f(other.x - top);
     }
-    const float factor = __builtin_amdgcn_exp2f(state.top - top);
-    for (int v = 1; v < kAttnWaves; ++v) {
-        __syncthreads();
-        if (wave == v) {
+    state.rescale(__builtin_amdgcn_exp2f(state.top - top));
+    constexpr int kValues = kBlocks * 16 * kWave;
+#pragma unroll
+    for (int active = kFewWaves / 2; active > 0; active /= 2) {
+        if (active < kFewWaves / 2) __syncthreads();
+        if (wave >= active && wave < 2 * active) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sums[(b * 16 + r) * kWave + lane] = state.acc[b][r] * factor;
+                for (int r = 0; r < 16; ++r)
+                    sums[(wave - active) * kValues + (b * 16 + r) * kWave + lane] = state.acc[b][r];
             }
         }
         __syncthreads();
-        if (wave == 0) {
-            if (v == 1) state.rescale(factor);
+        if (wave < active) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) state.acc[b][r] += sums[(b * 16 + r) * kWave + lane];
+                for (int r = 0; r < 16; ++r) state.acc[b][r] += sums[wave * kValues + (b * 16 + r) * kWave + lane];
             }
         }
     }
@@ -286,7 +304,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
                       reinterpret_cast<AttnRowScratch*>(shared));
 }
 
-// Joins the parts of a row: a wave a (query row, head).
+// Joins the parts (at most 64) of a row: a wave a (query row, head).
 template <typename T>
 __global__ void __launch_bounds__(kAttnBlock)
 join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
@@ -295,36 +313,35 @@ join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     const long long items = static_cast<long long>(a.queries) * a.heads;
     const long long at = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
     if (at >= items) return;
-    const int row = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
-    const int e = query_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
-    const AttnSequence s = attn_sequence(a, e);
-    const int i = row - s.q0;
-    const bool sees = attn_seen(a, s.nk, i + s.shift()).total() > 0;
-    float acc[kAttnMaxDim / kWave] = {}, top = kAttnFloor, sum = 0.0f;
-    if (sees) {
-        for (int z = 0; z < splits; ++z) top = fmaxf(top, part.states[z * items + at].x);
-        for (int z = 0; z < splits; ++z) {
-            const float2 state = part.states[z * items + at];
-            const float factor = __builtin_amdgcn_exp2f(state.x - top);
-            sum += state.y * factor;
+    const float2 state = lane < splits ? part.states[lane * items + at] : float2{kAttnFloor, 0.0f};
+    const float top = wave_max(state.x);
+    const float factor = __builtin_amdgcn_exp2f(state.x - top);
+    const float sum = wave_sum(state.y * factor);
+    float acc[kAttnMaxDim / kWave] = {};
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) {
+        const float share = __shfl(factor, z);
 #pragma unroll
-            for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
-                const int d = lane + c * kWave;
-                if (d < a.dim) acc[c] += part.values[(z * items + at) * a.dim + d] * factor;
-            }
+        for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
+            const int d = min(lane + c * kWave, a.dim - 1);
+            acc[c] += part.values[(z * items + at) * a.dim + d] * share;
         }
     }
-    bool finite = true;
+    bool finite = sum > 0.0f;
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
-        if (sees) acc[c] = lane + c * kWave < a.dim ? acc[c] / sum : 0.0f;
+        acc[c] /= sum;
         finite = finite && fabsf(acc[c]) < INFINITY;
     }
+    // Rows that see nothing, and those that are not finite.
     if (__any(!finite)) {
-        attend_row<T>(a, s, i, head, out, lse, &scratch[wave]);
+        const int row = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
+        const int e = query_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
+        const AttnSequence s = attn_sequence(a, e);
+        attend_row<T>(a, s, row - s.q0, head, out, lse, &scratch[wave]);
         return;
     }
-    if (lse && lane == 0) lse[at] = sees ? top + log2f(sum) : INFINITY;
+    if (lse && lane == 0) lse[at] = top + log2f(sum);
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
         const int d = lane + c * kWave;
@@ -363,24 +380,24 @@ inline AttnLayout attn_layout(const lattice_attention& a) {
 template <typename T, int DP>
 int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, T* out, float* lse,
                   hipStream_t stream) {
+    // Tiles twice as large are no faster (scan of heads of 32: 152 us for 143).
     constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
     typedef AttnTile<T, DP, kTile> Tile;
     const dim3 grid(static_cast<unsigned>(l.slots), a.kv_heads, l.splits);
     if (l.few) {
-        constexpr int kFew = 32;
-        constexpr size_t kLds = std::max<size_t>(kAttnWaves * 2 * AttnTile<T, DP, kFew>::kBytes,
-                                                 kAttnWaves * 32 * sizeof(float2) + DP / 32 * 16 * kWave * 4);
+        constexpr int kFew = 32, kFewWaves = few_waves<T, DP>();
+        constexpr size_t kLds =
+            std::max<size_t>(kFewWaves * 2 * AttnTile<T, DP, kFew>::kBytes,
+                             kFewWaves * 32 * sizeof(float2) + kFewWaves / 2 * DP / 32 * 16 * kWave * sizeof(float));
         static_assert(kLds >= sizeof(AttnRowScratch) && kLds <= 160 * 1024);
-        const auto kernel = attend_few<T, DP, kFew>;
-        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-        kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, lse);
+        const auto kernel = attend_few<T, DP, kFew, kFewWaves>;
+        LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
+        kernel<<<grid, kFewWaves * kWave, kLds, stream>>>(a, l.splits, part, out, lse);
     } else {
         constexpr size_t kLds = std::max<size_t>(4 * Tile::kBytes, kAttnWaves * sizeof(AttnRowScratch));
         static_assert(kLds <= 160 * 1024);
         const auto kernel = attend_tiles<T, DP, kTile>;
-        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
         kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, lse);
     }
     LATTICE_LAUNCH_CHECK();

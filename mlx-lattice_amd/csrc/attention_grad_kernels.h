@@ -133,6 +133,7 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
     }
     const float log_sum = w.valid ? lse[at] : INFINITY;
     if (w.valid && half == 0) states[query_state(a, group, row, w.head)] = float2{log_sum, along};
+    const AttnMask mask(a, s.nk, w.p);
     f32x16_attn acc[kBlocks] = {};
     SlopeScale<T> slopes;
     const int p_low = static_cast<int>(t.first / group) + s.shift();
@@ -149,24 +150,17 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
         const int j0 = tiles.tile(index) * KT;
         const char* k_tile = shared + (index & 1) * 2 * Tile::kBytes;
         const char* v_tile = k_tile + Tile::kBytes;
-        const bool none = j0 > w.p_high + a.right || (j0 + KT - 1 < w.p_low - a.left && j0 >= a.sinks);
-        const bool all = j0 + KT <= s.nk && j0 + KT - 1 <= w.p_low + a.right &&
-                         (j0 >= w.p_high - a.left || j0 + KT <= a.sinks);
-        if (!none) {
 #pragma unroll
-            for (int part = 0; part < KT / 32; ++part) {
-                f32x16_attn p = tile_product<Tile, T, DP>(k_tile, 32 * part, q);
-                f32x16_attn dp = tile_product<Tile, T, DP>(v_tile, 32 * part, d);
-                if (!all) {
+        for (int row0 = 0; row0 < KT; row0 += 32) {
+            const AttnView view = attn_view(a, s.nk, w.p_low, w.p_high, j0 + row0, 32);
+            if (view == kSeesNone) continue;
+            f32x16_attn p = tile_product<Tile, T, DP>(k_tile, row0, q, f32x16_attn{});
+            f32x16_attn dp = tile_product<Tile, T, DP>(v_tile, row0, d, f32x16_attn{});
+            if (view == kSeesSome) mask.apply(p, j0 + row0, j0 + row0 < a.sinks);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!attn_visible(a, s.nk, w.p, j0 + 32 * part + result_row(r))) p[r] = -INFINITY;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
-                add_slopes<Tile, T>(acc, slopes, k_tile, 32 * part, dp);
-            }
+            for (int r = 0; r < 16; ++r)
+                dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
+            add_slopes<Tile, T>(acc, slopes, k_tile, row0, dp);
         }
         __syncthreads();
     }
@@ -184,7 +178,7 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
 
 // ROWS (query, head) pairs r0 .. of a sequence and key head in LDS: q and
 // grad_out rows, and of each its lse (+inf past the rows there are, so that
-// its shares are zero), delta and position.
+// its shares are zero) less the shares' scale, -delta and position.
 template <typename T, int DP, int ROWS>
 struct QueryTile {
     typedef AttnTile<T, DP, ROWS> Tile;
@@ -207,7 +201,7 @@ struct QueryTiles {
     const float2* states;
     long long q_stride, d_stride;
     int thread, wave, q_row, q_head, d_row, d_head, shift;
-    uint32_t group;
+    GroupDivide by_group;
     bool aligned;
     int own_query;
     int q_offsets[kCopies], d_offsets[kCopies];
@@ -219,11 +213,12 @@ struct QueryTiles {
     };
 
     __device__ QueryTiles(const lattice_attention& a, const AttnSequence& s, int kv, uint32_t heads,
-                          const float2* all_states, const T* all_grad_out, int of_thread) {
+                          const float2* all_states, const T* all_grad_out, int of_thread)
+        : by_group(heads) {
         constexpr int kSize = sizeof(T);
         thread = of_thread;
         wave = __builtin_amdgcn_readfirstlane(thread / kWave);
-        group = heads;
+        const uint32_t group = heads;
         shift = s.shift();
         q_stride = a.q_row_stride;
         d_stride = static_cast<long long>(a.heads) * a.dim;
@@ -241,21 +236,21 @@ struct QueryTiles {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const uint32_t n = h0 + Tile::template copy_row<THREADS>(i, thread);
-            const int query = n / group, head = n - query * group;
+            const int query = by_group(n), head = n - query * by_group.group;
             const int piece = Tile::template copy_piece<THREADS>(i, thread, d_head / 16);
             q_offsets[i] = query * q_row + head * q_head + piece;
             d_offsets[i] = query * d_row + head * d_head + piece;
         }
-        own_query = (h0 + thread) / group;
+        own_query = by_group(h0 + thread);
     }
     // Starts the copies of pairs r0 .. of `rows`; rows past them hold other
     // rows or zeros, whose shares are zero.
     __device__ State copy(char* to, uint32_t r0, uint32_t rows) {
-        const uint32_t i0 = r0 / group, h0 = r0 - i0 * group;
+        const uint32_t group = by_group.group, i0 = by_group(r0), h0 = r0 - i0 * group;
         if (!aligned) places(h0);
         const uint32_t count = min(rows - r0, static_cast<uint32_t>(ROWS));
         // The range ends with the last query's last head.
-        const int last = (h0 + count - 1) / group;
+        const int last = by_group(h0 + count - 1);
         Tile::template copy<THREADS>(to, q + i0 * q_stride,
                                      last * q_row + static_cast<int>(group - 1) * q_head + d_head, q_offsets, wave);
         Tile::template copy<THREADS>(to + Tile::kBytes, grad_out + i0 * d_stride,
@@ -271,14 +266,16 @@ struct QueryTiles {
     __device__ void store(char* to, const State& state) const {
         if (thread >= ROWS) return;
         float* at = reinterpret_cast<float*>(to + 2 * Tile::kBytes);
-        at[thread] = state.lse;
-        at[ROWS + thread] = state.delta;
+        at[thread] = state.lse - kShareLog2<T>;
+        at[ROWS + thread] = -state.delta;
         reinterpret_cast<int*>(at)[2 * ROWS + thread] = state.position;
     }
 };
 
 // Adds the queries of a tile to a wave's 32 keys; `masked`: a lane's key is
-// seen from the positions lo .. hi alone.
+// seen from the positions lo .. hi alone.  (A form of its own for tiles without
+// a mask costs more registers than it saves branches: 855 for 787 us at heads
+// of 128, 133 for 121 at 64.)
 template <typename T, int DP, int QT>
 __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k, const AttnOperand<T, DP>& v,
                                    float scale, int lo, int hi, bool masked, f32x16_attn (&acc_k)[DP / 32],
@@ -290,8 +287,22 @@ __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k
     const float* states = Queries::states(tile);
 #pragma unroll
     for (int part = 0; part < QT / 32; ++part) {
-        f32x16_attn p = tile_product<Tile, T, DP>(tile, 32 * part, k);
-        f32x16_attn ds = tile_product<Tile, T, DP>(d_tile, 32 * part, v);
+        f32x16_attn p = tile_product<Tile, T, DP>(tile, 32 * part, k, f32x16_attn{});
+        // dp - delta.  The product may start from -delta; with one wave a SIMD
+        // (heads of 128) that read would hold it up, and delta is added after.
+        constexpr bool kFromDelta = DP < 128;
+        f32x16_attn ds = {};
+        if constexpr (kFromDelta) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 delta = *reinterpret_cast<const float4*>(states + QT + 32 * part + 8 * g + 4 * half);
+                ds[4 * g] = delta.x;
+                ds[4 * g + 1] = delta.y;
+                ds[4 * g + 2] = delta.z;
+                ds[4 * g + 3] = delta.w;
+            }
+        }
+        ds = tile_product<Tile, T, DP>(d_tile, 32 * part, v, ds);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int row = 32 * part + 8 * g + 4 * half;
@@ -303,14 +314,15 @@ __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k
                     if (position[i] < lo || position[i] > hi) p[4 * g + i] = -INFINITY;
             }
             const float4 lse = *reinterpret_cast<const float4*>(states + row);
-            const float4 delta = *reinterpret_cast<const float4*>(states + QT + row);
             const float log_sum[4] = {lse.x, lse.y, lse.z, lse.w};
+            float4 delta{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!kFromDelta) delta = *reinterpret_cast<const float4*>(states + QT + row);
             const float along[4] = {delta.x, delta.y, delta.z, delta.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 4 * g + i;
-                p[r] = __builtin_amdgcn_exp2f(p[r] * scale - (log_sum[i] - kShareLog2<T>));
-                ds[r] = p[r] * (ds[r] - along[i]);
+                p[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum[i]);
+                ds[r] = p[r] * (kFromDelta ? ds[r] : ds[r] + along[i]);
             }
         }
         add_columns<Tile, T>(acc_v, d_tile, 32 * part, p);
@@ -369,9 +381,7 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
         if (r0 < to) source.store(tile, source.copy(tile, r0, to));
         __syncthreads();
         if (r0 < to) {
-            const int p_low = static_cast<int>(r0 / group) + s.shift();
-            add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, p_low <= j0 + 31 + a.left, acc_k,
-                                   acc_v, slopes);
+            add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, true, acc_k, acc_v, slopes);
         }
     }
     scale_sums(acc_k, 1.0f / slopes.factor());
@@ -395,56 +405,62 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
     if (wave == 0) store_part(parts.past_of(a, blockIdx.x, kv, blockIdx.z, kFirstValues<DP>), acc_k, acc_v);
 }
 
-// Adds the parts of 32 first keys of a sequence and key head, the window's
-// first and the others in slot order.
+// Adds the parts of 32 first keys and eight channels of a sequence and key
+// head, the window's first and the others in slot order: 256 values of dk and
+// as many of dv, which lie side by side in a part.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kAttnBlock)
 join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
                 const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
-    constexpr int kHeld = kFirstValues<DP> / kAttnBlock;
     __shared__ AttnRowScratch scratch[kAttnWaves];
     __shared__ uint32_t spoilt;
     const uint32_t group = a.heads / a.kv_heads;
-    const int e = blockIdx.x + 1, kv = blockIdx.y, j0 = blockIdx.z * 32;
+    const int e = blockIdx.x + 1, kv = blockIdx.y;
+    const int tile = blockIdx.z / (DP / 8), eighth = blockIdx.z % (DP / 8), j0 = tile * 32, d0 = eighth * 8;
     const AttnSequence s = attn_sequence(a, e);
     const int keys = min(a.sinks, s.nk);
-    if (j0 >= keys) return;
+    if (j0 >= keys || d0 >= a.dim) return;
     const int lane = lane_id(), wave = threadIdx.x / kWave;
     const int j = j0 + (lane & 31);
     const uint32_t slot = s.q0 * group / kFirstRows + e, slots = (s.nq * group + kFirstRows - 1) / kFirstRows;
-    float sum[kHeld];
-    const float* window = parts.window_of(a, e, kv, blockIdx.z, kFirstValues<DP>);
+    const int of_k = eighth * kAttnBlock + threadIdx.x, of_v = of_k + DP * 32;
+    const float* at = parts.window_of(a, e, kv, tile, kFirstValues<DP>);
+    float sum_k = at[of_k], sum_v = at[of_v];
+    constexpr int kAhead = 8;  // parts in flight
+    for (uint32_t u = 0; u < slots; u += kAhead) {
+        float past_k[kAhead], past_v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) sum[i] = window[i * kAttnBlock + threadIdx.x];
-    for (uint32_t u = 0; u < slots; ++u) {
-        const float* past = parts.past_of(a, slot + u, kv, blockIdx.z, kFirstValues<DP>);
+        for (int i = 0; i < kAhead; ++i) {
+            const bool here = u + i < slots;
+            const float* past = parts.past_of(a, slot + (here ? u + i : 0), kv, tile, kFirstValues<DP>);
+            past_k[i] = here ? past[of_k] : 0.0f;
+            past_v[i] = here ? past[of_v] : 0.0f;
+        }
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) sum[i] += past[i * kAttnBlock + threadIdx.x];
+        for (int i = 0; i < kAhead; ++i) {
+            sum_k += past_k[i];
+            sum_v += past_v[i];
+        }
     }
     const float share = __builtin_amdgcn_exp2f(-kShareLog2<T>);
+    sum_k *= a.scale * share;
+    sum_v *= share;
     if (threadIdx.x == 0) spoilt = 0;
     __syncthreads();
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        sum[i] *= i < kHeld / 2 ? a.scale * share : share;
-        finite = finite && fabsf(sum[i]) < INFINITY;
-    }
-    if (!finite && j < keys) atomicOr(&spoilt, 1u << (lane & 31));
+    if (j < keys && !(fabsf(sum_k) < INFINITY && fabsf(sum_v) < INFINITY)) atomicOr(&spoilt, 1u << (lane & 31));
     __syncthreads();
     const uint32_t again = spoilt;
     if (j < keys && !(again >> (lane & 31) & 1)) {
-        const long long at = ((static_cast<long long>(s.k0) + j) * a.kv_heads + kv) * a.dim;
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int value = (i % (kHeld / 2)) * kAttnWaves + wave;  // register of the part
-            const int d = value / 16 * 32 + result_row(value % 16);
-            if (d < a.dim) (i < kHeld / 2 ? grad_k : grad_v)[at + d] = static_cast<T>(sum[i]);
+        const int d = d0 + 4 * (lane >> 5) + wave;
+        const long long to = ((static_cast<long long>(s.k0) + j) * a.kv_heads + kv) * a.dim + d;
+        if (d < a.dim) {
+            grad_k[to] = static_cast<T>(sum_k);
+            grad_v[to] = static_cast<T>(sum_v);
         }
     }
     for (int n = wave; n < 32; n += kAttnWaves) {
         if (again >> n & 1)
-            grad_key_row<T>(a, s, j0 + n, kv, lse, states, grad_out, grad_k, grad_v, &scratch[wave]);
+            grad_key_row<T>(a, s, j0 + n, kv, lse, states, grad_out, grad_k, grad_v, &scratch[wave], d0, d0 + 8);
     }
 }
 
@@ -502,12 +518,12 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
         if (index + 1 < count) state = source.copy(next, first_row(index + 1), rows);
         const char* tile = shared + (index & 1) * Queries::kBytes;
         const uint32_t r0 = first_row(index);
-        const int p_low = static_cast<int>(r0 / group) + s.shift();
-        const int p_high = static_cast<int>((min(r0 + QT, rows) - 1) / group) + s.shift();
         // In the window, or past it: of the first keys alone.
         const bool outside = index >= window_tiles;
         const int lo = !outside ? j - a.right : j < a.sinks ? j + a.left + 1 : INT_MAX;
         const int hi = outside ? INT_MAX : j + a.left;
+        const int p_low = static_cast<int>(source.by_group(r0)) + s.shift();
+        const int p_high = static_cast<int>(source.by_group(min(r0 + QT, rows) - 1)) + s.shift();
         const bool none = outside ? j_wave >= a.sinks || p_high <= j_wave + a.left
                                   : p_high < j_wave - a.right || p_low > j_wave + 31 + a.left;
         const bool all = !outside && j_wave + 31 <= p_low + a.right && j_wave >= p_high - a.left;
@@ -549,8 +565,7 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
         constexpr size_t kLds = std::max<size_t>(4 * AttnTile<T, DP, kTile>::kBytes,
                                                  kAttnWaves * sizeof(AttnRowScratch));
         const auto kernel = grad_query_tiles<T, DP, kTile>;
-        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
         const long long slots = static_cast<long long>(a.queries) * group / (32 * kAttnWaves) + a.sequences + 2;
         kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, lse, grad_out,
                                                                                             grad_q, states);
@@ -562,8 +577,7 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
                                                  kFirstValues<DP> * sizeof(float));
         static_assert(kLds <= 160 * 1024);
         const auto kernel = grad_first_keys<T, DP>;
-        LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                            hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+        LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
         kernel<<<dim3(l.first_slots, a.kv_heads, l.first_tiles), kAttnBlock, kLds, stream>>>(a, states, grad_out,
                                                                                             parts);
         LATTICE_LAUNCH_CHECK();
@@ -572,14 +586,13 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
         std::max<size_t>(2 * QueryTile<T, DP, kTile>::kBytes, kAttnWaves * sizeof(AttnRowScratch));
     static_assert(kLds <= 160 * 1024);
     const auto kernel = grad_key_tiles<T, DP, kTile>;
-    LATTICE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
     const long long slots = a.keys / (32 * kAttnWaves) + a.sequences + 2;
     kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
                                                                                         parts, grad_k, grad_v);
     LATTICE_LAUNCH_CHECK();
     if (l.first_tiles && a.sequences) {
-        join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles), kAttnBlock, 0, stream>>>(
+        join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles * (DP / 8)), kAttnBlock, 0, stream>>>(
             a, lse, states, grad_out, parts, grad_k, grad_v);
         LATTICE_LAUNCH_CHECK();
     }

@@ -211,11 +211,10 @@ struct AttnOperand {
     }
 };
 
-// Rows row0 .. row0 + 31 of the tile times the operand's rows.
+// c + rows row0 .. row0 + 31 of the tile times the operand's rows.
 template <typename Tile, typename T, int DP>
-__device__ inline f32x16_attn tile_product(const char* tile, int row0, const AttnOperand<T, DP>& b) {
+__device__ inline f32x16_attn tile_product(const char* tile, int row0, const AttnOperand<T, DP>& b, f32x16_attn c) {
     const int lane = lane_id();
-    f32x16_attn c = {};
 #pragma unroll
     for (int step = 0; step < AttnOperand<T, DP>::kSteps; ++step)
         c = AttnMath<T>::product(Tile::row_frag(tile, row0 + (lane & 31), step, lane >> 5), b.f[step], c);
@@ -243,6 +242,52 @@ __device__ inline bool finite_columns(const f32x16_attn (&acc)[BLOCKS], float fa
     }
     return largest < 0x7f800000u;
 }
+
+// What a lane's query sees, as a test of two instructions: lo <= j <= lo +
+// span, or a first key.
+struct AttnMask {
+    int lo, hi, sinks;
+    uint32_t span;
+    __device__ AttnMask(const lattice_attention& a, int nk, int p)
+        : lo(p - a.left), hi(min(nk - 1, p + a.right)), sinks(a.sinks), span(hi - lo) {}
+    // The scores of keys j0 + result_row(r); `first`: some are first keys.
+    __device__ void apply(f32x16_attn& x, int j0, bool first) const {
+        const int j = j0 + 4 * (lane_id() >> 5);
+        if (first) {
+            const int bound = min(sinks - 1, hi);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int at = j + 8 * (r / 4) + r % 4;
+                if (static_cast<uint32_t>(at - lo) > span && at > bound) x[r] = -INFINITY;
+            }
+        } else {
+            const uint32_t from = j - lo;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (from + 8 * (r / 4) + r % 4 > span) x[r] = -INFINITY;
+        }
+    }
+};
+
+// How the positions p_low .. p_high see the keys j0 .. j0 + count.
+enum AttnView { kSeesNone, kSeesSome, kSeesAll };
+__device__ inline AttnView attn_view(const lattice_attention& a, int nk, int p_low, int p_high, int j0, int count) {
+    const int end = j0 + count;
+    if (j0 >= nk || j0 > p_high + a.right || (end <= p_low - a.left && j0 >= a.sinks)) return kSeesNone;
+    const bool all = end <= nk && end - 1 <= p_low + a.right && (j0 >= p_high - a.left || end <= a.sinks);
+    return all ? kSeesAll : kSeesSome;
+}
+
+// r / group, with one product for the division.
+struct GroupDivide {
+    uint32_t group, magic;
+    __device__ explicit GroupDivide(uint32_t g) : group(g), magic(g > 1 ? 0xffffffffu / g + 1 : 0) {}
+    __device__ uint32_t operator()(uint32_t r) const {
+        if (group == 1) return r;
+        const uint32_t q = __umulhi(r, magic);
+        return q * group > r ? q - 1 : q;
+    }
+};
 
 // The tiles of KT keys that a range of positions sees: first those of the
 // first keys that lie before the window's, then the window's.

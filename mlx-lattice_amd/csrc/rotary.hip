@@ -75,7 +75,9 @@ __device__ inline void rotary_table(float2* table, const RotaryAxes& axes, const
     }
 }
 
-// x rows of dim = chunks * V channels, chunks <= 64.
+// x rows of dim = chunks * V channels, chunks <= 64.  A lane has a piece of a
+// row and walks the row's heads, so that its cosines and sines stay in
+// registers; the waves that are left over share the heads.
 template <typename T, int V>
 __global__ void __launch_bounds__(kRotaryBlock)
 rotary_rows(const T* __restrict__ x, long long x_row, long long x_head, int rows, int heads, int dim,
@@ -84,12 +86,11 @@ rotary_rows(const T* __restrict__ x, long long x_row, long long x_head, int rows
     typedef RowVec<T, V> Vec;
     extern __shared__ float2 table[];
     __shared__ __align__(16) T stage[kRotaryWaves][kRotaryUnroll][kWave * V];
-    const int wave = threadIdx.x / kWave, lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
     const int chunks = dim / V;
-    const int wave_heads = kWave / chunks;
+    const int wave_rows = kWave / chunks;
     const int sub = lane / chunks, c0 = (lane - sub * chunks) * V;
-    const bool used = sub < wave_heads;
-    int pair[V], from[V];
+    int from[V], pair[V];
     float turn[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -98,48 +99,53 @@ rotary_rows(const T* __restrict__ x, long long x_row, long long x_head, int rows
         from[j] = sub * dim + ch.partner;
         turn[j] = ch.sign;
     }
-    const int head_groups = (heads + wave_heads - 1) / wave_heads;
     const long long first = static_cast<long long>(blockIdx.x) * block_rows;
     const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
     rotary_table(table, axes, positions, frequencies, first, count, sign);
     __syncthreads();
-    const int items = count * head_groups;
-    for (int base = wave; base < items; base += kRotaryWaves * kRotaryUnroll) {
-        Vec in[kRotaryUnroll];
-        int row[kRotaryUnroll], head[kRotaryUnroll];
-        bool live[kRotaryUnroll];
+    const int groups = (count + wave_rows - 1) / wave_rows;
+    const int shares = max(1, kRotaryWaves / groups);  // waves a group of rows
+    for (int unit = wave; unit < groups * shares; unit += kRotaryWaves) {
+        const int row = unit / shares * wave_rows + sub;
+        const bool live = sub < wave_rows && row < count;
+        float cosine[V], sine[V];
 #pragma unroll
-        for (int u = 0; u < kRotaryUnroll; ++u) {
-            const int item = base + u * kRotaryWaves;
-            row[u] = item / head_groups;
-            head[u] = (item - row[u] * head_groups) * wave_heads + sub;
-            live[u] = item < items && used && head[u] < heads;
-            if (live[u]) in[u] = Vec::load(x + (first + row[u]) * x_row + head[u] * x_head + c0);
+        for (int j = 0; j < V; ++j) {
+            const float2 t = live && pair[j] >= 0 ? table[row * axes.pairs + pair[j]] : float2{1.0f, 0.0f};
+            cosine[j] = t.x;
+            sine[j] = turn[j] * t.y;
         }
+        const T* in = x + (first + row) * x_row + c0;
+        T* out = y + (first + row) * heads * dim + c0;
+        for (int base = unit % shares; base < heads; base += shares * kRotaryUnroll) {
+            Vec v[kRotaryUnroll];
 #pragma unroll
-        for (int u = 0; u < kRotaryUnroll; ++u)
-            if (live[u]) in[u].store(&stage[wave][u][lane * V]);
-        // The wave alone reads what it wrote, in order.
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int u = 0; u < kRotaryUnroll; ++u) {
-            if (!live[u]) continue;
-            Vec out;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (pair[j] < 0) {
-                    out.e[j] = in[u].e[j];
-                } else {
-                    const float2 t = table[row[u] * axes.pairs + pair[j]];
-                    const float other = static_cast<float>(stage[wave][u][from[j]]);
-                    out.set(j, in[u].at(j) * t.x + turn[j] * (other * t.y));
-                }
+            for (int u = 0; u < kRotaryUnroll; ++u) {
+                const int head = base + u * shares;
+                if (live && head < heads) v[u] = Vec::load(in + head * x_head);
             }
-            out.store(y + ((first + row[u]) * heads + head[u]) * dim + c0);
+#pragma unroll
+            for (int u = 0; u < kRotaryUnroll; ++u)
+                if (live && base + u * shares < heads) v[u].store(&stage[wave][u][lane * V]);
+            // The wave alone reads what it wrote, in order.
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int u = 0; u < kRotaryUnroll; ++u) {
+                const int head = base + u * shares;
+                if (!live || head >= heads) continue;
+                Vec turned;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    // Channels past the axes are copied, whatever they hold.
+                    const float other = pair[j] < 0 ? 0.0f : static_cast<float>(stage[wave][u][from[j]]);
+                    turned.set(j, v[u].at(j) * cosine[j] + other * sine[j]);
+                }
+                turned.store(out + head * dim);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
