@@ -99,53 +99,60 @@ rotary_rows(const T* __restrict__ x, long long x_row, long long x_head, int rows
         from[j] = sub * dim + ch.partner;
         turn[j] = ch.sign;
     }
-    const long long first = static_cast<long long>(blockIdx.x) * block_rows;
-    const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
-    rotary_table(table, axes, positions, frequencies, first, count, sign);
-    __syncthreads();
-    const int groups = (count + wave_rows - 1) / wave_rows;
-    const int shares = max(1, kRotaryWaves / groups);  // waves a group of rows
-    for (int unit = wave; unit < groups * shares; unit += kRotaryWaves) {
-        const int row = unit / shares * wave_rows + sub;
-        const bool live = sub < wave_rows && row < count;
-        float cosine[V], sine[V];
+    for (long long first = static_cast<long long>(blockIdx.x) * block_rows; first < rows;
+         first += static_cast<long long>(gridDim.x) * block_rows) {
+        const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
+        rotary_table(table, axes, positions, frequencies, first, count, sign);
+        __syncthreads();
+        const int groups = (count + wave_rows - 1) / wave_rows;
+        const int shares = max(1, kRotaryWaves / groups);  // waves a group of rows
+        for (int unit = wave; unit < groups * shares; unit += kRotaryWaves) {
+            const int row = unit / shares * wave_rows + sub;
+            const bool live = sub < wave_rows && row < count;
+            float cosine[V], sine[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 t = live && pair[j] >= 0 ? table[row * axes.pairs + pair[j]] : float2{1.0f, 0.0f};
-            cosine[j] = t.x;
-            sine[j] = turn[j] * t.y;
-        }
-        const T* in = x + (first + row) * x_row + c0;
-        T* out = y + (first + row) * heads * dim + c0;
-        for (int base = unit % shares; base < heads; base += shares * kRotaryUnroll) {
-            Vec v[kRotaryUnroll];
-#pragma unroll
-            for (int u = 0; u < kRotaryUnroll; ++u) {
-                const int head = base + u * shares;
-                if (live && head < heads) v[u] = Vec::load(in + head * x_head);
+            for (int j = 0; j < V; ++j) {
+                const float2 t = live && pair[j] >= 0 ? table[row * axes.pairs + pair[j]] : float2{1.0f, 0.0f};
+                cosine[j] = t.x;
+                sine[j] = turn[j] * t.y;
             }
+            const T* in = x + (first + row) * x_row + c0;
+            T* out = y + (first + row) * heads * dim + c0;
+            // Neighbouring heads, which share lines, together.
+            const int share = (heads + shares - 1) / shares;
+            const int end = min(heads, (unit % shares + 1) * share);
+            for (int base = unit % shares * share; base < end; base += kRotaryUnroll) {
+                Vec v[kRotaryUnroll];
 #pragma unroll
-            for (int u = 0; u < kRotaryUnroll; ++u)
-                if (live && base + u * shares < heads) v[u].store(&stage[wave][u][lane * V]);
-            // The wave alone reads what it wrote, in order.
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int u = 0; u < kRotaryUnroll; ++u) {
-                const int head = base + u * shares;
-                if (!live || head >= heads) continue;
-                Vec turned;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // Channels past the axes are copied, whatever they hold.
-                    const float other = pair[j] < 0 ? 0.0f : static_cast<float>(stage[wave][u][from[j]]);
-                    turned.set(j, v[u].at(j) * cosine[j] + other * sine[j]);
+                for (int u = 0; u < kRotaryUnroll; ++u) {
+                    const int head = base + u;
+                    if (live && head < end) v[u] = Vec::load(in + head * x_head);
                 }
-                turned.store(out + head * dim);
+#pragma unroll
+                for (int u = 0; u < kRotaryUnroll; ++u)
+                    if (live && base + u < end) v[u].store(&stage[wave][u][lane * V]);
+                // The wave alone reads what it wrote, in order.
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int u = 0; u < kRotaryUnroll; ++u) {
+                    const int head = base + u;
+                    if (!live || head >= end) continue;
+                    Vec turned;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float other = static_cast<float>(stage[wave][u][from[j]]);
+                        turned.set(j, v[u].at(j) * cosine[j] + other * sine[j]);
+                        // Channels past the axes are copied, whatever they hold.
+                        if (pair[j] < 0) turned.e[j] = v[u].e[j];
+                    }
+                    turned.store(out + head * dim);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
         }
+        __syncthreads();
     }
 }
 
@@ -188,9 +195,14 @@ int rotary_of(const void* x, long long x_row, long long x_head, int rows, int he
     const int block_rows = static_cast<int>(std::max<long long>(
         1, std::min<long long>(std::max(1, 512 / std::max(1, axes.pairs)), (rows + 1023ll) / 1024)));
     const unsigned grid = static_cast<unsigned>((static_cast<long long>(rows) + block_rows - 1) / block_rows);
+    // Working out a lane's eight channels of a 16-bit type is worth more than
+    // an even end: blocks that stay (five a unit) take 101 us over 200k rows of
+    // 16 heads of 32, a block for every table 107; with four channels (fp32,
+    // 60k rows of 6 heads of 64) 46 and 43.
+    const unsigned resident = sizeof(T) == 2 ? std::min(grid, 256u * 5u) : grid;
     const size_t lds = static_cast<size_t>(block_rows) * axes.pairs * sizeof(float2);
     if (row_vector<T>(dim, {x, y}, {x_row, x_head}) == kMost && dim / kMost <= kWave) {
-        rotary_rows<T, kMost><<<grid, kRotaryBlock, lds, stream>>>(in, x_row, x_head, rows, heads, dim, positions,
+        rotary_rows<T, kMost><<<resident, kRotaryBlock, lds, stream>>>(in, x_row, x_head, rows, heads, dim, positions,
                                                                    frequencies, axes, sign, block_rows, out);
     } else {
         rotary_channels<T><<<grid, kRotaryBlock, lds, stream>>>(in, x_row, x_head, rows, heads, dim, positions,
