@@ -90,7 +90,7 @@ __device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T,
 }
 
 // A tile of KT keys: at once where every row sees every key, else 32 keys at a
-// time, those that some row sees.  Heads of 128 take every tile at once: a
+// time, those that some row sees.  Heads of 96 and 128 take every tile at once: a
 // second form of the loop costs them more registers than it saves products
 // (16k causal rows, window 4096: 612 us with it, 572 without; 120k rows of
 // heads of 32, window 257: 143 with it, 171 without).
@@ -100,11 +100,11 @@ __device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>&
                                    const AttnMask& mask, int j0) {
     const AttnView view = attn_view(a, nk, w.p_low, w.p_high, j0, KT);
     if (view == kSeesNone) return;
-    if (KT > 32 && (DP >= 128 || view == kSeesAll)) {
+    if (KT > 32 && (DP >= 96 || view == kSeesAll)) {
         attend_keys<KT / 32, T, DP, KT>(state, q, keys, values, 0, scale, mask, j0, view == kSeesSome);
         return;
     }
-    if (KT > 32 && DP >= 128) return;
+    if (KT > 32 && DP >= 96) return;
     for (int row0 = 0; row0 < KT; row0 += 32) {
         const AttnView part = attn_view(a, nk, w.p_low, w.p_high, j0 + row0, 32);
         if (part != kSeesNone)
@@ -217,7 +217,7 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
 }
 
 // Waves a block for few queries: two tiles a wave fit the LDS of a unit.
-template <typename T, int DP> constexpr int few_waves() { return DP * static_cast<int>(sizeof(T)) <= 256 ? 8 : 4; }
+template <typename T, int DP> constexpr int few_waves() { return kTileDim<DP> * static_cast<int>(sizeof(T)) <= 256 ? 8 : 4; }
 
 // 32 rows a block, for few queries: each wave takes its own tiles
 // of KT keys, with no wait for the others, and the waves' parts are joined in
@@ -415,6 +415,7 @@ int attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part
     T* o = static_cast<T*>(out);
     if (a.dim <= 32) return launch_attend<T, 32>(a, l, part, o, lse, stream);
     if (a.dim <= 64) return launch_attend<T, 64>(a, l, part, o, lse, stream);
+    if (a.dim <= 96) return launch_attend<T, 96>(a, l, part, o, lse, stream);
     return launch_attend<T, 128>(a, l, part, o, lse, stream);
 }
 

@@ -35,8 +35,7 @@ inline GradLayout grad_layout(const lattice_attention& a) {
     if (a.sinks > 0 && a.sinks <= 128 && a.left < a.keys && pairs >= 512ll * std::max(1, a.sequences)) {
         l.first_slots = static_cast<int>(pairs / kFirstRows + a.sequences + 2);
         l.first_tiles = (a.sinks + 31) / 32;
-        const int dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
-        const size_t values = static_cast<size_t>(a.kv_heads) * l.first_tiles * 2 * dp * 32;
+        const size_t values = static_cast<size_t>(a.kv_heads) * l.first_tiles * 2 * attn_width(a.dim) * 32;
         l.past_values = l.first_slots * values;
         l.window_values = (a.sequences + 2) * values;
     }

@@ -111,13 +111,13 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
     const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
-    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const float scale = a.scale * kAttnLog2e;
     const AttnRows w = attn_rows(s, kv, group, t.first + 32 * wave);
     const long long row = static_cast<long long>(s.q0) + w.i;
     const long long at = row * a.heads + w.head;
     Operand q, d;
     q.load(static_cast<const T*>(a.q) + row * a.q_row_stride + w.head * a.q_head_stride, a.dim, w.valid,
-           a.scale < 0.0f);
+           false);
     d.load(grad_out + at * a.dim, a.dim, w.valid, false);
     float along = 0.0f;
     {
@@ -364,9 +364,9 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
     const bool valid = j < s.nk;
     const long long row = static_cast<long long>(s.k0) + min(j, s.nk - 1);
     AttnOperand<T, DP> k, v;
-    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, a.scale < 0.0f);
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, false);
     v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
-    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const float scale = a.scale * kAttnLog2e;
     f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
     SlopeScale<T> slopes;
     QueryTiles<T, DP, QT, kWave> source(a, s, kv, group, states, grad_out, lane);
@@ -464,10 +464,16 @@ join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2
     }
 }
 
+// Two waves a SIMD leave 256 registers a lane: enough up to heads of 96 (25k
+// rows of 8 heads of 80, window 330: 123 us, with one wave 228).  At 128 the
+// sums alone take half of them and a second wave spills (8k rows of 16 heads,
+// window 4096: 1735 us, with one wave 787; with the keys read from LDS 959).
+template <typename T, int DP> constexpr int kKeyWaves = DP <= 64 || (DP <= 96 && sizeof(T) == 2) ? 2 : 1;
+
 // grad_k and grad_v: 128 keys a block, 32 a wave, over the tiles of (query,
 // head) pairs that see them.
 template <typename T, int DP, int QT>
-__global__ void __launch_bounds__(kAttnBlock, DP <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kAttnBlock, kKeyWaves<T, DP>)
 grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
                const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
     constexpr int kBlocks = DP / 32;
@@ -487,9 +493,9 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const bool valid = j < s.nk;
     const long long row = static_cast<long long>(s.k0) + min(j, owned - 1);
     AttnOperand<T, DP> k, v;
-    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, a.scale < 0.0f);
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, false);
     v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
-    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const float scale = a.scale * kAttnLog2e;
     f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
     SlopeScale<T> slopes;
     QueryTiles<T, DP, QT, kAttnBlock> source(a, s, kv, group, states, grad_out, threadIdx.x);
@@ -612,6 +618,7 @@ int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out
     T* dv = static_cast<T*>(grad_v);
     if (a.dim <= 32) return launch_grad<T, 32>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
     if (a.dim <= 64) return launch_grad<T, 64>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
+    if (a.dim <= 96) return launch_grad<T, 96>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
     return launch_grad<T, 128>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
 }
 

@@ -50,6 +50,11 @@ template <> struct AttnMath<float> {
     }
 };
 
+// Kernels are made for heads of up to DP = 32, 64, 96 and 128 channels; a
+// tile's rows lie a power of two apart.
+inline int attn_width(int dim) { return (dim + 31) / 32 * 32; }
+template <int DP> constexpr int kTileDim = DP == 96 ? 128 : DP;
+
 // ROWS rows of DP channels (zeros past the channels there are) in LDS, in
 // 16-byte pieces.  LDS serves 256 bytes a cycle from 64 banks: 16 lanes that
 // read a piece each of 16 rows, or 32 that read 64 bytes of each of 4 rows
@@ -58,7 +63,7 @@ template <> struct AttnMath<float> {
 template <typename T, int DP, int ROWS>
 struct AttnTile {
     typedef typename AttnMath<T>::Frag Frag;
-    static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+    static constexpr int kRowBytes = kTileDim<DP> * static_cast<int>(sizeof(T));
     static constexpr int kPieces = kRowBytes / 16;
     static constexpr int kBytes = ROWS * kRowBytes;
     static constexpr int kElems = 16 / static_cast<int>(sizeof(T));
