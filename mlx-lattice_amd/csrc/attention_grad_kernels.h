@@ -472,8 +472,8 @@ template <typename T, int DP> constexpr int kKeyWaves = DP <= 64 || (DP <= 96 &&
 
 // grad_k and grad_v: 128 keys a block, 32 a wave, over the tiles of (query,
 // head) pairs that see them.
-template <typename T, int DP, int QT>
-__global__ void __launch_bounds__(kAttnBlock, kKeyWaves<T, DP>)
+template <typename T, int DP, int QT, int WAVES>
+__global__ void __launch_bounds__(kAttnBlock, WAVES)
 grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
                const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
     constexpr int kBlocks = DP / 32;
@@ -591,7 +591,7 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
     constexpr size_t kLds =
         std::max<size_t>(2 * QueryTile<T, DP, kTile>::kBytes, kAttnWaves * sizeof(AttnRowScratch));
     static_assert(kLds <= 160 * 1024);
-    const auto kernel = grad_key_tiles<T, DP, kTile>;
+    const auto kernel = grad_key_tiles<T, DP, kTile, kKeyWaves<T, DP>>;
     LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
     const long long slots = a.keys / (32 * kAttnWaves) + a.sequences + 2;
     kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
