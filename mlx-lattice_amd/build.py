@@ -37,6 +37,7 @@ HOST_SOURCES = [
     'native/features/pooling/pooling.cpp',
     'native/features/quantization/quantization.cpp',
     'native/features/transformer/transformer.cpp',
+    'native/features/transformer/autograd.cpp',
     'native/bindings/module.cpp',
 ]
 

@@ -77,24 +77,5 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     window = (left, right, int(sinks), float(scale))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or v.requires_grad):
-        return _WindowAttention.apply(q, k, v, *layout, window)
+        return ext.window_attention_node(q, k, v, *layout, *window)
     return ext.window_attention(q, k, v, *layout, *window, False)[0]
-
-
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, offsets, key_offsets, key_lengths, window):
-        out, lse = ext.window_attention(q, k, v, offsets, key_offsets,
-                                        key_lengths, *window, True)
-        ctx.save_for_backward(q, k, v, out, lse, offsets, key_offsets,
-                              key_lengths)
-        ctx.window = window
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        q, k, v, out, lse, *layout = ctx.saved_tensors
-        grads = ext.window_attention_grad(grad_out, out, lse, q, k, v, *layout,
-                                          *ctx.window)
-        return (*grads, None, None, None, None)

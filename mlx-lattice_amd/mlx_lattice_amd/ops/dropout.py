@@ -43,19 +43,5 @@ def dropout(x: SparseTensor | torch.Tensor, p: float, *, seed: int,
     key = (int(seed) & _WORD, int(offset) & _WORD, threshold, scale)
     if torch.is_grad_enabled() and (
             x.requires_grad or residual is not None and residual.requires_grad):
-        return _Dropout.apply(x, residual, key)
+        return ext.dropout_node(x, residual, *key)
     return ext.dropout(x, residual, *key)
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, key):
-        ctx.key = key
-        return ext.dropout(x, residual, *key)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        need_x, need_residual, _ = ctx.needs_input_grad
-        return (ext.dropout(grad_y, None, *ctx.key) if need_x else None,
-                grad_y if need_residual else None, None)

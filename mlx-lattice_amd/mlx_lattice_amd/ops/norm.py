@@ -29,25 +29,8 @@ def layer_norm(x: SparseTensor | torch.Tensor,
             raise ValueError('a sparse tensor has its own active_rows.')
         return x.replace(feats=layer_norm(x.feats, weight, bias, eps=eps,
                                           active_rows=x.active_rows))
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNorm.apply(x, weight, bias, eps, active_rows)
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight is not None and weight.requires_grad
+            or bias is not None and bias.requires_grad):
+        return ext.layer_norm_node(x, weight, bias, eps, active_rows)
     return ext.layer_norm(x, weight, bias, eps, active_rows, False)[0]
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, active_rows):
-        y, statistics = ext.layer_norm(x, weight, bias, eps, active_rows, True)
-        ctx.save_for_backward(x, weight, statistics, active_rows)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        x, weight, statistics, active_rows = ctx.saved_tensors
-        _, need_weight, need_bias, _, _ = ctx.needs_input_grad
-        grad_x, grad_weight, grad_bias = ext.layer_norm_grad(
-            grad_y, x, weight, statistics, active_rows, need_weight, need_bias)
-        return (grad_x, grad_weight if need_weight else None,
-                grad_bias if need_bias else None, None, None)

@@ -40,24 +40,7 @@ def rotary_positions(x: torch.Tensor, positions: torch.Tensor,
     """
     dims = [int(d) for d in dims]
     if torch.is_grad_enabled() and x.requires_grad:
-        return _RotaryPositions.apply(x, positions, frequencies, dims,
-                                      interleaved)
+        return ext.rotary_positions_node(x, positions, frequencies, dims,
+                                         interleaved)
     return ext.rotary_positions(x, positions, frequencies, dims, interleaved,
                                 False)
-
-
-class _RotaryPositions(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, frequencies, dims, interleaved):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.layout = (dims, interleaved)
-        return ext.rotary_positions(x, positions, frequencies, dims,
-                                    interleaved, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        positions, frequencies = ctx.saved_tensors
-        return (ext.rotary_positions(grad_y, positions, frequencies,
-                                     *ctx.layout, True),
-                None, None, None, None)

@@ -427,4 +427,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("key_offsets"),
           py::arg("key_lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"), py::arg("scale"),
           "Gradients of the windowed attention: (grad_q, grad_k, grad_v).");
+    m.def("layer_norm_node", &ln::layer_norm_node, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),
+          py::arg("active_rows"), "layer_norm as a differentiable node.");
+    m.def("dropout_node", &ln::dropout_node, py::arg("x"), py::arg("residual"), py::arg("seed"), py::arg("offset"),
+          py::arg("threshold"), py::arg("scale"), "dropout as a differentiable node.");
+    m.def("rotary_positions_node", &ln::rotary_positions_node, py::arg("x"), py::arg("positions"),
+          py::arg("frequencies"), py::arg("dims"), py::arg("interleaved"),
+          "rotary_positions as a differentiable node.");
+    m.def("window_attention_node", &ln::window_attention_node, py::arg("q"), py::arg("k"), py::arg("v"),
+          py::arg("offsets"), py::arg("key_offsets"), py::arg("key_lengths"), py::arg("left"), py::arg("right"),
+          py::arg("sinks"), py::arg("scale"), "window_attention as a differentiable node.");
 }

@@ -82,7 +82,8 @@ std::tuple<at::Tensor, at::Tensor> layer_norm(const at::Tensor& x_in, const c10:
     const at::Tensor x = unit_rows(x_in);
     const int rows = row_count(x, "x");
     at::Tensor y = at::empty(x.sizes(), x.options());
-    at::Tensor statistics = at::empty({keep_statistics ? rows : 0, 2}, x.options().dtype(at::kFloat));
+    at::Tensor statistics;
+    if (keep_statistics) statistics = at::empty({rows, 2}, x.options().dtype(at::kFloat));
     check_status(lattice_hip_layer_norm(dtype, x.data_ptr(), row_stride(x), rows, static_cast<int>(x.size(1)),
                                         or_null(weight), or_null(bias), static_cast<float>(eps), active, y.data_ptr(),
                                         keep_statistics ? statistics.data_ptr<float>() : nullptr, current_stream(x)));
@@ -110,8 +111,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor&
     const at::Tensor x = unit_rows(x_in), dy = unit_rows(grad_y);
     const int rows = row_count(x, "x"), channels = static_cast<int>(x.size(1));
     at::Tensor dx = at::empty(x.sizes(), x.options());
-    at::Tensor dw = at::empty({grad_weight ? channels : 0}, x.options());
-    at::Tensor db = at::empty({grad_bias ? channels : 0}, x.options());
+    at::Tensor dw, db;
+    if (grad_weight) dw = at::empty({channels}, x.options());
+    if (grad_bias) db = at::empty({channels}, x.options());
     at::Tensor ws;
     size_t bytes = 0;
     if (grad_weight || grad_bias) {
@@ -120,8 +122,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor&
     }
     check_status(lattice_hip_layer_norm_grad(
         dtype, dy.data_ptr(), row_stride(dy), x.data_ptr(), row_stride(x), rows, channels, or_null(weight),
-        statistics.data_ptr<float>(), active, dx.data_ptr(), grad_weight ? dw.data_ptr() : nullptr,
-        grad_bias ? db.data_ptr() : nullptr, or_null(ws), bytes, current_stream(x)));
+        statistics.data_ptr<float>(), active, dx.data_ptr(), or_null(dw), or_null(db), or_null(ws), bytes, current_stream(x)));
     return {dx, dw, db};
 }
 
@@ -294,7 +295,8 @@ std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q, const a
     const c10::OptionalDeviceGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
     const Attention a = attention_of(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
     at::Tensor out = at::empty(a.q.sizes(), q.options());
-    at::Tensor lse = at::empty({keep_lse ? q.size(0) : 0, q.size(1)}, q.options().dtype(at::kFloat));
+    at::Tensor lse;
+    if (keep_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
     const size_t bytes = lattice_hip_window_attention_workspace_bytes(&a.args);
     at::Tensor ws;
     if (bytes) ws = workspace(bytes, q);

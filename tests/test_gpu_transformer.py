@@ -182,6 +182,42 @@ def test_attention_after_a_strided_conv():
         ops.batch_offsets(down, 0)
 
 
+def test_gradients_cannot_be_differentiated_again():
+    """With create_graph the first gradients are as ever; a second
+    differentiation says that it cannot."""
+    import mlx_lattice_amd.ops as ops
+
+    x = torch.randn((12, 2, 16), device='cuda', requires_grad=True)
+    at = torch.tensor([0, 12], dtype=torch.int32, device='cuda')
+    places = torch.arange(12, dtype=torch.int32, device='cuda')[:, None]
+    frequencies = ops.rotary_frequencies((16,), device='cuda')
+    for call in (lambda: ops.window_attention(x, x, x, offsets=at),
+                 lambda: ops.rotary_positions(x, places, frequencies,
+                                              dims=(16,)),
+                 lambda: ops.layer_norm(x.view(12, 32)),
+                 lambda: ops.dropout(x, 0.5, seed=1)):
+        out = call()
+        dy = torch.ones_like(out)
+        plain, = torch.autograd.grad(call(), x, dy)
+        kept, = torch.autograd.grad(out, x, dy, create_graph=True)
+        assert torch.equal(plain, kept.detach())
+        with pytest.raises(RuntimeError, match='differentiated once'):
+            kept.square().sum().backward()
+
+
+def test_only_the_gradients_asked_for():
+    import mlx_lattice_amd.ops as ops
+
+    x, y = (torch.randn((9, 8), device='cuda', requires_grad=True)
+            for _ in range(2))
+    w = torch.ones(8, device='cuda', requires_grad=True)
+    out = ops.dropout(ops.layer_norm(x.detach(), w), 0.25, seed=2, residual=y)
+    dw, dy = torch.autograd.grad(out.sum(), (w, y))
+    assert dw.shape == w.shape and torch.equal(dy, torch.ones_like(y))
+    ops.layer_norm(x, None, w).sum().backward()
+    assert torch.equal(w.grad, torch.full_like(w, 9.0))
+
+
 def test_refusals():
     import mlx_lattice_amd.nn as lnn
 
