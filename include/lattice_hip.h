@@ -809,8 +809,8 @@ int lattice_hip_rotary_positions(int dtype, const void* x,
  * zero.  What a row does not see never reaches it, whatever its value.
  * q [queries, heads, dim], k and v [keys, kv_heads, dim]: strides in
  * elements, unit stride in dim, rows in whole 16-byte pieces on 16-byte
- * boundaries, row strides under 16 MiB; dim up to 128.  Head h reads key
- * head h * kv_heads / heads.
+ * boundaries, rows under 4 MiB apart and the query heads of a key head within
+ * 512 MiB; dim up to 128.  Head h reads key head h * kv_heads / heads.
  * Offsets are device int32 and clamped to the rows there are. */
 typedef struct lattice_attention {
     int dtype, queries, keys, heads, kv_heads, dim, sequences;

@@ -303,8 +303,13 @@ inline const char* attn_fault(const lattice_attention* a) {
                                  a->k_head_stride, a->v_row_stride, a->v_head_stride};
     for (long long s : strides)
         if (s < 0 || s % piece != 0) return "attention strides must be whole 16-byte pieces.";
-    if (std::max({a->q_row_stride, a->k_row_stride, a->v_row_stride}) >= piece << 20)
-        return "attention row strides must be under 16 MiB.";
+    // Within a tile, places are counted in 32 bits: rows of a tile and the heads
+    // of a group lie within 2^30 bytes.
+    if (std::max({a->q_row_stride, a->k_row_stride, a->v_row_stride, static_cast<long long>(a->heads) * a->dim}) >=
+        piece << 18)
+        return "attention rows must be under 4 MiB apart.";
+    if (a->q_head_stride >= (piece << 25) / (a->heads / a->kv_heads))
+        return "the query heads of a key head must lie within 512 MiB.";
     if (a->dim % piece != 0) return "attention rows must be whole 16-byte pieces.";
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) %
         16 != 0)

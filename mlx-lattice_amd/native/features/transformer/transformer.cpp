@@ -191,18 +191,20 @@ namespace {
 
 int64_t piece_of(const at::Tensor& t) { return 16 / t.element_size(); }
 
-bool in_pieces(const at::Tensor& t) {
+// group: heads that are read together.
+bool in_pieces(const at::Tensor& t, int64_t group) {
     const int64_t piece = piece_of(t);
-    return t.stride(2) == 1 && (t.size(0) <= 1 || (t.stride(0) % piece == 0 && t.stride(0) < piece << 20)) &&
-           (t.size(1) <= 1 || t.stride(1) % piece == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return t.stride(2) == 1 && (t.size(0) <= 1 || (t.stride(0) % piece == 0 && t.stride(0) < piece << 18)) &&
+           (t.size(1) <= 1 || (t.stride(1) % piece == 0 && t.stride(1) < (piece << 25) / group)) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
-// Heads of whole 16-byte pieces on 16-byte boundaries: `t` itself, or a copy
-// with the channels padded by zeros, which add nothing to a product.
-at::Tensor pieces(const at::Tensor& t) {
+// Heads of whole 16-byte pieces on 16-byte boundaries, not too far apart: `t`
+// itself, or a copy with the channels padded by zeros, which add nothing to a
+// product.
+at::Tensor pieces(const at::Tensor& t, int64_t group = 1) {
     const int64_t piece = piece_of(t), dim = t.size(2), padded = (dim + piece - 1) / piece * piece;
     if (padded != dim) return at::constant_pad_nd(t, {0, padded - dim}).contiguous();
-    if (t.numel() == 0 || in_pieces(t)) return t;
+    if (t.numel() == 0 || in_pieces(t, group)) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -247,7 +249,7 @@ Attention attention_of(const at::Tensor& q, const at::Tensor& k, const at::Tenso
         lengths = ci32(*key_lengths);
     }
     constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
-    Attention a{{}, pieces(q), pieces(k), pieces(v)};
+    Attention a{{}, pieces(q, q.size(1) / k.size(1)), pieces(k), pieces(v)};
     const auto head_stride = [](const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; };
     a.args.dtype = dtype;
     a.args.queries = row_count(q, "q");

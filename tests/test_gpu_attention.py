@@ -290,6 +290,62 @@ def test_cache_past_32_bits():
         assert_within(got, ref, bound)
 
 
+@pytest.mark.parametrize('dim', (32, 128))
+def test_rows_and_heads_far_apart(dim):
+    """Query heads and rows that no tile's 32-bit places reach."""
+    gen = torch.Generator(device='cuda').manual_seed(11)
+    store = torch.zeros(5 << 28, dtype=torch.float16, device='cuda')
+    q = store.as_strided((70, 4, dim), (dim, 1 << 28, 1))
+    k = store[1 << 20:].as_strided((70, 2, dim), (1 << 23, dim, 1))
+    for t in (q, k):
+        t.copy_(_normal(gen, torch.float16, *t.shape))
+    v = _normal(gen, torch.float16, 70, 2, dim)
+    dy = _normal(gen, torch.float16, 70, 4, dim)
+    _check(q, k, v, dy, [(0, 70, 0, 70)], 20, 3, 2, offsets=_offsets((70,)))
+
+
+@pytest.mark.parametrize('dtype, dim', ((torch.float32, 128),
+                                        (torch.float16, 128),
+                                        (torch.bfloat16, 32)))
+def test_captured_graph_replays(dtype, dim):
+    """Forward and gradients, few queries and many, in a captured graph whose
+    inputs change between replays."""
+    from mlx_lattice_amd._native import ext
+
+    gen = torch.Generator(device='cuda').manual_seed(12)
+    q, dy = (torch.zeros((700, 4, dim), dtype=dtype, device='cuda')
+             for _ in range(2))
+    k, v = (torch.zeros((700, 2, dim), dtype=dtype, device='cuda')
+            for _ in range(2))
+    at, token = _offsets((300, 400)), _offsets((1, 1))
+    window = (60, 10, 2, dim ** -0.5)
+
+    def passes():
+        out, lse = ext.window_attention(q, k, v, at, at, None, *window, True)
+        grads = ext.window_attention_grad(dy, out, lse, q, k, v, at, at, None,
+                                          *window)
+        few = _ops().window_attention(q[:2], k, v, offsets=token,
+                                      key_offsets=at)
+        return [out, *grads, few]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = passes()
+    for _ in range(3):
+        for t in (q, k, v, dy):
+            t.copy_(_normal(gen, dtype, *t.shape))
+        want = passes()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, eager in zip(captured, want):
+            assert torch.equal(got, eager)
+
+
 def test_other_stream():
     gen = torch.Generator(device='cuda').manual_seed(9)
     q, k, v, dy = (_normal(gen, torch.float16, 500, h, 32)
