@@ -57,7 +57,7 @@ __device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T,
     typedef AttnTile<T, DP, KT> Tile;
     f32x16_attn s[PARTS];
 #pragma unroll
-    for (int part = 0; part < PARTS; ++part) 
+    for (int part = 0; part < PARTS; ++part)
         s[part] = tile_product<Tile, T, DP>(keys, row0 + 32 * part, q, f32x16_attn{});
     if (masked) {
 #pragma unroll
@@ -89,26 +89,26 @@ __device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T,
     for (int part = 0; part < PARTS; ++part) add_columns<Tile, T>(state.acc, values, row0 + 32 * part, s[part]);
 }
 
-// A tile of KT keys: at once where every row sees every key, else 32 keys at a
-// time, those that some row sees.  Heads of 96 and 128 take every tile at once: a
-// second form of the loop costs them more registers than it saves products
-// (16k causal rows, window 4096: 612 us with it, 572 without; 120k rows of
-// heads of 32, window 257: 143 with it, 171 without).
+// A tile of KT keys: 32 at a time, those that some row sees; in one step for
+// heads of 96 and 128, whose sums leave registers for two waves a SIMD either
+// way.  (120k rows of heads of 32, window 257: 131 us, 171 in one step; 60k rows
+// of heads of 64, window 513: 67 and 74; 16k causal rows of heads of 128, window
+// 4096: 612 and 572.  A form of each, by what the rows see, costs registers:
+// 143, 74, 612.)
 template <typename T, int DP, int KT>
 __device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>& state, const AttnOperand<T, DP>& q,
                                    const char* keys, const char* values, float scale, int nk, const AttnRows& w,
                                    const AttnMask& mask, int j0) {
     const AttnView view = attn_view(a, nk, w.p_low, w.p_high, j0, KT);
     if (view == kSeesNone) return;
-    if (KT > 32 && (DP >= 96 || view == kSeesAll)) {
+    if constexpr (KT > 32 && DP >= 96) {
         attend_keys<KT / 32, T, DP, KT>(state, q, keys, values, 0, scale, mask, j0, view == kSeesSome);
-        return;
-    }
-    if (KT > 32 && DP >= 96) return;
-    for (int row0 = 0; row0 < KT; row0 += 32) {
-        const AttnView part = attn_view(a, nk, w.p_low, w.p_high, j0 + row0, 32);
-        if (part != kSeesNone)
-            attend_keys<1, T, DP, KT>(state, q, keys, values, row0, scale, mask, j0 + row0, part == kSeesSome);
+    } else {
+        for (int row0 = 0; row0 < KT; row0 += 32) {
+            const AttnView part = attn_view(a, nk, w.p_low, w.p_high, j0 + row0, 32);
+            if (part != kSeesNone)
+                attend_keys<1, T, DP, KT>(state, q, keys, values, row0, scale, mask, j0 + row0, part == kSeesSome);
+        }
     }
 }
 

@@ -62,6 +62,36 @@ __device__ inline void add_slopes(f32x16_attn (&acc)[BLOCKS], SlopeScale<T>& sca
     add_columns<Tile, T>(acc, tile, row0, ds);
 }
 
+// Adds the waves' sums pairwise into the first wave's; `lds` holds half of the
+// waves'.
+template <int BLOCKS>
+__device__ inline void join_waves(f32x16_attn (&acc)[BLOCKS], float* lds, int wave) {
+    const int lane = lane_id();
+    constexpr int kValues = BLOCKS * 16 * kWave;
+#pragma unroll
+    for (int active = kAttnWaves / 2; active > 0; active /= 2) {
+        __syncthreads();
+        if (wave >= active && wave < 2 * active) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    lds[(wave - active) * kValues + (b * 16 + r) * kWave + lane] = acc[b][r];
+            }
+        }
+        __syncthreads();
+        if (wave < active) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[b][r] += lds[wave * kValues + (b * 16 + r) * kWave + lane];
+            }
+        }
+    }
+    __syncthreads();
+}
+template <int DP> constexpr size_t kJoinBytes = kAttnWaves / 2 * (DP / 32) * 16 * kWave * sizeof(float);
+
 // Stores column n of acc times `factor` into row n's `to` (dim channels);
 // lanes without a row pass valid = false.
 template <typename T, int BLOCKS>
@@ -96,7 +126,9 @@ __device__ inline long long query_state(const lattice_attention& a, uint32_t gro
 }
 
 // grad_q, laid out as the forward pass; keeps lse and delta for the keys' pass.
-template <typename T, int DP, int KT>
+// FEW: 32 rows a block, whose tiles the waves take in turn, each with its own
+// copies; their sums are joined.
+template <typename T, int DP, int KT, bool FEW>
 __global__ void __launch_bounds__(kAttnBlock, DP <= 64 || sizeof(T) == 2 ? 2 : 1)
 grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __restrict__ lse,
                  const T* __restrict__ grad_out, T* __restrict__ grad_q, float2* __restrict__ states) {
@@ -108,11 +140,12 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
     const int half = lane_id() >> 5;
     const uint32_t group = a.heads / a.kv_heads;
     const int kv = blockIdx.y;
-    const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
+    constexpr int kRows = FEW ? 32 : 32 * kAttnWaves;
+    const AttnSlot t = attn_slot<kRows>(a, group, blockIdx.x);
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
     const float scale = a.scale * kAttnLog2e;
-    const AttnRows w = attn_rows(s, kv, group, t.first + 32 * wave);
+    const AttnRows w = attn_rows(s, kv, group, t.first + (FEW ? 0 : 32 * wave));
     const long long row = static_cast<long long>(s.q0) + w.i;
     const long long at = row * a.heads + w.head;
     Operand q, d;
@@ -132,24 +165,31 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
         along += other_half(along);
     }
     const float log_sum = w.valid ? lse[at] : INFINITY;
-    if (w.valid && half == 0) states[query_state(a, group, row, w.head)] = float2{log_sum, along};
+    if (w.valid && half == 0 && (!FEW || wave == 0))
+        states[query_state(a, group, row, w.head)] = float2{log_sum, along};
     const AttnMask mask(a, s.nk, w.p);
     f32x16_attn acc[kBlocks] = {};
     SlopeScale<T> slopes;
     const int p_low = static_cast<int>(t.first / group) + s.shift();
-    const int p_high = static_cast<int>((min(t.first + 32 * kAttnWaves, t.rows) - 1) / group) + s.shift();
+    const int p_high = static_cast<int>((min(t.first + kRows, t.rows) - 1) / group) + s.shift();
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, p_low, p_high);
-    const KeyTiles<T, DP, KT, kAttnBlock> source(a, s, kv, threadIdx.x);
-    const auto copy = [&](int index) {
-        source.copy(shared + (index & 1) * 2 * Tile::kBytes, tiles.tile(index) * KT, s.nk);
-    };
-    if (tiles.count) copy(0);
-    __syncthreads();
-    for (int index = 0; index < tiles.count; ++index) {
-        if (index + 1 < tiles.count) copy(index + 1);
+    constexpr int kThreads = FEW ? kWave : kAttnBlock, kStep = FEW ? kAttnWaves : 1;
+    const KeyTiles<T, DP, KT, kThreads> source(a, s, kv, FEW ? lane_id() : threadIdx.x);
+    if constexpr (!FEW) {
+        if (tiles.count) source.copy(shared, tiles.tile(0) * KT, s.nk);
+        __syncthreads();
+    }
+    for (int index = FEW ? wave : 0; index < tiles.count; index += kStep) {
         const int j0 = tiles.tile(index) * KT;
-        const char* k_tile = shared + (index & 1) * 2 * Tile::kBytes;
+        char* k_tile = shared + (FEW ? wave : index & 1) * 2 * Tile::kBytes;
         const char* v_tile = k_tile + Tile::kBytes;
+        if constexpr (FEW) {
+            source.copy(k_tile, j0, s.nk);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wave_fence();
+        } else if (index + 1 < tiles.count) {
+            source.copy(shared + ((index + 1) & 1) * 2 * Tile::kBytes, tiles.tile(index + 1) * KT, s.nk);
+        }
 #pragma unroll
         for (int row0 = 0; row0 < KT; row0 += 32) {
             const AttnView view = attn_view(a, s.nk, w.p_low, w.p_high, j0 + row0, 32);
@@ -162,12 +202,19 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
                 dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
             add_slopes<Tile, T>(acc, slopes, k_tile, row0, dp);
         }
-        __syncthreads();
+        if constexpr (FEW)
+            wave_fence();
+        else
+            __syncthreads();
+    }
+    if constexpr (SlopeScale<T>::kUsed) scale_sums(acc, 1.0f / slopes.factor());
+    if constexpr (FEW) {
+        join_waves(acc, reinterpret_cast<float*>(shared), wave);
+        if (wave != 0) return;
     }
     // A row that is not finite is made again from what it sees alone.
-    const float factor = a.scale / slopes.factor();
-    uint32_t again = spoilt_columns(w.valid, finite_columns(acc, factor));
-    store_columns(acc, factor, grad_q + at * a.dim, a.dim, w.valid && !(again >> (lane_id() & 31) & 1));
+    uint32_t again = spoilt_columns(w.valid, finite_columns(acc, a.scale));
+    store_columns(acc, a.scale, grad_q + at * a.dim, a.dim, w.valid && !(again >> (lane_id() & 31) & 1));
     while (again) {
         const int n = __ffs(again) - 1;
         again &= again - 1;
@@ -377,31 +424,16 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
     char* tile = shared + wave * Queries::kBytes;
     for (uint32_t base = from; base < to; base += QT * kAttnWaves) {
         const uint32_t r0 = base + QT * wave;
-        __syncthreads();
-        if (r0 < to) source.store(tile, source.copy(tile, r0, to));
-        __syncthreads();
-        if (r0 < to) {
-            add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, true, acc_k, acc_v, slopes);
-        }
+        if (r0 >= to) break;
+        source.store(tile, source.copy(tile, r0, to));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wave_fence();
+        add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, true, acc_k, acc_v, slopes);
+        wave_fence();
     }
-    scale_sums(acc_k, 1.0f / slopes.factor());
-    // The waves' sums are added in wave order.
-    float* sums = reinterpret_cast<float*>(shared);
-    for (int u = 1; u < kAttnWaves; ++u) {
-        __syncthreads();
-        if (wave == u) store_part(sums, acc_k, acc_v);
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    acc_k[b][r] += sums[(b * 16 + r) * kWave + lane];
-                    acc_v[b][r] += sums[((kBlocks + b) * 16 + r) * kWave + lane];
-                }
-            }
-        }
-    }
+    if constexpr (SlopeScale<T>::kUsed) scale_sums(acc_k, 1.0f / slopes.factor());
+    join_waves(acc_k, reinterpret_cast<float*>(shared), wave);
+    join_waves(acc_v, reinterpret_cast<float*>(shared), wave);
     if (wave == 0) store_part(parts.past_of(a, blockIdx.x, kv, blockIdx.z, kFirstValues<DP>), acc_k, acc_v);
 }
 
@@ -471,13 +503,14 @@ join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2
 template <typename T, int DP> constexpr int kKeyWaves = DP <= 64 || (DP <= 96 && sizeof(T) == 2) ? 2 : 1;
 
 // grad_k and grad_v: 128 keys a block, 32 a wave, over the tiles of (query,
-// head) pairs that see them.
-template <typename T, int DP, int QT, int WAVES>
+// head) pairs that see them.  FEW: 32 keys a block, whose tiles the waves take in
+// turn, each with its own copies; their sums are joined.
+template <typename T, int DP, int QT, bool FEW, int WAVES>
 __global__ void __launch_bounds__(kAttnBlock, WAVES)
 grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
                const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
     constexpr int kBlocks = DP / 32;
-    constexpr int kKeys = 32 * kAttnWaves;
+    constexpr int kKeys = FEW ? 32 : 32 * kAttnWaves, kThreads = FEW ? kWave : kAttnBlock;
     typedef QueryTile<T, DP, QT> Queries;
     extern __shared__ __align__(128) char shared[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
@@ -489,7 +522,7 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const int owned = max(0, key_rows(a).start(e + 1) - s.k0);
     const int j0 = static_cast<int>(blockIdx.x - slot_of(s.k0, e)) * kKeys;
     if (j0 >= owned) return;
-    const int j_wave = j0 + 32 * wave, j = j_wave + (lane & 31);
+    const int j_wave = j0 + (FEW ? 0 : 32 * wave), j = j_wave + (lane & 31);
     const bool valid = j < s.nk;
     const long long row = static_cast<long long>(s.k0) + min(j, owned - 1);
     AttnOperand<T, DP> k, v;
@@ -498,7 +531,7 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const float scale = a.scale * kAttnLog2e;
     f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
     SlopeScale<T> slopes;
-    QueryTiles<T, DP, QT, kAttnBlock> source(a, s, kv, group, states, grad_out, threadIdx.x);
+    QueryTiles<T, DP, QT, kThreads> source(a, s, kv, group, states, grad_out, FEW ? lane : threadIdx.x);
     const uint32_t rows = s.nq * group;
     // The pairs whose window holds a key of the block.
     const int i_from = max(0, j0 - a.right - s.shift());
@@ -516,14 +549,23 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const auto first_row = [&](int index) {
         return (index < window_tiles ? from + index : past + (index - window_tiles)) * QT;
     };
-    if (count > 0) source.store(shared, source.copy(shared, first_row(0), rows));
-    __syncthreads();
-    for (int index = 0; index < count; ++index) {
+    constexpr int kStep = FEW ? kAttnWaves : 1;
+    if constexpr (!FEW) {
+        if (count > 0) source.store(shared, source.copy(shared, first_row(0), rows));
+        __syncthreads();
+    }
+    for (int index = FEW ? wave : 0; index < count; index += kStep) {
+        char* tile = shared + (FEW ? wave : index & 1) * Queries::kBytes;
         char* next = shared + ((index + 1) & 1) * Queries::kBytes;
-        typename QueryTiles<T, DP, QT, kAttnBlock>::State state{};
-        if (index + 1 < count) state = source.copy(next, first_row(index + 1), rows);
-        const char* tile = shared + (index & 1) * Queries::kBytes;
+        typename QueryTiles<T, DP, QT, kThreads>::State state{};
         const uint32_t r0 = first_row(index);
+        if constexpr (FEW) {
+            source.store(tile, source.copy(tile, r0, rows));
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wave_fence();
+        } else if (index + 1 < count) {
+            state = source.copy(next, first_row(index + 1), rows);
+        }
         // In the window, or past it: of the first keys alone.
         const bool outside = index >= window_tiles;
         const int lo = !outside ? j - a.right : j < a.sinks ? j + a.left + 1 : INT_MAX;
@@ -534,10 +576,19 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
                                   : p_high < j_wave - a.right || p_low > j_wave + 31 + a.left;
         const bool all = !outside && j_wave + 31 <= p_low + a.right && j_wave >= p_high - a.left;
         if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, !all, acc_k, acc_v, slopes);
-        if (index + 1 < count) source.store(next, state);
-        __syncthreads();
+        if constexpr (FEW) {
+            wave_fence();
+        } else {
+            if (index + 1 < count) source.store(next, state);
+            __syncthreads();
+        }
     }
-    scale_sums(acc_k, 1.0f / slopes.factor());
+    if constexpr (SlopeScale<T>::kUsed) scale_sums(acc_k, 1.0f / slopes.factor());
+    if constexpr (FEW) {
+        join_waves(acc_k, reinterpret_cast<float*>(shared), wave);
+        join_waves(acc_v, reinterpret_cast<float*>(shared), wave);
+        if (wave != 0) return;
+    }
     const int first_keys = parts.tiles ? min(a.sinks, s.nk) : 0;
     if (j_wave < first_keys) store_part(parts.window_of(a, e, kv, j_wave / 32, kFirstValues<DP>), acc_k, acc_v);
     // Keys past the sequence's get zeros; a key whose sums are not finite is
@@ -562,25 +613,55 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     }
 }
 
+template <typename T, int DP, bool FEW>
+int launch_grad_query(const lattice_attention& a, const T* out, const float* lse, const T* grad_out, T* grad_q,
+                      float2* states, hipStream_t stream) {
+    constexpr int kTile = sizeof(T) == 2 && !FEW ? 64 : 32, kRows = FEW ? 32 : 32 * kAttnWaves;
+    constexpr size_t kLds = std::max({(FEW ? kAttnWaves : 2) * size_t{2} * AttnTile<T, DP, kTile>::kBytes,
+                                      FEW ? kJoinBytes<DP> : 0, kAttnWaves * sizeof(AttnRowScratch)});
+    static_assert(kLds <= 160 * 1024);
+    const auto kernel = grad_query_tiles<T, DP, kTile, FEW>;
+    LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
+    const long long slots = static_cast<long long>(a.queries) * (a.heads / a.kv_heads) / kRows + a.sequences + 2;
+    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, lse, grad_out, grad_q,
+                                                                                        states);
+    LATTICE_LAUNCH_CHECK();
+    return LATTICE_OK;
+}
+
+template <typename T, int DP, bool FEW>
+int launch_grad_keys(const lattice_attention& a, const float* lse, const float2* states, const T* grad_out,
+                     const FirstParts& parts, T* grad_k, T* grad_v, hipStream_t stream) {
+    constexpr int kTile = sizeof(T) == 2 && !FEW ? 64 : 32, kKeys = FEW ? 32 : 32 * kAttnWaves;
+    constexpr size_t kLds = std::max({(FEW ? kAttnWaves : 2) * size_t{QueryTile<T, DP, kTile>::kBytes},
+                                      FEW ? kJoinBytes<DP> : 0, kAttnWaves * sizeof(AttnRowScratch)});
+    static_assert(kLds <= 160 * 1024);
+    const auto kernel = grad_key_tiles<T, DP, kTile, FEW, FEW ? 1 : kKeyWaves<T, DP>>;
+    LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
+    const long long slots = a.keys / kKeys + a.sequences + 2;
+    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
+                                                                                        parts, grad_k, grad_v);
+    LATTICE_LAUNCH_CHECK();
+    return LATTICE_OK;
+}
+
+// Whether tiles of 128 of `rows` rows would leave units idle: below one block a
+// unit the form for few rows is faster (156 blocks of heads of 64: 33 us for 38;
+// 32 blocks, window 3556: 35 for 101), above it the other (312: 45 for 53).
+inline bool grad_few(long long rows) { return rows < 128ll * 256; }
+
 template <typename T, int DP>
 int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, const float* lse, const T* grad_out,
                 T* grad_q, T* grad_k, T* grad_v, float2* states, const FirstParts& parts, hipStream_t stream) {
-    constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
-    const int group = a.heads / a.kv_heads;
     if (a.queries) {
-        constexpr size_t kLds = std::max<size_t>(4 * AttnTile<T, DP, kTile>::kBytes,
-                                                 kAttnWaves * sizeof(AttnRowScratch));
-        const auto kernel = grad_query_tiles<T, DP, kTile>;
-        LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
-        const long long slots = static_cast<long long>(a.queries) * group / (32 * kAttnWaves) + a.sequences + 2;
-        kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, lse, grad_out,
-                                                                                            grad_q, states);
-        LATTICE_LAUNCH_CHECK();
+        const int rc = grad_few(static_cast<long long>(a.queries) * a.heads)
+                           ? launch_grad_query<T, DP, true>(a, out, lse, grad_out, grad_q, states, stream)
+                           : launch_grad_query<T, DP, false>(a, out, lse, grad_out, grad_q, states, stream);
+        if (rc != LATTICE_OK) return rc;
     }
     if (a.keys == 0) return LATTICE_OK;
     if (l.first_tiles) {
-        constexpr size_t kLds = std::max<size_t>(kAttnWaves * QueryTile<T, DP, 32>::kBytes,
-                                                 kFirstValues<DP> * sizeof(float));
+        constexpr size_t kLds = std::max<size_t>(kAttnWaves * QueryTile<T, DP, 32>::kBytes, kJoinBytes<DP>);
         static_assert(kLds <= 160 * 1024);
         const auto kernel = grad_first_keys<T, DP>;
         LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
@@ -588,15 +669,10 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
                                                                                             parts);
         LATTICE_LAUNCH_CHECK();
     }
-    constexpr size_t kLds =
-        std::max<size_t>(2 * QueryTile<T, DP, kTile>::kBytes, kAttnWaves * sizeof(AttnRowScratch));
-    static_assert(kLds <= 160 * 1024);
-    const auto kernel = grad_key_tiles<T, DP, kTile, kKeyWaves<T, DP>>;
-    LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
-    const long long slots = a.keys / (32 * kAttnWaves) + a.sequences + 2;
-    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
-                                                                                        parts, grad_k, grad_v);
-    LATTICE_LAUNCH_CHECK();
+    const int rc = grad_few(static_cast<long long>(a.keys) * a.kv_heads)
+                       ? launch_grad_keys<T, DP, true>(a, lse, states, grad_out, parts, grad_k, grad_v, stream)
+                       : launch_grad_keys<T, DP, false>(a, lse, states, grad_out, parts, grad_k, grad_v, stream);
+    if (rc != LATTICE_OK) return rc;
     if (l.first_tiles && a.sequences) {
         join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles * (DP / 8)), kAttnBlock, 0, stream>>>(
             a, lse, states, grad_out, parts, grad_k, grad_v);
