@@ -360,17 +360,23 @@ inline AttnLayout attn_layout(const lattice_attention& a) {
     const int group = a.heads / a.kv_heads;
     const long long pairs = static_cast<long long>(a.queries) * group;
     const int sequences = std::max(1, a.sequences);
+    // The keys that a block sees, were the rows spread evenly over the sequences.
+    const auto seen_by = [&](int m) {
+        const long long span = static_cast<long long>(a.left) + a.right + std::min(m, a.queries) + a.sinks;
+        return std::min<long long>(span, (static_cast<long long>(a.keys) + sequences - 1) / sequences);
+    };
     AttnLayout l;
-    // Few rows a sequence leave three of four waves of a large tile idle.
-    l.few = pairs <= 32ll * sequences;
+    // Few rows a sequence leave three of four waves of a large tile idle; few
+    // rows in all leave units idle where there are too few keys to split (2.9k
+    // rows fp32, 4 heads of 128, window 414: 58 us, in large tiles 148; 256 rows
+    // of 8 heads against 8k keys: 38, split in large tiles 35).
+    l.few = pairs <= 32ll * sequences || (pairs * a.kv_heads < 128ll * 256 && seen_by(128) < 2048);
     const int m = l.few ? 32 : 128;
     l.slots = pairs / m + a.sequences + 2;
-    // Blocks that have rows, and the keys that one sees, were the rows spread
-    // evenly over the sequences.
+    // Blocks that have rows.
     const long long busy =
         std::max<long long>((pairs + m - 1) / m, std::min<long long>(sequences, a.queries)) * a.kv_heads;
-    const long long span = static_cast<long long>(a.left) + a.right + std::min(m, a.queries) + a.sinks;
-    const long long seen = std::min<long long>(span, (static_cast<long long>(a.keys) + sequences - 1) / sequences);
+    const long long seen = seen_by(m);
     // Two blocks a compute unit, each with at least 512 keys.
     const long long wanted = std::min<long long>((512 + busy - 1) / busy, seen / 512);
     l.splits = static_cast<int>(std::max<long long>(1, std::min<long long>(wanted, 64)));
