@@ -22,6 +22,11 @@ struct FirstParts {
 };
 constexpr uint32_t kFirstRows = 1024;
 
+// Whether tiles of 128 of `rows` rows would leave units idle: below one block a
+// unit the form for few rows is faster (156 blocks of heads of 64: 33 us for 38;
+// 32 blocks, window 3556: 35 for 101), above it the other (312: 45 for 53).
+inline bool grad_few(long long rows) { return rows < 128ll * 256; }
+
 // What a call needs besides its outputs.
 struct GradLayout {
     size_t states, past_values, window_values;
@@ -31,8 +36,10 @@ inline GradLayout grad_layout(const lattice_attention& a) {
     GradLayout l{static_cast<size_t>(a.queries) * a.heads, 0, 0, 0, 0};
     const long long pairs = static_cast<long long>(a.queries) * (a.heads / a.kv_heads);
     // The first keys' queries past the window are a pass of their own where
-    // sequences are long: one block would walk all of a sequence.
-    if (a.sinks > 0 && a.sinks <= 128 && a.left < a.keys && pairs >= 512ll * std::max(1, a.sequences)) {
+    // sequences are long: one block would walk all of a sequence.  In the form
+    // for few rows its four waves do, and two launches are saved.
+    const long long alone = grad_few(static_cast<long long>(a.keys) * a.kv_heads) ? 2048 : 512;
+    if (a.sinks > 0 && a.sinks <= 128 && a.left < a.keys && pairs >= alone * std::max(1, a.sequences)) {
         l.first_slots = static_cast<int>(pairs / kFirstRows + a.sequences + 2);
         l.first_tiles = (a.sinks + 31) / 32;
         const size_t values = static_cast<size_t>(a.kv_heads) * l.first_tiles * 2 * attn_width(a.dim) * 32;

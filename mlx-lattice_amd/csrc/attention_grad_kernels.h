@@ -645,11 +645,6 @@ int launch_grad_keys(const lattice_attention& a, const float* lse, const float2*
     return LATTICE_OK;
 }
 
-// Whether tiles of 128 of `rows` rows would leave units idle: below one block a
-// unit the form for few rows is faster (156 blocks of heads of 64: 33 us for 38;
-// 32 blocks, window 3556: 35 for 101), above it the other (312: 45 for 53).
-inline bool grad_few(long long rows) { return rows < 128ll * 256; }
-
 template <typename T, int DP>
 int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, const float* lse, const T* grad_out,
                 T* grad_q, T* grad_k, T* grad_v, float2* states, const FirstParts& parts, hipStream_t stream) {

@@ -36,18 +36,20 @@ def _run(q, k, v, dy, **kwargs):
     return [out, *torch.autograd.grad(out, leaves, dy)]
 
 
-def _check(q, k, v, dy, spans, left, right, sinks, scale=None, **kwargs):
+def _check(q, k, v, dy, spans, left, right, sinks, scale=None, device='cpu',
+           **kwargs):
     got = _run(q, k, v, dy, left=left, right=right, sinks=sinks, scale=scale,
                **kwargs)
     want = attention_f64(q, k, v, spans, left, right, sinks,
-                         scale or q.shape[-1] ** -0.5, dy)
+                         scale or q.shape[-1] ** -0.5, dy, device)
     for name, value, like, (ref, bound) in zip(('out', 'dq', 'dk', 'dv'), got,
                                                (q, q, k, v), want):
         assert value.dtype == like.dtype and value.shape == like.shape
         assert_within(value, ref, bound, name)
 
 
-def _self(lengths, heads, kv_heads, dim, dtype, left, right, sinks, seed=0):
+def _self(lengths, heads, kv_heads, dim, dtype, left, right, sinks, seed=0,
+          device='cpu'):
     gen = torch.Generator(device='cuda').manual_seed(seed)
     rows = sum(lengths)
     qkv = _normal(gen, dtype, rows, heads + 2 * kv_heads, dim)
@@ -57,7 +59,8 @@ def _self(lengths, heads, kv_heads, dim, dtype, left, right, sinks, seed=0):
         at += n
     _check(qkv[:, :heads], qkv[:, heads:heads + kv_heads],
            qkv[:, heads + kv_heads:], _normal(gen, dtype, rows, heads, dim),
-           spans, left, right, sinks, offsets=_offsets(lengths))
+           spans, left, right, sinks, offsets=_offsets(lengths),
+           device=device)
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -90,6 +93,56 @@ def test_any_number_of_channels(dim, dtype):
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_many_short_sequences(dtype):
     _self(tuple(i % 4 for i in range(700)), 2, 1, 32, dtype, 2, 1, 1)
+
+
+# Rows enough for tiles of 128, 32768 rows of key heads and more; the first
+# keys' long sums in a pass of their own (long sequences) and without.
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths, heads, kv_heads, dim, left, right, sinks', [
+    ((3000, 2501, 3100), 8, 4, 64, 90, 40, 5),
+    ((1500, 0, 700, 1, 411) + (61,) * 110, 8, 4, 32, 70, 9, 3),
+    ((4100, 4200), 12, 4, 80, 130, 0, 37),
+    ((3400, 33, 5000), 4, 4, 128, 33, 64, 1),
+    ((2900, 2800, 2700), 4, 4, 24, 10, 200, 150),
+    ((5600,), 6, 6, 96, 300, 0, 0)])
+def test_many_rows(lengths, heads, kv_heads, dim, left, right, sinks, dtype):
+    _self(lengths, heads, kv_heads, dim, dtype, left, right, sinks,
+          device='cuda')
+
+
+# Few rows that see thousands of keys: tiles of 128 whose keys are split.
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths, heads, kv_heads, dim, left, right, sinks', [
+    ((2600,), 2, 1, 64, None, 0, 0), ((3001,), 2, 2, 32, 2500, 100, 7),
+    ((2500, 70), 2, 1, 128, None, None, 0), ((2300,), 1, 1, 96, 2290, 0, 1)])
+def test_split_keys(lengths, heads, kv_heads, dim, left, right, sinks, dtype):
+    _self(lengths, heads, kv_heads, dim, dtype, left, right, sinks,
+          device='cuda')
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('value', (float('nan'), float('inf')))
+def test_what_is_not_seen_never_arrives_in_large_tiles(value, dtype):
+    """A row of k, v, q or the cotangent that is not finite, in tiles of 128:
+    rows past two windows of it neither see it nor share a sum with one that
+    does.  Those that share a tile with it are made again by themselves and
+    differ in rounding; rows some tiles away are those of the clean call."""
+    gen = torch.Generator(device='cuda').manual_seed(13)
+    kwargs = {'left': 40, 'right': 3, 'sinks': 0, 'offsets': _offsets((9000,))}
+    place = torch.arange(9000, device='cuda')
+    past = (place - 4321).abs() > 86
+    far = (place - 4321).abs() > 86 + 4 * 128
+    for name in ('k', 'v', 'dy', 'q'):
+        t = {n: _normal(gen, dtype, 9000, 4, 32) for n in ('q', 'k', 'v', 'dy')}
+        clean = _run(t['q'], t['k'], t['v'], t['dy'], **kwargs)
+        want = attention_f64(t['q'], t['k'], t['v'], [(0, 9000, 0, 9000)], 40,
+                             3, 0, 32 ** -0.5, t['dy'], 'cuda')
+        t[name][4321] = value
+        got = _run(t['q'], t['k'], t['v'], t['dy'], **kwargs)
+        for a, b, (ref, bound) in zip(got, clean, want):
+            assert torch.equal(a[far], b[far])
+            assert_within(a[past], ref[past], bound[past], name)
+        assert not torch.isfinite(got[1][4310:4340]).all()
 
 
 def _cache(q_lengths, k_lengths, capacity, heads, kv_heads, dim, dtype, left,

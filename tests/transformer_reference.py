@@ -126,23 +126,24 @@ def visible(nq, nk, left, right, sinks):
     return seen
 
 
-def attention_f64(q, k, v, spans, left, right, sinks, scale, dy=None):
+def attention_f64(q, k, v, spans, left, right, sinks, scale, dy=None,
+                  device='cpu'):
     """``spans``: (first query row, queries, first key row, keys) of each
     sequence.  A list of (value, bound): out, or out, dq, dk and dv.  What a
     query does not see is left out of its sums altogether."""
     u, tiny = UNIT[q.dtype], TINY[q.dtype]
     step = u + FLOAT_SUM
-    q64, k64, v64 = (t.detach().cpu().double() for t in (q, k, v))
+    q64, k64, v64 = (t.detach().to(device).double() for t in (q, k, v))
     heads, group = q64.shape[1], q64.shape[1] // k64.shape[1]
     grad = dy is not None
     zero = [torch.zeros_like(q64) for _ in range(4)]
     out, out_bound, dq, dq_bound = zero
     dk, dk_bound, dv, dv_bound = (torch.zeros_like(k64) for _ in range(4))
-    d64 = dy.detach().cpu().double() if grad else None
+    d64 = dy.detach().to(device).double() if grad else None
     for q0, nq, k0, nk in spans:
         if not nq or not nk:
             continue
-        seen = visible(nq, nk, left, right, sinks)
+        seen = visible(nq, nk, left, right, sinks).to(device)
         for h in range(heads):
             g = h // group
             rows, keys = slice(q0, q0 + nq), slice(k0, k0 + nk)
