@@ -823,23 +823,26 @@ typedef struct lattice_attention {
     const int32_t *offsets, *key_offsets, *key_lengths;
 } lattice_attention;
 
-/* out [queries, heads, dim] contiguous.  lse (NULL: not kept) gets the
- * float32 [queries, heads] log2 of each row's softmax sum, for the gradient
- * (+inf on empty rows). */
+/* out [queries, heads, dim] contiguous.  For the gradient: lse (NULL: not
+ * kept) gets the float32 [queries, heads] log2 of each row's softmax sum (+inf
+ * on empty rows), out_rest (NULL: not kept; unused in float32) what rounding
+ * took from out, like out. */
 size_t lattice_hip_window_attention_workspace_bytes(
     const lattice_attention* args);
 int lattice_hip_window_attention(const lattice_attention* args, void* out,
-                                 float* lse, void* workspace,
+                                 float* lse, void* out_rest, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
 /* Its gradients for the cotangent grad_out (contiguous, like out): grad_q,
  * grad_k, grad_v contiguous; every row is written, in an order of sums fixed
- * by the shapes and offsets. */
+ * by the shapes and offsets.  out_rest NULL: grad_q and grad_k are less exact
+ * by out's rounding. */
 size_t lattice_hip_window_attention_grad_workspace_bytes(
     const lattice_attention* args);
 int lattice_hip_window_attention_grad(const lattice_attention* args,
-                                      const void* out, const float* lse,
-                                      const void* grad_out, void* grad_q,
+                                      const void* out, const void* out_rest,
+                                      const float* lse, const void* grad_out,
+                                      void* grad_q,
                                       void* grad_k, void* grad_v,
                                       void* workspace, size_t workspace_bytes,
                                       void* stream);

@@ -125,12 +125,26 @@ __device__ inline void stage_row(float* to, const T* from, int dim) {
     for (int d = lane_id(); d < dim; d += kWave) to[d] = static_cast<float>(from[d]);
 }
 
+// What a forward pass keeps for the gradient (NULL: nothing): log2 of each
+// row's softmax sum, and what rounding took from out, in its type.
+template <typename T>
+struct AttnKept {
+    float* lse;
+    T* rest;
+};
+// An infinity leaves none.
+template <typename T>
+__device__ inline T rounding_rest(float value, T rounded) {
+    const float rest = value - static_cast<float>(rounded);
+    return static_cast<T>(fabsf(rest) < INFINITY ? rest : 0.0f);
+}
+
 // The forward pass of one query row and head, keys in order 64 at a time, one
 // a lane, with the running maximum and sum; then a channel a lane.  A key that
 // the row does not see is not read.
 template <typename T>
 __device__ inline void attend_row(const lattice_attention& a, const AttnSequence& s, int i, int head, T* out,
-                                  float* lse, AttnRowScratch* scratch) {
+                                  const AttnKept<T>& kept, AttnRowScratch* scratch) {
     const int lane = lane_id();
     const int kv = static_cast<int>(static_cast<long long>(head) * a.kv_heads / a.heads);
     const long long row = static_cast<long long>(s.q0) + i;
@@ -166,11 +180,15 @@ __device__ inline void attend_row(const lattice_attention& a, const AttnSequence
             acc[c] = acc[c] * old + add;
         }
     }
-    if (lse && lane == 0) lse[row * a.heads + head] = total ? top + log2f(sum) : INFINITY;
+    if (kept.lse && lane == 0) kept.lse[row * a.heads + head] = total ? top + log2f(sum) : INFINITY;
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
         const int d = lane + c * kWave;
-        if (d < a.dim) out[(row * a.heads + head) * a.dim + d] = static_cast<T>(total ? acc[c] / sum : 0.0f);
+        if (d >= a.dim) continue;
+        const float value = total ? acc[c] / sum : 0.0f;
+        const T rounded = static_cast<T>(value);
+        out[(row * a.heads + head) * a.dim + d] = rounded;
+        if (kept.rest) kept.rest[(row * a.heads + head) * a.dim + d] = rounding_rest(value, rounded);
     }
 }
 

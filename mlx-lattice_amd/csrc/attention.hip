@@ -119,7 +119,7 @@ __device__ inline void attend_tile(const lattice_attention& a, AttnState<T, DP>&
 template <typename T, int DP>
 __device__ inline void write_rows(const lattice_attention& a, const AttnSequence& s, const AttnRows& w,
                                   AttnState<T, DP>& state, bool partial, int split, const AttnPart& part, T* out,
-                                  float* lse, AttnRowScratch* scratch) {
+                                  const AttnKept<T>& kept, AttnRowScratch* scratch) {
     const int half = lane_id() >> 5;
     const float sum = state.sum + other_half(state.sum);
     const long long at = (static_cast<long long>(s.q0) + w.i) * a.heads + w.head;
@@ -151,7 +151,7 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
     const uint64_t spoilt = ballot(w.valid && !finite_columns(state.acc, 1.0f));
     uint32_t again = static_cast<uint32_t>(spoilt) | static_cast<uint32_t>(spoilt >> 32);
     if (w.valid && !(again >> (lane_id() & 31) & 1)) {
-        if (lse && half == 0) lse[at] = sees ? state.top + __builtin_amdgcn_logf(sum) : INFINITY;
+        if (kept.lse && half == 0) kept.lse[at] = sees ? state.top + __builtin_amdgcn_logf(sum) : INFINITY;
 #pragma unroll
         for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
 #pragma unroll
@@ -162,13 +162,18 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v.set(i, state.acc[b][4 * g + i]);
                 v.store(out + at * a.dim + d);
+                if (!kept.rest) continue;
+                RowVec<T, 4> rest;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rest.e[i] = rounding_rest(state.acc[b][4 * g + i], v.e[i]);
+                rest.store(kept.rest + at * a.dim + d);
             }
         }
     }
     while (again) {
         const int n = __ffs(again) - 1;
         again &= again - 1;
-        attend_row<T>(a, s, __shfl(w.i, n), __shfl(w.head, n), out, lse, scratch);
+        attend_row<T>(a, s, __shfl(w.i, n), __shfl(w.head, n), out, kept, scratch);
     }
 }
 
@@ -176,7 +181,7 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
 // Double-buffered: a tile is copied to LDS while the one before is used.
 template <typename T, int DP, int KT>
 __global__ void __launch_bounds__(kAttnBlock, 2)
-attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
+attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, AttnKept<T> kept) {
     typedef AttnTile<T, DP, KT> Tile;
     extern __shared__ __align__(128) char shared[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -212,7 +217,7 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
         attend_tile<T, DP, KT>(a, state, q, at, at + Tile::kBytes, scale, s.nk, w, mask, tiles.tile(index) * KT);
         __syncthreads();
     }
-    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, lse,
+    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, kept,
                       reinterpret_cast<AttnRowScratch*>(shared) + wave);
 }
 
@@ -224,7 +229,7 @@ template <typename T, int DP> constexpr int few_waves() { return kTileDim<DP> * 
 // LDS.
 template <typename T, int DP, int KT, int kFewWaves>
 __global__ void __launch_bounds__(kFewWaves * kWave)
-attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
+attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, AttnKept<T> kept) {
     typedef AttnTile<T, DP, KT> Tile;
     constexpr int kBlocks = AttnState<T, DP>::kBlocks;
     extern __shared__ __align__(128) char shared[];
@@ -300,14 +305,14 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     if (wave != 0) return;
     state.top = top;
     state.sum = lane < 32 ? sum : 0.0f;  // write_rows adds the halves
-    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, lse,
+    write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, kept,
                       reinterpret_cast<AttnRowScratch*>(shared));
 }
 
 // Joins the parts (at most 64) of a row: a wave a (query row, head).
 template <typename T>
 __global__ void __launch_bounds__(kAttnBlock)
-join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, float* __restrict__ lse) {
+join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, AttnKept<T> kept) {
     __shared__ AttnRowScratch scratch[kAttnWaves];
     const int wave = threadIdx.x / kWave, lane = lane_id();
     const long long items = static_cast<long long>(a.queries) * a.heads;
@@ -338,14 +343,17 @@ join_parts(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
         const int row = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
         const int e = query_rows(a).find(row, [](int start, int) { return static_cast<uint32_t>(start); });
         const AttnSequence s = attn_sequence(a, e);
-        attend_row<T>(a, s, row - s.q0, head, out, lse, &scratch[wave]);
+        attend_row<T>(a, s, row - s.q0, head, out, kept, &scratch[wave]);
         return;
     }
-    if (lse && lane == 0) lse[at] = top + log2f(sum);
+    if (kept.lse && lane == 0) kept.lse[at] = top + log2f(sum);
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / kWave; ++c) {
         const int d = lane + c * kWave;
-        if (d < a.dim) out[at * a.dim + d] = static_cast<T>(acc[c]);
+        if (d >= a.dim) continue;
+        const T rounded = static_cast<T>(acc[c]);
+        out[at * a.dim + d] = rounded;
+        if (kept.rest) kept.rest[at * a.dim + d] = rounding_rest(acc[c], rounded);
     }
 }
 
@@ -384,8 +392,8 @@ inline AttnLayout attn_layout(const lattice_attention& a) {
 }
 
 template <typename T, int DP>
-int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, T* out, float* lse,
-                  hipStream_t stream) {
+int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, T* out,
+                  const AttnKept<T>& kept, hipStream_t stream) {
     // Tiles twice as large are no faster (scan of heads of 32: 152 us for 143).
     constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
     typedef AttnTile<T, DP, kTile> Tile;
@@ -398,18 +406,18 @@ int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPar
         static_assert(kLds >= sizeof(AttnRowScratch) && kLds <= 160 * 1024);
         const auto kernel = attend_few<T, DP, kFew, kFewWaves>;
         LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
-        kernel<<<grid, kFewWaves * kWave, kLds, stream>>>(a, l.splits, part, out, lse);
+        kernel<<<grid, kFewWaves * kWave, kLds, stream>>>(a, l.splits, part, out, kept);
     } else {
         constexpr size_t kLds = std::max<size_t>(4 * Tile::kBytes, kAttnWaves * sizeof(AttnRowScratch));
         static_assert(kLds <= 160 * 1024);
         const auto kernel = attend_tiles<T, DP, kTile>;
         LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
-        kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, lse);
+        kernel<<<grid, kAttnBlock, kLds, stream>>>(a, l.splits, part, out, kept);
     }
     LATTICE_LAUNCH_CHECK();
     if (l.splits > 1) {
         join_parts<T><<<grid_for(static_cast<long long>(a.queries) * a.heads, kAttnWaves, 1u << 30), kAttnBlock, 0,
-                        stream>>>(a, l.splits, part, out, lse);
+                        stream>>>(a, l.splits, part, out, kept);
         LATTICE_LAUNCH_CHECK();
     }
     return LATTICE_OK;
@@ -417,12 +425,13 @@ int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPar
 
 template <typename T>
 int attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, void* out, float* lse,
-           hipStream_t stream) {
+           void* rest, hipStream_t stream) {
+    const AttnKept<T> kept{lse, sizeof(T) == 4 ? nullptr : static_cast<T*>(rest)};
     T* o = static_cast<T*>(out);
-    if (a.dim <= 32) return launch_attend<T, 32>(a, l, part, o, lse, stream);
-    if (a.dim <= 64) return launch_attend<T, 64>(a, l, part, o, lse, stream);
-    if (a.dim <= 96) return launch_attend<T, 96>(a, l, part, o, lse, stream);
-    return launch_attend<T, 128>(a, l, part, o, lse, stream);
+    if (a.dim <= 32) return launch_attend<T, 32>(a, l, part, o, kept, stream);
+    if (a.dim <= 64) return launch_attend<T, 64>(a, l, part, o, kept, stream);
+    if (a.dim <= 96) return launch_attend<T, 96>(a, l, part, o, kept, stream);
+    return launch_attend<T, 128>(a, l, part, o, kept, stream);
 }
 
 }  // namespace
@@ -439,8 +448,8 @@ extern "C" size_t lattice_hip_window_attention_workspace_bytes(const lattice_att
     return aligned_bytes(rows * a.dim * sizeof(float)) + aligned_bytes(rows * sizeof(float2));
 }
 
-extern "C" int lattice_hip_window_attention(const lattice_attention* args, void* out, float* lse, void* workspace,
-                                            size_t workspace_bytes, void* stream_ptr) {
+extern "C" int lattice_hip_window_attention(const lattice_attention* args, void* out, float* lse, void* out_rest,
+                                            void* workspace, size_t workspace_bytes, void* stream_ptr) {
     LATTICE_REQUIRE_ATTENTION(args);
     if (args->queries == 0) return LATTICE_OK;
     LATTICE_REQUIRE(out, "attention pointers must be non-null.");
@@ -455,7 +464,7 @@ extern "C" int lattice_hip_window_attention(const lattice_attention* args, void*
         LATTICE_REQUIRE(part.values && part.states, "attention workspace is too small.");
     }
     hipStream_t stream = as_stream(stream_ptr);
-    if (a.dtype == LATTICE_F32) return attend<float>(a, l, part, out, lse, stream);
-    if (a.dtype == LATTICE_F16) return attend<_Float16>(a, l, part, out, lse, stream);
-    return attend<__bf16>(a, l, part, out, lse, stream);
+    if (a.dtype == LATTICE_F32) return attend<float>(a, l, part, out, lse, out_rest, stream);
+    if (a.dtype == LATTICE_F16) return attend<_Float16>(a, l, part, out, lse, out_rest, stream);
+    return attend<__bf16>(a, l, part, out, lse, out_rest, stream);
 }

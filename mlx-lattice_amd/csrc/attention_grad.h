@@ -51,8 +51,8 @@ inline GradLayout grad_layout(const lattice_attention& a) {
 
 // The launches for rows of type T.
 template <typename T>
-int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out, const float* lse,
-                const void* grad_out, void* grad_q, void* grad_k, void* grad_v, float2* states,
+int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out, const void* out_rest,
+                const float* lse, const void* grad_out, void* grad_q, void* grad_k, void* grad_v, float2* states,
                 const FirstParts& parts, hipStream_t stream);
 
 }  // namespace lattice

@@ -20,14 +20,17 @@ extern "C" size_t lattice_hip_window_attention_grad_workspace_bytes(const lattic
            aligned_bytes(l.window_values * sizeof(float));
 }
 
-extern "C" int lattice_hip_window_attention_grad(const lattice_attention* args, const void* out, const float* lse,
-                                                 const void* grad_out, void* grad_q, void* grad_k, void* grad_v,
+extern "C" int lattice_hip_window_attention_grad(const lattice_attention* args, const void* out, const void* out_rest,
+                                                 const float* lse, const void* grad_out, void* grad_q, void* grad_k, void* grad_v,
                                                  void* workspace, size_t workspace_bytes, void* stream_ptr) {
     LATTICE_REQUIRE_ATTENTION(args);
     if (args->queries == 0 && args->keys == 0) return LATTICE_OK;
     LATTICE_REQUIRE(args->queries == 0 || (out && lse && grad_out && grad_q), "attention pointers must be non-null.");
     LATTICE_REQUIRE(args->keys == 0 || (grad_k && grad_v), "attention pointers must be non-null.");
-    LATTICE_REQUIRE((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(grad_out)) % 16 == 0,
+    LATTICE_REQUIRE((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest) |
+                     reinterpret_cast<uintptr_t>(grad_out)) %
+                            16 ==
+                        0,
                     "attention rows must lie on 16-byte boundaries.");
     const lattice_attention a = attn_bounded(*args);
     const GradLayout l = grad_layout(a);
@@ -40,8 +43,8 @@ extern "C" int lattice_hip_window_attention_grad(const lattice_attention* args, 
                     "attention gradient workspace is too small.");
     hipStream_t stream = as_stream(stream_ptr);
     if (a.dtype == LATTICE_F32)
-        return attend_grad<float>(a, l, out, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
+        return attend_grad<float>(a, l, out, out_rest, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
     if (a.dtype == LATTICE_F16)
-        return attend_grad<_Float16>(a, l, out, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
-    return attend_grad<__bf16>(a, l, out, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
+        return attend_grad<_Float16>(a, l, out, out_rest, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
+    return attend_grad<__bf16>(a, l, out, out_rest, lse, grad_out, grad_q, grad_k, grad_v, states, parts, stream);
 }

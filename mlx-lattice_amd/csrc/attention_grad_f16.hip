@@ -2,7 +2,7 @@
 
 namespace lattice {
 
-template int attend_grad<_Float16>(const lattice_attention&, const GradLayout&, const void*, const float*, const void*,
-                                 void*, void*, void*, float2*, const FirstParts&, hipStream_t);
+template int attend_grad<_Float16>(const lattice_attention&, const GradLayout&, const void*, const void*, const float*,
+                                   const void*, void*, void*, void*, float2*, const FirstParts&, hipStream_t);
 
 }  // namespace lattice

@@ -130,8 +130,8 @@ __device__ inline long long query_state(const lattice_attention& a, uint32_t gro
 // copies; their sums are joined.
 template <typename T, int DP, int KT, bool FEW>
 __global__ void __launch_bounds__(kAttnBlock, DP <= 64 || sizeof(T) == 2 ? 2 : 1)
-grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __restrict__ lse,
-                 const T* __restrict__ grad_out, T* __restrict__ grad_q, float2* __restrict__ states) {
+grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __restrict__ rest,
+                 const float* __restrict__ lse, const T* __restrict__ grad_out, T* __restrict__ grad_q, float2* __restrict__ states) {
     typedef AttnTile<T, DP, KT> Tile;
     typedef AttnOperand<T, DP> Operand;
     constexpr int kBlocks = DP / 32;
@@ -161,6 +161,16 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const float* __
 #pragma unroll
             for (int i = 0; i < Tile::kElems; ++i)
                 along += static_cast<float>(o.f[c][i]) * static_cast<float>(d.f[c][i]);
+        }
+        if (rest) {
+            // What rounding took from out would be a third of delta's error.
+            o.load(rest + at * a.dim, a.dim, w.valid, false);
+#pragma unroll
+            for (int c = 0; c < Operand::kSteps; ++c) {
+#pragma unroll
+                for (int i = 0; i < Tile::kElems; ++i)
+                    along += static_cast<float>(o.f[c][i]) * static_cast<float>(d.f[c][i]);
+            }
         }
         along += other_half(along);
     }
@@ -614,8 +624,8 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
 }
 
 template <typename T, int DP, bool FEW>
-int launch_grad_query(const lattice_attention& a, const T* out, const float* lse, const T* grad_out, T* grad_q,
-                      float2* states, hipStream_t stream) {
+int launch_grad_query(const lattice_attention& a, const T* out, const T* rest, const float* lse, const T* grad_out,
+                      T* grad_q, float2* states, hipStream_t stream) {
     constexpr int kTile = sizeof(T) == 2 && !FEW ? 64 : 32, kRows = FEW ? 32 : 32 * kAttnWaves;
     constexpr size_t kLds = std::max({(FEW ? kAttnWaves : 2) * size_t{2} * AttnTile<T, DP, kTile>::kBytes,
                                       FEW ? kJoinBytes<DP> : 0, kAttnWaves * sizeof(AttnRowScratch)});
@@ -623,8 +633,8 @@ int launch_grad_query(const lattice_attention& a, const T* out, const float* lse
     const auto kernel = grad_query_tiles<T, DP, kTile, FEW>;
     LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
     const long long slots = static_cast<long long>(a.queries) * (a.heads / a.kv_heads) / kRows + a.sequences + 2;
-    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, lse, grad_out, grad_q,
-                                                                                        states);
+    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, rest, lse, grad_out,
+                                                                                        grad_q, states);
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
 }
@@ -646,12 +656,12 @@ int launch_grad_keys(const lattice_attention& a, const float* lse, const float2*
 }
 
 template <typename T, int DP>
-int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, const float* lse, const T* grad_out,
-                T* grad_q, T* grad_k, T* grad_v, float2* states, const FirstParts& parts, hipStream_t stream) {
+int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, const T* rest, const float* lse,
+                const T* grad_out, T* grad_q, T* grad_k, T* grad_v, float2* states, const FirstParts& parts, hipStream_t stream) {
     if (a.queries) {
         const int rc = grad_few(static_cast<long long>(a.queries) * a.heads)
-                           ? launch_grad_query<T, DP, true>(a, out, lse, grad_out, grad_q, states, stream)
-                           : launch_grad_query<T, DP, false>(a, out, lse, grad_out, grad_q, states, stream);
+                           ? launch_grad_query<T, DP, true>(a, out, rest, lse, grad_out, grad_q, states, stream)
+                           : launch_grad_query<T, DP, false>(a, out, rest, lse, grad_out, grad_q, states, stream);
         if (rc != LATTICE_OK) return rc;
     }
     if (a.keys == 0) return LATTICE_OK;
@@ -679,18 +689,19 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
 }  // namespace
 
 template <typename T>
-int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out, const float* lse,
-                const void* grad_out, void* grad_q, void* grad_k, void* grad_v, float2* states,
+int attend_grad(const lattice_attention& a, const GradLayout& l, const void* out, const void* out_rest,
+                const float* lse, const void* grad_out, void* grad_q, void* grad_k, void* grad_v, float2* states,
                 const FirstParts& parts, hipStream_t stream) {
     const T* o = static_cast<const T*>(out);
+    const T* rest = sizeof(T) == 4 ? nullptr : static_cast<const T*>(out_rest);
     const T* dy = static_cast<const T*>(grad_out);
     T* dq = static_cast<T*>(grad_q);
     T* dk = static_cast<T*>(grad_k);
     T* dv = static_cast<T*>(grad_v);
-    if (a.dim <= 32) return launch_grad<T, 32>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
-    if (a.dim <= 64) return launch_grad<T, 64>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
-    if (a.dim <= 96) return launch_grad<T, 96>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
-    return launch_grad<T, 128>(a, l, o, lse, dy, dq, dk, dv, states, parts, stream);
+    if (a.dim <= 32) return launch_grad<T, 32>(a, l, o, rest, lse, dy, dq, dk, dv, states, parts, stream);
+    if (a.dim <= 64) return launch_grad<T, 64>(a, l, o, rest, lse, dy, dq, dk, dv, states, parts, stream);
+    if (a.dim <= 96) return launch_grad<T, 96>(a, l, o, rest, lse, dy, dq, dk, dv, states, parts, stream);
+    return launch_grad<T, 128>(a, l, o, rest, lse, dy, dq, dk, dv, states, parts, stream);
 }
 
 }  // namespace lattice

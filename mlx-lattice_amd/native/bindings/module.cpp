@@ -422,9 +422,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("dims"), py::arg("interleaved"), py::arg("inverse"), "Rotary positions of several axes.");
     m.def("window_attention", &ln::window_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"),
           py::arg("key_offsets"), py::arg("key_lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"),
-          py::arg("scale"), py::arg("keep_lse"), "Attention over a sliding window: (out, lse).");
+          py::arg("scale"), py::arg("keep"), "Attention over a sliding window: (out, lse, rest).");
     m.def("window_attention_grad", &ln::window_attention_grad, py::arg("cotangent"), py::arg("out"), py::arg("lse"),
-          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("key_offsets"),
+          py::arg("rest"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("key_offsets"),
           py::arg("key_lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"), py::arg("scale"),
           "Gradients of the windowed attention: (grad_q, grad_k, grad_v).");
     m.def("layer_norm_node", &ln::layer_norm_node, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),

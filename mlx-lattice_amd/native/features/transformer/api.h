@@ -28,16 +28,18 @@ at::Tensor dropout(const at::Tensor& x, const c10::optional<at::Tensor>& residua
 at::Tensor rotary_positions(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies,
                             const std::vector<int>& dims, bool interleaved, bool inverse);
 
-// (out, lse); lse is undefined (None) unless kept for the gradient.
-std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                    const at::Tensor& offsets, const at::Tensor& key_offsets,
-                                                    const c10::optional<at::Tensor>& key_lengths, int64_t left,
-                                                    int64_t right, int64_t sinks, double scale, bool keep_lse);
+// (out, lse, rest); the last two are undefined (None) unless kept for the
+// gradient, rest (what rounding took from out) in float32 too.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+    const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right,
+    int64_t sinks, double scale, bool keep);
 // (grad_q, grad_k, grad_v).
 std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_grad(
-    const at::Tensor& grad_out, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& q,
-    const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& key_offsets,
-    const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right, int64_t sinks, double scale);
+    const at::Tensor& grad_out, const at::Tensor& out, const at::Tensor& lse, const c10::optional<at::Tensor>& rest,
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+    const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right,
+    int64_t sinks, double scale);
 
 // The same operators as differentiable nodes of torch's graph.
 at::Tensor layer_norm_node(const at::Tensor& x, const c10::optional<at::Tensor>& weight,

@@ -105,9 +105,9 @@ struct WindowAttention : Function<WindowAttention> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                               const at::Tensor& offsets, const at::Tensor& key_offsets, const MaybeTensor& key_lengths,
                               int64_t left, int64_t right, int64_t sinks, double scale) {
-        auto [out, lse] = window_attention(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale,
+        auto [out, lse, rest] = window_attention(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale,
                                            true);
-        ctx->save_for_backward({q, k, v, out, lse, offsets, key_offsets, or_undefined(key_lengths)});
+        ctx->save_for_backward({q, k, v, out, lse, offsets, key_offsets, or_undefined(key_lengths), rest});
         ctx->saved_data["left"] = left;
         ctx->saved_data["right"] = right;
         ctx->saved_data["sinks"] = sinks;
@@ -117,8 +117,8 @@ struct WindowAttention : Function<WindowAttention> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         auto& data = ctx->saved_data;
-        auto [dq, dk, dv] = window_attention_grad(grads[0], saved[3], saved[4], saved[0], saved[1], saved[2],
-                                                  saved[5], saved[6], or_none(saved[7]), data["left"].toInt(),
+        auto [dq, dk, dv] = window_attention_grad(grads[0], saved[3], saved[4], or_none(saved[8]), saved[0], saved[1],
+                                                  saved[2], saved[5], saved[6], or_none(saved[7]), data["left"].toInt(),
                                                   data["right"].toInt(), data["sinks"].toInt(),
                                                   data["scale"].toDouble());
         return once({dq, dk, dv, {}, {}, {}, {}, {}, {}, {}});

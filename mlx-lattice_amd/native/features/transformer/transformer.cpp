@@ -290,27 +290,31 @@ at::Tensor whole_pieces(const at::Tensor& t) {
 
 }  // namespace
 
-std::tuple<at::Tensor, at::Tensor> window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                    const at::Tensor& offsets, const at::Tensor& key_offsets,
-                                                    const c10::optional<at::Tensor>& key_lengths, int64_t left,
-                                                    int64_t right, int64_t sinks, double scale, bool keep_lse) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+    const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right,
+    int64_t sinks, double scale, bool keep) {
     const c10::OptionalDeviceGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
     const Attention a = attention_of(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
     at::Tensor out = at::empty(a.q.sizes(), q.options());
-    at::Tensor lse;
-    if (keep_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    at::Tensor lse, rest;
+    if (keep) {
+        lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+        if (q.scalar_type() != at::kFloat) rest = at::empty(a.q.sizes(), q.options());
+    }
     const size_t bytes = lattice_hip_window_attention_workspace_bytes(&a.args);
     at::Tensor ws;
     if (bytes) ws = workspace(bytes, q);
-    check_status(lattice_hip_window_attention(&a.args, out.data_ptr(), keep_lse ? lse.data_ptr<float>() : nullptr,
-                                              or_null(ws), bytes, current_stream(q)));
-    return {unpadded(out, q.size(2)), lse};
+    check_status(lattice_hip_window_attention(&a.args, out.data_ptr(), keep ? lse.data_ptr<float>() : nullptr,
+                                              or_null(rest), or_null(ws), bytes, current_stream(q)));
+    return {unpadded(out, q.size(2)), lse, rest};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_grad(
-    const at::Tensor& grad_out_in, const at::Tensor& out_in, const at::Tensor& lse, const at::Tensor& q,
-    const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& key_offsets,
-    const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right, int64_t sinks, double scale) {
+    const at::Tensor& grad_out_in, const at::Tensor& out_in, const at::Tensor& lse,
+    const c10::optional<at::Tensor>& rest, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& offsets, const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths,
+    int64_t left, int64_t right, int64_t sinks, double scale) {
     const c10::OptionalDeviceGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
     const Attention a = attention_of(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
     require_same(grad_out_in, q, "the cotangent");
@@ -323,13 +327,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_grad(
         throw std::invalid_argument("lse must be that of the forward call.");
     }
     const at::Tensor grad_out = whole_pieces(grad_out_in), out = whole_pieces(out_in);
+    if (rest && rest->defined() &&
+        (rest->sizes() != a.q.sizes() || rest->scalar_type() != q.scalar_type() || !rest->is_contiguous() ||
+         rest->device() != q.device())) {
+        throw std::invalid_argument("rest must be that of the forward call.");
+    }
     at::Tensor dq = at::empty(a.q.sizes(), q.options());
     at::Tensor dk = at::empty(a.k.sizes(), q.options()), dv = at::empty(a.k.sizes(), q.options());
     const size_t bytes = lattice_hip_window_attention_grad_workspace_bytes(&a.args);
     at::Tensor ws;
     if (bytes) ws = workspace(bytes, q);
-    check_status(lattice_hip_window_attention_grad(&a.args, out.data_ptr(), lse.data_ptr<float>(),
-                                                   grad_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    check_status(lattice_hip_window_attention_grad(&a.args, out.data_ptr(), data_or_null(rest),
+                                                   lse.data_ptr<float>(), grad_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                                    or_null(ws), bytes, current_stream(q)));
     const int64_t dim = q.size(2);
     return {unpadded(dq, dim), unpadded(dk, dim), unpadded(dv, dim)};

@@ -374,9 +374,10 @@ def test_captured_graph_replays(dtype, dim):
     window = (60, 10, 2, dim ** -0.5)
 
     def passes():
-        out, lse = ext.window_attention(q, k, v, at, at, None, *window, True)
-        grads = ext.window_attention_grad(dy, out, lse, q, k, v, at, at, None,
-                                          *window)
+        out, lse, rest = ext.window_attention(q, k, v, at, at, None, *window,
+                                              True)
+        grads = ext.window_attention_grad(dy, out, lse, rest, q, k, v, at, at,
+                                          None, *window)
         few = _ops().window_attention(q[:2], k, v, offsets=token,
                                       key_offsets=at)
         return [out, *grads, few]

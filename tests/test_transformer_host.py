@@ -73,10 +73,10 @@ def test_attention_refusals(changes, message):
     lib = _library()
     args = _attention(**changes)
     rc = lib.lattice_hip_window_attention(
-        ctypes.byref(args), 4096, None, None, ctypes.c_size_t(0), None)
+        ctypes.byref(args), 4096, None, None, None, ctypes.c_size_t(0), None)
     assert rc == 1 and message in lib.lattice_hip_last_error()
     rc = lib.lattice_hip_window_attention_grad(
-        ctypes.byref(args), 4096, 4096, 4096, 4096, 4096, 4096, None,
+        ctypes.byref(args), 4096, None, 4096, 4096, 4096, 4096, 4096, None,
         ctypes.c_size_t(0), None)
     assert rc == 1 and message in lib.lattice_hip_last_error()
     assert lib.lattice_hip_window_attention_workspace_bytes(
@@ -85,7 +85,7 @@ def test_attention_refusals(changes, message):
 
 def test_attention_workspaces():
     lib = _library()
-    rc = lib.lattice_hip_window_attention(None, None, None, None,
+    rc = lib.lattice_hip_window_attention(None, None, None, None, None,
                                           ctypes.c_size_t(0), None)
     assert rc == 1 and b'non-null' in lib.lattice_hip_last_error()
     # Enough rows of their own: no workspace.
@@ -97,13 +97,14 @@ def test_attention_workspaces():
     size = lib.lattice_hip_window_attention_workspace_bytes(ctypes.byref(args))
     assert size >= 2 * 4 * (64 * 4 + 8)
     rc = lib.lattice_hip_window_attention(
-        ctypes.byref(args), 4096, None, 4096, ctypes.c_size_t(size - 1), None)
+        ctypes.byref(args), 4096, None, None, 4096, ctypes.c_size_t(size - 1),
+        None)
     assert rc == 1 and b'workspace' in lib.lattice_hip_last_error()
     size = lib.lattice_hip_window_attention_grad_workspace_bytes(
         ctypes.byref(args))
     assert size >= 4 * 8
     rc = lib.lattice_hip_window_attention_grad(
-        ctypes.byref(args), 4096, 4096, 4096, 4096, 4096, 4096, 4096,
+        ctypes.byref(args), 4096, None, 4096, 4096, 4096, 4096, 4096, 4096,
         ctypes.c_size_t(size - 1), None)
     assert rc == 1 and b'workspace' in lib.lattice_hip_last_error()
 
