@@ -314,12 +314,13 @@ layer_norm_grad_columns(const T* __restrict__ dy, long long dy_stride, const T* 
 }
 
 // partials [count][2][channels] -> grad_weight and grad_bias: 16 columns a
-// block, 16 slices of the partials added in slice order.
+// block, 64 slices of the partials added in slice order.
+constexpr int kFinishBlock = 1024, kFinishSlices = kFinishBlock / 16;
 template <typename T>
-__global__ void __launch_bounds__(kNormBlock)
+__global__ void __launch_bounds__(kFinishBlock)
 layer_norm_grad_finish(const float* __restrict__ partials, int count, int channels, T* __restrict__ grad_weight,
                        T* __restrict__ grad_bias) {
-    __shared__ float shared[16][17];
+    __shared__ float shared[kFinishSlices][17];
     const int at = threadIdx.x & 15, slice = threadIdx.x >> 4;
     const long long column = static_cast<long long>(blockIdx.x) * 16 + at;
     const long long columns = 2ll * channels;
@@ -328,17 +329,18 @@ layer_norm_grad_finish(const float* __restrict__ partials, int count, int channe
         // Four chains of additions keep four reads in flight.
         float chain[4] = {};
         int i = slice;
-        for (; i + 48 < count; i += 64) {
+        for (; i + 3 * kFinishSlices < count; i += 4 * kFinishSlices) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) chain[u] += partials[(i + 16ll * u) * columns + column];
+            for (int u = 0; u < 4; ++u)
+                chain[u] += partials[(i + static_cast<long long>(kFinishSlices) * u) * columns + column];
         }
-        for (; i < count; i += 16) chain[0] += partials[static_cast<long long>(i) * columns + column];
+        for (; i < count; i += kFinishSlices) chain[0] += partials[static_cast<long long>(i) * columns + column];
         sum = (chain[0] + chain[1]) + (chain[2] + chain[3]);
     }
     shared[slice][at] = sum;
     __syncthreads();
     if (slice != 0 || column >= columns) return;
-    for (int s = 1; s < 16; ++s) sum += shared[s][at];
+    for (int s = 1; s < kFinishSlices; ++s) sum += shared[s][at];
     if (column < channels) {
         if (grad_weight) grad_weight[column] = static_cast<T>(sum);
     } else if (grad_bias) {
@@ -421,7 +423,7 @@ int launch_norm_grad(const T* dy, long long dy_stride, const T* x, long long x_s
 #undef LATTICE_NORM_ROWS
     LATTICE_LAUNCH_CHECK();
     if (partials) {
-        layer_norm_grad_finish<T><<<(2 * channels + 15) / 16, kNormBlock, 0, stream>>>(partials, blocks, channels,
+        layer_norm_grad_finish<T><<<(2 * channels + 15) / 16, kFinishBlock, 0, stream>>>(partials, blocks, channels,
                                                                                       grad_weight, grad_bias);
         LATTICE_LAUNCH_CHECK();
     }
@@ -520,10 +522,10 @@ extern "C" int lattice_hip_layer_norm_grad(int dtype, const void* grad_y, long l
         // No partials: the sums are zero.
         const unsigned blocks = static_cast<unsigned>((2 * channels + 15) / 16);
         if (dtype == LATTICE_F32) {
-            layer_norm_grad_finish<float><<<blocks, kNormBlock, 0, stream>>>(
+            layer_norm_grad_finish<float><<<blocks, kFinishBlock, 0, stream>>>(
                 nullptr, 0, channels, static_cast<float*>(grad_weight), static_cast<float*>(grad_bias));
         } else {  // zero has the same bits in both 16-bit types
-            layer_norm_grad_finish<_Float16><<<blocks, kNormBlock, 0, stream>>>(
+            layer_norm_grad_finish<_Float16><<<blocks, kFinishBlock, 0, stream>>>(
                 nullptr, 0, channels, static_cast<_Float16*>(grad_weight), static_cast<_Float16*>(grad_bias));
         }
         LATTICE_LAUNCH_CHECK();
