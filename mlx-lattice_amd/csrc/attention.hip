@@ -7,7 +7,20 @@
 //
 // The rows of a tile are (query, head) pairs of the heads that share a key
 // head, so that each key is staged once for all of them and the band of keys
-// that a tile sees is as narrow as may be.
+// that a tile sees is as narrow as may be.  A wave holds 32 rows: q as the right
+// operand in registers, the scores transposed, so that a lane has one row's and
+// the softmax needs one exchange between two lanes a step.
+//
+// Shares are rounded to the rows' type for the second product, as q, k and v
+// are; maximum, sums and results are fp32.
+//
+// Bound by the exponentials and the other vector instructions of the softmax,
+// 7 issue slots a score beside the products' 4 (heads of 32) to 16 (128) cycles;
+// few queries by reading the keys.  120,000 rows of 8 heads of 32, window 257,
+// fp16: 131 us (246 TFLOP/s).  16,384 causal rows of 16 heads of 128 over 4,
+// window 4096, bf16: 569 us under the profiler, 540 without (894 TFLOP/s; a
+// library product of 8192^3 1191).  One query of 16 heads of 128 over 4 against
+// 32 caches of 24,000 keys, fp16: 298 us (5.5 TB/s).
 
 #include "attention_tiles.h"
 

@@ -15,6 +15,10 @@
 // row per block, and a second launch adds the partials in a fixed order.
 // Rows wider than 256 vectors take a block each and are read again from the
 // caches.
+//
+// 400,000 x 128 fp16: forward 40 us (5.1 TB/s of the 5.4 that a copy of that
+// size reaches), gradient 64 us (4.8 TB/s; 64 bytes of sums a lane cost it some
+// of its waves), the partials' sum 4 us.  20,000 x 32 fp32: 3.7 us, a launch.
 
 #include "rows.h"
 
