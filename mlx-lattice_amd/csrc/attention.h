@@ -164,7 +164,8 @@ __device__ inline void attend_row(const lattice_attention& a, const AttnSequence
         if (lane < count) x = row_dot(scratch->a, k + seen.key(base + lane) * a.k_row_stride, a.dim) * scale;
         const float next = fmaxf(top, wave_max(x));
         const float old = top == next ? 1.0f : exp2f(top - next);
-        const float p = lane < count ? exp2f(x - next) : 0.0f;
+        // Of -inf before any other score, no share (alone, 0 / 0 in the end).
+        const float p = x != -INFINITY ? exp2f(x - next) : 0.0f;
         top = next;
         sum = sum * old + wave_sum(p);
         wave_fence();
@@ -240,8 +241,8 @@ __device__ inline void grad_query_row(const lattice_attention& a, const AttnSequ
 
 // grad_k and grad_v of one key row and key head: states holds (lse, delta) by
 // key head, row and head, channels from_dim .. to_dim are written; over the
-// queries that see it
-// and the heads that share it, (query, head) pairs 64 at a time, one a lane.
+// queries that see it and the heads that share it, (query, head) pairs 64 at a
+// time, one a lane.
 template <typename T>
 __device__ inline void grad_key_row(const lattice_attention& a, const AttnSequence& s, int j, int kv,
                                     const float* lse, const float2* states, const T* grad_out, T* grad_k, T* grad_v,

@@ -488,6 +488,7 @@ extern "C" int lattice_hip_layer_norm(int dtype, const void* x, long long x_stri
     LATTICE_REQUIRE(dtype == LATTICE_F32 || dtype == LATTICE_F16 || dtype == LATTICE_BF16,
                     "layer norm supports float32, float16 and bfloat16.");
     LATTICE_REQUIRE(rows >= 0 && channels > 0 && x_stride >= 0, "layer norm shapes must be positive.");
+    LATTICE_REQUIRE(channels < 1 << 30, "layer norm takes up to 2^30 - 1 channels.");
     LATTICE_REQUIRE(eps >= 0.0f, "eps must be non-negative.");
     if (rows == 0) return LATTICE_OK;
     LATTICE_REQUIRE(x && y, "layer norm pointers must be non-null.");
@@ -514,6 +515,7 @@ extern "C" int lattice_hip_layer_norm_grad(int dtype, const void* grad_y, long l
                     "layer norm supports float32, float16 and bfloat16.");
     LATTICE_REQUIRE(rows >= 0 && channels > 0 && x_stride >= 0 && grad_y_stride >= 0,
                     "layer norm shapes must be positive.");
+    LATTICE_REQUIRE(channels < 1 << 30, "layer norm takes up to 2^30 - 1 channels.");
     const bool sums = grad_weight || grad_bias;
     LATTICE_REQUIRE(rows == 0 || (grad_y && x && statistics && grad_x), "layer norm pointers must be non-null.");
     LATTICE_REQUIRE(!sums || rows == 0 ||

@@ -282,6 +282,26 @@ def test_what_is_not_seen_never_arrives(value, dtype):
             assert not torch.isfinite(got[0][40:51]).all()
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows, start', ((200, 100), (9000, 4100)))
+def test_scores_of_minus_infinity(rows, start, dtype):
+    """Keys whose scores are -inf have no share, also in rows that are made
+    again since a key that they do not see is not finite: such a row starts
+    with 64 and more of the former."""
+    gen = torch.Generator(device='cuda').manual_seed(17)
+    q, k, v = (_normal(gen, dtype, rows, 4, 32) for _ in 'qkv')
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[max(0, start - 200):start, :, 0] = float('-inf')
+    k[start + 80] = float('nan')
+    v[start + 80] = float('nan')
+    got = _ops().window_attention(q, k, v, left=170, right=0,
+                                  offsets=_offsets((rows,)))
+    at = slice(start, start + 80)
+    want, bound = attention_f64(q[at], k[at], v[at], [(0, 80, 0, 80)], 170, 0,
+                                0, 32 ** -0.5)[0]
+    assert_within(got[at], want, bound)
+
+
 def test_gradient_against_differences():
     gen = torch.Generator(device='cuda').manual_seed(6)
     leaves = [_normal(gen, torch.float32, 60, h, 16).requires_grad_()
