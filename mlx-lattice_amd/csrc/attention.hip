@@ -190,6 +190,21 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
     }
 }
 
+// Starts the copy of tile `index` + 1 (below `to`) into `next` and adds tile
+// `index`, which lies in `tile`.  That the two do not overlap lets the reads of
+// one pass the copies of the other: without the qualifiers the compiler waits
+// for all copies before it reads a transposed operand.
+template <typename T, int DP, int KT, typename Source>
+__device__ __forceinline__ void attend_step(const lattice_attention& a, AttnState<T, DP>& state,
+                                            const AttnOperand<T, DP>& q, const Source& source,
+                                            const AttnTiles& tiles, int index, int to, char* __restrict__ next,
+                                            const char* __restrict__ tile, float scale, int nk, const AttnRows& w,
+                                            const AttnMask& mask) {
+    if (index + 1 < to) source.copy(next, tiles.tile(index + 1) * KT, nk);
+    attend_tile<T, DP, KT>(a, state, q, tile, tile + AttnTile<T, DP, KT>::kBytes, scale, nk, w, mask,
+                           tiles.tile(index) * KT);
+}
+
 // 128 rows a block, 32 a wave, over tiles of KT keys that the waves share.
 // Double-buffered: a tile is copied to LDS while the one before is used.
 template <typename T, int DP, int KT>
@@ -219,15 +234,13 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
     const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
     const KeyTiles<T, DP, KT, kAttnBlock> source(a, s, kv, threadIdx.x);
-    const auto copy = [&](int index) {
-        source.copy(shared + (index & 1) * 2 * Tile::kBytes, tiles.tile(index) * KT, s.nk);
-    };
-    if (from < to) copy(from);
+    if (from < to) source.copy(shared + (from & 1) * 2 * Tile::kBytes, tiles.tile(from) * KT, s.nk);
+    wait_for_copies();
     __syncthreads();
     for (int index = from; index < to; ++index) {
-        if (index + 1 < to) copy(index + 1);
-        const char* at = shared + (index & 1) * 2 * Tile::kBytes;
-        attend_tile<T, DP, KT>(a, state, q, at, at + Tile::kBytes, scale, s.nk, w, mask, tiles.tile(index) * KT);
+        attend_step<T, DP, KT>(a, state, q, source, tiles, index, to, shared + (~index & 1) * 2 * Tile::kBytes,
+                               shared + (index & 1) * 2 * Tile::kBytes, scale, s.nk, w, mask);
+        wait_for_copies();
         __syncthreads();
     }
     write_rows<T, DP>(a, s, w, state, splits > 1, split, part, out, kept,
@@ -270,7 +283,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     for (int index = from + wave; index < to; index += kFewWaves) {
         const int j0 = tiles.tile(index) * KT;
         source.copy(mine, j0, s.nk);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wait_for_copies();
         wave_fence();
         attend_tile<T, DP, KT>(a, state, q, mine, mine + Tile::kBytes, scale, s.nk, w, mask, j0);
         wave_fence();

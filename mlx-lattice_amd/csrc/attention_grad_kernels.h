@@ -132,6 +132,40 @@ __device__ inline long long query_state(const lattice_attention& a, uint32_t gro
     return (static_cast<long long>(kv) * a.queries + row) * group + (head - kv * group);
 }
 
+// Adds the keys j0 .. of a tile to the sums of a wave's 32 rows.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void add_keys(const lattice_attention& a, int nk, const AttnOperand<T, DP>& q,
+                                         const AttnOperand<T, DP>& d, const char* k_tile, float scale, float log_sum,
+                                         float along, const AttnRows& w, const AttnMask& mask, int j0,
+                                         f32x16_attn (&acc)[DP / 32], SlopeScale<T>& slopes) {
+    typedef AttnTile<T, DP, KT> Tile;
+    const char* v_tile = k_tile + Tile::kBytes;
+#pragma unroll
+    for (int row0 = 0; row0 < KT; row0 += 32) {
+        const AttnView view = attn_view(a, nk, w.p_low, w.p_high, j0 + row0, 32);
+        if (view == kSeesNone) continue;
+        f32x16_attn p = tile_product<Tile, T, DP>(k_tile, row0, q, f32x16_attn{});
+        f32x16_attn dp = tile_product<Tile, T, DP>(v_tile, row0, d, f32x16_attn{});
+        if (view == kSeesSome) mask.apply(p, j0 + row0, j0 + row0 < a.sinks);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
+        add_slopes<Tile, T>(acc, slopes, k_tile, row0, dp);
+    }
+}
+
+// The same, with the copy of the keys j_next .. (negative: none) into `next`
+// under way: see attend_step.
+template <typename T, int DP, int KT, typename Source>
+__device__ __forceinline__ void grad_query_step(const lattice_attention& a, int nk, const Source& source, int j_next,
+                                                char* __restrict__ next, const AttnOperand<T, DP>& q,
+                                                const AttnOperand<T, DP>& d, const char* __restrict__ tile,
+                                                float scale, float log_sum, float along, const AttnRows& w,
+                                                const AttnMask& mask, int j0, f32x16_attn (&acc)[DP / 32],
+                                                SlopeScale<T>& slopes) {
+    if (j_next >= 0) source.copy(next, j_next, nk);
+    add_keys<T, DP, KT>(a, nk, q, d, tile, scale, log_sum, along, w, mask, j0, acc, slopes);
+}
+
 // grad_q, laid out as the forward pass; keeps lse and delta for the keys' pass.
 // FEW: 32 rows a block, whose tiles the waves take in turn, each with its own
 // copies; their sums are joined.
@@ -194,35 +228,25 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __rest
     const KeyTiles<T, DP, KT, kThreads> source(a, s, kv, FEW ? lane_id() : threadIdx.x);
     if constexpr (!FEW) {
         if (tiles.count) source.copy(shared, tiles.tile(0) * KT, s.nk);
+        wait_for_copies();
         __syncthreads();
     }
     for (int index = FEW ? wave : 0; index < tiles.count; index += kStep) {
+        char* tile = shared + (FEW ? wave : index & 1) * 2 * Tile::kBytes;
         const int j0 = tiles.tile(index) * KT;
-        char* k_tile = shared + (FEW ? wave : index & 1) * 2 * Tile::kBytes;
-        const char* v_tile = k_tile + Tile::kBytes;
         if constexpr (FEW) {
-            source.copy(k_tile, j0, s.nk);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            source.copy(tile, j0, s.nk);
+            wait_for_copies();
             wave_fence();
-        } else if (index + 1 < tiles.count) {
-            source.copy(shared + ((index + 1) & 1) * 2 * Tile::kBytes, tiles.tile(index + 1) * KT, s.nk);
-        }
-#pragma unroll
-        for (int row0 = 0; row0 < KT; row0 += 32) {
-            const AttnView view = attn_view(a, s.nk, w.p_low, w.p_high, j0 + row0, 32);
-            if (view == kSeesNone) continue;
-            f32x16_attn p = tile_product<Tile, T, DP>(k_tile, row0, q, f32x16_attn{});
-            f32x16_attn dp = tile_product<Tile, T, DP>(v_tile, row0, d, f32x16_attn{});
-            if (view == kSeesSome) mask.apply(p, j0 + row0, j0 + row0 < a.sinks);
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                dp[r] = __builtin_amdgcn_exp2f(p[r] * scale - log_sum) * (dp[r] - along);
-            add_slopes<Tile, T>(acc, slopes, k_tile, row0, dp);
-        }
-        if constexpr (FEW)
+            add_keys<T, DP, KT>(a, s.nk, q, d, tile, scale, log_sum, along, w, mask, j0, acc, slopes);
             wave_fence();
-        else
+        } else {
+            const int next = index + 1 < tiles.count ? tiles.tile(index + 1) * KT : -1;
+            grad_query_step<T, DP, KT>(a, s.nk, source, next, shared + (~index & 1) * 2 * Tile::kBytes, q, d, tile,
+                                       scale, log_sum, along, w, mask, j0, acc, slopes);
+            wait_for_copies();
             __syncthreads();
+        }
     }
     if constexpr (SlopeScale<T>::kUsed) scale_sums(acc, 1.0f / slopes.factor());
     if constexpr (FEW) {
@@ -394,6 +418,20 @@ __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k
     }
 }
 
+// The same (none: nothing is added), with the copy of the queries r_next ..
+// into `next` under way: see attend_step.  What it holds of their states.
+template <typename T, int DP, int QT, typename Source>
+__device__ __forceinline__ typename Source::State
+grad_key_step(Source& source, bool more, uint32_t r_next, uint32_t rows, char* __restrict__ next,
+              const char* __restrict__ tile, const AttnOperand<T, DP>& k, const AttnOperand<T, DP>& v, float scale,
+              int lo, int hi, bool none, bool masked, f32x16_attn (&acc_k)[DP / 32], f32x16_attn (&acc_v)[DP / 32],
+              SlopeScale<T>& slopes) {
+    typename Source::State state{};
+    if (more) state = source.copy(next, r_next, rows);
+    if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, masked, acc_k, acc_v, slopes);
+    return state;
+}
+
 template <int DP> constexpr int kFirstValues = 2 * DP * 32;
 
 template <int BLOCKS>
@@ -443,7 +481,7 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
         const uint32_t r0 = base + QT * wave;
         if (r0 >= to) break;
         source.store(tile, source.copy(tile, r0, to));
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wait_for_copies();
         wave_fence();
         add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, true, acc_k, acc_v, slopes);
         wave_fence();
@@ -569,20 +607,12 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     constexpr int kStep = FEW ? kAttnWaves : 1;
     if constexpr (!FEW) {
         if (count > 0) source.store(shared, source.copy(shared, first_row(0), rows));
+        wait_for_copies();
         __syncthreads();
     }
     for (int index = FEW ? wave : 0; index < count; index += kStep) {
         char* tile = shared + (FEW ? wave : index & 1) * Queries::kBytes;
-        char* next = shared + ((index + 1) & 1) * Queries::kBytes;
-        typename QueryTiles<T, DP, QT, kThreads>::State state{};
         const uint32_t r0 = first_row(index);
-        if constexpr (FEW) {
-            source.store(tile, source.copy(tile, r0, rows));
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            wave_fence();
-        } else if (index + 1 < count) {
-            state = source.copy(next, first_row(index + 1), rows);
-        }
         // In the window, or past it: of the first keys alone.
         const bool outside = index >= window_tiles;
         const int lo = !outside ? j - a.right : j < a.sinks ? j + a.left + 1 : INT_MAX;
@@ -592,11 +622,19 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
         const bool none = outside ? j_wave >= a.sinks || p_high <= j_wave + a.left
                                   : p_high < j_wave - a.right || p_low > j_wave + 31 + a.left;
         const bool all = !outside && j_wave + 31 <= p_low + a.right && j_wave >= p_high - a.left;
-        if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, !all, acc_k, acc_v, slopes);
         if constexpr (FEW) {
+            source.store(tile, source.copy(tile, r0, rows));
+            wait_for_copies();
+            wave_fence();
+            if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, !all, acc_k, acc_v, slopes);
             wave_fence();
         } else {
-            if (index + 1 < count) source.store(next, state);
+            char* next = shared + (~index & 1) * Queries::kBytes;
+            const bool more = index + 1 < count;
+            const auto state = grad_key_step<T, DP, QT>(source, more, more ? first_row(index + 1) : 0, rows, next, tile,
+                                                        k, v, scale, lo, hi, none, !all, acc_k, acc_v, slopes);
+            if (more) source.store(next, state);
+            wait_for_copies();
             __syncthreads();
         }
     }

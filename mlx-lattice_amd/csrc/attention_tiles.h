@@ -108,6 +108,9 @@ struct AttnTile {
     }
 };
 
+// Until the copies that this wave started are in LDS.
+__device__ inline void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // Transposed operand of a product over rows: channel 32 block + L % 32 of the
 // tile's rows in the order in which a lane's registers 8 step .. 8 step + 7
 // hold them: rows 16 step + 4 h + 0 .. 3 and 16 step + 8 + 4 h + 0 .. 3.
