@@ -19,10 +19,11 @@ struct RowPartition {
     const int32_t* offsets;
     int count, rows;
 
+    // Read whether needed or not, so that reads of several need not wait for
+    // each other.
     __device__ int start(int e) const {
-        if (e <= 0) return 0;
-        if (e > count + 1) return rows;
-        return min(max(offsets[e - 1], 0), rows);
+        const int at = min(max(offsets[min(max(e - 1, 0), count)], 0), rows);
+        return e <= 0 ? 0 : e > count + 1 ? rows : at;
     }
     __device__ bool real(int e) const { return e >= 1 && e <= count; }
 

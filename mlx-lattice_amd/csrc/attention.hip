@@ -82,7 +82,7 @@ __device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T,
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, s[part][r]);
     }
-    most = fmaxf(most, other_half(most)) * scale;
+    most = halves_max(most) * scale;
     if (__any(most > state.top + kAttnLag)) {
         const float next = fmaxf(state.top, most);
         state.rescale(__builtin_amdgcn_exp2f(state.top - next));
@@ -134,7 +134,7 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
                                   AttnState<T, DP>& state, bool partial, int split, const AttnPart& part, T* out,
                                   const AttnKept<T>& kept, AttnRowScratch* scratch) {
     const int half = lane_id() >> 5;
-    const float sum = state.sum + other_half(state.sum);
+    const float sum = halves_sum(state.sum);
     const long long at = (static_cast<long long>(s.q0) + w.i) * a.heads + w.head;
     if (partial) {
         if (!w.valid) return;
@@ -190,6 +190,11 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
     }
 }
 
+// The first of `count` tiles (at most 2^24) that split `split` of at most 64 has.
+__device__ inline int split_tile(int count, int split, int splits) {
+    return splits == 1 ? count * split : static_cast<int>(static_cast<uint32_t>(count) * split / splits);
+}
+
 // Starts the copy of tile `index` + 1 (below `to`) into `next` and adds tile
 // `index`, which lies in `tile`.  That the two do not overlap lets the reads of
 // one pass the copies of the other: without the qualifiers the compiler waits
@@ -231,8 +236,7 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     const int p_low = static_cast<int>(t.first / group) + s.shift();
     const int p_high = static_cast<int>((min(t.first + 32 * kAttnWaves, t.rows) - 1) / group) + s.shift();
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, p_low, p_high);
-    const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
-    const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
+    const int from = split_tile(tiles.count, split, splits), to = split_tile(tiles.count, split + 1, splits);
     const KeyTiles<T, DP, KT, kAttnBlock> source(a, s, kv, threadIdx.x);
     if (from < to) source.copy(shared + (from & 1) * 2 * Tile::kBytes, tiles.tile(from) * KT, s.nk);
     wait_for_copies();
@@ -276,8 +280,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     AttnState<T, DP> state;
     state.clear();
     const AttnTiles tiles = attn_tiles<KT>(a, s.nk, w.p_low, w.p_high);
-    const int from = static_cast<int>(static_cast<long long>(tiles.count) * split / splits);
-    const int to = static_cast<int>(static_cast<long long>(tiles.count) * (split + 1) / splits);
+    const int from = split_tile(tiles.count, split, splits), to = split_tile(tiles.count, split + 1, splits);
     const KeyTiles<T, DP, KT, kWave> source(a, s, kv, lane_id());
     char* mine = shared + wave * 2 * Tile::kBytes;
     for (int index = from + wave; index < to; index += kFewWaves) {
@@ -291,7 +294,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     // Every wave's sums to the largest maximum, then pairwise into the first
     // wave's.
     const int lane = lane_id();
-    state.sum += other_half(state.sum);
+    state.sum = halves_sum(state.sum);
     __syncthreads();
     float2* states = reinterpret_cast<float2*>(shared);
     float* sums = reinterpret_cast<float*>(shared + kFewWaves * 32 * sizeof(float2));

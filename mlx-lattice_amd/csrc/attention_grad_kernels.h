@@ -213,7 +213,7 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __rest
                     along += static_cast<float>(o.f[c][i]) * static_cast<float>(d.f[c][i]);
             }
         }
-        along += other_half(along);
+        along = halves_sum(along);
     }
     const float log_sum = w.valid ? lse[at] : INFINITY;
     if (w.valid && half == 0 && (!FEW || wave == 0))

@@ -229,7 +229,19 @@ __device__ inline f32x16_attn tile_product(const char* tile, int row0, const Att
     return c;
 }
 
-__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
+// The maximum and sum over both halves of a wave, in both.
+__device__ inline float2 both_halves(float v) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return float2{__uint_as_float(halves[0]), __uint_as_float(halves[1])};
+}
+__device__ inline float halves_max(float v) {
+    const float2 both = both_halves(v);
+    return fmaxf(both.x, both.y);
+}
+__device__ inline float halves_sum(float v) {
+    const float2 both = both_halves(v);
+    return both.x + both.y;
+}
 
 // Row of a result's register r.
 __device__ inline int result_row(int r) { return 8 * (r / 4) + 4 * (lane_id() >> 5) + r % 4; }
