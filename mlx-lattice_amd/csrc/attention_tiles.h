@@ -263,29 +263,38 @@ __device__ inline bool finite_columns(const f32x16_attn (&acc)[BLOCKS], float fa
     return largest < 0x7f800000u;
 }
 
-// What a lane's query sees, as a test of two instructions: lo <= j <= lo +
-// span, or a first key.
+// What a lane's query sees: lo <= j <= hi, or a first key (j <= hi).
 struct AttnMask {
     int lo, hi, sinks;
-    uint32_t span;
     __device__ AttnMask(const lattice_attention& a, int nk, int p)
-        : lo(p - a.left), hi(min(nk - 1, p + a.right)), sinks(a.sinks), span(hi - lo) {}
-    // The scores of keys j0 + result_row(r); `first`: some are first keys.
+        : lo(p - a.left), hi(min(nk - 1, p + a.right)), sinks(a.sinks) {}
+    // The scores of keys j0 + result_row(r); `first`: some are first keys.  Most
+    // tiles cross one end of the window, and each end has its own test.
     __device__ void apply(f32x16_attn& x, int j0, bool first) const {
         const int j = j0 + 4 * (lane_id() >> 5);
-        if (first) {
-            const int bound = min(sinks - 1, hi);
+        const int most = hi - j, least = lo - j;
+        if (__any(most < kLastRow)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int at = j + 8 * (r / 4) + r % 4;
-                if (static_cast<uint32_t>(at - lo) > span && at > bound) x[r] = -INFINITY;
-            }
-        } else {
-            const uint32_t from = j - lo;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (from + 8 * (r / 4) + r % 4 > span) x[r] = -INFINITY;
+            for (int r = 0; r < 16; ++r) hide(x, r, row(r) > most);
         }
+        if (first) {
+            const int firsts = sinks - j;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) hide(x, r, row(r) < least && row(r) >= firsts);
+        }
+        if (!first && __any(least > 0)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) hide(x, r, row(r) < least);
+        }
+    }
+
+   private:
+    static constexpr int kLastRow = 27;
+    __device__ static constexpr int row(int r) { return 8 * (r / 4) + r % 4; }
+    // In order: 16 tests at once would take more scalar registers than there are.
+    __device__ static void hide(f32x16_attn& x, int r, bool hidden) {
+        x[r] = hidden ? -INFINITY : x[r];
+        if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 };
 
