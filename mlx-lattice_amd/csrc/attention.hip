@@ -155,11 +155,11 @@ __device__ inline void write_rows(const lattice_attention& a, const AttnSequence
         return;
     }
     const bool sees = attn_seen(a, s.nk, w.p).total() > 0;
-    const float inv = 1.0f / sum;
+    const float inv = sees ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int b = 0; b < AttnState<T, DP>::kBlocks; ++b) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) state.acc[b][r] = sees ? state.acc[b][r] * inv : 0.0f;
+        for (int r = 0; r < 16; ++r) state.acc[b][r] *= inv;
     }
     const uint64_t spoilt = ballot(w.valid && !finite_columns(state.acc, 1.0f));
     uint32_t again = static_cast<uint32_t>(spoilt) | static_cast<uint32_t>(spoilt >> 32);

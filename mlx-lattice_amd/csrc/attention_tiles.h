@@ -209,12 +209,14 @@ struct AttnOperand {
     __device__ void load(const T* row, int dim, bool valid, bool negate) {
         const int half = lane_id() >> 5;
         constexpr int kShare = AttnMath<T>::kStep / 2;
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+        const Words signs = Words{} + (!negate ? 0u : sizeof(T) == 2 ? 0x80008000u : 0x80000000u);
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
             const int d = (2 * c + half) * kShare;
-            f[c] = Frag{};
-            if (valid && d < dim) f[c] = *reinterpret_cast<const Frag*>(row + d);
-            if (negate) f[c] = -f[c];
+            Words words{};
+            if (valid && d < dim) words = *reinterpret_cast<const Words*>(row + d);
+            f[c] = __builtin_bit_cast(Frag, words ^ signs);
         }
     }
 };
