@@ -493,13 +493,16 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
 }
 
 // Adds the parts of 32 first keys and eight channels of a sequence and key
-// head, the window's first and the others in slot order: 256 values of dk and
-// as many of dv, which lie side by side in a part.
+// head: 256 values of dk and as many of dv, which lie side by side in a part.
+// Four groups of threads take a quarter of the slots each, in slot order, after
+// the window's part; their sums are added in order.
+constexpr int kJoinGroups = 4, kJoinBlock = kJoinGroups * kAttnBlock;
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAttnBlock)
+__global__ void __launch_bounds__(kJoinBlock)
 join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2* __restrict__ states,
                 const T* __restrict__ grad_out, FirstParts parts, T* __restrict__ grad_k, T* __restrict__ grad_v) {
     __shared__ AttnRowScratch scratch[kAttnWaves];
+    __shared__ float2 sums[kJoinGroups - 1][kAttnBlock];
     __shared__ uint32_t spoilt;
     const uint32_t group = a.heads / a.kv_heads;
     const int e = blockIdx.x + 1, kv = blockIdx.y;
@@ -507,18 +510,25 @@ join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2
     const AttnSequence s = attn_sequence(a, e);
     const int keys = min(a.sinks, s.nk);
     if (j0 >= keys || d0 >= a.dim) return;
-    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    const uint32_t quarter = threadIdx.x / kAttnBlock, thread = threadIdx.x % kAttnBlock;
+    const int lane = lane_id(), wave = thread / kWave;
     const int j = j0 + (lane & 31);
     const uint32_t slot = s.q0 * group / kFirstRows + e, slots = (s.nq * group + kFirstRows - 1) / kFirstRows;
-    const int of_k = eighth * kAttnBlock + threadIdx.x, of_v = of_k + DP * 32;
-    const float* at = parts.window_of(a, e, kv, tile, kFirstValues<DP>);
-    float sum_k = at[of_k], sum_v = at[of_v];
+    const int of_k = eighth * kAttnBlock + thread, of_v = of_k + DP * 32;
+    float sum_k = 0.0f, sum_v = 0.0f;
+    if (quarter == 0) {
+        const float* at = parts.window_of(a, e, kv, tile, kFirstValues<DP>);
+        sum_k = at[of_k];
+        sum_v = at[of_v];
+    }
     constexpr int kAhead = 8;  // parts in flight
-    for (uint32_t u = 0; u < slots; u += kAhead) {
+    const uint32_t share_slots = (slots + kJoinGroups - 1) / kJoinGroups;
+    const uint32_t to = min(slots, (quarter + 1) * share_slots);
+    for (uint32_t u = quarter * share_slots; u < to; u += kAhead) {
         float past_k[kAhead], past_v[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const bool here = u + i < slots;
+            const bool here = u + i < to;
             const float* past = parts.past_of(a, slot + (here ? u + i : 0), kv, tile, kFirstValues<DP>);
             past_k[i] = here ? past[of_k] : 0.0f;
             past_v[i] = here ? past[of_v] : 0.0f;
@@ -529,13 +539,23 @@ join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2
             sum_v += past_v[i];
         }
     }
+    if (quarter > 0) sums[quarter - 1][thread] = float2{sum_k, sum_v};
+    if (threadIdx.x == 0) spoilt = 0;
+    __syncthreads();
+    if (quarter == 0) {
+#pragma unroll
+        for (int g = 0; g < kJoinGroups - 1; ++g) {
+            sum_k += sums[g][thread].x;
+            sum_v += sums[g][thread].y;
+        }
+    }
     const float share = __builtin_amdgcn_exp2f(-kShareLog2<T>);
     sum_k *= a.scale * share;
     sum_v *= share;
-    if (threadIdx.x == 0) spoilt = 0;
+    if (quarter == 0 && j < keys && !(fabsf(sum_k) < INFINITY && fabsf(sum_v) < INFINITY))
+        atomicOr(&spoilt, 1u << (lane & 31));
     __syncthreads();
-    if (j < keys && !(fabsf(sum_k) < INFINITY && fabsf(sum_v) < INFINITY)) atomicOr(&spoilt, 1u << (lane & 31));
-    __syncthreads();
+    if (quarter > 0) return;
     const uint32_t again = spoilt;
     if (j < keys && !(again >> (lane & 31) & 1)) {
         const int d = d0 + 4 * (lane >> 5) + wave;
@@ -724,7 +744,7 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
                        : launch_grad_keys<T, DP, false>(a, lse, states, grad_out, parts, grad_k, grad_v, stream);
     if (rc != LATTICE_OK) return rc;
     if (l.first_tiles && a.sequences) {
-        join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles * (DP / 8)), kAttnBlock, 0, stream>>>(
+        join_first_keys<T, DP><<<dim3(a.sequences, a.kv_heads, l.first_tiles * (DP / 8)), kJoinBlock, 0, stream>>>(
             a, lse, states, grad_out, parts, grad_k, grad_v);
         LATTICE_LAUNCH_CHECK();
     }
