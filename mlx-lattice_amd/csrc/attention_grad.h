@@ -20,9 +20,9 @@ struct FirstParts {
         return window + ((static_cast<long long>(e) * a.kv_heads + kv) * tiles + tile) * values;
     }
 };
-// Pairs of a slot.  (The parts of 60k rows of 4 heads of 64 over 2: 17.5 us, in
-// slots of 1024 20.5, of 256 23.4; of 20k rows of 4 heads of 32, fp32: 17.6, 28.1
-// and 15.6; their sum grows with the number of slots.)
+// Pairs of a slot.  (The parts of 60k rows of 4 heads of 64 over 2, one block a
+// unit: 17.5 us, in slots of 1024 20.5, of 256 23.4; of 20k rows of 4 heads of
+// 32, fp32: 17.6, 28.1 and 15.6; their sum grows with the number of slots.)
 constexpr uint32_t kFirstRows = 512;
 
 // Whether tiles of 128 of `rows` rows would leave units idle: below one block a

@@ -360,13 +360,19 @@ struct QueryTiles {
     }
 };
 
-// Adds the queries of a tile to a wave's 32 keys; `masked`: a lane's key is
-// seen from the positions lo .. hi alone.  (A form of its own for tiles without
-// a mask costs more registers than it saves branches: 855 for 787 us at heads
-// of 128, 133 for 121 at 64.)
+// Which positions of a tile a lane's key is seen from: lo .. hi; `below`,
+// `above`: some tile's position is below some lane's lo, above some hi.
+struct QueryMask {
+    int lo, hi;
+    bool below, above;
+};
+
+// Adds the queries of a tile to a wave's 32 keys.  (A form of its own for tiles
+// without a mask costs more registers than it saves branches: 855 for 787 us at
+// heads of 128, 133 for 121 at 64.)
 template <typename T, int DP, int QT>
 __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k, const AttnOperand<T, DP>& v,
-                                   float scale, int lo, int hi, bool masked, f32x16_attn (&acc_k)[DP / 32],
+                                   float scale, const QueryMask& mask, f32x16_attn (&acc_k)[DP / 32],
                                    f32x16_attn (&acc_v)[DP / 32], SlopeScale<T>& slopes) {
     typedef QueryTile<T, DP, QT> Queries;
     typedef typename Queries::Tile Tile;
@@ -394,12 +400,25 @@ __device__ inline void add_queries(const char* tile, const AttnOperand<T, DP>& k
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int row = 32 * part + 8 * g + 4 * half;
-            if (masked) {
+            if (mask.below || mask.above) {
                 const int4 at = *reinterpret_cast<const int4*>(states + 2 * QT + row);
                 const int position[4] = {at.x, at.y, at.z, at.w};
+                // One end at a time where registers are left for the branches (8 heads of
+                // 80: 122.5 -> 117.7 us; of 128: 782 -> 818).
+                if constexpr (DP < 128) {
+                    if (mask.below) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (position[i] < lo || position[i] > hi) p[4 * g + i] = -INFINITY;
+                        for (int i = 0; i < 4; ++i) p[4 * g + i] = position[i] < mask.lo ? -INFINITY : p[4 * g + i];
+                    }
+                    if (mask.above) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[4 * g + i] = position[i] > mask.hi ? -INFINITY : p[4 * g + i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (position[i] < mask.lo || position[i] > mask.hi) p[4 * g + i] = -INFINITY;
+                }
             }
             const float4 lse = *reinterpret_cast<const float4*>(states + row);
             const float log_sum[4] = {lse.x, lse.y, lse.z, lse.w};
@@ -424,11 +443,11 @@ template <typename T, int DP, int QT, typename Source>
 __device__ __forceinline__ typename Source::State
 grad_key_step(Source& source, bool more, uint32_t r_next, uint32_t rows, char* __restrict__ next,
               const char* __restrict__ tile, const AttnOperand<T, DP>& k, const AttnOperand<T, DP>& v, float scale,
-              int lo, int hi, bool none, bool masked, f32x16_attn (&acc_k)[DP / 32], f32x16_attn (&acc_v)[DP / 32],
+              const QueryMask& mask, bool none, f32x16_attn (&acc_k)[DP / 32], f32x16_attn (&acc_v)[DP / 32],
               SlopeScale<T>& slopes) {
     typename Source::State state{};
     if (more) state = source.copy(next, r_next, rows);
-    if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, masked, acc_k, acc_v, slopes);
+    if (!none) add_queries<T, DP, QT>(tile, k, v, scale, mask, acc_k, acc_v, slopes);
     return state;
 }
 
@@ -447,9 +466,15 @@ __device__ inline void store_part(float* to, const f32x16_attn (&acc_k)[BLOCKS],
     }
 }
 
+// Two waves a SIMD leave 256 registers a lane: enough up to heads of 96 (25k
+// rows of 8 heads of 80, window 330: 123 us, with one wave 228).  At 128 the
+// sums alone take half of them and a second wave spills (8k rows of 16 heads,
+// window 4096: 1735 us, with one wave 787; with the keys read from LDS 959).
+template <typename T, int DP> constexpr int kKeyWaves = DP <= 64 || (DP <= 96 && sizeof(T) == 2) ? 2 : 1;
+
 // The part of a slot: each wave takes every fourth tile of 32 pairs.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kAttnBlock)
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(kAttnBlock, WAVES)
 grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T* __restrict__ grad_out,
                 FirstParts parts) {
     constexpr int QT = 32;
@@ -477,13 +502,14 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
     const uint32_t from = max(t.first, static_cast<uint32_t>(min(i_from, s.nq)) * group / QT * QT);
     const uint32_t to = min(t.first + kFirstRows, t.rows);
     char* tile = shared + wave * Queries::kBytes;
+    const QueryMask mask{j + a.left + 1, INT_MAX, true, false};
     for (uint32_t base = from; base < to; base += QT * kAttnWaves) {
         const uint32_t r0 = base + QT * wave;
         if (r0 >= to) break;
         source.store(tile, source.copy(tile, r0, to));
         wait_for_copies();
         wave_fence();
-        add_queries<T, DP, QT>(tile, k, v, scale, j + a.left + 1, INT_MAX, true, acc_k, acc_v, slopes);
+        add_queries<T, DP, QT>(tile, k, v, scale, mask, acc_k, acc_v, slopes);
         wave_fence();
     }
     if constexpr (SlopeScale<T>::kUsed) scale_sums(acc_k, 1.0f / slopes.factor());
@@ -571,12 +597,6 @@ join_first_keys(lattice_attention a, const float* __restrict__ lse, const float2
     }
 }
 
-// Two waves a SIMD leave 256 registers a lane: enough up to heads of 96 (25k
-// rows of 8 heads of 80, window 330: 123 us, with one wave 228).  At 128 the
-// sums alone take half of them and a second wave spills (8k rows of 16 heads,
-// window 4096: 1735 us, with one wave 787; with the keys read from LDS 959).
-template <typename T, int DP> constexpr int kKeyWaves = DP <= 64 || (DP <= 96 && sizeof(T) == 2) ? 2 : 1;
-
 // grad_k and grad_v: 128 keys a block, 32 a wave, over the tiles of (query,
 // head) pairs that see them.  FEW: 32 keys a block, whose tiles the waves take in
 // turn, each with its own copies; their sums are joined.
@@ -641,18 +661,18 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
         const int p_high = static_cast<int>(source.by_group(min(r0 + QT, rows) - 1)) + s.shift();
         const bool none = outside ? j_wave >= a.sinks || p_high <= j_wave + a.left
                                   : p_high < j_wave - a.right || p_low > j_wave + 31 + a.left;
-        const bool all = !outside && j_wave + 31 <= p_low + a.right && j_wave >= p_high - a.left;
+        const QueryMask mask{lo, hi, outside || p_low < j_wave + 31 - a.right, !outside && p_high > j_wave + a.left};
         if constexpr (FEW) {
             source.store(tile, source.copy(tile, r0, rows));
             wait_for_copies();
             wave_fence();
-            if (!none) add_queries<T, DP, QT>(tile, k, v, scale, lo, hi, !all, acc_k, acc_v, slopes);
+            if (!none) add_queries<T, DP, QT>(tile, k, v, scale, mask, acc_k, acc_v, slopes);
             wave_fence();
         } else {
             char* next = shared + (~index & 1) * Queries::kBytes;
             const bool more = index + 1 < count;
             const auto state = grad_key_step<T, DP, QT>(source, more, more ? first_row(index + 1) : 0, rows, next, tile,
-                                                        k, v, scale, lo, hi, none, !all, acc_k, acc_v, slopes);
+                                                        k, v, scale, mask, none, acc_k, acc_v, slopes);
             if (more) source.store(next, state);
             wait_for_copies();
             __syncthreads();
@@ -733,7 +753,7 @@ int launch_grad(const lattice_attention& a, const GradLayout& l, const T* out, c
     if (l.first_tiles) {
         constexpr size_t kLds = std::max<size_t>(kAttnWaves * QueryTile<T, DP, 32>::kBytes, kJoinBytes<DP>);
         static_assert(kLds <= 160 * 1024);
-        const auto kernel = grad_first_keys<T, DP>;
+        const auto kernel = grad_first_keys<T, DP, kKeyWaves<T, DP>>;
         LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
         kernel<<<dim3(l.first_slots, a.kv_heads, l.first_tiles), kAttnBlock, kLds, stream>>>(a, states, grad_out,
                                                                                             parts);
