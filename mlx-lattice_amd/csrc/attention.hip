@@ -17,10 +17,10 @@
 // Bound by the exponentials and the other vector instructions of the softmax,
 // 7 issue slots a score beside the products' 4 (heads of 32) to 16 (128) cycles;
 // few queries by reading the keys.  120,000 rows of 8 heads of 32, window 257,
-// fp16: 131 us (246 TFLOP/s).  16,384 causal rows of 16 heads of 128 over 4,
-// window 4096, bf16: 569 us under the profiler, 540 without (894 TFLOP/s; a
+// fp16: 127 us (249 TFLOP/s).  16,384 causal rows of 16 heads of 128 over 4,
+// window 4096, bf16: 557 us under the profiler, 534 without (904 TFLOP/s; a
 // library product of 8192^3 1191).  One query of 16 heads of 128 over 4 against
-// 32 caches of 24,000 keys, fp16: 298 us (5.5 TB/s).
+// 32 caches of 24,000 keys, fp16: 297 us (5.5 TB/s).
 
 #include "attention_tiles.h"
 
@@ -423,7 +423,7 @@ inline AttnLayout attn_layout(const lattice_attention& a) {
 template <typename T, int DP>
 int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPart& part, T* out,
                   const AttnKept<T>& kept, hipStream_t stream) {
-    // Tiles twice as large are no faster (scan of heads of 32: 152 us for 143).
+    // Tiles twice as large are no faster (120k rows of heads of 32: 132 us for 127).
     constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
     typedef AttnTile<T, DP, kTile> Tile;
     const dim3 grid(static_cast<unsigned>(l.slots), a.kv_heads, l.splits);

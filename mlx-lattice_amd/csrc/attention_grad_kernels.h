@@ -2,9 +2,9 @@
 //
 // Bound as the forward pass by the vector instructions between the products (an
 // exponential, four others and two roundings a score and pass).  60,001 rows of
-// 4 heads of 64 over 2, window 513, bf16: grad_q 85 us, grad_k and grad_v 119,
-// the first keys' long sums 21 + 10; 20,000 rows of 4 heads of 32, window 128,
-// fp32: 62, 67, 29 + 4 (fp32 products have a sixteenth of the 16-bit rate, and
+// 4 heads of 64 over 2, window 513, bf16: grad_q 87 us, grad_k and grad_v 114,
+// the first keys' long sums 16 + 10; 20,000 rows of 4 heads of 32, window 128,
+// fp32: 60, 65, 17 + 4 (fp32 products have a sixteenth of the 16-bit rate, and
 // eight or nine short steps leave a block waiting for its copies).
 #pragma once
 
