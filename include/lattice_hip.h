@@ -811,7 +811,9 @@ int lattice_hip_rotary_positions(int dtype, const void* x,
  * elements, unit stride in dim, rows in whole 16-byte pieces on 16-byte
  * boundaries, rows under 4 MiB apart and the query heads of a key head within
  * 512 MiB; dim up to 128.  Head h reads key head h * kv_heads / heads.
- * Offsets are device int32 and clamped to the rows there are. */
+ * Offsets are device int32, must not decrease, and are clamped to the rows
+ * there are; offsets that decrease leave results unspecified, some of them
+ * unwritten, but nothing outside the tensors is touched. */
 typedef struct lattice_attention {
     int dtype, queries, keys, heads, kv_heads, dim, sequences;
     int left, right, sinks;

@@ -615,7 +615,7 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const int e = key_rows(a).find(blockIdx.x, slot_of);
     const AttnSequence s = attn_sequence(a, e);
     const int owned = max(0, key_rows(a).start(e + 1) - s.k0);
-    const int j0 = static_cast<int>(blockIdx.x - slot_of(s.k0, e)) * kKeys;
+    const int j0 = slot_first<kKeys>(blockIdx.x, slot_of(s.k0, e), owned);
     if (j0 >= owned) return;
     const int j_wave = j0 + (FEW ? 0 : 32 * wave), j = j_wave + (lane & 31);
     const bool valid = j < s.nk;

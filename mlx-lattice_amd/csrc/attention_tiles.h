@@ -355,6 +355,15 @@ __device__ inline AttnRows attn_rows(const AttnSequence& s, int kv, uint32_t gro
     return w;
 }
 
+// The first of `rows` rows of a slot of M, where the sequence's slots begin at
+// `start`: `rows` itself, none, where the slot is not the sequence's.  Offsets
+// that decrease can lead the search to a sequence that starts past the slot.
+template <int M>
+__device__ inline uint32_t slot_first(uint32_t slot, uint32_t start, uint32_t rows) {
+    const uint32_t tile = slot - start;
+    return tile < (rows + M - 1) / M ? tile * M : rows;
+}
+
 // Which sequence, tile of M rows and key head a block has.
 struct AttnSlot {
     AttnSequence s;
@@ -368,7 +377,7 @@ __device__ inline AttnSlot attn_slot(const lattice_attention& a, uint32_t group,
     AttnSlot t;
     t.s = attn_sequence(a, e);
     t.rows = t.s.nq * group;
-    t.first = (slot - slot_of(t.s.q0, e)) * M;
+    t.first = slot_first<M>(slot, slot_of(t.s.q0, e), t.rows);
     return t;
 }
 

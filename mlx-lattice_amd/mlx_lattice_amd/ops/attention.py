@@ -56,7 +56,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     key rows of ``key_offsets`` (``offsets`` by default), of which
     ``key_lengths[s]`` are filled (all by default): a cache of ``B`` sequences
     of ``L`` rows has ``key_offsets = arange(B + 1) * L``.  All three are int32
-    on the device and are not read back.
+    on the device and are not read back; offsets must not decrease, and are
+    clamped to the rows there are.
 
     Query ``i`` of ``nq``, in a sequence of ``nk`` keys, has position ``p = i +
     nk - nq``: queries sit at the end of the keys.  It sees key ``j`` where

@@ -486,3 +486,72 @@ def test_refusals():
     refused('key_lengths must have', q, k, k, key_lengths=at)
     refused('HIP device tensor', q.cpu(), k.cpu(), k.cpu())
     refused('HIP device tensor', q, k, k, offsets=at.cpu())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', (1500, 40000))
+def test_offsets_that_decrease_stay_inside(rows, dtype):
+    """The results are unspecified, but no row outside the tensors is written,
+    and none is read: what surrounds the inputs is NaN, what surrounds the
+    results stays as it is, and what is written is finite."""
+    import ctypes
+
+    from test_transformer_host import Attention, _library
+
+    lib = _library()
+    gen = torch.Generator(device='cuda').manual_seed(23)
+    around, dim, heads = 2000, 32, 2
+    span = slice(around, around + rows)
+
+    def guarded(count, fill, of=dtype):
+        return torch.full((rows + 2 * around, count, dim), fill, dtype=of,
+                          device='cuda')
+
+    def at(t):
+        return t[span].data_ptr()
+
+    inputs = {n: guarded(c, float('nan'))
+              for n, c in (('q', heads), ('k', 1), ('v', 1), ('dy', heads),
+                           ('y', heads), ('rest', heads))}
+    for t in inputs.values():
+        t[span] = _normal(gen, dtype, rows, t.shape[1], dim)
+    inputs['rest'][span] = 0
+    lse = torch.full((rows + 2 * around, heads), float('nan'), device='cuda')
+    lse[span] = 8.0
+    results = [guarded(c, 3.0) for c in (heads, heads, 1, 1)]
+    states = torch.full((rows + 2 * around, heads), 3.0, device='cuda')
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    for shares in ((0.9, 0.3, 0.35, 0.05, 0.1), (1.0, 0.0), (0.5, 1.0, 0.2)):
+        offsets = torch.tensor([int(s * rows) for s in shares],
+                               dtype=torch.int32, device='cuda')
+        args = Attention(
+            dtype=code, queries=rows, keys=rows, heads=heads, kv_heads=1,
+            dim=dim, sequences=len(shares) - 1, left=60, right=10, sinks=3,
+            scale=dim ** -0.5, q=at(inputs['q']), k=at(inputs['k']),
+            v=at(inputs['v']), q_row_stride=heads * dim, q_head_stride=dim,
+            k_row_stride=dim, k_head_stride=dim, v_row_stride=dim,
+            v_head_stride=dim, offsets=offsets.data_ptr(),
+            key_offsets=offsets.data_ptr(), key_lengths=None)
+        sizes = [getattr(lib, f'lattice_hip_window_attention{n}'
+                         '_workspace_bytes')(ctypes.byref(args))
+                 for n in ('', '_grad')]
+        space = torch.zeros(max(*sizes, 1), dtype=torch.uint8, device='cuda')
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+        def pointers(*values):
+            return [ctypes.c_void_p(v) for v in values]
+
+        assert lib.lattice_hip_window_attention(
+            ctypes.byref(args), *pointers(at(results[0]), at(states), None,
+                                          space.data_ptr()),
+            ctypes.c_size_t(sizes[0]), stream) == 0
+        assert lib.lattice_hip_window_attention_grad(
+            ctypes.byref(args), *pointers(
+                at(inputs['y']), None if code == 0 else at(inputs['rest']),
+                at(lse), at(inputs['dy']), *(at(t) for t in results[1:]),
+                space.data_ptr()), ctypes.c_size_t(sizes[1]), stream) == 0
+        torch.cuda.synchronize()
+        for t in (*results, states):
+            assert (t[:around] == 3).all() and (t[span.stop:] == 3).all()
+        for t in results:
+            assert torch.isfinite(t[span]).all()
