@@ -109,6 +109,10 @@ __device__ inline void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// Until the wave has what it read from LDS: before a copy, which takes no turn
+// among its LDS accesses, overwrites what they read.
+__device__ inline void wait_for_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 template <typename T>
 __device__ inline float row_dot(const float* __restrict__ a, const T* __restrict__ b, int dim) {
     float sum = 0.0f;

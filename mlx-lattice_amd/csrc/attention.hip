@@ -289,7 +289,7 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
         wait_for_copies();
         wave_fence();
         attend_tile<T, DP, KT>(a, state, q, mine, mine + Tile::kBytes, scale, s.nk, w, mask, j0);
-        wave_fence();
+        wait_for_reads();
     }
     // Every wave's sums to the largest maximum, then pairwise into the first
     // wave's.

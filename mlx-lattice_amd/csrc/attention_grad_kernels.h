@@ -239,7 +239,7 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __rest
             wait_for_copies();
             wave_fence();
             add_keys<T, DP, KT>(a, s.nk, q, d, tile, scale, log_sum, along, w, mask, j0, acc, slopes);
-            wave_fence();
+            wait_for_reads();
         } else {
             const int next = index + 1 < tiles.count ? tiles.tile(index + 1) * KT : -1;
             grad_query_step<T, DP, KT>(a, s.nk, source, next, shared + (~index & 1) * 2 * Tile::kBytes, q, d, tile,
@@ -510,7 +510,7 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
         wait_for_copies();
         wave_fence();
         add_queries<T, DP, QT>(tile, k, v, scale, mask, acc_k, acc_v, slopes);
-        wave_fence();
+        wait_for_reads();
     }
     if constexpr (SlopeScale<T>::kUsed) scale_sums(acc_k, 1.0f / slopes.factor());
     join_waves(acc_k, reinterpret_cast<float*>(shared), wave);
@@ -667,7 +667,7 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
             wait_for_copies();
             wave_fence();
             if (!none) add_queries<T, DP, QT>(tile, k, v, scale, mask, acc_k, acc_v, slopes);
-            wave_fence();
+            wait_for_reads();
         } else {
             char* next = shared + (~index & 1) * Queries::kBytes;
             const bool more = index + 1 < count;

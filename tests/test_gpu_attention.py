@@ -493,7 +493,8 @@ def test_refusals():
 def test_offsets_that_decrease_stay_inside(rows, dtype):
     """The results are unspecified, but no row outside the tensors is written,
     and none is read: what surrounds the inputs is NaN, what surrounds the
-    results stays as it is, and what is written is finite."""
+    results and the workspace stays as it is, and what is written is finite.
+    (A first key's part would lie some thousand parts before the others.)"""
     import ctypes
 
     from test_transformer_host import Attention, _library
@@ -535,7 +536,10 @@ def test_offsets_that_decrease_stay_inside(rows, dtype):
         sizes = [getattr(lib, f'lattice_hip_window_attention{n}'
                          '_workspace_bytes')(ctypes.byref(args))
                  for n in ('', '_grad')]
-        space = torch.zeros(max(*sizes, 1), dtype=torch.uint8, device='cuda')
+        guard = 32 << 20
+        store = torch.full((max(sizes) + 2 * guard,), 3, dtype=torch.uint8,
+                           device='cuda')
+        space = store[guard:-guard].zero_()
         stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
         def pointers(*values):
@@ -553,5 +557,6 @@ def test_offsets_that_decrease_stay_inside(rows, dtype):
         torch.cuda.synchronize()
         for t in (*results, states):
             assert (t[:around] == 3).all() and (t[span.stop:] == 3).all()
+        assert (store[:guard] == 3).all() and (store[-guard:] == 3).all()
         for t in results:
             assert torch.isfinite(t[span]).all()
