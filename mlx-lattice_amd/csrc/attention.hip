@@ -223,13 +223,12 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
-    const bool negate = a.scale < 0.0f;
-    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const float scale = exponent_scale(a);
     const AttnRows w = attn_rows(s, kv, group, t.first + 32 * wave);
     AttnOperand<T, DP> q;
     q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
                w.head * a.q_head_stride,
-           a.dim, w.valid, negate);
+           a.dim, w.valid, a.scale < 0.0f);
     const AttnMask mask(a, s.nk, w.p);
     AttnState<T, DP> state;
     state.clear();
@@ -269,13 +268,12 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     const AttnSlot t = attn_slot<32>(a, group, blockIdx.x);
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
-    const bool negate = a.scale < 0.0f;
-    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const float scale = exponent_scale(a);
     const AttnRows w = attn_rows(s, kv, group, t.first);
     AttnOperand<T, DP> q;
     q.load(static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + w.i) * a.q_row_stride +
                w.head * a.q_head_stride,
-           a.dim, w.valid, negate);
+           a.dim, w.valid, a.scale < 0.0f);
     const AttnMask mask(a, s.nk, w.p);
     AttnState<T, DP> state;
     state.clear();

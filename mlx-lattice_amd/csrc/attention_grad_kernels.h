@@ -185,13 +185,13 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __rest
     const AttnSlot t = attn_slot<kRows>(a, group, blockIdx.x);
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
-    const float scale = a.scale * kAttnLog2e;
+    const float scale = exponent_scale(a);
     const AttnRows w = attn_rows(s, kv, group, t.first + (FEW ? 0 : 32 * wave));
     const long long row = static_cast<long long>(s.q0) + w.i;
     const long long at = row * a.heads + w.head;
     Operand q, d;
     q.load(static_cast<const T*>(a.q) + row * a.q_row_stride + w.head * a.q_head_stride, a.dim, w.valid,
-           false);
+           a.scale < 0.0f);
     d.load(grad_out + at * a.dim, a.dim, w.valid, false);
     float along = 0.0f;
     {
@@ -491,9 +491,10 @@ grad_first_keys(lattice_attention a, const float2* __restrict__ states, const T*
     const bool valid = j < s.nk;
     const long long row = static_cast<long long>(s.k0) + min(j, s.nk - 1);
     AttnOperand<T, DP> k, v;
-    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, false);
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid,
+           a.scale < 0.0f);
     v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
-    const float scale = a.scale * kAttnLog2e;
+    const float scale = exponent_scale(a);
     f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
     SlopeScale<T> slopes;
     QueryTiles<T, DP, QT, kWave> source(a, s, kv, group, states, grad_out, lane);
@@ -621,9 +622,10 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const bool valid = j < s.nk;
     const long long row = static_cast<long long>(s.k0) + min(j, owned - 1);
     AttnOperand<T, DP> k, v;
-    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid, false);
+    k.load(static_cast<const T*>(a.k) + row * a.k_row_stride + kv * a.k_head_stride, a.dim, valid,
+           a.scale < 0.0f);
     v.load(static_cast<const T*>(a.v) + row * a.v_row_stride + kv * a.v_head_stride, a.dim, valid, false);
-    const float scale = a.scale * kAttnLog2e;
+    const float scale = exponent_scale(a);
     f32x16_attn acc_k[kBlocks] = {}, acc_v[kBlocks] = {};
     SlopeScale<T> slopes;
     QueryTiles<T, DP, QT, kThreads> source(a, s, kv, group, states, grad_out, FEW ? lane : threadIdx.x);

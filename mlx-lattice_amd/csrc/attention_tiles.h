@@ -10,6 +10,8 @@
 // product, whose left operand is read in the same order of rows.
 #pragma once
 
+#include <cfloat>
+
 #include "attention.h"
 
 namespace lattice {
@@ -220,6 +222,15 @@ struct AttnOperand {
         }
     }
 };
+
+// The scale of the scores in the exponent.  Positive, so that the -inf of a
+// key that is not seen stays -inf: the sign goes into one operand of the scores
+// (a.scale < 0), and a scale of zero becomes the smallest normal number, whose
+// product with a score below 1e30 vanishes beside every exponent.
+__device__ inline float exponent_scale(const lattice_attention& a) {
+    const float size = fabsf(a.scale);
+    return (size < FLT_MIN ? FLT_MIN : size) * kAttnLog2e;
+}
 
 // c + rows row0 .. row0 + 31 of the tile times the operand's rows.
 template <typename Tile, typename T, int DP>

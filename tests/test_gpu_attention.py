@@ -560,3 +560,40 @@ def test_offsets_that_decrease_stay_inside(rows, dtype):
         assert (store[:guard] == 3).all() and (store[-guard:] == 3).all()
         for t in results:
             assert torch.isfinite(t[span]).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths, heads, kv_heads, dim, left, right, sinks', [
+    ((300, 77), 4, 2, 32, 40, 3, 2), ((129,), 2, 2, 128, None, 0, 0),
+    ((4000, 4600), 8, 4, 64, 90, 0, 5), ((9000,), 4, 4, 32, 33, 64, 0)])
+def test_negative_scale(lengths, heads, kv_heads, dim, left, right, sinks,
+                        dtype):
+    """A negative scale is the positive one with the sign in the queries or the
+    keys, bit for bit: no row is made again by itself since a mask met the
+    sign.  (A gradient is compared where its sums have the same operands: the
+    matrix cores' sums are not symmetric in sign.)"""
+    gen = torch.Generator(device='cuda').manual_seed(19)
+    rows = sum(lengths)
+    q, k, v, dy = (_normal(gen, dtype, rows, h, dim)
+                   for h in (heads, kv_heads, kv_heads, heads))
+    kwargs = {'left': left, 'right': right, 'sinks': sinks,
+              'offsets': _offsets(lengths)}
+    out, dq, dk, dv = _run(q, k, v, dy, scale=-0.2, **kwargs)
+    of_q = _run(-q, k, v, dy, scale=0.2, **kwargs)
+    of_k = _run(q, -k, v, dy, scale=0.2, **kwargs)
+    for a, b in ((out, of_q[0]), (out, of_k[0]), (dv, of_q[3]), (dv, of_k[3]),
+                 (dq, -of_q[1]), (dk, -of_k[2])):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths, dim', (((300, 77), 32), ((9000,), 64)))
+def test_scale_of_zero(lengths, dim, dtype):
+    """Every key that is seen has the same share, as with queries of zero."""
+    gen = torch.Generator(device='cuda').manual_seed(20)
+    q, k, v, dy = (_normal(gen, dtype, sum(lengths), 4, dim) for _ in range(4))
+    kwargs = {'left': 50, 'right': 3, 'sinks': 2, 'offsets': _offsets(lengths)}
+    out, dq, dk, dv = _run(q, k, v, dy, scale=0.0, **kwargs)
+    want = _run(torch.zeros_like(q), k, v, dy, scale=1.0, **kwargs)
+    assert torch.equal(out, want[0]) and torch.equal(dv, want[3])
+    assert not dq.any() and not dk.any()
