@@ -27,20 +27,29 @@
 namespace lattice {
 namespace {
 
-// The share of a softmax over some of a row's keys: sum over them of
-// exp2(x - top) and of that times v.
+// The part of a softmax over some of a row's keys: the sum over them of
+// exp2(x - top), and of that times v.
 struct AttnPart {
     float* values;  // [splits][queries * heads][dim]
     float2* states;  // [splits][queries * heads]: (top, sum)
 };
 
-// A row's running maximum starts far below every score but above -inf, so
-// that what is masked (-inf) keeps an exponent of zero.
+// A row's top starts far below every score but above -inf, so that what is
+// masked (-inf) has a share of zero.
 constexpr float kAttnFloor = -3.0e38f;
-// The maximum in use may lag behind the scores by this many powers of two
-// before the sums are scaled down to a new one; the shares stay below 2^8,
-// far inside every type.
-constexpr float kAttnLag = 8.0f;
+// Shares are exp2(score - top), where top is the running maximum less kBase and
+// may lag behind the scores by kLag powers of two more before the sums are
+// scaled down to a new one: shares stay within 2^(kBase + kLag).  In half
+// precision, where a share below 2^-14 loses bits and one below 2^-25 is lost
+// (the sum of shares is not rounded), they fill the type's range instead: a
+// share keeps all bits down to 2^-25 of the largest and some down to 2^-36, so
+// that a tail of 2^24 equal keys is right to half a rounding of the result.
+template <typename T> struct ShareRange {
+    static constexpr float kBase = 0.0f, kLag = 8.0f;
+};
+template <> struct ShareRange<_Float16> {
+    static constexpr float kBase = 11.0f, kLag = 4.0f;
+};
 
 template <typename T, int DP>
 struct AttnState {
@@ -83,8 +92,9 @@ __device__ inline void attend_keys(AttnState<T, DP>& state, const AttnOperand<T,
         for (int r = 0; r < 16; ++r) most = fmaxf(most, s[part][r]);
     }
     most = halves_max(most) * scale;
-    if (__any(most > state.top + kAttnLag)) {
-        const float next = fmaxf(state.top, most);
+    typedef ShareRange<T> Range;
+    if (__any(most > state.top + (Range::kBase + Range::kLag))) {
+        const float next = fmaxf(state.top, most - Range::kBase);
         state.rescale(__builtin_amdgcn_exp2f(state.top - next));
         state.top = next;
     }

@@ -597,3 +597,31 @@ def test_scale_of_zero(lengths, dim, dtype):
     want = _run(torch.zeros_like(q), k, v, dy, scale=1.0, **kwargs)
     assert torch.equal(out, want[0]) and torch.equal(dv, want[3])
     assert not dq.any() and not dk.any()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('first', (True, False))
+@pytest.mark.parametrize('queries', (1, 300, 66000))
+def test_long_tail_under_one_large_score(queries, first, dtype):
+    """One key 17.4 above 40,000 others, whose shares of 2^-25 come to a
+    thousandth of the result: the first key and the last, few queries, keys
+    that are split, and tiles of many queries."""
+    keys = 40001
+    q = torch.zeros((queries, 1, 32), dtype=dtype, device='cuda')
+    k = torch.zeros((keys, 1, 32), dtype=dtype, device='cuda')
+    v = torch.ones_like(k)
+    # 4 x 4.34375 has the same value in every type.
+    at = 0 if first else keys - 1
+    q[..., 0], k[at, 0, 0], v[at] = 4, 4.34375, 0
+    got = _ops().window_attention(q, k, v, offsets=_offsets((queries,)),
+                                  key_offsets=_offsets((keys,)), scale=1.0)
+    tail = (keys - 1) * 2.718281828459045 ** -17.375
+    want = torch.full(got.shape, tail / (1 + tail), dtype=torch.float64)
+    # The result is rounded, and so are the shares: in half precision to
+    # eleven bits or, as small as these, at least ten.  The sums are made in
+    # float32 over products of two keys (float32) or sixteen, in order.
+    unit = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11,
+            torch.bfloat16: 2.0 ** -8}[dtype]
+    share = 2.0 ** -10 if dtype == torch.float16 else unit
+    steps = keys / (2 if dtype == torch.float32 else 16)
+    assert_within(got, want, want * (unit + share + steps * 2.0 ** -24))
