@@ -49,6 +49,12 @@ class Dropout(nn.Module):
     ``seed`` is the layer's own; ``calls`` counts its training passes and is
     the generator's offset, so that each pass has a mask of its own and a run
     repeats from the two numbers.
+
+    A pass that checkpointing makes again in the backward pass has the mask of
+    the first: it is known by a number drawn from torch's CPU generator, whose
+    state checkpointing restores.  Where the first cannot be told (the state
+    was not kept, several passes began with the same, or it lies more than
+    4096 passes back), a pass inside a backward pass is an error.
     """
 
     def __init__(self, p: float, *, seed: int) -> None:
@@ -58,6 +64,8 @@ class Dropout(nn.Module):
         self.p = p
         self.seed = seed
         self.calls = 0
+        # The offsets of the last passes by the number drawn; None: of several.
+        self._offsets: dict[int, int | None] = {}
 
     def forward(self, x: SparseTensor, *,
                 residual: SparseTensor | None = None) -> SparseTensor:
@@ -67,9 +75,27 @@ class Dropout(nn.Module):
             if not x.same_coords(residual):
                 raise ValueError('sparse tensor coordinates must match.')
             return x.replace(feats=x.feats + residual.feats)
-        self.calls += 1
-        return dropout(x, self.p, seed=self.seed, offset=self.calls - 1,
+        return dropout(x, self.p, seed=self.seed, offset=self._offset(),
                        residual=residual)
+
+    def _offset(self) -> int:
+        drawn = int(torch.randint(2 ** 62, (), device='cpu'))
+        if torch._C._current_graph_task_id() != -1:
+            offset = self._offsets.get(drawn)
+            if offset is None:
+                raise RuntimeError(
+                    'a dropout pass inside a backward pass must repeat an '
+                    "earlier one, known by the state of torch's CPU "
+                    'generator: checkpoint with preserve_rng_state, and give '
+                    'each pass a state of its own.')
+            return offset
+        offset = self.calls
+        self.calls += 1
+        same = self._offsets.get(drawn, offset) == offset
+        self._offsets[drawn] = offset if same else None
+        if len(self._offsets) > 4096:
+            del self._offsets[next(iter(self._offsets))]
+        return offset
 
 
 class WindowAttention(nn.Module):
