@@ -43,12 +43,21 @@ class LayerNorm(nn.Module):
         return layer_norm(x, self.weight, self.bias, eps=self.eps)
 
 
+def _draw() -> int:
+    """A number of torch's CPU generator."""
+    return int(torch.randint(2 ** 62, (), device='cpu'))
+
+
 class Dropout(nn.Module):
     """Dropout delegating to :func:`dropout`, with a residual.
 
-    ``seed`` is the layer's own; ``calls`` counts its training passes and is
-    the generator's offset, so that each pass has a mask of its own and a run
-    repeats from the two numbers.
+    ``seed`` is the layer's own, by default drawn from torch's CPU generator,
+    as initial weights are (ranks that build their layers from the same state
+    and train on different rows give seeds of their own); ``calls`` counts the
+    layer's training passes and is the generator's offset, so that each pass
+    has a mask of its own and a run repeats from the two numbers.  Both are in
+    ``state_dict``: a resumed run goes on with the masks.  A seed that was
+    given stays when a state is loaded.
 
     A pass that checkpointing makes again in the backward pass has the mask of
     the first: it is known by a number drawn from torch's CPU generator, whose
@@ -57,12 +66,15 @@ class Dropout(nn.Module):
     4096 passes back), a pass inside a backward pass is an error.
     """
 
-    def __init__(self, p: float, *, seed: int) -> None:
+    def __init__(self, p: float, *, seed: int | None = None) -> None:
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError('p must be between 0 and 1.')
         self.p = p
-        self.seed = seed
+        self._drawn_seed = seed is None
+        # Without dropout nothing is drawn, and a network's weights are those
+        # of its seed.
+        self.seed = _draw() if seed is None and p > 0.0 else seed
         self.calls = 0
         # The offsets of the last passes by the number drawn; None: of several.
         self._offsets: dict[int, int | None] = {}
@@ -75,11 +87,39 @@ class Dropout(nn.Module):
             if not x.same_coords(residual):
                 raise ValueError('sparse tensor coordinates must match.')
             return x.replace(feats=x.feats + residual.feats)
-        return dropout(x, self.p, seed=self.seed, offset=self._offset(),
+        offset = self._offset()
+        if self.seed is None:  # p was zero before
+            # Leaves the generator as a pass made again will find it.
+            state = torch.get_rng_state()
+            self.seed = _draw()
+            torch.set_rng_state(state)
+        return dropout(x, self.p, seed=self.seed, offset=offset,
                        residual=residual)
 
+    def get_extra_state(self) -> torch.Tensor:
+        seed = 0 if self.seed is None else self.seed
+        # 64 bits of a seed are in use; a tensor holds them as signed.
+        seed = (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63
+        return torch.tensor([self.calls, seed, self.seed is not None],
+                            device='cpu')
+
+    def set_extra_state(self, state: torch.Tensor) -> None:
+        self.calls, seed, known = state.tolist()
+        if self._drawn_seed and known:
+            self.seed = seed
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict,
+                              missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(
+            state_dict, prefix, local_metadata, strict, missing_keys,
+            unexpected_keys, error_msgs)
+        # A state from before the layer had one leaves its masks as they are.
+        key = prefix + '_extra_state'
+        if key in missing_keys:
+            missing_keys.remove(key)
+
     def _offset(self) -> int:
-        drawn = int(torch.randint(2 ** 62, (), device='cpu'))
+        drawn = _draw()
         if torch._C._current_graph_task_id() != -1:
             offset = self._offsets.get(drawn)
             if offset is None:
@@ -160,21 +200,25 @@ class WindowAttention(nn.Module):
 
 class VoxelTransformerBlock(nn.Module):
     """Pre-norm block: ``x + dropout(attention(norm(x)))``, then the same with
-    a ReLU layer of ``hidden`` channels (4 times the channels by default)."""
+    a ReLU layer of ``hidden`` channels (4 times the channels by default).
+
+    ``seed`` gives the two dropouts the seeds ``2 * seed`` and ``2 * seed +
+    1``; by default each draws its own.
+    """
 
     def __init__(self, channels: int, heads: int, *, hidden: int | None = None,
-                 p: float = 0.0, seed: int = 0, device=None,
+                 p: float = 0.0, seed: int | None = None, device=None,
                  dtype: torch.dtype = torch.float32, **attention) -> None:
         super().__init__()
         hidden = 4 * channels if hidden is None else hidden
         made = {'device': device, 'dtype': dtype}
         self.norm1 = LayerNorm(channels, **made)
         self.attention = WindowAttention(channels, heads, **attention, **made)
-        self.drop1 = Dropout(p, seed=2 * seed)
+        self.drop1 = Dropout(p, seed=None if seed is None else 2 * seed)
         self.norm2 = LayerNorm(channels, **made)
         self.expand = SubmConv3d(channels, hidden, kernel_size=1, **made)
         self.contract = SubmConv3d(hidden, channels, kernel_size=1, **made)
-        self.drop2 = Dropout(p, seed=2 * seed + 1)
+        self.drop2 = Dropout(p, seed=None if seed is None else 2 * seed + 1)
 
     def forward(self, x: SparseTensor, *,
                 offsets: torch.Tensor | None = None) -> SparseTensor:

@@ -1,4 +1,5 @@
-"""Dropout layers where a pass is made again: checkpointing."""
+"""Dropout layers' masks: passes that checkpointing makes again, seeds, and
+states that are saved and loaded."""
 
 from __future__ import annotations
 
@@ -9,7 +10,7 @@ from torch.utils.checkpoint import checkpoint
 
 def _masked(x, p, *, seed, offset, residual=None):
     """Stands in for the operator: a mask made from the two numbers."""
-    generator = torch.Generator().manual_seed(seed * 1000 + offset)
+    generator = torch.Generator().manual_seed(seed % 2 ** 50 * 1000 + offset)
     mask = torch.rand(x.shape, generator=generator) >= p
     return x * mask / (1 - p) + (0 if residual is None else residual)
 
@@ -75,6 +76,77 @@ def test_only_the_last_passes_are_kept(layers):
     assert len(drop._offsets) == 4096 and drop.calls == 4101
     with pytest.raises(RuntimeError, match='earlier one'):
         first.sum().backward()
+
+
+def _blocks(layers, count=2, **kwargs):
+    return [layers.VoxelTransformerBlock(8, 2, **kwargs) for _ in range(count)]
+
+
+def test_layers_without_a_seed_draw_their_own(layers):
+    torch.manual_seed(5)
+    blocks = _blocks(layers, 3, p=0.1)
+    seeds = [d.seed for b in blocks for d in (b.drop1, b.drop2)]
+    assert len(set(seeds)) == 6
+    torch.manual_seed(5)
+    again = _blocks(layers, 3, p=0.1)
+    assert seeds == [d.seed for b in again for d in (b.drop1, b.drop2)]
+    given, = _blocks(layers, 1, p=0.1, seed=4)
+    assert (given.drop1.seed, given.drop2.seed) == (8, 9)
+
+
+def test_no_dropout_draws_nothing(layers):
+    torch.manual_seed(5)
+    want = torch.get_rng_state()
+    drop = layers.Dropout(0.0)
+    assert torch.equal(torch.get_rng_state(), want)
+    x = torch.ones(4)
+    assert drop(x) is x and torch.equal(torch.get_rng_state(), want)
+    # Turned on later, in passes that are made again.
+    drops = torch.nn.Sequential(drop, layers.Dropout(0.0))
+    drops[0].p = drops[1].p = 0.5
+    x.requires_grad_()
+    out = checkpoint(drops, x, use_reentrant=False)
+    grad, = torch.autograd.grad(out.sum(), x)
+    assert torch.equal(grad, out.detach())
+    assert drops[0].seed != drops[1].seed
+
+
+def test_a_resumed_run_goes_on_with_the_masks(layers, tmp_path):
+    x = torch.ones(64)
+    torch.manual_seed(6)
+    block, = _blocks(layers, 1, p=0.5)
+    for _ in range(3):
+        block.drop1(x)
+    torch.save(block.state_dict(), tmp_path / 'state.pt')
+    want = [block.drop1(x), block.drop2(x)]
+    other, = _blocks(layers, 1, p=0.5)
+    state = torch.load(tmp_path / 'state.pt', weights_only=True)
+    other.load_state_dict(state)
+    assert (other.drop1.calls, other.drop2.calls) == (3, 0)
+    for a, b in zip(want, [other.drop1(x), other.drop2(x)]):
+        assert torch.equal(a, b)
+    # A seed that was given is the caller's; the count goes on.
+    given, = _blocks(layers, 1, p=0.5, seed=2)
+    given.load_state_dict(state)
+    assert (given.drop1.seed, given.drop1.calls) == (4, 3)
+    for seed in (-1, 2 ** 63 + 5, 2 ** 64 - 1, 2 ** 70 + 3):
+        drop = layers.Dropout(0.5, seed=seed)
+        fresh = layers.Dropout(0.5)
+        fresh.load_state_dict(drop.state_dict())
+        assert (fresh.seed - seed) % 2 ** 64 == 0
+
+
+def test_states_without_masks_still_load(layers):
+    block, other = _blocks(layers, p=0.5)
+    state = {k: v for k, v in block.state_dict().items()
+             if not k.endswith('_extra_state')}
+    seed = other.drop1.seed
+    other.load_state_dict(state)
+    assert other.drop1.seed == seed
+    assert torch.equal(other.expand.weight, block.expand.weight)
+    with pytest.raises(RuntimeError, match='expand.weight'):
+        other.load_state_dict({k: v for k, v in state.items()
+                               if k != 'expand.weight'})
 
 
 @pytest.mark.gpu
