@@ -177,9 +177,8 @@ class WindowAttention(nn.Module):
     def forward(self, x: SparseTensor, *,
                 offsets: torch.Tensor | None = None) -> SparseTensor:
         """``offsets``: the scans' row offsets, which the layers of a level
-        can share; ``batch_offsets(x)`` by default.  A tensor of several scans
-        that has lost its ``batch_counts``, as strided convs give it, needs
-        ``batch_offsets(x, batches)``."""
+        can share; ``batch_offsets(x)`` by default, which for a tensor without
+        ``batch_counts``, as strided convs give it, waits for the device."""
         if offsets is None:
             offsets = batch_offsets(x)
         packed = self.project(x).feats.view(x.capacity, -1, self.dim)

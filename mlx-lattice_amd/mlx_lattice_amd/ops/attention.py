@@ -13,11 +13,13 @@ __all__ = ['batch_offsets', 'window_attention']
 _ALL = 2 ** 31 - 1
 
 
-def batch_offsets(x: SparseTensor, batches: int = 1) -> torch.Tensor:
+def batch_offsets(x: SparseTensor, batches: int | None = None) -> torch.Tensor:
     """Row offsets ``(B + 1,)`` of the scans of ``x``, int32 on its device.
 
     From ``batch_counts`` where ``x`` has them; else its active rows hold the
-    scans 0 to ``batches - 1`` (a strided conv's output has no counts).  Rows
+    scans 0 to ``batches - 1`` (a strided conv's output has no counts).  Without
+    ``batches`` their number is read from the last active row's batch column,
+    which waits for the device; layers of a level can share the offsets.  Rows
     of a scan are adjacent and scans in order, as ``sparse_collate`` lays them
     and strided convs keep them.
     """
@@ -27,6 +29,8 @@ def batch_offsets(x: SparseTensor, batches: int = 1) -> torch.Tensor:
         for count in counts:
             offsets.append(offsets[-1] + count)
         return torch.tensor(offsets, dtype=torch.int32, device=x.device)
+    if batches is None:
+        batches = 1 if counts is not None else _scans(x)
     if batches < 1:
         raise ValueError('batches must be positive.')
     if counts is not None or batches == 1:
@@ -36,6 +40,18 @@ def batch_offsets(x: SparseTensor, batches: int = 1) -> torch.Tensor:
     return torch.searchsorted(
         scan, torch.arange(batches + 1, dtype=scan.dtype, device=x.device),
         out_int32=True)
+
+
+def _scans(x: SparseTensor) -> int:
+    if x.capacity == 0:
+        return 1
+    if x.device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+        raise ValueError('without batch_counts the number of scans is read '
+                         'from the device, which a captured graph cannot: '
+                         'give batches, or offsets made before.')
+    last = (x.active_rows - 1).clamp(min=0).long()
+    scan = torch.where(x.active_rows > 0, x.batch_indices[last], 0)
+    return max(0, int(scan)) + 1
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
