@@ -21,14 +21,15 @@ def batch_offsets(x: SparseTensor, batches: int | None = None) -> torch.Tensor:
     ``batches`` their number is read from the last active row's batch column,
     which waits for the device; layers of a level can share the offsets.  Rows
     of a scan are adjacent and scans in order, as ``sparse_collate`` lays them
-    and strided convs keep them.
+    and strided convs keep them.  Rows past the active ones are in no scan.
     """
     counts = x.batch_counts
     if counts is not None and len(counts) > 1:
         offsets = [0]
         for count in counts:
             offsets.append(offsets[-1] + count)
-        return torch.tensor(offsets, dtype=torch.int32, device=x.device)
+        made = torch.tensor(offsets, dtype=torch.int32, device=x.device)
+        return torch.minimum(made, x.active_rows)
     if batches is None:
         batches = 1 if counts is not None else _scans(x)
     if batches < 1:

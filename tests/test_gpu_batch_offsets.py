@@ -32,6 +32,18 @@ def test_scans_are_found_in_the_batch_column(scans, active, want):
     assert ops.batch_offsets(x, 1).tolist() == [0, active]
 
 
+def test_rows_that_are_not_active_are_in_no_scan():
+    import mlx_lattice_amd.ops as ops
+    from mlx_lattice_amd import SparseTensor
+
+    coords, feats = _rows([0, 0, 0, 1, 1, 1, 1])
+    for active, want in ((7, [0, 3, 7]), (5, [0, 3, 5]), (2, [0, 2, 2])):
+        x = SparseTensor(coords, feats, batch_counts=(3, 4),
+                         active_rows=torch.tensor([active], dtype=torch.int32,
+                                                  device='cuda'))
+        assert ops.batch_offsets(x).tolist() == want
+
+
 def test_a_strided_level_keeps_its_scans_apart():
     import mlx_lattice_amd.nn as lnn
     import mlx_lattice_amd.ops as ops
