@@ -28,8 +28,7 @@ def batch_offsets(x: SparseTensor, batches: int | None = None) -> torch.Tensor:
         offsets = [0]
         for count in counts:
             offsets.append(offsets[-1] + count)
-        made = torch.tensor(offsets, dtype=torch.int32, device=x.device)
-        return torch.minimum(made, x.active_rows)
+        return torch.minimum(_on_device(offsets, x.device), x.active_rows)
     if batches is None:
         batches = 1 if counts is not None else _scans(x)
     if batches < 1:
@@ -43,13 +42,25 @@ def batch_offsets(x: SparseTensor, batches: int | None = None) -> torch.Tensor:
         out_int32=True)
 
 
+def _refuse_capture(device: torch.device, what: str) -> None:
+    if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+        raise ValueError(f'{what}, which a captured graph cannot: give '
+                         'offsets made before.')
+
+
+def _on_device(offsets: list[int], device: torch.device) -> torch.Tensor:
+    """Copied from pinned memory: the host does not wait for the device."""
+    _refuse_capture(device, 'offsets of batch_counts are copied from the host')
+    return torch.tensor(offsets, dtype=torch.int32,
+                        pin_memory=device.type == 'cuda').to(
+                            device, non_blocking=True)
+
+
 def _scans(x: SparseTensor) -> int:
     if x.capacity == 0:
         return 1
-    if x.device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
-        raise ValueError('without batch_counts the number of scans is read '
-                         'from the device, which a captured graph cannot: '
-                         'give batches, or offsets made before.')
+    _refuse_capture(x.device, 'without batch_counts the number of scans is '
+                    'read from the device')
     last = (x.active_rows - 1).clamp(min=0).long()
     scan = torch.where(x.active_rows > 0, x.batch_indices[last], 0)
     return max(0, int(scan)) + 1

@@ -73,3 +73,26 @@ def test_a_captured_graph_refuses_to_count(monkeypatch):
     with pytest.raises(ValueError, match='captured graph'):
         ops.batch_offsets(x)
     assert ops.batch_offsets(x, 2).tolist() == [0, 1, 2]
+    x = SparseTensor(coords, feats, batch_counts=(1, 1))
+    with pytest.raises(ValueError, match='captured graph'):
+        ops.batch_offsets(x)
+
+
+def test_counts_reach_the_device_without_a_host_wait():
+    import mlx_lattice_amd.nn as lnn
+    import mlx_lattice_amd.ops as ops
+    from mlx_lattice_amd import SparseTensor
+
+    coords, feats = _rows([0] * 30 + [1] * 20)
+    x = SparseTensor(coords, feats, batch_counts=(30, 20))
+    layer = lnn.WindowAttention(16, 2, left=5, right=5, device='cuda')
+    want = layer(x).feats
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode('error')
+    try:
+        offsets = [ops.batch_offsets(x) for _ in range(50)]
+        got = layer(x).feats
+    finally:
+        torch.cuda.set_sync_debug_mode(0)
+    assert all(o.tolist() == [0, 30, 50] for o in offsets)
+    assert torch.equal(got, want)
