@@ -204,7 +204,7 @@ bool in_pieces(const at::Tensor& t, int64_t group) {
 at::Tensor pieces(const at::Tensor& t, int64_t group = 1) {
     const int64_t piece = piece_of(t), dim = t.size(2), padded = (dim + piece - 1) / piece * piece;
     if (padded != dim) return at::constant_pad_nd(t, {0, padded - dim}).contiguous();
-    if (t.numel() == 0 || in_pieces(t, group)) return t;
+    if (in_pieces(t, group)) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
 

@@ -625,3 +625,19 @@ def test_long_tail_under_one_large_score(queries, first, dtype):
     share = 2.0 ** -10 if dtype == torch.float16 else unit
     steps = keys / (2 if dtype == torch.float32 else 16)
     assert_within(got, want, want * (unit + share + steps * 2.0 ** -24))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_no_rows_in_any_layout(dtype):
+    """Slices without rows are taken in every layout, as slices with rows."""
+    gen = torch.Generator(device='cuda').manual_seed(21)
+    q, dy = (_normal(gen, dtype, 5, 2, 32) for _ in range(2))
+    wide = _normal(gen, dtype, 5, 4, 33)
+    none = wide[:0, :2, 1:]
+    kwargs = {'offsets': _offsets((5,)), 'key_offsets': _offsets((0,))}
+    for value in _run(q, none, none, dy, **kwargs):
+        assert not value.any()
+    for value, like in zip(_run(none, q, q, none, offsets=_offsets((0,)),
+                                key_offsets=_offsets((5,))),
+                           (none, none, q, q)):
+        assert value.shape == like.shape and not value.any()
