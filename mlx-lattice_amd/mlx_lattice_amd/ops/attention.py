@@ -98,8 +98,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     head are summed over its query heads, in a fixed order.
     """
     left, right = (_ALL if b is None else int(b) for b in (left, right))
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
+    if scale is None:  # a head without channels is refused below
+        scale = max([1, *q.shape[-1:]]) ** -0.5
     if key_offsets is None:
         key_offsets = offsets
     layout = (offsets, key_offsets, key_lengths)

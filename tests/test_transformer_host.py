@@ -176,3 +176,14 @@ def test_operators_refuse_host_tensors():
                              ops.rotary_frequencies((8,)), dims=(8,))
     with pytest.raises(ValueError, match='even'):
         ops.rotary_frequencies((5,))
+
+
+@pytest.mark.parametrize('shape', ((3, 2, 0), (3, 0), (0,), ()))
+def test_attention_refuses_heads_without_channels(shape):
+    """With the default scale, which has no value there."""
+    import mlx_lattice_amd.ops as ops
+
+    x = torch.zeros(shape)
+    at = torch.tensor([0, 3], dtype=torch.int32)
+    with pytest.raises(ValueError, match='attention heads must have|shape'):
+        ops.window_attention(x, x, x, offsets=at)
