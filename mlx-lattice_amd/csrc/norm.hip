@@ -427,7 +427,7 @@ int launch_norm_grad(const T* dy, long long dy_stride, const T* x, long long x_s
 #undef LATTICE_NORM_ROWS
     LATTICE_LAUNCH_CHECK();
     if (partials) {
-        layer_norm_grad_finish<T><<<(2 * channels + 15) / 16, kFinishBlock, 0, stream>>>(partials, blocks, channels,
+        layer_norm_grad_finish<T><<<static_cast<unsigned>((2ll * channels + 15) / 16), kFinishBlock, 0, stream>>>(partials, blocks, channels,
                                                                                       grad_weight, grad_bias);
         LATTICE_LAUNCH_CHECK();
     }
@@ -526,7 +526,7 @@ extern "C" int lattice_hip_layer_norm_grad(int dtype, const void* grad_y, long l
     if (rows == 0) {
         if (!sums) return LATTICE_OK;
         // No partials: the sums are zero.
-        const unsigned blocks = static_cast<unsigned>((2 * channels + 15) / 16);
+        const unsigned blocks = static_cast<unsigned>((2ll * channels + 15) / 16);
         if (dtype == LATTICE_F32) {
             layer_norm_grad_finish<float><<<blocks, kFinishBlock, 0, stream>>>(
                 nullptr, 0, channels, static_cast<float*>(grad_weight), static_cast<float*>(grad_bias));

@@ -230,6 +230,7 @@ extern "C" int lattice_hip_rotary_positions(int dtype, const void* x, long long 
                     "rotary positions support float32, float16 and bfloat16.");
     LATTICE_REQUIRE(rows >= 0 && heads > 0 && dim > 0 && dim <= kRotaryMaxDim,
                     "rotary heads must have between 1 and 1024 channels.");
+    LATTICE_REQUIRE(static_cast<long long>(heads) * dim < 1ll << 31, "rotary rows take up to 2^31 - 1 values.");
     LATTICE_REQUIRE(x_row_stride >= 0 && x_head_stride >= 0 && position_stride >= 0,
                     "rotary strides must be non-negative.");
     LATTICE_REQUIRE(axes >= 1 && axes <= kRotaryAxes && dims, "rotary positions need between 1 and 4 axes.");

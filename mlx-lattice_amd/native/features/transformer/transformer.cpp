@@ -21,11 +21,16 @@ int dtype_code(const at::Tensor& t, const char* what) {
     }
 }
 
+constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
+
 int row_count(const at::Tensor& t, const char* what) {
-    if (t.size(0) > std::numeric_limits<int32_t>::max()) {
-        throw std::invalid_argument(std::string(what) + " has too many rows.");
-    }
+    if (t.size(0) > kMost) throw std::invalid_argument(std::string(what) + " has too many rows.");
     return static_cast<int>(t.size(0));
+}
+
+// The kernels count the values of a row in 32 bits.
+void require_row_values(int64_t heads, int64_t dim, const char* what) {
+    if (dim > 0 && heads > (kMost - 64) / dim) throw std::invalid_argument(std::string(what) + " are too wide.");
 }
 
 void require_same(const at::Tensor& t, const at::Tensor& like, const char* what) {
@@ -74,6 +79,7 @@ std::tuple<at::Tensor, at::Tensor> layer_norm(const at::Tensor& x_in, const c10:
                                               const c10::optional<at::Tensor>& active_rows, bool keep_statistics) {
     if (x_in.dim() != 2 || x_in.size(1) < 1) throw std::invalid_argument("layer norm rows must have shape (N, C).");
     const int dtype = dtype_code(x_in, "layer norm rows");
+    require_row_values(1, x_in.size(1), "layer norm rows");
     if (!(eps >= 0.0)) throw std::invalid_argument("eps must be non-negative.");
     require_device(x_in, "x");
     const at::DeviceGuard guard(x_in.device());
@@ -97,6 +103,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor&
                                                                bool grad_weight, bool grad_bias) {
     if (x_in.dim() != 2 || x_in.size(1) < 1) throw std::invalid_argument("layer norm rows must have shape (N, C).");
     const int dtype = dtype_code(x_in, "layer norm rows");
+    require_row_values(1, x_in.size(1), "layer norm rows");
     require_device(x_in, "x");
     require_same(grad_y, x_in, "the cotangent");
     if (grad_y.sizes() != x_in.sizes()) throw std::invalid_argument("the cotangent must match the output shape.");
@@ -150,6 +157,7 @@ at::Tensor rotary_positions(const at::Tensor& x_in, const at::Tensor& positions_
         throw std::invalid_argument("rotary rows must have shape (N, heads, dim).");
     }
     const int dtype = dtype_code(x_in, "rotary rows");
+    require_row_values(x_in.size(1), x_in.size(2), "rotary rows");
     if (x_in.size(2) > 1024) throw std::invalid_argument("rotary heads must have between 1 and 1024 channels.");
     if (dims.empty() || dims.size() > 4) throw std::invalid_argument("rotary positions need between 1 and 4 axes.");
     int64_t pairs = 0;
@@ -220,6 +228,8 @@ Attention attention_of(const at::Tensor& q, const at::Tensor& k, const at::Tenso
         throw std::invalid_argument("q, k and v must have shape (N, heads, dim).");
     }
     const int dtype = dtype_code(q, "q, k and v");
+    require_row_values(q.size(1), q.size(2), "q, k and v");
+    require_row_values(k.size(1), k.size(2), "q, k and v");
     if (k.sizes() != v.sizes()) throw std::invalid_argument("k and v must have the same shape.");
     if (q.size(2) != k.size(2)) throw std::invalid_argument("q, k and v must share the channels of a head.");
     if (q.size(2) < 1 || q.size(2) > 128) {
@@ -248,7 +258,6 @@ Attention attention_of(const at::Tensor& q, const at::Tensor& k, const at::Tenso
         if (!key_lengths->is_contiguous()) throw std::invalid_argument("key_lengths must be contiguous.");
         lengths = ci32(*key_lengths);
     }
-    constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
     Attention a{{}, pieces(q, q.size(1) / k.size(1)), pieces(k), pieces(v)};
     const auto head_stride = [](const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; };
     a.args.dtype = dtype;

@@ -235,3 +235,24 @@ def test_example():
     assert losses[-1] < losses[0]
     # Outputs of size one in bfloat16: two roundings of 2^-8, and the shares'.
     assert example.serve(rows=90) < 2.0 ** -5
+
+
+def test_rows_too_wide_are_refused():
+    """Rows of 2^32 values and some, whose count in 32 bits is the some."""
+    import mlx_lattice_amd.ops as ops
+
+    one = torch.zeros((1, 1, 1), dtype=torch.float16, device='cuda')
+    many = 2 ** 32 + 8
+    with pytest.raises(ValueError, match='too wide'):
+        ops.layer_norm(one[0].expand(1, many))
+    heads = one.expand(1, many, 8)
+    places = torch.zeros((1, 1), dtype=torch.int32, device='cuda')
+    with pytest.raises(ValueError, match='too wide'):
+        ops.rotary_positions(heads, places,
+                             ops.rotary_frequencies((8,), device='cuda'),
+                             dims=(8,))
+    at = torch.tensor([0, 1], dtype=torch.int32, device='cuda')
+    with pytest.raises(ValueError, match='too wide'):
+        ops.window_attention(heads, heads, heads, offsets=at)
+    with pytest.raises(ValueError, match='too wide'):
+        ops.window_attention(heads[:, :8], heads, heads, offsets=at)

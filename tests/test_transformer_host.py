@@ -187,3 +187,12 @@ def test_attention_refuses_heads_without_channels(shape):
     at = torch.tensor([0, 3], dtype=torch.int32)
     with pytest.raises(ValueError, match='attention heads must have|shape'):
         ops.window_attention(x, x, x, offsets=at)
+
+
+def test_rotary_rows_of_too_many_values():
+    lib = _library()
+    long = ctypes.c_longlong
+    rc = lib.lattice_hip_rotary_positions(
+        0, 4096, long(64), long(32), 2, 1 << 26, 32, 4096, 0, long(3), 4096, 1,
+        (ctypes.c_int32 * 1)(16), 0, 0, 4096, None)
+    assert rc == 1 and b'2^31' in lib.lattice_hip_last_error()
