@@ -786,9 +786,9 @@ int lattice_hip_dropout(int dtype, const void* x, const void* residual,
  * positions[row, a] * frequencies[pair] radians (times -1 if `inverse`),
  * frequencies holding sum(dims) / 2 float64 values in section order; the
  * other channels are copied.  A pair is (i, i + dims[a] / 2) of its section,
- * or (2 i, 2 i + 1) if `interleaved`.  heads * dim < 2^31.  positions: int32, or float32 if
- * float_positions, position_stride elements between rows.  The angle is
- * reduced in float64. */
+ * or (2 i, 2 i + 1) if `interleaved`.  heads * dim < 2^31.  positions: int32,
+ * or float32 if float_positions, position_stride elements between rows.  The
+ * angle is reduced in float64. */
 int lattice_hip_rotary_positions(int dtype, const void* x,
                                  long long x_row_stride,
                                  long long x_head_stride, int rows, int heads,

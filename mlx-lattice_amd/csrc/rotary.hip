@@ -167,24 +167,27 @@ rotary_channels(const T* __restrict__ x, long long x_row, long long x_head, int 
                 RotaryPositions positions, const double* __restrict__ frequencies, RotaryAxes axes, float sign,
                 int block_rows, T* __restrict__ y) {
     extern __shared__ float2 table[];
-    const long long first = static_cast<long long>(blockIdx.x) * block_rows;
-    const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
-    rotary_table(table, axes, positions, frequencies, first, count, sign);
-    __syncthreads();
     const long long width = static_cast<long long>(heads) * dim;
-    for (long long i = threadIdx.x; i < count * width; i += kRotaryBlock) {
-        const int row = static_cast<int>(i / width);
-        const int at = static_cast<int>(i - row * width);
-        const int head = at / dim;
-        const RotaryChannel ch = rotary_channel(axes, at - head * dim);
-        const T* in = x + (first + row) * x_row + head * x_head;
-        T out = in[at - head * dim];
-        if (ch.pair >= 0) {
-            const float2 t = table[row * axes.pairs + ch.pair];
-            out = static_cast<T>(static_cast<float>(out) * t.x +
-                                 ch.sign * (static_cast<float>(in[ch.partner]) * t.y));
+    for (long long first = static_cast<long long>(blockIdx.x) * block_rows; first < rows;
+         first += static_cast<long long>(gridDim.x) * block_rows) {
+        const int count = static_cast<int>(min(static_cast<long long>(block_rows), rows - first));
+        rotary_table(table, axes, positions, frequencies, first, count, sign);
+        __syncthreads();
+        for (long long i = threadIdx.x; i < count * width; i += kRotaryBlock) {
+            const int row = static_cast<int>(i / width);
+            const int at = static_cast<int>(i - row * width);
+            const int head = at / dim;
+            const RotaryChannel ch = rotary_channel(axes, at - head * dim);
+            const T* in = x + (first + row) * x_row + head * x_head;
+            T out = in[at - head * dim];
+            if (ch.pair >= 0) {
+                const float2 t = table[row * axes.pairs + ch.pair];
+                out = static_cast<T>(static_cast<float>(out) * t.x +
+                                     ch.sign * (static_cast<float>(in[ch.partner]) * t.y));
+            }
+            y[first * width + i] = out;
         }
-        y[first * width + i] = out;
+        __syncthreads();
     }
 }
 
@@ -198,7 +201,8 @@ int rotary_of(const void* x, long long x_row, long long x_head, int rows, int he
     // A table of about 512 pairs a block, fewer where that leaves units idle.
     const int block_rows = static_cast<int>(std::max<long long>(
         1, std::min<long long>(std::max(1, 512 / std::max(1, axes.pairs)), (rows + 1023ll) / 1024)));
-    const unsigned grid = static_cast<unsigned>((static_cast<long long>(rows) + block_rows - 1) / block_rows);
+    // A launch takes fewer than 2^32 threads; far fewer blocks fill the chip.
+    const unsigned grid = grid_for(rows, block_rows, 1u << 22);
     // Working out a lane's eight channels of a 16-bit type is worth more than
     // an even end: blocks that stay (five a unit) take 101 us over 200k rows of
     // 16 heads of 32, a block for every table 107; with four channels (fp32)

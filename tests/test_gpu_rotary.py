@@ -115,3 +115,18 @@ def test_refusals():
         ops.rotary_frequencies((3,))
     with pytest.raises(ValueError, match='base'):
         ops.rotary_frequencies((4,), 0.0)
+
+
+def test_more_rows_than_blocks_of_a_launch():
+    """Rows of many pairs, a block each: 2^24 blocks of 256 threads are more
+    than a launch takes."""
+    rows, dim = 2 ** 24 + 5, 1022
+    x = torch.randn((1, 1, dim), device='cuda').half()
+    places = torch.full((1, 1), 7, dtype=torch.int32, device='cuda')
+    kwargs = {'frequencies': _ops().rotary_frequencies((dim,), device='cuda'),
+              'dims': (dim,)}
+    want = _ops().rotary_positions(x, places, **kwargs)
+    got = _ops().rotary_positions(x.expand(rows, 1, dim),
+                                  places.expand(rows, 1), **kwargs)
+    for part in got.split(1 << 20):
+        assert torch.equal(part, want.expand_as(part))
