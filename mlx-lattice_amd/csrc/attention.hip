@@ -229,8 +229,8 @@ attend_tiles(lattice_attention a, int splits, AttnPart part, T* __restrict__ out
     extern __shared__ __align__(128) char shared[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t group = a.heads / a.kv_heads;
-    const int kv = blockIdx.y, split = blockIdx.z;
-    const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, blockIdx.x);
+    const int kv = blockIdx.y, split = block_part(splits);
+    const AttnSlot t = attn_slot<32 * kAttnWaves>(a, group, block_slot(splits));
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
     const float scale = exponent_scale(a);
@@ -274,8 +274,8 @@ attend_few(lattice_attention a, int splits, AttnPart part, T* __restrict__ out, 
     extern __shared__ __align__(128) char shared[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t group = a.heads / a.kv_heads;
-    const int kv = blockIdx.y, split = blockIdx.z;
-    const AttnSlot t = attn_slot<32>(a, group, blockIdx.x);
+    const int kv = blockIdx.y, split = block_part(splits);
+    const AttnSlot t = attn_slot<32>(a, group, block_slot(splits));
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
     const float scale = exponent_scale(a);
@@ -434,7 +434,7 @@ int launch_attend(const lattice_attention& a, const AttnLayout& l, const AttnPar
     // Tiles twice as large are no faster (120k rows of heads of 32: 132 us for 127).
     constexpr int kTile = sizeof(T) == 2 ? 64 : 32;
     typedef AttnTile<T, DP, kTile> Tile;
-    const dim3 grid(static_cast<unsigned>(l.slots), a.kv_heads, l.splits);
+    const dim3 grid = slot_grid(l.slots, a.kv_heads, l.splits);
     if (l.few) {
         constexpr int kFew = 32, kFewWaves = few_waves<T, DP>();
         constexpr size_t kLds =

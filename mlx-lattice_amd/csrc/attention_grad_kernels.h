@@ -182,7 +182,7 @@ grad_query_tiles(lattice_attention a, const T* __restrict__ out, const T* __rest
     const uint32_t group = a.heads / a.kv_heads;
     const int kv = blockIdx.y;
     constexpr int kRows = FEW ? 32 : 32 * kAttnWaves;
-    const AttnSlot t = attn_slot<kRows>(a, group, blockIdx.x);
+    const AttnSlot t = attn_slot<kRows>(a, group, block_slot(1));
     const AttnSequence s = t.s;
     if (t.first >= t.rows) return;
     const float scale = exponent_scale(a);
@@ -613,10 +613,11 @@ grad_key_tiles(lattice_attention a, const float* __restrict__ lse, const float2*
     const uint32_t group = a.heads / a.kv_heads;
     const int kv = blockIdx.y;
     const auto slot_of = [](int start, int e) { return static_cast<uint32_t>(start) / kKeys + e; };
-    const int e = key_rows(a).find(blockIdx.x, slot_of);
+    const uint32_t slot = block_slot(1);
+    const int e = key_rows(a).find(slot, slot_of);
     const AttnSequence s = attn_sequence(a, e);
     const int owned = max(0, key_rows(a).start(e + 1) - s.k0);
-    const int j0 = slot_first<kKeys>(blockIdx.x, slot_of(s.k0, e), owned);
+    const int j0 = slot_first<kKeys>(slot, slot_of(s.k0, e), owned);
     if (j0 >= owned) return;
     const int j_wave = j0 + (FEW ? 0 : 32 * wave), j = j_wave + (lane & 31);
     const bool valid = j < s.nk;
@@ -720,7 +721,7 @@ int launch_grad_query(const lattice_attention& a, const T* out, const T* rest, c
     const auto kernel = grad_query_tiles<T, DP, kTile, FEW>;
     LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
     const long long slots = static_cast<long long>(a.queries) * (a.heads / a.kv_heads) / kRows + a.sequences + 2;
-    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, out, rest, lse, grad_out,
+    kernel<<<slot_grid(slots, a.kv_heads, 1), kAttnBlock, kLds, stream>>>(a, out, rest, lse, grad_out,
                                                                                         grad_q, states);
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
@@ -736,7 +737,7 @@ int launch_grad_keys(const lattice_attention& a, const float* lse, const float2*
     const auto kernel = grad_key_tiles<T, DP, kTile, FEW, FEW ? 1 : kKeyWaves<T, DP>>;
     LATTICE_HIP_TRY(allow_lds(reinterpret_cast<const void*>(kernel), kLds));
     const long long slots = a.keys / kKeys + a.sequences + 2;
-    kernel<<<dim3(static_cast<unsigned>(slots), a.kv_heads), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
+    kernel<<<slot_grid(slots, a.kv_heads, 1), kAttnBlock, kLds, stream>>>(a, lse, states, grad_out,
                                                                                         parts, grad_k, grad_v);
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;

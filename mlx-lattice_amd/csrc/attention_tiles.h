@@ -366,6 +366,17 @@ __device__ inline AttnRows attn_rows(const AttnSequence& s, int kv, uint32_t gro
     return w;
 }
 
+// A launch takes fewer than 2^32 threads along x: slots past 2^22 go on along
+// z, above its own `parts`.
+inline dim3 slot_grid(long long slots, int kv_heads, int parts) {
+    const long long x = std::min(slots, 1ll << 22);
+    return dim3(static_cast<unsigned>(x), kv_heads, static_cast<unsigned>((slots + x - 1) / x * parts));
+}
+__device__ inline uint32_t block_slot(uint32_t parts) {
+    return blockIdx.x + gridDim.x * (parts == 1 ? blockIdx.z : blockIdx.z / parts);
+}
+__device__ inline int block_part(uint32_t parts) { return parts == 1 ? 0 : blockIdx.z % parts; }
+
 // The first of `rows` rows of a slot of M, where the sequence's slots begin at
 // `start`: `rows` itself, none, where the slot is not the sequence's.  Offsets
 // that decrease can lead the search to a sequence that starts past the slot.

@@ -641,3 +641,17 @@ def test_no_rows_in_any_layout(dtype):
                                 key_offsets=_offsets((5,))),
                            (none, none, q, q)):
         assert value.shape == like.shape and not value.any()
+
+
+def test_more_sequences_than_blocks_of_a_launch():
+    """2^24 sequences of a row each: 2^32 threads and more."""
+    rows = 2 ** 24 + 3
+    gen = torch.Generator(device='cuda').manual_seed(22)
+    q, k, v, dy = (_normal(gen, torch.float16, rows, 1, 8) for _ in range(4))
+    offsets = torch.arange(rows + 1, dtype=torch.int32, device='cuda')
+    out, dq, dk, dv = _run(q, k, v, dy, offsets=offsets)
+    # The one key has the whole share.
+    assert torch.equal(out, v) and torch.equal(dv, dy)
+    # delta is float32's sum of eight products.
+    for grad in (dq, dk):
+        assert float(grad.abs().max()) < 1e-4
