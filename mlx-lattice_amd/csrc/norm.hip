@@ -326,31 +326,37 @@ layer_norm_grad_finish(const float* __restrict__ partials, int count, int channe
                        T* __restrict__ grad_bias) {
     __shared__ float shared[kFinishSlices][17];
     const int at = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const long long column = static_cast<long long>(blockIdx.x) * 16 + at;
     const long long columns = 2ll * channels;
-    float sum = 0.0f;
-    if (column < columns) {
-        // Four chains of additions keep four reads in flight.
-        float chain[4] = {};
-        int i = slice;
-        for (; i + 3 * kFinishSlices < count; i += 4 * kFinishSlices) {
+    for (long long first = blockIdx.x * 16ll; first < columns; first += gridDim.x * 16ll) {
+        const long long column = first + at;
+        float sum = 0.0f;
+        if (column < columns) {
+            // Four chains of additions keep four reads in flight.
+            float chain[4] = {};
+            int i = slice;
+            for (; i + 3 * kFinishSlices < count; i += 4 * kFinishSlices) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                chain[u] += partials[(i + static_cast<long long>(kFinishSlices) * u) * columns + column];
+                for (int u = 0; u < 4; ++u)
+                    chain[u] += partials[(i + static_cast<long long>(kFinishSlices) * u) * columns + column];
+            }
+            for (; i < count; i += kFinishSlices) chain[0] += partials[static_cast<long long>(i) * columns + column];
+            sum = (chain[0] + chain[1]) + (chain[2] + chain[3]);
         }
-        for (; i < count; i += kFinishSlices) chain[0] += partials[static_cast<long long>(i) * columns + column];
-        sum = (chain[0] + chain[1]) + (chain[2] + chain[3]);
-    }
-    shared[slice][at] = sum;
-    __syncthreads();
-    if (slice != 0 || column >= columns) return;
-    for (int s = 1; s < kFinishSlices; ++s) sum += shared[s][at];
-    if (column < channels) {
-        if (grad_weight) grad_weight[column] = static_cast<T>(sum);
-    } else if (grad_bias) {
-        grad_bias[column - channels] = static_cast<T>(sum);
+        shared[slice][at] = sum;
+        __syncthreads();
+        if (slice == 0 && column < columns) {
+            for (int s = 1; s < kFinishSlices; ++s) sum += shared[s][at];
+            if (column < channels) {
+                if (grad_weight) grad_weight[column] = static_cast<T>(sum);
+            } else if (grad_bias) {
+                grad_bias[column - channels] = static_cast<T>(sum);
+            }
+        }
+        __syncthreads();
     }
 }
+// A launch takes fewer than 2^32 threads.
+inline unsigned finish_blocks(int channels) { return grid_for(2ll * channels, 16, 1u << 20); }
 
 // Lanes and vectors a lane for rows of `vectors` vectors.
 struct NormShape {
@@ -427,8 +433,8 @@ int launch_norm_grad(const T* dy, long long dy_stride, const T* x, long long x_s
 #undef LATTICE_NORM_ROWS
     LATTICE_LAUNCH_CHECK();
     if (partials) {
-        layer_norm_grad_finish<T><<<static_cast<unsigned>((2ll * channels + 15) / 16), kFinishBlock, 0, stream>>>(partials, blocks, channels,
-                                                                                      grad_weight, grad_bias);
+        layer_norm_grad_finish<T><<<finish_blocks(channels), kFinishBlock, 0, stream>>>(partials, blocks, channels,
+                                                                               grad_weight, grad_bias);
         LATTICE_LAUNCH_CHECK();
     }
     return LATTICE_OK;
@@ -526,7 +532,7 @@ extern "C" int lattice_hip_layer_norm_grad(int dtype, const void* grad_y, long l
     if (rows == 0) {
         if (!sums) return LATTICE_OK;
         // No partials: the sums are zero.
-        const unsigned blocks = static_cast<unsigned>((2ll * channels + 15) / 16);
+        const unsigned blocks = finish_blocks(channels);
         if (dtype == LATTICE_F32) {
             layer_norm_grad_finish<float><<<blocks, kFinishBlock, 0, stream>>>(
                 nullptr, 0, channels, static_cast<float*>(grad_weight), static_cast<float*>(grad_bias));

@@ -159,3 +159,25 @@ def test_refusals():
         ops.layer_norm(x, weight, bias, eps=-1.0)
     with pytest.raises(ValueError, match='active_rows'):
         ops.layer_norm(x, active_rows=torch.zeros(2, device='cuda'))
+
+
+def test_more_channels_than_blocks_of_a_launch():
+    """The sums of 2^26 columns and more, 16 a block of 1024 threads."""
+    channels = 2 ** 25 + 24
+    x, weight, bias, dy = _inputs(2, channels, torch.float16)
+    leaves = [t.requires_grad_() for t in (x, weight, bias)]
+    y = _ops().layer_norm(*leaves)
+    _, dw, db = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        wide = x.double()
+        var, mean = torch.var_mean(wide, 1, unbiased=False, keepdim=True)
+        normed = (wide - mean) / torch.sqrt(var + 1e-5)
+        size = (wide.abs() + wide.abs().mean(1, keepdim=True)) / torch.sqrt(
+            var + 1e-5)
+        terms = dy.double()
+        # As the bounds of layer_norm_f64, of sums of two terms.
+        for got, want, most in ((dw, terms * normed, terms.abs() * size),
+                                (db, terms, terms.abs())):
+            off = (got.double() - want.sum(0)).abs()
+            assert (off <= 2.0 ** -11 * want.sum(0).abs()
+                    + 2.0 ** -16 * most.sum(0) + 2.0 ** -24).all()
