@@ -3,7 +3,9 @@
 #include <ATen/DeviceGuard.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <limits>
+#include <stdexcept>
 #include <string>
 
 #include "foundation/runtime.h"
@@ -32,6 +34,16 @@ int row_count(const at::Tensor& t, const char* what) {
 void require_row_values(int64_t heads, int64_t dim, const char* what) {
     if (dim > 0 && heads > (kMost - 64) / dim) throw std::invalid_argument(std::string(what) + " are too wide.");
 }
+
+// A tangent of forward-mode differentiation would be lost.
+void refuse_tangents(std::initializer_list<at::Tensor> tensors) {
+    for (const at::Tensor& t : tensors) {
+        if (t.defined() && t._fw_grad(/*level=*/0).defined())
+            throw std::runtime_error("the transformer operators have no forward-mode derivatives.");
+    }
+}
+
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); }
 
 void require_same(const at::Tensor& t, const at::Tensor& like, const char* what) {
     require_device(t, what);
@@ -77,6 +89,7 @@ void* or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr
 std::tuple<at::Tensor, at::Tensor> layer_norm(const at::Tensor& x_in, const c10::optional<at::Tensor>& weight_in,
                                               const c10::optional<at::Tensor>& bias_in, double eps,
                                               const c10::optional<at::Tensor>& active_rows, bool keep_statistics) {
+    refuse_tangents({x_in, or_undefined(weight_in), or_undefined(bias_in)});
     if (x_in.dim() != 2 || x_in.size(1) < 1) throw std::invalid_argument("layer norm rows must have shape (N, C).");
     const int dtype = dtype_code(x_in, "layer norm rows");
     require_row_values(1, x_in.size(1), "layer norm rows");
@@ -101,6 +114,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor&
                                                                const at::Tensor& statistics,
                                                                const c10::optional<at::Tensor>& active_rows,
                                                                bool grad_weight, bool grad_bias) {
+    refuse_tangents({grad_y, x_in, or_undefined(weight_in)});
     if (x_in.dim() != 2 || x_in.size(1) < 1) throw std::invalid_argument("layer norm rows must have shape (N, C).");
     const int dtype = dtype_code(x_in, "layer norm rows");
     require_row_values(1, x_in.size(1), "layer norm rows");
@@ -135,6 +149,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_grad(const at::Tensor&
 
 at::Tensor dropout(const at::Tensor& x_in, const c10::optional<at::Tensor>& residual_in, uint64_t seed,
                    uint64_t offset, uint64_t threshold, double scale) {
+    refuse_tangents({x_in, or_undefined(residual_in)});
     const int dtype = dtype_code(x_in, "dropout values");
     require_device(x_in, "x");
     const at::DeviceGuard guard(x_in.device());
@@ -153,6 +168,7 @@ at::Tensor dropout(const at::Tensor& x_in, const c10::optional<at::Tensor>& resi
 
 at::Tensor rotary_positions(const at::Tensor& x_in, const at::Tensor& positions_in, const at::Tensor& frequencies_in,
                             const std::vector<int>& dims, bool interleaved, bool inverse) {
+    refuse_tangents({x_in, positions_in, frequencies_in});
     if (x_in.dim() != 3 || x_in.size(1) < 1 || x_in.size(2) < 1) {
         throw std::invalid_argument("rotary rows must have shape (N, heads, dim).");
     }
@@ -303,6 +319,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
     const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right,
     int64_t sinks, double scale, bool keep) {
+    refuse_tangents({q, k, v});
     const c10::OptionalDeviceGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
     const Attention a = attention_of(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
     at::Tensor out = at::empty(a.q.sizes(), q.options());
@@ -324,6 +341,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_grad(
     const c10::optional<at::Tensor>& rest, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& offsets, const at::Tensor& key_offsets, const c10::optional<at::Tensor>& key_lengths,
     int64_t left, int64_t right, int64_t sinks, double scale) {
+    refuse_tangents({grad_out_in, q, k, v});
     const c10::OptionalDeviceGuard guard(q.is_cuda() ? c10::make_optional(q.device()) : c10::nullopt);
     const Attention a = attention_of(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
     require_same(grad_out_in, q, "the cotangent");

@@ -256,3 +256,36 @@ def test_rows_too_wide_are_refused():
         ops.window_attention(heads, heads, heads, offsets=at)
     with pytest.raises(ValueError, match='too wide'):
         ops.window_attention(heads[:, :8], heads, heads, offsets=at)
+
+
+@pytest.mark.parametrize('grad', (False, True))
+def test_forward_mode_is_refused(grad):
+    """A tangent of any input would be lost."""
+    import torch.autograd.forward_ad as fwd
+
+    import mlx_lattice_amd.ops as ops
+
+    rows = torch.randn((12, 32), device='cuda', requires_grad=grad)
+    heads = rows.view(12, 2, 16)
+    weight = torch.ones(32, device='cuda')
+    at = torch.tensor([0, 12], dtype=torch.int32, device='cuda')
+    places = torch.arange(12., device='cuda')[:, None]
+    frequencies = ops.rotary_frequencies((16,), device='cuda')
+    for call, *inputs in (
+            (ops.layer_norm, rows, weight, weight),
+            (lambda x, r: ops.dropout(x, 0.5, seed=1, residual=r), rows, rows),
+            (lambda x, p: ops.rotary_positions(x, p, frequencies, dims=(16,)),
+             heads, places),
+            (lambda q, k, v: ops.window_attention(q, k, v, offsets=at),
+             heads, heads, heads)):
+        plain = call(*inputs)
+        with fwd.dual_level():
+            assert torch.equal(call(*inputs), plain)
+            for i, primal in enumerate(inputs):
+                dual = fwd.make_dual(primal, torch.ones_like(primal))
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    call(*inputs[:i], dual, *inputs[i + 1:])
+            if grad:
+                dual = fwd.make_dual(plain.detach(), torch.ones_like(plain))
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    torch.autograd.grad(plain, rows, dual)
