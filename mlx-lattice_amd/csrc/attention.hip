@@ -12,15 +12,22 @@
 // the softmax needs one exchange between two lanes a step.
 //
 // Shares are rounded to the rows' type for the second product, as q, k and v
-// are; maximum, sums and results are fp32.
+// are; maximum, sums and results are fp32.  That is one more rounding of a
+// row's result, which does not grow with the number of keys (error against
+// float64 2.9e-4 in half precision and 2.4e-3 in bfloat16, of which the result's
+// own rounding makes 2.1e-4 and 1.7e-3).
 //
-// Bound by the exponentials and the other vector instructions of the softmax,
-// 7 issue slots a score beside the products' 4 (heads of 32) to 16 (128) cycles;
-// few queries by reading the keys.  120,000 rows of 8 heads of 32, window 257,
-// fp16: 127 us (249 TFLOP/s).  16,384 causal rows of 16 heads of 128 over 4,
-// window 4096, bf16: 557 us under the profiler, 534 without (904 TFLOP/s; a
-// library product of 8192^3 1191).  One query of 16 heads of 128 over 4 against
-// 32 caches of 24,000 keys, fp16: 297 us (5.5 TB/s).
+// Bound, by the counters, by the vector instructions of the softmax (eight a
+// score): their pipe is busy 62 % of the time at heads of 32 and 47 % at 64,
+// beside 13 and 19 % of the matrix cores; neighbouring tiles of rows, which lie
+// on different dies, each read their keys beyond the L2 (846 MB at 120,000 rows
+// of heads of 32, 6.6 TB/s).  At heads of 128 both pipes are busy about evenly
+// (42 and 45 %, two waves a SIMD), few queries wait for the keys.  120,000 rows
+// of 8 heads of 32, window 257, fp16: 127 us (249 TFLOP/s).  16,384 causal rows
+// of 16 heads of 128 over 4, window 4096, bf16: 534 us under the profiler, 518
+// without (931 TFLOP/s; a library product of 8192^3 1191); fp32: 4.9 ms (98 of
+// 154).  One query of 16 heads of 128 over 4 against 32 caches of 24,000 keys,
+// fp16: 298 us (5.5 TB/s); fp32: 831 (4.0).
 
 #include "attention_tiles.h"
 

@@ -1,11 +1,14 @@
 // Kernels of the windowed attention's gradients and their launches.
 //
-// Bound as the forward pass by the vector instructions between the products (an
-// exponential, four others and two roundings a score and pass).  60,001 rows of
-// 4 heads of 64 over 2, window 513, bf16: grad_q 87 us, grad_k and grad_v 114,
-// the first keys' long sums 16 + 10; 20,000 rows of 4 heads of 32, window 128,
-// fp32: 60, 65, 17 + 4 (fp32 products have a sixteenth of the 16-bit rate, and
-// eight or nine short steps leave a block waiting for its copies).
+// grad_q is bound as the forward pass by the vector instructions between the
+// products (an exponential, four others and two roundings a score; their pipe
+// is busy 40 % of the time, the matrix cores 25); grad_k and grad_v by waits, with
+// one or two waves a SIMD for the registers of their sums (vector 25 %, matrix
+// cores 24, half of a wave's time in waits).  60,001 rows of 4 heads of 64 over
+// 2, window 513, bf16: grad_q 89 us, grad_k and grad_v 113, the first keys' long
+// sums 17 + 9; 20,000 rows of 4 heads of 32, window 128, fp32: 60, 65, 17 + 4
+// (fp32 products have a sixteenth of the 16-bit rate: matrix cores 35 %; eight or
+// nine short steps leave a block waiting for its copies, 45 % of a wave's time).
 #pragma once
 
 #include "attention_grad.h"
