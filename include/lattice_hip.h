@@ -768,6 +768,41 @@ int lattice_hip_layer_norm_grad(int dtype, const void* grad_y,
                                 void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* The junction of two parts of a block over `channels` of each row:
+ *   sum = residual + scale * gate * u,  u = norm(x) * post_weight + post_bias
+ *   (post_norm) or x,   normed = norm(sum) * weight + bias,
+ * where norm(z) = (z - mean) / sqrt(var + eps), or z / sqrt(mean z^2 + eps)
+ * (rms), and the second is of the sum as it is stored.  x and residual
+ * [rows, channels] with elements between rows as given, sum and normed
+ * contiguous.  Vectors have `channels` values of the rows' type (NULL: weights
+ * and gate 1, biases 0).  Rows at and past *active_rows (device int32, NULL:
+ * all rows are active) become zeros in both results.  statistics (NULL: not
+ * kept) gets, 16-byte aligned, float4 (mean, 1 / deviation) of the sum and of
+ * x (post_norm, else 0) of every row. */
+typedef struct lattice_residual_norm {
+    int dtype, rows, channels, rms, post_norm;
+    float scale, eps;
+    const void *x, *residual;
+    long long x_stride, residual_stride;
+    const void *weight, *bias, *gate, *post_weight, *post_bias;
+    const int32_t* active_rows;
+} lattice_residual_norm;
+int lattice_hip_residual_norm(const lattice_residual_norm* args, void* sum,
+                              void* normed, float* statistics, void* stream);
+
+/* Its gradients: grad_x and grad_residual [rows, channels] contiguous (zero on
+ * inactive rows), and, unless NULL, the vectors' [channels], summed over the
+ * active rows in an order fixed by the shape.  sum and statistics as the
+ * forward call gave them; the cotangents grad_sum and grad_normed are
+ * contiguous (NULL: zero). */
+size_t lattice_hip_residual_norm_grad_workspace_bytes(int rows, int channels);
+int lattice_hip_residual_norm_grad(
+    const lattice_residual_norm* args, const void* sum,
+    const float* statistics, const void* grad_sum, const void* grad_normed,
+    void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
+    void* grad_gate, void* grad_post_weight, void* grad_post_bias,
+    void* workspace, size_t workspace_bytes, void* stream);
+
 /* Dropout: y[e] = residual[e] + (kept(e) ? x[e] * scale : 0) over `count`
  * contiguous values (residual NULL: 0).  Element e is kept when word e % 4 of
  * Philox 4x32-10 (Salmon et al., SC 2011) over the counter (e / 4, offset)
@@ -848,6 +883,66 @@ int lattice_hip_window_attention_grad(const lattice_attention* args,
                                       void* grad_k, void* grad_v,
                                       void* workspace, size_t workspace_bytes,
                                       void* stream);
+
+/* ------------------------------------------------------- 8-bit caches -- */
+/* Keys and values of `sequences` x `kv_heads` x 32 * `blocks` tokens in one
+ * byte each, with a power of two for each block of 32 tokens and key head: a
+ * code c of a block with exponent e stands for c * 2^e.  Heads of `dim` (up to
+ * 128) channels lie in rows of width = dim rounded up to 32, zeros behind:
+ *   keys   [sequences, kv_heads, 32 * blocks, width],
+ *   values [sequences, kv_heads, blocks, width, 32] (a block's tokens
+ *          innermost, as the product with the softmax's shares reads them),
+ *   exponents int8 [sequences, kv_heads, blocks].
+ * Codes are OCP e4m3 (no infinities) or int8.  Codes on 16-byte boundaries. */
+enum { LATTICE_CODE_E4M3 = 0, LATTICE_CODE_INT8 = 1 };
+typedef struct lattice_cache {
+    int code, sequences, kv_heads, blocks, dim;
+    void *keys, *values;
+    int8_t *key_exponents, *value_exponents;
+} lattice_cache;
+
+/* Appends rows.  Sequence s gets the rows offsets[s] .. offsets[s + 1] of k and
+ * v [rows, kv_heads, dim] (strides in elements, unit stride in dim) as the
+ * last of its lengths[s] tokens.  A block that gets new tokens takes as its
+ * exponent the least, at least -126, that leaves the largest finite magnitude
+ * of the new tokens at most 448 (e4m3) or 127 (int8), or that of its earlier
+ * tokens, if it has any and theirs is larger; earlier codes are divided by the
+ * power of two between.  Quotients are rounded to the nearest code, half to
+ * even.  Infinities and NaN become NaN in e4m3, the largest code and 0 in
+ * int8.  Tokens outside 0 .. 32 * blocks are not written, other tokens keep
+ * their bytes.  offsets [sequences + 1] and lengths [sequences] are device
+ * int32; offsets must not decrease and are clamped to the rows there are. */
+int lattice_hip_cache_write(const lattice_cache* cache, int dtype,
+                            const void* k, long long k_row_stride,
+                            long long k_head_stride, const void* v,
+                            long long v_row_stride, long long v_head_stride,
+                            int rows, const int32_t* offsets,
+                            const int32_t* lengths, void* stream);
+
+/* k and v [sequences, 32 * blocks, kv_heads, dim] contiguous: what the codes
+ * stand for, rounded once; zeros at and past a sequence's length. */
+int lattice_hip_cache_read(const lattice_cache* cache, int dtype,
+                           const int32_t* lengths, void* k, void* v,
+                           void* stream);
+
+/* Attention over a cache: as lattice_hip_window_attention, where sequence s
+ * has the keys and values of the first lengths[s] tokens of the cache and its
+ * queries sit at their end: query i of nq has position lengths[s] - nq + i.
+ * out [queries, heads, dim] contiguous. */
+typedef struct lattice_cache_attention {
+    int dtype, queries, heads;
+    int left, right, sinks;
+    float scale;
+    const void* q;
+    long long q_row_stride, q_head_stride;
+    const int32_t *offsets, *lengths;
+} lattice_cache_attention;
+size_t lattice_hip_cache_attention_workspace_bytes(
+    const lattice_cache* cache, const lattice_cache_attention* args);
+int lattice_hip_cache_attention(const lattice_cache* cache,
+                                const lattice_cache_attention* args, void* out,
+                                void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 #ifdef __cplusplus
 }

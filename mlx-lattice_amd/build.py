@@ -29,14 +29,17 @@ INCLUDE = REPO / 'include'
 ARCH = 'gfx950'
 
 HIP_SOURCES = ['scan.hip', 'sort.hip', 'coords.hip', 'conv.hip', 'conv_grad.hip', 'pool.hip', 'quantize.hip',
-               'norm.hip', 'dropout.hip', 'rotary.hip', 'attention.hip', 'attention_grad.hip',
-               'attention_grad_f32.hip', 'attention_grad_f16.hip', 'attention_grad_bf16.hip']
+               'norm.hip', 'residual_norm.hip', 'dropout.hip', 'rotary.hip', 'attention.hip', 'attention_grad.hip',
+               'attention_grad_f32.hip', 'attention_grad_f16.hip', 'attention_grad_bf16.hip', 'cache.hip',
+               'cache_attention.hip', 'cache_attention_f32.hip', 'cache_attention_f16.hip', 'cache_attention_bf16.hip']
 HOST_SOURCES = [
     'native/features/coordinates/relations.cpp',
     'native/features/convolution/api.cpp',
     'native/features/pooling/pooling.cpp',
     'native/features/quantization/quantization.cpp',
     'native/features/transformer/transformer.cpp',
+    'native/features/transformer/cache.cpp',
+    'native/features/transformer/residual_norm.cpp',
     'native/features/transformer/autograd.cpp',
     'native/bindings/module.cpp',
 ]

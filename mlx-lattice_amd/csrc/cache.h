@@ -1,0 +1,114 @@
+// A cache of keys and values in 8 bits: its codes, its sequences and what every
+// entry checks.
+#pragma once
+
+#include "attention_tiles.h"
+
+namespace lattice {
+
+constexpr int kCacheBlock = 32;        // tokens that share an exponent
+constexpr int kCacheLeast = -126;      // the least exponent: 2^e and 2^-e are normal numbers
+constexpr int kCacheLongest = 1 << 29;  // lengths are clamped to it, so that positions stay inside 32 bits
+
+// 2^e for e in -126 .. 127.
+__device__ inline float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+typedef __bf16 bf16x2_cache __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_cache __attribute__((ext_vector_type(2)));
+
+// What a code type does: the exponent that holds a magnitude, codes from
+// values, and values (whole in any of the operand types: codes have at most 7
+// significant bits) from codes.
+struct CodeE4m3 {
+    // 448 = 1.75 * 2^8.
+    static constexpr int kShift = 9;
+    static constexpr uint32_t kMostMantissa = 0x600000;
+
+    __device__ static uint8_t code(float x) {
+        const float finite = fabsf(x) < INFINITY ? x : __uint_as_float(0x7fc00000u);
+        return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(finite, finite, 0, false));
+    }
+    __device__ static float value(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8(c, 0); }
+    // The values of four codes.
+    __device__ static void values(uint32_t w, bf16x2_cache* v) {
+        v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+        v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+    }
+    __device__ static void values(uint32_t w, f16x2_cache* v) {
+        v[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        v[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    }
+};
+struct CodeInt8 {
+    static constexpr int kShift = 7;
+    static constexpr uint32_t kMostMantissa = 0x7e0000;  // 127 = 1.984375 * 2^6
+
+    __device__ static uint8_t code(float x) {
+        const float bounded = fminf(fmaxf(rintf(x), -127.0f), 127.0f);
+        return static_cast<uint8_t>(static_cast<int8_t>(x == x ? bounded : 0.0f));
+    }
+    __device__ static float value(uint8_t c) { return static_cast<float>(static_cast<int8_t>(c)); }
+    __device__ static void values(uint32_t w, bf16x2_cache* v) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            v[i] = bf16x2_cache{static_cast<__bf16>(value(w >> 16 * i & 0xff)),
+                                static_cast<__bf16>(value(w >> (16 * i + 8) & 0xff))};
+    }
+    // 1024 + (c + 128) has the bits 0x6400 | (c + 128) in half precision.
+    __device__ static void values(uint32_t w, f16x2_cache* v) {
+        const uint32_t biased = w ^ 0x80808080u;
+        const f16x2_cache bias{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+        v[0] = __builtin_bit_cast(f16x2_cache, __builtin_amdgcn_perm(0x64646464u, biased, 0x04010400u)) - bias;
+        v[1] = __builtin_bit_cast(f16x2_cache, __builtin_amdgcn_perm(0x64646464u, biased, 0x04030402u)) - bias;
+    }
+};
+
+// The exponent of a block whose largest magnitude is `most`.
+template <typename Code>
+__device__ inline int block_exponent(float most) {
+    const uint32_t bits = __float_as_uint(most);
+    const int e = static_cast<int>(bits >> 23) - 126 - Code::kShift + ((bits & 0x7fffffu) > Code::kMostMantissa);
+    return max(e, kCacheLeast);
+}
+
+// A sequence: its rows q0 .. q0 + nq, the last of `length` tokens, of which the
+// cache has `nk`; row i is token i + shift.
+struct CacheSequence {
+    int q0, nq, nk, length;
+    __device__ int shift() const { return length - nq; }
+};
+__device__ inline CacheSequence cache_sequence(const RowPartition& rows, const int32_t* lengths, int capacity, int e) {
+    CacheSequence s;
+    s.q0 = rows.start(e);
+    s.nq = max(0, rows.start(e + 1) - s.q0);
+    s.length = rows.real(e) ? min(max(lengths[e - 1], 0), kCacheLongest) : 0;
+    s.nk = min(s.length, capacity);
+    return s;
+}
+
+__host__ __device__ inline int cache_width(const lattice_cache& c) { return (c.dim + 31) / 32 * 32; }
+
+// What every entry checks; NULL, or what is wrong.
+inline const char* cache_fault(const lattice_cache* c) {
+    if (!c) return "cache arguments must be non-null.";
+    if (c->code != LATTICE_CODE_E4M3 && c->code != LATTICE_CODE_INT8) return "caches hold e4m3 or int8 codes.";
+    if (c->sequences < 0 || c->kv_heads < 1 || c->blocks < 0) return "cache shapes must be positive.";
+    if (c->sequences >= 1 << 24 || c->kv_heads >= 1 << 16 || c->blocks >= 1 << 23)
+        return "caches have under 2^24 sequences, 2^16 key heads and 2^28 tokens.";
+    if (c->dim < 1 || c->dim > kAttnMaxDim) return "cache heads must have between 1 and 128 channels.";
+    if (c->sequences == 0 || c->blocks == 0) return nullptr;
+    if (!c->keys || !c->values || !c->key_exponents || !c->value_exponents) return "cache pointers must be non-null.";
+    if ((reinterpret_cast<uintptr_t>(c->keys) | reinterpret_cast<uintptr_t>(c->values)) % 16 != 0)
+        return "cache codes must lie on 16-byte boundaries.";
+    return nullptr;
+}
+
+#define LATTICE_REQUIRE_CACHE(cache)                              \
+    do {                                                          \
+        if (const char* fault_ = ::lattice::cache_fault(cache)) { \
+            ::lattice::set_error(fault_);                         \
+            return LATTICE_ERROR_INVALID_ARGUMENT;                \
+        }                                                         \
+    } while (0)
+
+}  // namespace lattice

@@ -1,0 +1,37 @@
+// Attention over an 8-bit cache: what its units of translation share.
+#pragma once
+
+#include "cache.h"
+
+namespace lattice {
+
+// A part of a row's softmax, over some of its tokens: the largest score (log2),
+// the sum of exp2(score - top), and the sum of that times v.
+struct CachePart {
+    float* values;   // [splits][queries * heads][dim]
+    float2* states;  // [splits][queries * heads]: (top, sum)
+};
+
+// How a call is laid out.
+struct CacheLayout {
+    bool share;       // the waves of a block share rows and split their tokens, or have rows of their own
+    int tiles;        // tiles of 16 (query, head) pairs a wave
+    int splits;       // blocks that split a row's tokens
+    long long slots;  // tiles of rows at most
+    int rows() const { return 16 * tiles * (share ? 1 : kAttnWaves); }
+};
+
+// Both structures, with bounds that keep positions inside 32 bits.
+struct CacheCall {
+    lattice_cache cache;
+    lattice_cache_attention args;
+};
+
+int cache_attend_f32(const CacheCall& call, const CacheLayout& layout, const CachePart& part, void* out,
+                     hipStream_t stream);
+int cache_attend_f16(const CacheCall& call, const CacheLayout& layout, const CachePart& part, void* out,
+                     hipStream_t stream);
+int cache_attend_bf16(const CacheCall& call, const CacheLayout& layout, const CachePart& part, void* out,
+                      hipStream_t stream);
+
+}  // namespace lattice

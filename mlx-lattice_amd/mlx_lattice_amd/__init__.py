@@ -11,6 +11,7 @@ from mlx_lattice_amd.core import (
     CoordinateMapKey,
     KernelRelation,
     KernelSpec,
+    QuantizedCache,
     QuantizedWeight,
     SparseTensor,
     dequantize_weight,
@@ -24,6 +25,7 @@ __all__ = [
     'CoordinateMapKey',
     'KernelRelation',
     'KernelSpec',
+    'QuantizedCache',
     'QuantizedWeight',
     'SparseTensor',
     'dequantize_weight',

@@ -1,3 +1,4 @@
+from mlx_lattice_amd.core.cache import QuantizedCache
 from mlx_lattice_amd.core.coords import CoordinateManager, CoordinateMapKey
 from mlx_lattice_amd.core.coords.quantization import (
     PointVoxelMap,
@@ -25,6 +26,7 @@ __all__ = [
     'KernelRelation',
     'KernelSpec',
     'PointVoxelMap',
+    'QuantizedCache',
     'QuantizedWeight',
     'RelationCSRView',
     'RelationEdges',

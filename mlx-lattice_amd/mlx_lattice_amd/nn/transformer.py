@@ -11,15 +11,18 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from mlx_lattice_amd.core import SparseTensor
+from mlx_lattice_amd.core import QuantizedCache, SparseTensor
 from mlx_lattice_amd.nn.conv import SubmConv3d
 from mlx_lattice_amd.ops import (
     batch_offsets,
+    cache_attention,
     dropout,
     layer_norm,
+    residual_norm,
     rotary_frequencies,
     rotary_positions,
     window_attention,
+    write_cache,
 )
 
 __all__ = ['Dropout', 'LayerNorm', 'VoxelTransformerBlock', 'WindowAttention']
@@ -174,21 +177,43 @@ class WindowAttention(nn.Module):
         self.out = SubmConv3d(channels, channels, kernel_size=1, bias=bias,
                               device=device, dtype=dtype)
 
+    def make_cache(self, batches: int, capacity: int, *,
+                   dtype: torch.dtype = torch.float8_e4m3fn
+                   ) -> QuantizedCache:
+        """An empty 8-bit cache for ``batches`` scans of up to ``capacity``
+        rows, on the layer's device."""
+        return QuantizedCache.empty(batches, capacity, self.kv_heads, self.dim,
+                                    dtype=dtype,
+                                    device=self.project.weight.device)
+
     def forward(self, x: SparseTensor, *,
-                offsets: torch.Tensor | None = None) -> SparseTensor:
+                offsets: torch.Tensor | None = None,
+                cache: QuantizedCache | None = None,
+                lengths: torch.Tensor | None = None) -> SparseTensor:
         """``offsets``: the scans' row offsets, which the layers of a level
         can share; ``batch_offsets(x)`` by default, which for a tensor without
-        ``batch_counts``, as strided convs give it, waits for the device."""
+        ``batch_counts``, as strided convs give it, waits for the device.
+
+        With a ``cache`` the rows of ``x`` are new rows of streamed scans: they
+        are appended to it and see what it holds, ``lengths`` ``(B,)`` counting
+        the rows of each scan with the new ones (int32, on the device)."""
+        if (cache is None) != (lengths is None):
+            raise ValueError('cache and lengths go together.')
         if offsets is None:
             offsets = batch_offsets(x)
         packed = self.project(x).feats.view(x.capacity, -1, self.dim)
         turned = packed[:, :self.heads + self.kv_heads]
         turned = rotary_positions(turned, x.coords[:, 1:],
                                   self._on(x.device), dims=self.dims)
-        rows = window_attention(
-            turned[:, :self.heads], turned[:, self.heads:],
-            packed[:, self.heads + self.kv_heads:], left=self.left,
-            right=self.right, sinks=self.sinks, offsets=offsets)
+        queries, keys = turned[:, :self.heads], turned[:, self.heads:]
+        values = packed[:, self.heads + self.kv_heads:]
+        window = {'left': self.left, 'right': self.right, 'sinks': self.sinks,
+                  'offsets': offsets}
+        if cache is None:
+            rows = window_attention(queries, keys, values, **window)
+        else:
+            write_cache(cache, keys, values, offsets=offsets, lengths=lengths)
+            rows = cache_attention(queries, cache, lengths=lengths, **window)
         return self.out(x.replace(feats=rows.view(x.capacity, -1)))
 
     def _on(self, device: torch.device) -> torch.Tensor:
@@ -202,11 +227,13 @@ class VoxelTransformerBlock(nn.Module):
     a ReLU layer of ``hidden`` channels (4 times the channels by default).
 
     ``seed`` gives the two dropouts the seeds ``2 * seed`` and ``2 * seed +
-    1``; by default each draws its own.
+    1``; by default each draws its own.  With ``layer_scale`` each part is
+    multiplied by a gate a channel, which starts at that value.
     """
 
     def __init__(self, channels: int, heads: int, *, hidden: int | None = None,
-                 p: float = 0.0, seed: int | None = None, device=None,
+                 p: float = 0.0, seed: int | None = None,
+                 layer_scale: float | None = None, device=None,
                  dtype: torch.dtype = torch.float32, **attention) -> None:
         super().__init__()
         hidden = 4 * channels if hidden is None else hidden
@@ -218,10 +245,26 @@ class VoxelTransformerBlock(nn.Module):
         self.expand = SubmConv3d(channels, hidden, kernel_size=1, **made)
         self.contract = SubmConv3d(hidden, channels, kernel_size=1, **made)
         self.drop2 = Dropout(p, seed=None if seed is None else 2 * seed + 1)
+        self.gate1, self.gate2 = (
+            None if layer_scale is None else nn.Parameter(
+                torch.full((channels,), float(layer_scale), device=device,
+                           dtype=dtype), requires_grad=False)
+            for _ in range(2))
 
     def forward(self, x: SparseTensor, *,
-                offsets: torch.Tensor | None = None) -> SparseTensor:
-        mixed = self.attention(self.norm1(x), offsets=offsets)
-        x = self.drop1(mixed, residual=x)
-        inner = self.expand(self.norm2(x), activation='relu')
-        return self.drop2(self.contract(inner), residual=x)
+                offsets: torch.Tensor | None = None,
+                cache: QuantizedCache | None = None,
+                lengths: torch.Tensor | None = None) -> SparseTensor:
+        """``cache`` and ``lengths``: as :class:`WindowAttention` takes them."""
+        mixed = self.attention(self.norm1(x), offsets=offsets, cache=cache,
+                               lengths=lengths)
+        if self.gate1 is None:
+            x = self.drop1(mixed, residual=x)
+            inner = self.expand(self.norm2(x), activation='relu')
+            return self.drop2(self.contract(inner), residual=x)
+        x, normed = residual_norm(
+            self.drop1(mixed), x, self.norm2.weight, self.norm2.bias,
+            gate=self.gate1, eps=self.norm2.eps)
+        inner = self.expand(normed, activation='relu')
+        inner = self.drop2(self.contract(inner))
+        return x.replace(feats=torch.addcmul(x.feats, inner.feats, self.gate2))

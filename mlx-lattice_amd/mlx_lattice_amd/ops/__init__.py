@@ -2,6 +2,7 @@ from mlx_lattice_amd.core.coords.builders import (
     build_relation_implicit_gemm_view,
 )
 from mlx_lattice_amd.ops.attention import batch_offsets, window_attention
+from mlx_lattice_amd.ops.cache import cache_attention, read_cache, write_cache
 from mlx_lattice_amd.ops.conv import (
     conv3d,
     conv_transpose3d,
@@ -40,6 +41,7 @@ from mlx_lattice_amd.ops.relations import (
     target_kernel_relation,
     transposed_kernel_relation,
 )
+from mlx_lattice_amd.ops.residual_norm import residual_norm
 from mlx_lattice_amd.ops.rotary import rotary_frequencies, rotary_positions
 from mlx_lattice_amd.ops.tensor import sparse_collate
 
@@ -53,6 +55,7 @@ __all__ = [
     'build_submanifold_kernel_relation',
     'build_target_kernel_relation',
     'build_transposed_kernel_relation',
+    'cache_attention',
     'conv3d',
     'conv_transpose3d',
     'devoxelize',
@@ -68,6 +71,8 @@ __all__ = [
     'layer_norm',
     'max_pool3d',
     'pool3d',
+    'read_cache',
+    'residual_norm',
     'rotary_frequencies',
     'rotary_positions',
     'sparse_collate',
@@ -80,4 +85,5 @@ __all__ = [
     'voxelize',
     'voxelize_with_quantization',
     'window_attention',
+    'write_cache',
 ]

@@ -437,4 +437,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("window_attention_node", &ln::window_attention_node, py::arg("q"), py::arg("k"), py::arg("v"),
           py::arg("offsets"), py::arg("key_offsets"), py::arg("key_lengths"), py::arg("left"), py::arg("right"),
           py::arg("sinks"), py::arg("scale"), "window_attention as a differentiable node.");
+    m.def("residual_norm", &ln::residual_norm, py::arg("x"), py::arg("residual"), py::arg("vectors"),
+          py::arg("scale"), py::arg("post_norm"), py::arg("rms"), py::arg("eps"), py::arg("active_rows"),
+          py::arg("keep_statistics"),
+          "The junction of two parts of a block: (sum, normed, statistics); vectors are (weight, bias, gate, "
+          "post_weight, post_bias).");
+    m.def("residual_norm_grad", &ln::residual_norm_grad, py::arg("grad_sum"), py::arg("grad_normed"), py::arg("sum"),
+          py::arg("statistics"), py::arg("x"), py::arg("residual"), py::arg("vectors"), py::arg("scale"),
+          py::arg("post_norm"), py::arg("rms"), py::arg("eps"), py::arg("active_rows"), py::arg("wanted"),
+          "Gradients of the junction: of x, residual and the wanted vectors.");
+    m.def("residual_norm_node", &ln::residual_norm_node, py::arg("x"), py::arg("residual"), py::arg("vectors"),
+          py::arg("scale"), py::arg("post_norm"), py::arg("rms"), py::arg("eps"), py::arg("active_rows"),
+          "residual_norm as a differentiable node: (sum, normed).");
+    m.def("cache_write", &ln::cache_write, py::arg("parts"), py::arg("dim"), py::arg("k"), py::arg("v"),
+          py::arg("offsets"), py::arg("lengths"),
+          "Append rows to an 8-bit cache; parts are (keys, values, key_exponents, value_exponents).");
+    m.def("cache_read", &ln::cache_read, py::arg("parts"), py::arg("dim"), py::arg("lengths"), py::arg("dtype"),
+          "The keys and values that an 8-bit cache stands for.");
+    m.def("cache_attention", &ln::cache_attention, py::arg("q"), py::arg("parts"), py::arg("dim"),
+          py::arg("offsets"), py::arg("lengths"), py::arg("left"), py::arg("right"), py::arg("sinks"),
+          py::arg("scale"), "Attention over an 8-bit cache.");
 }

@@ -125,6 +125,53 @@ struct WindowAttention : Function<WindowAttention> {
     }
 };
 
+struct ResidualNorm : Function<ResidualNorm> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual,
+                                 const MaybeTensor& weight, const MaybeTensor& bias, const MaybeTensor& gate,
+                                 const MaybeTensor& post_weight, const MaybeTensor& post_bias, double scale,
+                                 bool post_norm, bool rms, double eps, const MaybeTensor& active_rows) {
+        const JoinVectors vectors{weight, bias, gate, post_weight, post_bias};
+        auto [sum, normed, statistics] = residual_norm(x, residual, vectors, scale, post_norm, rms, eps, active_rows,
+                                                       true);
+        variable_list saved{x, residual, sum, statistics, or_undefined(active_rows)};
+        std::vector<bool> wanted;
+        for (const MaybeTensor& v : vectors) {
+            saved.push_back(or_undefined(v));
+            wanted.push_back(wants_grad(v));
+        }
+        ctx->save_for_backward(saved);
+        ctx->saved_data["wanted"] = c10::List<bool>({wanted[0], wanted[1], wanted[2], wanted[3], wanted[4]});
+        ctx->saved_data["x"] = wants_grad(x);
+        ctx->saved_data["residual"] = wants_grad(residual);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["post_norm"] = post_norm;
+        ctx->saved_data["rms"] = rms;
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return {sum, normed};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(12);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        auto& data = ctx->saved_data;
+        const JoinVectors vectors{or_none(saved[5]), or_none(saved[6]), or_none(saved[7]), or_none(saved[8]),
+                                  or_none(saved[9])};
+        const auto list = data["wanted"].toBoolList();
+        std::array<bool, 5> wanted;
+        for (int i = 0; i < 5; ++i) wanted[i] = list.get(i);
+        variable_list made = residual_norm_grad(
+            or_none(grads[0]), or_none(grads[1]), saved[2], saved[3], saved[0], saved[1], vectors,
+            data["scale"].toDouble(), data["post_norm"].toBool(), data["rms"].toBool(), data["eps"].toDouble(),
+            or_none(saved[4]), wanted);
+        if (!data["x"].toBool()) made[0] = at::Tensor();
+        if (!data["residual"].toBool()) made[1] = at::Tensor();
+        made = once(std::move(made));
+        for (int i = 0; i < 7; ++i) out[i] = made[i];
+        return out;
+    }
+};
+
 }  // namespace
 
 at::Tensor layer_norm_node(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
@@ -150,6 +197,15 @@ at::Tensor window_attention_node(const at::Tensor& q, const at::Tensor& k, const
                                  const c10::optional<at::Tensor>& key_lengths, int64_t left, int64_t right,
                                  int64_t sinks, double scale) {
     return WindowAttention::apply(q, k, v, offsets, key_offsets, key_lengths, left, right, sinks, scale);
+}
+
+std::tuple<at::Tensor, at::Tensor> residual_norm_node(const at::Tensor& x, const at::Tensor& residual,
+                                                      const JoinVectors& vectors, double scale, bool post_norm,
+                                                      bool rms, double eps,
+                                                      const c10::optional<at::Tensor>& active_rows) {
+    const variable_list out = ResidualNorm::apply(x, residual, vectors[0], vectors[1], vectors[2], vectors[3],
+                                                  vectors[4], scale, post_norm, rms, eps, active_rows);
+    return {out[0], out[1]};
 }
 
 }  // namespace lattice_native
