@@ -14,12 +14,19 @@ struct CachePart {
 
 // How a call is laid out.
 struct CacheLayout {
-    bool share;       // the waves of a block share rows and split their tokens, or have rows of their own
+    bool share;       // the waves of a block share their pairs and split the tokens, or have pairs of their own
     int tiles;        // tiles of 16 (query, head) pairs a wave
-    int splits;       // blocks that split a row's tokens
-    long long slots;  // tiles of rows at most
+    int splits;       // blocks that split a pair's tokens
+    long long slots;  // blocks of pairs at most
     int rows() const { return 16 * tiles * (share ? 1 : kAttnWaves); }
 };
+
+// Most tiles of pairs that fit a wave's registers.
+template <typename T> constexpr int cache_most_tiles(int width) {
+    return sizeof(T) == 4 ? (width == 32 ? 4 : 2) : width <= 64 ? 4 : width == 96 ? 3 : 2;
+}
+// Where widening a block's codes once for four waves, by way of LDS, is faster.
+template <typename T> constexpr bool cache_many(int width) { return width == 128 && sizeof(T) == 2; }
 
 // Both structures, with bounds that keep positions inside 32 bits.
 struct CacheCall {

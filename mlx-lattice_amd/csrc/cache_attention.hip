@@ -27,12 +27,15 @@ const char* cache_attention_fault(const lattice_cache* c, const lattice_cache_at
     return nullptr;
 }
 
+constexpr int kUnits = 512;  // blocks that fill the chip, two a unit
+
 CacheCall cache_call(const lattice_cache& c, const lattice_cache_attention& a) {
     CacheCall call{c, a};
-    // Nothing lies further than the cache and the queries are long.
-    const int most = c.blocks * kCacheBlock + a.queries;
-    call.args.left = std::min(a.left, most);
-    call.args.right = std::min(a.right, most);
+    // Positions stay below 2^29 + 2^28, the sums with these inside 32 bits.
+    constexpr int kFar = 1 << 30;
+    static_assert(kCacheLongest <= 1 << 29);
+    call.args.left = std::min(a.left, kFar);
+    call.args.right = std::min(a.right, kFar);
     call.args.sinks = std::min(a.sinks, c.blocks * kCacheBlock);
     return call;
 }
@@ -40,22 +43,39 @@ CacheCall cache_call(const lattice_cache& c, const lattice_cache_attention& a) {
 CacheLayout cache_layout(const CacheCall& call) {
     const lattice_cache& c = call.cache;
     const lattice_cache_attention& a = call.args;
-    const int group = a.heads / c.kv_heads;
+    const int group = a.heads / c.kv_heads, width = cache_width(c);
     const long long pairs = static_cast<long long>(a.queries) * group;
     const int sequences = std::max(1, c.sequences);
-    CacheLayout l;
-    l.share = pairs / 32 * c.kv_heads < 1024;
-    l.tiles = l.share ? 1 : 2;
-    l.slots = pairs / l.rows() + c.sequences + 2;
-    l.splits = 1;
-    if (l.share) {
-        const long long busy =
-            std::max<long long>((pairs + l.rows() - 1) / l.rows(), std::min<long long>(sequences, a.queries)) * c.kv_heads;
-        const long long seen = std::min<long long>(static_cast<long long>(a.left) + a.right + a.sinks +
-                                                       std::min(a.queries, l.rows()),
-                                                   static_cast<long long>(c.blocks) * kCacheBlock);
-        l.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({(512 + busy - 1) / busy, seen / 256, 64})));
+    // Blocks that have rows.
+    const auto blocks = [&](int rows) {
+        return std::max<long long>((pairs + rows - 1) / rows, std::min<long long>(sequences, a.queries)) * c.kv_heads;
+    };
+    const auto filled = [&](int rows) { return 2 * pairs > static_cast<long long>(rows) * sequences; };
+    CacheLayout l{true, 1, 1, 0};
+    const bool f32 = a.dtype == LATTICE_F32;
+    if ((f32 ? cache_many<float>(width) : cache_many<_Float16>(width)) && filled(32 * kAttnWaves) &&
+        blocks(32 * kAttnWaves) >= kUnits) {
+        l.share = false;
+        l.tiles = 2;
+    } else {
+        // The largest tiles that are mostly filled and, their tokens split, give
+        // every unit its blocks.
+        const long long seen = std::min<long long>(
+            static_cast<long long>(a.left) + a.right + a.sinks + std::min(a.queries, 16),
+            static_cast<long long>(c.blocks) * kCacheBlock);
+        const int most = f32 ? cache_most_tiles<float>(width) : cache_most_tiles<_Float16>(width);
+        for (int tiles : {most, 2, 1}) {
+            const long long own = blocks(16 * tiles), parts = std::min<long long>(64, seen / (tiles > 1 ? 2048 : 512));
+            if (tiles > 1 && (!filled(16 * tiles) || own * std::max(1ll, parts) < kUnits / 2)) continue;
+            l.tiles = tiles;
+            if (own < kUnits) {
+                const long long wanted = (tiles > 1 ? 2 : 4) * kUnits;
+                l.splits = static_cast<int>(std::max(1ll, std::min(parts, (wanted + own - 1) / own)));
+            }
+            break;
+        }
     }
+    l.slots = pairs / l.rows() + c.sequences + 2;
     return l;
 }
 

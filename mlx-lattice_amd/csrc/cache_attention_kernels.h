@@ -90,17 +90,25 @@ struct CacheTerms {
 // A block's codes as a lane holds them: of two rows of keys, and of DP / 16
 // channels of values.
 template <int DP>
-struct CacheCodes {
-    uint2 k[2][DP / 32], v[DP / 16];
-    int key_exponent, value_exponent;
+struct CacheKeys {
+    uint2 w[2][DP / 32];
+    int exponent;
+};
+template <int DP>
+struct CacheValues {
+    uint2 w[DP / 16];
+    int exponent;
 };
 
-// The channels that a lane gives to step `c` of the first product: 16 bytes a
-// load serve two steps, a rest of 32 channels 8 bytes one.
-template <int DP>
+// The channels that a lane gives to step `c` of the first product.  WIDE: 16
+// bytes a load serve two steps, a rest of 32 channels 8 bytes one.
+template <int DP, bool WIDE>
 __device__ constexpr int key_channel(int c, int g) {
-    return c < DP / 64 * 2 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : DP / 64 * 64 + 8 * g;
+    return !WIDE ? 32 * c + 8 * g : c < DP / 64 * 2 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : DP / 64 * 64 + 8 * g;
 }
+// The token of row `n` of the first product's half `i`: a lane ends with the
+// scores of tokens 8 g .. 8 g + 7.
+__device__ constexpr int key_token(int i, int n) { return 8 * (n >> 2) + 4 * i + (n & 3); }
 
 template <int DP>
 struct CacheReader {
@@ -115,46 +123,56 @@ struct CacheReader {
         key_exponents = c.key_exponents + at;
         value_exponents = c.value_exponents + at;
         const int n = lane_id() & 15, g = lane_id() >> 4;
-        key_place = (8 * (n >> 2) + (n & 3)) * DP;
+        key_place = key_token(0, n) * DP;
         value_place = n * kCacheBlock + 8 * g;
     }
-    __device__ void load(CacheCodes<DP>& to, int block) const {
+    __device__ void load(CacheKeys<DP>& to, int block) const {
         const uint8_t* k = keys + static_cast<long long>(block) * (kCacheBlock * DP);
-        const uint8_t* v = values + static_cast<long long>(block) * (kCacheBlock * DP);
         const int g = lane_id() >> 4;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c) {
                 const uint4 w = *reinterpret_cast<const uint4*>(k + key_place + 4 * i * DP + 64 * c + 16 * g);
-                to.k[i][2 * c] = uint2{w.x, w.y};
-                to.k[i][2 * c + 1] = uint2{w.z, w.w};
+                to.w[i][2 * c] = uint2{w.x, w.y};
+                to.w[i][2 * c + 1] = uint2{w.z, w.w};
             }
             if constexpr (DP % 64 != 0)
-                to.k[i][DP / 32 - 1] =
+                to.w[i][DP / 32 - 1] =
                     *reinterpret_cast<const uint2*>(k + key_place + 4 * i * DP + DP / 64 * 64 + 8 * g);
         }
+        to.exponent = key_exponents[block];
+    }
+    __device__ void load(CacheValues<DP>& to, int block) const {
+        const uint8_t* v = values + static_cast<long long>(block) * (kCacheBlock * DP);
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t)
-            to.v[t] = *reinterpret_cast<const uint2*>(v + value_place + 16 * t * kCacheBlock);
-        to.key_exponent = key_exponents[block];
-        to.value_exponent = value_exponents[block];
+            to.w[t] = *reinterpret_cast<const uint2*>(v + value_place + 16 * t * kCacheBlock);
+        to.exponent = value_exponents[block];
     }
 };
 
-// A share is exp2(score - top), where top is the running maximum and may lag
-// behind the scores by kLag powers of two.  Shares times 2^(e - unit + kFill) go
-// into the second product: at most 2^(kUnitLag + kFill), where the running unit
-// lags.  In half precision, which loses bits below 2^-14, they fill the range:
-// a product keeps all bits down to 2^-26 of the largest.
-constexpr float kCacheLag = 8.0f;
+// What goes into the second product is 2^(score - top + e - unit + kFill), e the
+// exponent of the block's values: top and unit are running maxima of the scores
+// and of (score - top + e).  They move where the eight of a lane add up to more
+// than kMost, so that nothing is compared on the way.  In half precision, which
+// loses bits below 2^-14, they fill the range: a product keeps all bits down to
+// 2^-25 of the largest.
 template <typename T> struct CacheRange {
-    static constexpr int kFill = 0, kUnitLag = 8;
+    static constexpr int kFill = 0;
+    static constexpr float kMost = 2048.0f;
 };
 template <> struct CacheRange<_Float16> {
-    static constexpr int kFill = 13, kUnitLag = 2;
+    static constexpr int kFill = 12;
+    static constexpr float kMost = 40000.0f;
 };
+// The power of two that is taken into the exponent is no less, so that sums of
+// shares are not lost where a block's values are next to nothing.
+constexpr int kCacheLeastShift = -60;
 constexpr int kCacheNoUnit = -(1 << 20);
+// A row's top starts far below every score but above -inf, so that what is
+// masked (-inf) has a share of zero.
+constexpr float kCacheFloor = -3.0e38f;
 
 // What a pair sees.
 struct CacheRow {
@@ -167,14 +185,14 @@ template <typename T, int DP, int R>
 struct CacheState {
     f32x4_attn acc[R][DP / 16];
     float top[R], sum[R];
-    int unit[R];  // acc is in units of 2^unit
+    int unit[R];  // sums are in units of 2^top, acc in units of 2^(top + unit)
 
     __device__ void clear() {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) acc[r][t] = f32x4_attn{};
-            top[r] = -3.0e38f;
+            top[r] = kCacheFloor;
             sum[r] = 0.0f;
             unit[r] = kCacheNoUnit;
         }
@@ -195,89 +213,127 @@ __device__ inline float pair_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// 2^e, zero far below.
-__device__ inline float bounded_power(int e) { return e < -126 ? 0.0f : power_of_two(min(e, 126)); }
+// 2^e for e up to 127, zero below -126 (the bits of zero).
+__device__ inline float bounded_power(int e) { return power_of_two(max(e, -127)); }
 
-// Adds the tokens j0 .. j0 + 31 to the wave's pairs; `masked`: some are not seen
-// by some pair.
-template <typename T, typename Code, int DP, int R>
-__device__ inline void attend_codes(CacheState<T, DP, R>& state, const CacheTerms<T> (&q)[R][DP / 32],
-                                    const CacheCodes<DP>& codes, const CacheRow (&rows)[R], float scale, int sinks,
-                                    int nk, int j0, bool masked) {
-    typedef typename CacheMath<T>::Operand O;
-    typedef typename CacheOperand<O>::Frag Frag;
-    const int g = lane_id() >> 4;
-    f32x4_attn s[R][2];
+// Bytes of tokens behind the last stand for nothing: those of a lane's eight
+// that are kept of a block's first `count`.
+__device__ inline uint64_t kept_bytes(int count) {
+    const int mine = count - 8 * (lane_id() >> 4);
+    return mine <= 0 ? 0 : mine >= 8 ? ~0ull : ~0ull >> 8 * (8 - mine);
+}
+__device__ inline uint2 cut_bytes(uint2 w, uint64_t keep) {
+    return uint2{w.x & static_cast<uint32_t>(keep), w.y & static_cast<uint32_t>(keep >> 32)};
+}
+
+// The scores of a block's tokens, before any scale, 8 tokens a lane; key(i, c)
+// gives the first product's left operand.
+template <typename T, int DP, int R, typename Keys>
+__device__ inline void cache_scores(f32x4_attn (&s)[R][2], const CacheTerms<T> (&q)[R][DP / 32], const Keys& key) {
 #pragma unroll
     for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = f32x4_attn{};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int c = 0; c < DP / 32; ++c) {
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-            const Frag k = widen<Code, O>(codes.k[i][c]);
+        for (int i = 0; i < 2; ++i) {
+            const auto k = key(i, c);
 #pragma unroll
             for (int r = 0; r < R; ++r) s[r][i] = q[r][c].product(k, s[r][i]);
         }
     }
-    const int key_exponent = max(codes.key_exponent, kCacheLeast);
-    const int value_exponent = max(codes.value_exponent, kCacheLeast);
-    // Positive, so that -inf stays -inf.
-    const float factor = fmaxf(scale * power_of_two(key_exponent), FLT_MIN);
-    CacheTerms<T> p[R];
+}
+
+// 8 shares of a pair and their sum, whose exponent was lowered by `shift` less.
+struct CacheShares {
+    float y[8], sum;
+    int wanted, shift;
+
+    template <typename T, int DP, int R>
+    __device__ void make(const CacheState<T, DP, R>& state, int r, const f32x4_attn (&s)[2], float factor,
+                         int value_exponent) {
+        wanted = value_exponent - state.unit[r] + CacheRange<T>::kFill;
+        shift = max(wanted, kCacheLeastShift);
+        const float base = static_cast<float>(shift) - state.top[r];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], factor, base));
+        sum = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+    }
+};
+
+// What tokens j0 .. j0 + 31 some pair does not see has no share.
+template <int R>
+__device__ inline void hide_scores(f32x4_attn (&s)[R][2], const CacheRow (&rows)[R], int sinks, int j0) {
+    const int j = j0 + 8 * (lane_id() >> 4);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[r][e / 4][e % 4];
-        if (masked) {
-            const int j = j0 + 8 * g;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool seen = j + e <= rows[r].hi && (j + e >= rows[r].lo || j + e < sinks);
-                x[e] = seen ? x[e] : -INFINITY;
-            }
-        }
-        float most = x[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) most = fmaxf(most, x[e]);
-        most *= factor;
-        if (__any(most > state.top[r] + kCacheLag)) {
-            const float next = fmaxf(state.top[r], pair_max(most));
-            const float old = __builtin_amdgcn_exp2f(state.top[r] - next);
-            state.rescale(r, old);
-            state.sum[r] *= old;
-            state.top[r] = next;
-        }
-        // The largest share times the block's power of two.
-        if (__any(most - state.top[r] + static_cast<float>(value_exponent) >
-                  static_cast<float>(state.unit[r] + CacheRange<T>::kUnitLag))) {
-            const float size = pair_max(most) - state.top[r] + static_cast<float>(value_exponent);
-            const int next = max(state.unit[r], static_cast<int>(ceilf(fmaxf(size, -512.0f))));
-            state.rescale(r, bounded_power(state.unit[r] - next));
-            state.unit[r] = next;
-        }
-        const float share = bounded_power(value_exponent - state.unit[r] + CacheRange<T>::kFill);
-        float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] = __builtin_amdgcn_exp2f(x[e] * factor - state.top[r]);
-            sum += x[e];
-            x[e] *= share;
+            const bool seen = j + e <= rows[r].hi && (j + e >= rows[r].lo || j + e < sinks);
+            s[r][e / 4][e % 4] = seen ? s[r][e / 4][e % 4] : -INFINITY;
         }
-        state.sum[r] += sum;
-        p[r].set(x);
     }
-    // Bytes behind the last token stand for nothing.
-    const int behind = nk - (j0 + 8 * g);
+}
+
+// Moves a row's maxima to what its scores ask for.
+template <typename T, int DP, int R>
+__device__ inline void move_maxima(CacheState<T, DP, R>& state, int r, const f32x4_attn (&s)[2], float factor,
+                                   int value_exponent) {
+    float most = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e / 4][e % 4]);
+    most = pair_max(most * factor);
+    const float top = fmaxf(state.top[r], most);
+    const float down = fminf(top - state.top[r], 1024.0f);
+    const float size = fmaxf(most - top + static_cast<float>(value_exponent), -512.0f);
+    const int unit = max(state.unit[r] - static_cast<int>(down), static_cast<int>(ceilf(size)));
+    state.sum[r] *= __builtin_amdgcn_exp2f(state.top[r] - top);
+    state.rescale(r, __builtin_amdgcn_exp2f(state.top[r] - top + static_cast<float>(state.unit[r] - unit)));
+    state.top[r] = top;
+    state.unit[r] = unit;
+}
+
+// The shares of the wave's pairs as the second product's operand.  One test a
+// block tells whether a maximum has to move.
+template <typename T, int DP, int R>
+__device__ inline void cache_shares(CacheTerms<T> (&p)[R], CacheState<T, DP, R>& state, const f32x4_attn (&s)[R][2],
+                                    float factor, int value_exponent) {
+    CacheShares x[R];
+    for (int tries = 0;; ++tries) {
+        bool moves = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            x[r].make(state, r, s[r], factor, value_exponent);
+            moves = moves || x[r].sum > CacheRange<T>::kMost;
+        }
+        if (!__any(moves) || tries > 0) break;
+#pragma unroll
+        for (int r = 0; r < R; ++r) move_maxima<T, DP, R>(state, r, s[r], factor, value_exponent);
+    }
+    bool low = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) low = low || x[r].wanted < kCacheLeastShift;
+    if (__any(low)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float rest = bounded_power(x[r].wanted - x[r].shift);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[r].y[e] *= rest;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        state.sum[r] += x[r].sum * bounded_power(-x[r].shift);
+        p[r].set(x[r].y);
+    }
+}
+
+// acc += values times shares; value(t) gives the second product's left operand.
+template <typename T, int DP, int R, typename Values>
+__device__ inline void add_cache_values(CacheState<T, DP, R>& state, const CacheTerms<T> (&p)[R],
+                                        const Values& value) {
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
-        uint2 w = codes.v[t];
-        if (masked && behind < 8) {
-            const uint64_t keep = behind <= 0 ? 0 : ~0ull >> 8 * (8 - behind);
-            w.x &= static_cast<uint32_t>(keep);
-            w.y &= static_cast<uint32_t>(keep >> 32);
-        }
-        const Frag v = widen<Code, O>(w);
+        const auto v = value(t);
 #pragma unroll
         for (int r = 0; r < R; ++r) state.acc[r][t] = p[r].product(v, state.acc[r][t]);
     }
@@ -376,52 +432,25 @@ __device__ inline AttnTiles cache_blocks(const lattice_cache_attention& a, int n
     return {first, from, first + max(0, hi / kCacheBlock - from + 1)};
 }
 
-// SHARE: the block's waves have the same R tiles of pairs and take turns at the
-// blocks of tokens; their parts are joined in LDS.  Otherwise each has R tiles
-// of its own.
-template <typename T, typename Code, int DP, int R, bool SHARE>
-__global__ void __launch_bounds__(kAttnBlock)
-cache_attend(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
-    constexpr int kTiles = DP / 16;
-    constexpr int kRows = 16 * R;
-    constexpr int kValues = R * kTiles * 4 * kWave;  // sums of a wave
-    __shared__ AttnRowScratch scratch[kAttnWaves];
-    __shared__ float2 states[SHARE ? kAttnWaves * kRows : 1];
-    __shared__ float sums[SHARE ? kAttnWaves / 2 * kValues : 1];
-    const lattice_cache& c = call.cache;
+// The queries of the wave's pairs, negated where the scale is negative.
+template <typename T, int DP, int R, bool WIDE>
+__device__ inline void cache_queries(CacheTerms<T> (&q)[R][DP / 32], const CacheCall& call, const CacheSequence& s,
+                                     const CacheRow (&rows)[R]) {
     const lattice_cache_attention& a = call.args;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
-    const int n = lane & 15, g = lane >> 4;
-    const uint32_t group = a.heads / c.kv_heads;
-    const int kv = blockIdx.y, split = block_part(splits);
-    constexpr int kSlot = SHARE ? kRows : kRows * kAttnWaves;
-    const RowPartition partition{a.offsets, c.sequences, a.queries};
-    const auto slot_of = [group](int start, int e) { return start * group / kSlot + e; };
-    const uint32_t slot = block_slot(splits);
-    const int e = partition.find(slot, slot_of);
-    const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
-    const uint32_t count = s.nq * group;
-    const uint32_t start = slot_first<kSlot>(slot, slot_of(s.q0, e), count);
-    const uint32_t first = start + (SHARE ? 0 : wave * kRows);
-    if (start >= count) return;
-    if (!SHARE && first >= count) return;
-
-    CacheRow rows[R];
-    cache_rows<R>(rows, call, s, kv, first);
-    CacheTerms<T> q[R][DP / 32];
+    constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+    const int g = lane_id() >> 4;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const T* row = static_cast<const T*>(a.q) + (static_cast<long long>(s.q0) + rows[r].i) * a.q_row_stride +
                        rows[r].head * a.q_head_stride;
-        constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
         for (int k = 0; k < DP / 32; ++k) {
             float x[8];
 #pragma unroll
             for (int h = 0; h < 8 / kPiece; ++h) {
-                const int channel = key_channel<DP>(k, g) + h * kPiece;
+                const int channel = key_channel<DP, WIDE>(k, g) + h * kPiece;
                 RowVec<T, kPiece> in;
-                const bool here = rows[r].valid && channel < c.dim;
+                const bool here = rows[r].valid && channel < call.cache.dim;
                 if (here) in = RowVec<T, kPiece>::load(row + channel);
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) {
@@ -432,98 +461,58 @@ cache_attend(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
             q[r][k].set(x);
         }
     }
-    const float scale = fabsf(a.scale) * kAttnLog2e;
-    const int p_low = static_cast<int>(first / group) + s.shift();
-    const int p_high = static_cast<int>((min(first + kRows, count) - 1) / group) + s.shift();
-    CacheState<T, DP, R> state;
-    state.clear();
-    if (partition.real(e)) {
-        const AttnTiles blocks = cache_blocks(a, s.nk, p_low, p_high);
-        const CacheReader<DP> reader(c, e - 1, kv);
-        const int parts = SHARE ? splits * kAttnWaves : 1, mine = SHARE ? split * kAttnWaves + wave : 0;
-        const int from = static_cast<int>(static_cast<long long>(blocks.count) * mine / parts);
-        const int to = static_cast<int>(static_cast<long long>(blocks.count) * (mine + 1) / parts);
-        CacheCodes<DP> codes;
-        if (from < to) reader.load(codes, blocks.tile(from));
-        for (int index = from; index < to; ++index) {
-            const CacheCodes<DP> now = codes;
-            if (index + 1 < to) reader.load(codes, blocks.tile(index + 1));
-            const int j0 = blocks.tile(index) * kCacheBlock, end = j0 + kCacheBlock;
-            const bool all = end <= s.nk && end - 1 <= p_low + a.right && (j0 >= p_high - a.left || end <= a.sinks);
-            attend_codes<T, Code, DP, R>(state, q, now, rows, scale, a.sinks, s.nk, j0, !all);
-        }
-    }
+}
+
+// How positions p_low .. p_high see a block of tokens from j0 on.
+struct CacheView {
+    int all_to, all_from, all_first;      // all of it
+    int some_to, some_from, some_first;  // some of it
+    __device__ CacheView(const lattice_cache_attention& a, int nk, int p_low, int p_high)
+        : all_to(min(nk, p_low + a.right + 1) - kCacheBlock),
+          all_from(p_high - a.left),
+          all_first(a.sinks - kCacheBlock),
+          some_to(min(nk, p_high + a.right + 1) - 1),
+          some_from(p_low - a.left - kCacheBlock + 1),
+          some_first(a.sinks - 1) {}
+    __device__ bool all(int j0) const { return j0 <= all_to && (j0 >= all_from || j0 <= all_first); }
+    __device__ bool some(int j0) const { return j0 <= some_to && (j0 >= some_from || j0 <= some_first); }
+};
+
+// The factor of a block's scores, positive, so that -inf stays -inf.
+__device__ inline float cache_factor(float scale, int key_exponent) {
+    return fmaxf(scale * power_of_two(max(key_exponent, kCacheLeast)), FLT_MIN);
+}
+
+// Sums over the four lanes of a pair, and products in units of one.
+template <typename T, int DP, int R>
+__device__ inline void close_state(CacheState<T, DP, R>& state) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         state.sum[r] = pair_sum(state.sum[r]);
-        // To units of one, in two steps of normal numbers.
-        const int half = (state.unit[r] - CacheRange<T>::kFill) / 2;
-        state.rescale(r, bounded_power(half));
-        state.rescale(r, bounded_power(state.unit[r] - CacheRange<T>::kFill - half));
+        // In two steps of normal numbers.
+        const int unit = state.unit[r] - CacheRange<T>::kFill;
+        state.rescale(r, bounded_power(unit / 2));
+        state.rescale(r, bounded_power(unit - unit / 2));
     }
-    if constexpr (SHARE) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (g == 0) states[wave * kRows + 16 * r + n] = float2{state.top[r], state.sum[r]};
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float top = -3.0e38f, sum = 0.0f;
-            for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, states[w * kRows + 16 * r + n].x);
-            for (int w = 0; w < kAttnWaves; ++w) {
-                const float2 other = states[w * kRows + 16 * r + n];
-                sum += other.y * __builtin_amdgcn_exp2f(other.x - top);
-            }
-            state.rescale(r, __builtin_amdgcn_exp2f(state.top[r] - top));
-            state.top[r] = top;
-            state.sum[r] = sum;
-        }
-#pragma unroll
-        for (int active = kAttnWaves / 2; active > 0; active /= 2) {
-            __syncthreads();
-            if (wave >= active && wave < 2 * active) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t)
-                        *reinterpret_cast<f32x4_attn*>(sums + (wave - active) * kValues +
-                                                       ((r * kTiles + t) * kWave + lane) * 4) = state.acc[r][t];
-                }
-            }
-            __syncthreads();
-            if (wave < active) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t)
-                        state.acc[r][t] += *reinterpret_cast<const f32x4_attn*>(
-                            sums + wave * kValues + ((r * kTiles + t) * kWave + lane) * 4);
-                }
-            }
-        }
-        if (wave != 0) return;
-    }
-    const long long items = static_cast<long long>(a.queries) * a.heads;
+}
+
+// Writes the wave's results.  One that is not finite is made again from its
+// definition.
+template <typename T, typename Code, int DP, int R>
+__device__ inline void write_pairs(const CacheCall& call, const CacheSequence& s, int sequence,
+                                   const CacheRow (&rows)[R], CacheState<T, DP, R>& state, T* out,
+                                   AttnRowScratch* scratch) {
+    const lattice_cache& c = call.cache;
+    const lattice_cache_attention& a = call.args;
+    const int n = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const long long at = (static_cast<long long>(s.q0) + rows[r].i) * a.heads + rows[r].head;
-        if (splits > 1) {
-            if (!rows[r].valid) continue;
-            const long long row = split * items + at;
-            if (g == 0) part.states[row] = float2{state.top[r], state.sum[r]};
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                const int d = 16 * t + 4 * g;
-                if (d < c.dim) *reinterpret_cast<f32x4_attn*>(part.values + row * c.dim + d) = state.acc[r][t];
-            }
-            continue;
-        }
         const bool sees = rows[r].hi >= max(0, rows[r].lo) || (a.sinks > 0 && rows[r].hi >= 0);
         const float inv = sees ? 1.0f / state.sum[r] : 0.0f;
         uint32_t largest = 0;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+        for (int t = 0; t < DP / 16; ++t) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 state.acc[r][t][i] *= inv;
@@ -535,7 +524,7 @@ cache_attend(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
         uint32_t again = static_cast<uint32_t>(spoilt | spoilt >> 16 | spoilt >> 32 | spoilt >> 48) & 0xffffu;
         if (rows[r].valid && !(again >> n & 1)) {
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
+            for (int t = 0; t < DP / 16; ++t) {
                 const int d = 16 * t + 4 * g;
                 if (d >= c.dim) continue;
                 RowVec<T, 4> v;
@@ -547,10 +536,312 @@ cache_attend(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
         while (again) {
             const int which = __ffs(again) - 1;
             again &= again - 1;
-            attend_pair<T, Code>(call, s, e - 1, __shfl(rows[r].i, which), __shfl(rows[r].head, which), out,
-                                 &scratch[wave]);
+            attend_pair<T, Code>(call, s, sequence, __shfl(rows[r].i, which), __shfl(rows[r].head, which), out,
+                                 scratch);
         }
     }
+}
+
+// For few queries: the block's waves have the same R tiles of pairs and take
+// each its share of the blocks of tokens, codes straight from memory to
+// registers; their parts are joined in LDS.
+template <typename T, typename Code, int DP, int R>
+__global__ void __launch_bounds__(kAttnBlock, 2)
+cache_attend_few(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
+    typedef typename CacheMath<T>::Operand O;
+    constexpr int kTiles = DP / 16;
+    constexpr int kRows = 16 * R;
+    constexpr int kValues = R * kTiles * 4 * kWave;  // sums of a wave
+    __shared__ AttnRowScratch scratch;
+    __shared__ float2 states[kAttnWaves * kRows];
+    __shared__ float sums[kAttnWaves / 2 * kValues];
+    const lattice_cache& c = call.cache;
+    const lattice_cache_attention& a = call.args;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+    const int n = lane & 15, g = lane >> 4;
+    const uint32_t group = a.heads / c.kv_heads;
+    const int kv = blockIdx.y, split = block_part(splits);
+    const RowPartition partition{a.offsets, c.sequences, a.queries};
+    const auto slot_of = [group](int start, int e) { return start * group / kRows + e; };
+    const uint32_t slot = block_slot(splits);
+    const int e = partition.find(slot, slot_of);
+    const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
+    const uint32_t count = s.nq * group;
+    const uint32_t first = slot_first<kRows>(slot, slot_of(s.q0, e), count);
+    if (first >= count) return;
+
+    const int p_low = static_cast<int>(first / group) + s.shift();
+    const int p_high = static_cast<int>((min(first + kRows, count) - 1) / group) + s.shift();
+    const AttnTiles blocks = partition.real(e) ? cache_blocks(a, s.nk, p_low, p_high) : AttnTiles{0, 0, 0};
+    const CacheReader<DP> reader(c, e - 1, kv);
+    const int parts = splits * kAttnWaves, mine = split * kAttnWaves + wave;
+    const int from = static_cast<int>(static_cast<long long>(blocks.count) * mine / parts);
+    const int to = static_cast<int>(static_cast<long long>(blocks.count) * (mine + 1) / parts);
+    // Codes are read into the registers that the block before has left, the first
+    // ones before the queries are.
+    CacheKeys<DP> keys;
+    CacheValues<DP> values;
+    if (from < to) {
+        reader.load(keys, blocks.tile(from));
+        reader.load(values, blocks.tile(from));
+    }
+    CacheRow rows[R];
+    cache_rows<R>(rows, call, s, kv, first);
+    CacheTerms<T> q[R][DP / 32];
+    cache_queries<T, DP, R, true>(q, call, s, rows);
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const CacheView view(a, s.nk, p_low, p_high);
+    CacheState<T, DP, R> state;
+    state.clear();
+    for (int index = from; index < to; ++index) {
+        const int next = blocks.tile(min(index + 1, to - 1));
+        const int j0 = blocks.tile(index) * kCacheBlock;
+        f32x4_attn scores[R][2];
+        cache_scores<T, DP, R>(scores, q, [&](int i, int k) { return widen<Code, O>(keys.w[i][k]); });
+        const float factor = cache_factor(scale, keys.exponent);
+        reader.load(keys, next);
+        CacheTerms<T> p[R];
+        if (!view.all(j0)) {
+            hide_scores<R>(scores, rows, a.sinks, j0);
+            const uint64_t keep = kept_bytes(s.nk - j0);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) values.w[t] = cut_bytes(values.w[t], keep);
+        }
+        cache_shares<T, DP, R>(p, state, scores, factor, max(values.exponent, kCacheLeast));
+        add_cache_values<T, DP, R>(state, p, [&](int t) { return widen<Code, O>(values.w[t]); });
+        reader.load(values, next);
+    }
+    close_state<T, DP, R>(state);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (g == 0) states[wave * kRows + 16 * r + n] = float2{state.top[r], state.sum[r]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float top = kCacheFloor, sum = 0.0f;
+        for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, states[w * kRows + 16 * r + n].x);
+        for (int w = 0; w < kAttnWaves; ++w) {
+            const float2 other = states[w * kRows + 16 * r + n];
+            sum += other.y * __builtin_amdgcn_exp2f(other.x - top);
+        }
+        state.rescale(r, __builtin_amdgcn_exp2f(state.top[r] - top));
+        state.top[r] = top;
+        state.sum[r] = sum;
+    }
+#pragma unroll
+    for (int active = kAttnWaves / 2; active > 0; active /= 2) {
+        __syncthreads();
+        if (wave >= active && wave < 2 * active) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    *reinterpret_cast<f32x4_attn*>(sums + (wave - active) * kValues +
+                                                   ((r * kTiles + t) * kWave + lane) * 4) = state.acc[r][t];
+            }
+        }
+        __syncthreads();
+        if (wave < active) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    state.acc[r][t] += *reinterpret_cast<const f32x4_attn*>(
+                        sums + wave * kValues + ((r * kTiles + t) * kWave + lane) * 4);
+            }
+        }
+    }
+    if (wave != 0) return;
+    if (splits == 1) {
+        write_pairs<T, Code, DP, R>(call, s, e - 1, rows, state, out, &scratch);
+        return;
+    }
+    const long long items = static_cast<long long>(a.queries) * a.heads;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (!rows[r].valid) continue;
+        const long long row =
+            split * items + (static_cast<long long>(s.q0) + rows[r].i) * a.heads + rows[r].head;
+        if (g == 0) part.states[row] = float2{state.top[r], state.sum[r]};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int d = 16 * t + 4 * g;
+            if (d < c.dim) *reinterpret_cast<f32x4_attn*>(part.values + row * c.dim + d) = state.acc[r][t];
+        }
+    }
+}
+
+// Blocks of tokens as operands in LDS, 16 bytes a lane each, written as they are
+// read: DP / 16 of a block's keys, or of its values.
+template <typename T, typename Code, int DP>
+struct CacheStage {
+    typedef typename CacheMath<T>::Operand O;
+    typedef typename CacheOperand<O>::Frag Frag;
+    static constexpr int kFrags = DP / 16;
+    static constexpr int kBytes = kFrags * kWave * 16;
+    // Operands that a wave makes; where they do not go around, the last waves
+    // have one less.
+    static constexpr int kMine = (kFrags + kAttnWaves - 1) / kAttnWaves;
+    struct Codes {
+        uint2 w[kMine];
+    };
+
+    const uint8_t* base;
+    uint32_t place[kMine];
+
+    // The keys or the values of `codes`.
+    __device__ CacheStage(const void* codes, long long at, bool values, int wave)
+        : base(static_cast<const uint8_t*>(codes) + at * kCacheBlock * DP) {
+        const int n = lane_id() & 15, g = lane_id() >> 4;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int f = min(wave + kAttnWaves * k, kFrags - 1);
+            place[k] = values ? (16 * f + n) * kCacheBlock + 8 * g
+                              : key_token(f / (DP / 32), n) * DP + key_channel<DP, false>(f % (DP / 32), g);
+        }
+    }
+    // Starts the reads of a block's codes.
+    __device__ void load(Codes& to, int block) const {
+        const uint8_t* from = base + static_cast<long long>(block) * (kCacheBlock * DP);
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) to.w[k] = *reinterpret_cast<const uint2*>(from + place[k]);
+    }
+    // Tokens from `count` on stand for nothing (values).
+    __device__ static void cut(Codes& codes, int count) {
+        const uint64_t keep = kept_bytes(count);
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) codes.w[k] = cut_bytes(codes.w[k], keep);
+    }
+    // Widens a block's codes into `to`.
+    __device__ static void write(char* to, const Codes& from, int wave) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            // The last ones twice, with the same bytes.
+            const int f = min(wave + kAttnWaves * k, kFrags - 1);
+            *reinterpret_cast<Frag*>(to + (f * kWave + lane_id()) * 16) = widen<Code, O>(from.w[k]);
+        }
+    }
+    __device__ static Frag operand(const char* from, int f) {
+        return *reinterpret_cast<const Frag*>(from + (f * kWave + lane_id()) * 16);
+    }
+};
+
+// For many queries: each wave has R tiles of pairs of its own; a block of tokens
+// is widened once for the four, into LDS.  A step makes the shares of one block
+// while the scores of the next are on their way through the matrix cores, then
+// adds the block's values while the codes of the next are widened.
+template <typename T, typename Code, int DP, int R>
+__global__ void __launch_bounds__(kAttnBlock, 2)
+cache_attend_many(CacheCall call, T* __restrict__ out) {
+    typedef CacheStage<T, Code, DP> Stage;
+    constexpr int kRows = 16 * R;
+    __shared__ AttnRowScratch scratch[kAttnWaves];
+    __shared__ __align__(16) char staged[4 * Stage::kBytes];
+    const lattice_cache& c = call.cache;
+    const lattice_cache_attention& a = call.args;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t group = a.heads / c.kv_heads;
+    const int kv = blockIdx.y;
+    constexpr int kSlot = kRows * kAttnWaves;
+    const RowPartition partition{a.offsets, c.sequences, a.queries};
+    const auto slot_of = [group](int start, int e) { return start * group / kSlot + e; };
+    const uint32_t slot = block_slot(1);
+    const int e = partition.find(slot, slot_of);
+    const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
+    const uint32_t count = s.nq * group;
+    const uint32_t start = slot_first<kSlot>(slot, slot_of(s.q0, e), count);
+    if (start >= count) return;
+    // A wave behind the last pair repeats it, unwritten.
+    const uint32_t first = start + wave * kRows, mine = min(first, count - 1);
+
+    CacheRow rows[R];
+    cache_rows<R>(rows, call, s, kv, first);
+    CacheTerms<T> q[R][DP / 32];
+    cache_queries<T, DP, R, false>(q, call, s, rows);
+    const float scale = fabsf(a.scale) * kAttnLog2e;
+    const int p_low = static_cast<int>(mine / group) + s.shift();
+    const int p_high = static_cast<int>((min(mine + kRows, count) - 1) / group) + s.shift();
+    CacheState<T, DP, R> state;
+    state.clear();
+    const AttnTiles blocks = partition.real(e)
+                                 ? cache_blocks(a, s.nk, static_cast<int>(start / group) + s.shift(),
+                                                static_cast<int>((min(start + kSlot, count) - 1) / group) + s.shift())
+                                 : AttnTiles{0, 0, 0};
+    if (blocks.count > 0) {
+        const long long at = (static_cast<long long>(e - 1) * c.kv_heads + kv) * c.blocks;
+        const Stage keys(c.keys, at, false, wave), values(c.values, at, true, wave);
+        const int8_t *key_exponents = c.key_exponents + at, *value_exponents = c.value_exponents + at;
+        const CacheView view(a, s.nk, p_low, p_high);
+        const int last = blocks.tile(blocks.count - 1);
+        const auto after = [&](int tile) {
+            return tile == last ? last : tile + 1 == blocks.first ? blocks.from : tile + 1;
+        };
+        const auto key_half = [&](int index) { return staged + (index & 1) * Stage::kBytes; };
+        const auto value_half = [&](int index) { return staged + (2 + (index & 1)) * Stage::kBytes; };
+        typename Stage::Codes k_codes, v_codes;
+        const auto cut = [&](int tile) {
+            const int tokens = s.nk - tile * kCacheBlock;
+            if (tokens < kCacheBlock) Stage::cut(v_codes, tokens);
+        };
+        // Ready are the first two blocks' keys and the first's values, on their way
+        // the third's keys and the second's values.
+        int tile = blocks.tile(0), next = after(tile), second = after(next);
+        keys.load(k_codes, tile);
+        values.load(v_codes, tile);
+        int key_exponent = key_exponents[tile], value_exponent = value_exponents[tile];
+        int next_key_exponent = key_exponents[next], next_value_exponent = value_exponents[next];
+        Stage::write(key_half(0), k_codes, wave);
+        cut(tile);
+        Stage::write(value_half(0), v_codes, wave);
+        keys.load(k_codes, next);
+        values.load(v_codes, next);
+        Stage::write(key_half(1), k_codes, wave);
+        keys.load(k_codes, second);
+        __syncthreads();
+        f32x4_attn scores[R][2];
+        cache_scores<T, DP, R>(scores, q, [&](int i, int k) {
+            return Stage::operand(key_half(0), i * (DP / 32) + k);
+        });
+        for (int index = 0; index < blocks.count; ++index) {
+            const int j0 = tile * kCacheBlock;
+            const int third = after(second);
+            __syncthreads();
+            // What lay there was last read before the barrier; long before the next
+            // one it is written.
+            Stage::write(key_half(index), k_codes, wave);
+            cut(next);
+            Stage::write(value_half(index + 1), v_codes, wave);
+            keys.load(k_codes, third);
+            values.load(v_codes, second);
+            const int second_key_exponent = key_exponents[second], second_value_exponent = value_exponents[second];
+            if (!view.all(j0)) hide_scores<R>(scores, rows, a.sinks, j0);
+            f32x4_attn following[R][2];
+            const char* key_now = key_half(index + 1);
+            cache_scores<T, DP, R>(following, q, [&](int i, int k) {
+                return Stage::operand(key_now, i * (DP / 32) + k);
+            });
+            CacheTerms<T> p[R];
+            cache_shares<T, DP, R>(p, state, scores, cache_factor(scale, key_exponent),
+                                   max(value_exponent, kCacheLeast));
+            const char* value_now = value_half(index);
+            add_cache_values<T, DP, R>(state, p, [&](int t) { return Stage::operand(value_now, t); });
+            tile = next;
+            next = second;
+            second = third;
+            key_exponent = next_key_exponent;
+            value_exponent = next_value_exponent;
+            next_key_exponent = second_key_exponent;
+            next_value_exponent = second_value_exponent;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                scores[r][0] = following[r][0];
+                scores[r][1] = following[r][1];
+            }
+        }
+    }
+    close_state<T, DP, R>(state);
+    write_pairs<T, Code, DP, R>(call, s, e - 1, rows, state, out, &scratch[wave]);
 }
 
 // Joins the parts (at most 64) of a pair: a wave a (query, head).
@@ -564,25 +855,26 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
     const long long items = static_cast<long long>(a.queries) * a.heads;
     const long long at = static_cast<long long>(blockIdx.x) * kAttnWaves + wave;
     if (at >= items) return;
-    const float2 state = lane < splits ? part.states[lane * items + at] : float2{-3.0e38f, 0.0f};
+    const float2 state = lane < splits ? part.states[lane * items + at] : float2{kCacheFloor, 0.0f};
     const float top = wave_max(state.x);
     const float factor = __builtin_amdgcn_exp2f(state.x - top);
     const float sum = wave_sum(state.y * factor);
-    float acc[kAttnMaxDim / kWave] = {};
-#pragma unroll 4
-    for (int z = 0; z < splits; ++z) {
+    // Each half of the wave has every second part, a lane four channels.
+    const int half = lane >> 5, d = (lane & 31) * 4;
+    const float* values = part.values + at * c.dim + min(d, c.dim - 4);
+    f32x4_attn acc{};
+#pragma unroll 8
+    for (int z0 = 0; z0 < splits; z0 += 2) {
+        // Both halves go around together: a lane that has left has no factor to give.
+        const int z = min(z0 + half, splits - 1);
         const float share = __shfl(factor, z);
-#pragma unroll
-        for (int b = 0; b < kAttnMaxDim / kWave; ++b) {
-            const int d = min(lane + b * kWave, c.dim - 1);
-            acc[b] += part.values[(z * items + at) * c.dim + d] * share;
-        }
+        acc += *reinterpret_cast<const f32x4_attn*>(values + z * items * c.dim) * (z0 + half < splits ? share : 0.0f);
     }
     bool finite = sum > 0.0f;
 #pragma unroll
-    for (int b = 0; b < kAttnMaxDim / kWave; ++b) {
-        acc[b] /= sum;
-        finite = finite && fabsf(acc[b]) < INFINITY;
+    for (int i = 0; i < 4; ++i) {
+        acc[i] = (acc[i] + __shfl_xor(acc[i], 32)) / sum;
+        finite = finite && fabsf(acc[i]) < INFINITY;
     }
     // Rows that see nothing, and those that are not finite.
     if (__any(!finite)) {
@@ -593,10 +885,11 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
         attend_pair<T, Code>(call, s, e - 1, row - s.q0, head, out, &scratch[wave]);
         return;
     }
+    if (half == 0 && d < c.dim) {
+        RowVec<T, 4> v;
 #pragma unroll
-    for (int b = 0; b < kAttnMaxDim / kWave; ++b) {
-        const int d = lane + b * kWave;
-        if (d < c.dim) out[at * c.dim + d] = static_cast<T>(acc[b]);
+        for (int i = 0; i < 4; ++i) v.set(i, acc[i]);
+        v.store(out + at * c.dim + d);
     }
 }
 
@@ -604,14 +897,16 @@ template <typename T, typename Code, int DP>
 int launch_cache_attend(const CacheCall& call, const CacheLayout& l, const CachePart& part, T* out,
                         hipStream_t stream) {
     const dim3 grid = slot_grid(l.slots, call.cache.kv_heads, l.splits);
-#define LATTICE_CACHE_ATTEND(TILES, SHARE) \
-    cache_attend<T, Code, DP, TILES, SHARE><<<grid, kAttnBlock, 0, stream>>>(call, l.splits, part, out)
-    if (l.share) {
-        LATTICE_CACHE_ATTEND(1, true);
-    } else {
-        LATTICE_CACHE_ATTEND(2, false);
+    const auto few = [&](auto kernel) { kernel<<<grid, kAttnBlock, 0, stream>>>(call, l.splits, part, out); };
+    if (!l.share) {
+        if constexpr (cache_many<T>(DP)) cache_attend_many<T, Code, DP, 2><<<grid, kAttnBlock, 0, stream>>>(call, out);
+    } else if (l.tiles == 1) {
+        few(cache_attend_few<T, Code, DP, 1>);
+    } else if (l.tiles == 2) {
+        few(cache_attend_few<T, Code, DP, 2>);
+    } else if (cache_most_tiles<T>(DP) > 2) {
+        few(cache_attend_few<T, Code, DP, cache_most_tiles<T>(DP)>);
     }
-#undef LATTICE_CACHE_ATTEND
     LATTICE_LAUNCH_CHECK();
     if (l.splits > 1) {
         cache_join<T, Code><<<grid_for(static_cast<long long>(call.args.queries) * call.args.heads, kAttnWaves,

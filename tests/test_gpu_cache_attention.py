@@ -253,6 +253,16 @@ def test_lengths_past_the_capacity():
             want = torch.softmax(scores, 0) @ values[0, seen, 0]
             assert (got[i, head].cpu().double() - want).abs().max() < 1e-5
     assert not got[10:].any()
+    # Without a bound every token is seen, however far the length.
+    for lengths in ((2000, 2 ** 29), (2 ** 31 - 1, 2 ** 31 - 1)):
+        for right in (0, None):
+            far = _ops().cache_attention(q, cache, offsets=at, right=right,
+                                         lengths=_ints(*lengths))
+            for i in range(20):
+                scores = keys[i // 10, :, 0] @ q[i, 0].cpu().double()
+                want = torch.softmax(scores / 32 ** 0.5,
+                                     0) @ values[i // 10, :, 0]
+                assert (far[i, 0].cpu().double() - want).abs().max() < 1e-5
     most = _ops().cache_attention(q, cache, offsets=at, left=5, sinks=3,
                                   lengths=_ints(2 ** 31 - 1, -7), right=0)
     sinks = _check(q[:1], cache, (1, 0), (64, 0), 0, 0, 3)
