@@ -24,9 +24,15 @@ struct CodeE4m3 {
     static constexpr int kShift = 9;
     static constexpr uint32_t kMostMantissa = 0x600000;
 
-    __device__ static uint8_t code(float x) {
-        const float finite = fabsf(x) < INFINITY ? x : __uint_as_float(0x7fc00000u);
-        return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(finite, finite, 0, false));
+    static constexpr bool kHasNan = true;
+
+    // Codes of one, two or four values times `factor`, the first in the lowest
+    // byte; what is not finite becomes NaN.
+    template <int N>
+    __device__ static uint32_t codes(const float (&x)[N], float factor) {
+        int out = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * factor, x[N > 1 ? 1 : 0] * factor, 0, false);
+        if constexpr (N == 4) out = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * factor, x[3] * factor, out, true);
+        return static_cast<uint32_t>(out) & (N == 4 ? ~0u : N == 2 ? 0xffffu : 0xffu);
     }
     __device__ static float value(uint8_t c) { return __builtin_amdgcn_cvt_f32_fp8(c, 0); }
     // The values of four codes.
@@ -43,9 +49,19 @@ struct CodeInt8 {
     static constexpr int kShift = 7;
     static constexpr uint32_t kMostMantissa = 0x7e0000;  // 127 = 1.984375 * 2^6
 
-    __device__ static uint8_t code(float x) {
-        const float bounded = fminf(fmaxf(rintf(x), -127.0f), 127.0f);
-        return static_cast<uint8_t>(static_cast<int8_t>(x == x ? bounded : 0.0f));
+    static constexpr bool kHasNan = false;
+
+    // As above, of products from -127 to 127: 1.5 2^23 more has the rounded
+    // product in its low bits.
+    template <int N>
+    __device__ static uint32_t codes(const float (&x)[N], float factor) {
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __float_as_uint(__builtin_fmaf(x[i], factor, 12582912.0f));
+        if constexpr (N == 1) return w[0] & 0xffu;
+        const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u);
+        if constexpr (N == 2) return low;
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u), low, 0x05040100u);
     }
     __device__ static float value(uint8_t c) { return static_cast<float>(static_cast<int8_t>(c)); }
     __device__ static void values(uint32_t w, bf16x2_cache* v) {

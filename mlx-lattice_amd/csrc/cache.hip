@@ -7,10 +7,10 @@
 // that codes do not depend on how the quotient is computed; recoding e4m3 is
 // exact but for its subnormals.
 //
-// A block of threads has one block of tokens of a key head, keys or values: it
-// alone reads and writes those bytes.  Rows are read with 16-byte loads,
-// reduced to the exponent, encoded into the block's image in LDS and merged
-// into its pieces of 16 bytes.
+// A wave has one block of tokens of a key head, keys or values: it alone reads and
+// writes those bytes.  A lane holds some successive tokens of some successive
+// channels, so that keys are encoded along its channels and values along its
+// tokens, and either is stored as it lies, with no exchange but the maximum's.
 
 #include "cache.h"
 
@@ -20,52 +20,128 @@ namespace {
 constexpr int kCacheThreads = 256;
 constexpr int kCacheImage = kCacheBlock * kAttnMaxDim;  // most bytes of a block
 
-__device__ inline float threads_max(float v, float* shared) {
-    v = wave_max(v);
-    if (lane_id() == 0) shared[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float most = shared[0];
-    for (int w = 1; w < kCacheThreads / kWave; ++w) most = fmaxf(most, shared[w]);
-    return most;
-}
-
 struct CacheSource {
     const void* rows;
     long long row_stride, head_stride;
 };
 
-// The place in a block's image of a token's channel.
-__device__ inline int image_place(bool values, int width, int token, int channel) {
-    return values ? channel * kCacheBlock + token : token * width + channel;
-}
-
 template <typename Code>
 __device__ inline uint32_t recode(uint32_t word, float factor) {
-    uint32_t out = 0;
+    const float x[4] = {Code::value(word & 0xff), Code::value(word >> 8 & 0xff), Code::value(word >> 16 & 0xff),
+                        Code::value(word >> 24)};
+    return Code::codes(x, factor);
+}
+
+// Codes of values, some of which are not finite if `odd`: an infinity has the
+// code of largest size, NaN its own or zero.
+template <typename Code, int N>
+__device__ inline uint32_t encode(const float (&x)[N], float factor, bool odd) {
+    if constexpr (!Code::kHasNan) {
+        if (odd) {
+            float y[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        out |= static_cast<uint32_t>(Code::code(Code::value(word >> 8 * i & 0xff) * factor)) << 8 * i;
-    return out;
+            for (int i = 0; i < N; ++i) y[i] = x[i] == x[i] ? __builtin_amdgcn_fmed3f(x[i] * factor, -127.0f, 127.0f) : 0.0f;
+            return Code::codes(y, 1.0f);
+        }
+    }
+    return Code::codes(x, factor);
 }
 
 // Slots: of 32 rows and two more a sequence, enough for the blocks its rows
 // touch.
 __device__ inline uint32_t write_slot(int start, int e) { return static_cast<uint32_t>(start) / kCacheBlock + 2u * e; }
 
-template <typename T, int V, typename Code>
+// Blocks of threads for the keys and values of a slot's heads.
+__host__ __device__ inline uint32_t write_groups(int kv_heads) {
+    return (2u * kv_heads + kCacheThreads / kWave - 1) / (kCacheThreads / kWave);
+}
+
+// N bytes as they are moved.
+template <int N> struct CacheBytes {
+    alignas(N < 4 ? 4 : N) uint32_t w[(N + 3) / 4];
+    __device__ static CacheBytes load(const uint8_t* p) {
+        CacheBytes b;
+        if constexpr (N >= 4) {
+            typedef typename RowBits<N>::type Bits;
+            *reinterpret_cast<Bits*>(b.w) = *reinterpret_cast<const Bits*>(p);
+        } else {
+            b.w[0] = N == 2 ? *reinterpret_cast<const uint16_t*>(p) : *p;
+        }
+        return b;
+    }
+    __device__ void store(uint8_t* p) const {
+        if constexpr (N >= 4) {
+            typedef typename RowBits<N>::type Bits;
+            *reinterpret_cast<Bits*>(p) = *reinterpret_cast<const Bits*>(w);
+        } else if constexpr (N == 2) {
+            *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+        } else {
+            *p = static_cast<uint8_t>(w[0]);
+        }
+    }
+};
+
+// The largest magnitude of rows' values, infinite or NaN if one of them is: the
+// bits of magnitudes are ordered.
+template <typename T, int V>
+struct Magnitude {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t bits = 0;
+    __device__ void add(const RowVec<T, V>& v) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) bits = max(bits, __float_as_uint(v.e[j]) & 0x7fffffffu);
+        } else if constexpr (V == 1) {
+            bits = max(bits, __builtin_bit_cast(uint16_t, v.e[0]) & 0x7fffu);
+        } else {
+            struct Words {
+                uint32_t w[V / 2];
+            };
+            const Words words = __builtin_bit_cast(Words, v);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j)
+                bits = __builtin_bit_cast(
+                    uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, bits),
+                                                        __builtin_bit_cast(u16x2, words.w[j] & 0x7fff7fffu)));
+        }
+    }
+    __device__ float value() const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(bits);
+        } else {
+            return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(max(bits & 0xffffu, bits >> 16))));
+        }
+    }
+};
+
+// How a wave's lanes hold a block of 32 tokens of DP channels, V of them a load:
+// kAcross lanes a row, kTokens successive tokens and kGroups vectors of channels a
+// lane.
+template <int DP, int V>
+struct CacheHold {
+    static constexpr int kVectors = DP / V;
+    static constexpr int kAcross = kVectors > 32 ? 64 : kVectors > 16 ? 32 : kVectors > 8 ? 16 : kVectors > 4 ? 8 : 4;
+    static constexpr int kGroups = (kVectors + kAcross - 1) / kAcross;
+    static constexpr int kTokens = kAcross / 2;  // 32 tokens over 64 / kAcross lanes
+};
+
+template <typename T, int V, typename Code, int DP>
 __global__ void __launch_bounds__(kCacheThreads)
 cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows, const int32_t* __restrict__ offsets,
                    const int32_t* __restrict__ lengths) {
     typedef RowVec<T, V> Vec;
-    constexpr int kHeld = kAttnMaxDim / (8 * V);  // vectors of a row that a thread holds, of 8 threads
-    __shared__ float shared[kCacheThreads / kWave];
-    __shared__ __align__(16) uint8_t image[kCacheImage];
-    const uint32_t slot = block_slot(2);
-    const bool values = block_part(2) != 0;
-    const int head = blockIdx.y;
+    typedef CacheHold<DP, V> Hold;
+    constexpr int kTokens = Hold::kTokens, kGroups = Hold::kGroups;
+    // The heads of a slot next to each other, as they lie in its rows.
+    const uint32_t groups = write_groups(c.kv_heads);
+    const uint64_t index = blockIdx.x + static_cast<uint64_t>(gridDim.x) * blockIdx.z;
+    const uint32_t slot = static_cast<uint32_t>(index / groups);
+    const int task = static_cast<int>(index % groups) * (kCacheThreads / kWave) + threadIdx.x / kWave;
     const RowPartition partition{offsets, c.sequences, rows};
     const int e = partition.find(slot, write_slot);
-    if (!partition.real(e)) return;
+    if (!partition.real(e) || task >= 2 * c.kv_heads) return;
+    const bool values = task & 1;
+    const int head = task >> 1;
     const CacheSequence s = cache_sequence(partition, lengths, c.blocks * kCacheBlock, e);
     const int first = max(s.shift(), 0);
     const long long block = first / kCacheBlock + static_cast<long long>(slot - write_slot(s.q0, e));
@@ -74,76 +150,146 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     const int begin = max(first, lo) - lo, end = min(s.nk - lo, kCacheBlock);
     if (begin >= end) return;
 
-    const int width = cache_width(c);
     const long long at = (static_cast<long long>(e - 1) * c.kv_heads + head) * c.blocks + block;
-    uint8_t* codes = static_cast<uint8_t*>(values ? c.values : c.keys) + at * kCacheBlock * width;
+    uint8_t* codes = static_cast<uint8_t*>(values ? c.values : c.keys) + at * kCacheBlock * DP;
     int8_t* exponent = (values ? c.value_exponents : c.key_exponents) + at;
     const CacheSource& source = values ? vals : keys;
-
-    const int token = threadIdx.x / 8, part = threadIdx.x % 8;
-    const bool fresh = token >= begin && token < end;
-    float x[kHeld][V];
-    float most = 0.0f;
-    const T* row = static_cast<const T*>(source.rows) +
-                   (static_cast<long long>(s.q0) + (lo + token - s.shift())) * source.row_stride +
-                   head * source.head_stride;
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-        const int channel = (part + 8 * k) * V;
-        Vec in;
-        const bool here = fresh && channel < c.dim;
-        if (here) in = Vec::load(row + channel);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            x[k][j] = here ? in.at(j) : 0.0f;
-            const float size = fabsf(x[k][j]);
-            most = fmaxf(most, size < INFINITY ? size : 0.0f);
-        }
-    }
     const int before = max(static_cast<int>(*exponent), kCacheLeast);
-    most = threads_max(most, shared);
-    int next = block_exponent<Code>(most);
-    if (begin > 0) next = max(next, before);
-    const float factor = power_of_two(-next), moved = power_of_two(max(before - next, kCacheLeast));
+    const int lane = lane_id();
+    const int token0 = lane / Hold::kAcross * kTokens, channel0 = lane % Hold::kAcross * V;
+    const T* from = static_cast<const T*>(source.rows) +
+                    (static_cast<long long>(s.q0) + (lo + token0 - s.shift())) * source.row_stride +
+                    head * source.head_stride + channel0;
+    Vec in[kTokens][kGroups];
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-        const int channel = (part + 8 * k) * V;
-        if (!fresh || channel >= width) continue;
+    for (int t = 0; t < kTokens; ++t) {
+        const bool fresh = token0 + t >= begin && token0 + t < end;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            image[image_place(values, width, token, channel + j)] = Code::code(x[k][j] * factor);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) *exponent = static_cast<int8_t>(next);
-    // The image's pieces of 16 bytes: a token's channels, or a channel's tokens.
-    for (int piece = threadIdx.x; piece < kCacheBlock * width / 16; piece += kCacheThreads) {
-        uint4* to = reinterpret_cast<uint4*>(codes) + piece;
-        const uint4 made = reinterpret_cast<const uint4*>(image)[piece];
-        const uint32_t words[4] = {made.x, made.y, made.z, made.w};
-        const int from = values ? 16 * (piece & 1) : 16 * piece / width;  // the first byte's token
-        const int step = values ? 1 : 0;
-        const int last = from + 15 * step;
-        if (from >= end || (last < begin && before == next)) continue;
-        if (from >= begin && last < end) {
-            *to = made;
-            continue;
+        for (int g = 0; g < kGroups; ++g) {
+            const int channel = channel0 + g * Hold::kAcross * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) in[t][g].set(j, 0.0f);
+            if (fresh && channel < c.dim) in[t][g] = Vec::load(from + t * source.row_stride + g * Hold::kAcross * V);
         }
-        const uint4 held = *to;
-        const uint32_t old[4] = {held.x, held.y, held.z, held.w};
-        uint32_t out[4];
+    }
+    // A lane's tokens of a channel lie together among the values; those that are
+    // not all new are merged into what is there.
+    constexpr int kBytes = kTokens > 16 ? 16 : kTokens, kParts = kTokens / kBytes;
+    const bool whole = token0 >= begin && token0 + kTokens <= end;
+    CacheBytes<kBytes> held[kGroups][V][kParts] = {};
+    if (values && !whole && token0 < end) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t again = before == next ? old[w] : recode<Code>(old[w], moved);
-            out[w] = 0;
+        for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = from + (4 * w + i) * step;
-                const uint32_t word = t < begin ? again : t < end ? words[w] : old[w];
-                out[w] |= word & 0xffu << 8 * i;
+            for (int j = 0; j < V; ++j) {
+                const int channel = channel0 + g * Hold::kAcross * V + j;
+                if (channel >= DP) continue;
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+                    held[g][j][part] =
+                        CacheBytes<kBytes>::load(codes + channel * kCacheBlock + token0 + part * kBytes);
             }
         }
-        *to = uint4{out[0], out[1], out[2], out[3]};
     }
+    Magnitude<T, V> largest;
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) largest.add(in[t][g]);
+    }
+    float most = largest.value();
+    const bool odd = __any(!(most < INFINITY));
+    if (odd) {  // of what is finite
+        most = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float size = fabsf(in[t][g].at(j));
+                    most = fmaxf(most, size < INFINITY ? size : 0.0f);
+                }
+            }
+        }
+    }
+    int next = block_exponent<Code>(wave_max(most));
+    if (begin > 0) next = max(next, before);
+    const bool moves = begin > 0 && next != before;
+    const float factor = power_of_two(-next), moved = power_of_two(max(before - next, kCacheLeast));
+    if (lane == 0) *exponent = static_cast<int8_t>(next);
+    if (!values) {
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            const int token = token0 + t;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int channel = channel0 + g * Hold::kAcross * V;
+                if (channel >= DP || token >= end || (token < begin && !moves)) continue;
+                uint8_t* to = codes + token * DP + channel;
+                CacheBytes<V> out;
+                if (token < begin) {
+                    out = CacheBytes<V>::load(to);
+#pragma unroll
+                    for (int w = 0; w < (V + 3) / 4; ++w) out.w[w] = recode<Code>(out.w[w], moved);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < (V + 3) / 4; ++w) {
+                        float x[V < 4 ? V : 4];
+#pragma unroll
+                        for (int i = 0; i < (V < 4 ? V : 4); ++i) x[i] = in[t][g].at(4 * w + i);
+                        out.w[w] = encode<Code>(x, factor, odd);
+                    }
+                }
+                out.store(to);
+            }
+        }
+        return;
+    }
+    const bool some = token0 < end && (moves || token0 + kTokens > begin);
+    if (!some) return;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int channel = channel0 + g * Hold::kAcross * V + j;
+            if (channel >= DP) continue;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                uint8_t* to = codes + channel * kCacheBlock + token0 + part * kBytes;
+                CacheBytes<kBytes> out;
+#pragma unroll
+                for (int w = 0; w < (kBytes + 3) / 4; ++w) {
+                    float x[kBytes < 4 ? kBytes : 4];
+#pragma unroll
+                    for (int i = 0; i < (kBytes < 4 ? kBytes : 4); ++i)
+                        x[i] = in[part * kBytes + 4 * w + i][g].at(j);
+                    out.w[w] = encode<Code>(x, factor, odd);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int w = 0; w < (kBytes + 3) / 4; ++w) {
+                        const uint32_t old = held[g][j][part].w[w];
+                        const uint32_t again = moves ? recode<Code>(old, moved) : old;
+                        uint32_t merged = 0;
+#pragma unroll
+                        for (int i = 0; i < (kBytes < 4 ? kBytes : 4); ++i) {
+                            const int token = token0 + part * kBytes + 4 * w + i;
+                            const uint32_t word = token < begin ? again : token < end ? out.w[w] : old;
+                            merged |= word & 0xffu << 8 * i;
+                        }
+                        out.w[w] = merged;
+                    }
+                }
+                out.store(to);
+            }
+        }
+    }
+}
+
+// The place in a block's image of a token's channel.
+__device__ inline int image_place(bool values, int width, int token, int channel) {
+    return values ? channel * kCacheBlock + token : token * width + channel;
 }
 
 // A block of tokens of a key head: keys as they lie, values by way of LDS.
@@ -184,18 +330,35 @@ cache_read_blocks(lattice_cache c, const int32_t* __restrict__ lengths, T* __res
     }
 }
 
+long long write_blocks(const lattice_cache& c, int rows) {
+    return (static_cast<long long>(rows) / kCacheBlock + 2ll * (c.sequences + 2)) * write_groups(c.kv_heads);
+}
+
+template <typename T, int V, typename Code>
+void launch_write(const lattice_cache& c, const CacheSource& k, const CacheSource& v, int rows,
+                  const int32_t* offsets, const int32_t* lengths, hipStream_t stream) {
+    const dim3 grid = slot_grid(write_blocks(c, rows), 1, 1);
+    const auto launch = [&](auto kernel) {
+        kernel<<<grid, kCacheThreads, 0, stream>>>(c, k, v, rows, offsets, lengths);
+    };
+    switch (cache_width(c)) {
+        case 32: return launch(cache_write_blocks<T, V, Code, 32>);
+        case 64: return launch(cache_write_blocks<T, V, Code, 64>);
+        case 96: return launch(cache_write_blocks<T, V, Code, 96>);
+        default: return launch(cache_write_blocks<T, V, Code, 128>);
+    }
+}
+
 template <typename T, typename Code>
 int write_of(const lattice_cache& c, const CacheSource& k, const CacheSource& v, int rows, const int32_t* offsets,
              const int32_t* lengths, hipStream_t stream) {
     constexpr int kMost = 16 / sizeof(T);
     const int vector = row_vector<T>(c.dim, {k.rows, v.rows},
                                      {k.row_stride, k.head_stride, v.row_stride, v.head_stride});
-    const long long slots = static_cast<long long>(rows) / kCacheBlock + 2ll * (c.sequences + 2);
-    const dim3 grid = slot_grid(slots, c.kv_heads, 2);
     if (vector == kMost) {
-        cache_write_blocks<T, kMost, Code><<<grid, kCacheThreads, 0, stream>>>(c, k, v, rows, offsets, lengths);
+        launch_write<T, kMost, Code>(c, k, v, rows, offsets, lengths, stream);
     } else {
-        cache_write_blocks<T, 1, Code><<<grid, kCacheThreads, 0, stream>>>(c, k, v, rows, offsets, lengths);
+        launch_write<T, 1, Code>(c, k, v, rows, offsets, lengths, stream);
     }
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
@@ -250,6 +413,7 @@ extern "C" int lattice_hip_cache_write(const lattice_cache* cache, int dtype, co
                     "cache row strides must be non-negative.");
     if (rows == 0 || cache->sequences == 0 || cache->blocks == 0) return LATTICE_OK;
     LATTICE_REQUIRE(k && v && offsets && lengths, "cache row pointers must be non-null.");
+    LATTICE_REQUIRE(write_blocks(*cache, rows) < 1ll << 37, "the cache has too many sequences and heads.");
     const CacheSource keys{k, k_row_stride, k_head_stride}, values{v, v_row_stride, v_head_stride};
     hipStream_t stream = as_stream(stream_ptr);
     if (cache->code == LATTICE_CODE_E4M3)
