@@ -18,7 +18,6 @@ namespace lattice {
 namespace {
 
 constexpr int kCacheThreads = 256;
-constexpr int kCacheImage = kCacheBlock * kAttnMaxDim;  // most bytes of a block
 
 struct CacheSource {
     const void* rows;
@@ -51,9 +50,22 @@ __device__ inline uint32_t encode(const float (&x)[N], float factor, bool odd) {
 // touch.
 __device__ inline uint32_t write_slot(int start, int e) { return static_cast<uint32_t>(start) / kCacheBlock + 2u * e; }
 
-// Blocks of threads for the keys and values of a slot's heads.
-__host__ __device__ inline uint32_t write_groups(int kv_heads) {
+// Blocks of threads for the keys and values of all heads.
+__host__ __device__ inline uint32_t head_groups(int kv_heads) {
     return (2u * kv_heads + kCacheThreads / kWave - 1) / (kCacheThreads / kWave);
+}
+
+// Places, slots or blocks of tokens, of `groups` blocks of threads each; those
+// past 2^22 blocks of threads go on along z.
+inline dim3 cache_grid(long long places, uint32_t groups) {
+    const long long x = std::min<long long>(places, (1 << 22) / groups);
+    return dim3(static_cast<unsigned>(x) * groups, 1, static_cast<unsigned>((places + x - 1) / x));
+}
+__device__ inline uint32_t cache_place(uint32_t groups) {
+    return blockIdx.x / groups + gridDim.x / groups * blockIdx.z;
+}
+inline bool cache_fits(const lattice_cache& c, long long places) {
+    return places < 1ll << 31 && places * head_groups(c.kv_heads) < 1ll << 36;
 }
 
 // N bytes as they are moved.
@@ -133,10 +145,9 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     typedef CacheHold<DP, V> Hold;
     constexpr int kTokens = Hold::kTokens, kGroups = Hold::kGroups;
     // The heads of a slot next to each other, as they lie in its rows.
-    const uint32_t groups = write_groups(c.kv_heads);
-    const uint64_t index = blockIdx.x + static_cast<uint64_t>(gridDim.x) * blockIdx.z;
-    const uint32_t slot = static_cast<uint32_t>(index / groups);
-    const int task = static_cast<int>(index % groups) * (kCacheThreads / kWave) + threadIdx.x / kWave;
+    const uint32_t groups = head_groups(c.kv_heads);
+    const uint32_t slot = cache_place(groups);
+    const int task = blockIdx.x % groups * (kCacheThreads / kWave) + threadIdx.x / kWave;
     const RowPartition partition{offsets, c.sequences, rows};
     const int e = partition.find(slot, write_slot);
     if (!partition.real(e) || task >= 2 * c.kv_heads) return;
@@ -287,57 +298,97 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     }
 }
 
-// The place in a block's image of a token's channel.
-__device__ inline int image_place(bool values, int width, int token, int channel) {
-    return values ? channel * kCacheBlock + token : token * width + channel;
+// The value of a lane's byte i, tokens or channels, of codes as they are moved.
+template <typename Code, int N>
+__device__ inline float value_of(const CacheBytes<N>& b, int i) {
+    return Code::value(static_cast<uint8_t>(b.w[i / 4] >> 8 * (i % 4)));
 }
 
-// A block of tokens of a key head: keys as they lie, values by way of LDS.
-template <typename T, int V, typename Code>
+// The inverse, of the same lanes: what is behind a sequence's last token is zero.
+template <typename T, int V, typename Code, int DP>
 __global__ void __launch_bounds__(kCacheThreads)
 cache_read_blocks(lattice_cache c, const int32_t* __restrict__ lengths, T* __restrict__ k, T* __restrict__ v) {
     typedef RowVec<T, V> Vec;
-    __shared__ __align__(16) uint8_t image[kCacheImage];
-    const int block = blockIdx.x % c.blocks, head = blockIdx.y;
-    const bool values = blockIdx.z != 0;
-    const int width = cache_width(c);
-    for (long long s = blockIdx.x / c.blocks; s < c.sequences; s += gridDim.x / c.blocks) {
-        const int lo = block * kCacheBlock;
-        const int filled = min(max(lengths[s], 0) - lo, kCacheBlock);
-        const long long at = (s * c.kv_heads + head) * c.blocks + block;
-        const uint4* codes =
-            reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(values ? c.values : c.keys) + at * kCacheBlock * width);
-        const float factor =
-            power_of_two(max(static_cast<int>((values ? c.value_exponents : c.key_exponents)[at]), kCacheLeast));
-        __syncthreads();
-        if (filled > 0) {
-            for (int piece = threadIdx.x; piece < kCacheBlock * width / 16; piece += kCacheThreads)
-                reinterpret_cast<uint4*>(image)[piece] = codes[piece];
+    typedef CacheHold<DP, V> Hold;
+    constexpr int kTokens = Hold::kTokens, kGroups = Hold::kGroups;
+    // The heads of a block next to each other, as they lie in its rows.
+    const uint32_t groups = head_groups(c.kv_heads);
+    const uint32_t place = cache_place(groups);
+    const int task = blockIdx.x % groups * (kCacheThreads / kWave) + threadIdx.x / kWave;
+    const long long s = place / c.blocks;
+    const int block = place % c.blocks;
+    if (s >= c.sequences || task >= 2 * c.kv_heads) return;
+    const bool values = task >= c.kv_heads;
+    const int head = values ? task - c.kv_heads : task;
+    const int lo = block * kCacheBlock;
+    const int filled = min(max(lengths[s], 0) - lo, kCacheBlock);
+    const long long at = (s * c.kv_heads + head) * c.blocks + block;
+    const uint8_t* codes = static_cast<const uint8_t*>(values ? c.values : c.keys) + at * kCacheBlock * DP;
+    const float factor =
+        power_of_two(max(static_cast<int>((values ? c.value_exponents : c.key_exponents)[at]), kCacheLeast));
+    const int lane = lane_id();
+    const int token0 = lane / Hold::kAcross * kTokens, channel0 = lane % Hold::kAcross * V;
+    T* out = (values ? v : k) + ((s * c.blocks * kCacheBlock + lo + token0) * c.kv_heads + head) * c.dim;
+    const long long stride = static_cast<long long>(c.kv_heads) * c.dim;
+    if (!values) {
+        CacheBytes<V> in[kTokens][kGroups] = {};
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int channel = channel0 + g * Hold::kAcross * V;
+                if (token0 + t < filled && channel < c.dim)
+                    in[t][g] = CacheBytes<V>::load(codes + (token0 + t) * DP + channel);
+            }
         }
-        __syncthreads();
-        T* out = (values ? v : k) + ((s * c.blocks * kCacheBlock + lo) * c.kv_heads + head) * c.dim;
-        const int vectors = c.dim / V;
-        for (int i = threadIdx.x; i < kCacheBlock * vectors; i += kCacheThreads) {
-            const int token = i / vectors, channel = i % vectors * V;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int channel = channel0 + g * Hold::kAcross * V;
+                Vec row;
+#pragma unroll
+                for (int j = 0; j < V; ++j) row.set(j, value_of<Code>(in[t][g], j) * factor);
+                if (channel < c.dim) row.store(out + t * stride + channel);
+            }
+        }
+        return;
+    }
+    constexpr int kBytes = kTokens > 16 ? 16 : kTokens, kParts = kTokens / kBytes;
+    CacheBytes<kBytes> in[kGroups][V][kParts] = {};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int channel = channel0 + g * Hold::kAcross * V + j;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+                if (token0 + part * kBytes < filled && channel < c.dim)
+                    in[g][j][part] = CacheBytes<kBytes>::load(codes + channel * kCacheBlock + token0 + part * kBytes);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int channel = channel0 + g * Hold::kAcross * V;
             Vec row;
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                row.set(j, token < filled
-                               ? Code::value(image[image_place(values, width, token, channel + j)]) * factor
-                               : 0.0f);
-            row.store(out + static_cast<long long>(token) * c.kv_heads * c.dim + channel);
+                row.set(j, token0 + t < filled ? value_of<Code>(in[g][j][t / kBytes], t % kBytes) * factor : 0.0f);
+            if (channel < c.dim) row.store(out + t * stride + channel);
         }
     }
 }
 
-long long write_blocks(const lattice_cache& c, int rows) {
-    return (static_cast<long long>(rows) / kCacheBlock + 2ll * (c.sequences + 2)) * write_groups(c.kv_heads);
+long long write_slots(const lattice_cache& c, int rows) {
+    return rows / kCacheBlock + 2ll * (c.sequences + 2);
 }
 
 template <typename T, int V, typename Code>
 void launch_write(const lattice_cache& c, const CacheSource& k, const CacheSource& v, int rows,
                   const int32_t* offsets, const int32_t* lengths, hipStream_t stream) {
-    const dim3 grid = slot_grid(write_blocks(c, rows), 1, 1);
+    const dim3 grid = cache_grid(write_slots(c, rows), head_groups(c.kv_heads));
     const auto launch = [&](auto kernel) {
         kernel<<<grid, kCacheThreads, 0, stream>>>(c, k, v, rows, offsets, lengths);
     };
@@ -364,18 +415,26 @@ int write_of(const lattice_cache& c, const CacheSource& k, const CacheSource& v,
     return LATTICE_OK;
 }
 
+template <typename T, int V, typename Code>
+void launch_read(const lattice_cache& c, const int32_t* lengths, T* k, T* v, hipStream_t stream) {
+    const dim3 grid = cache_grid(1ll * c.sequences * c.blocks, head_groups(c.kv_heads));
+    const auto launch = [&](auto kernel) { kernel<<<grid, kCacheThreads, 0, stream>>>(c, lengths, k, v); };
+    switch (cache_width(c)) {
+        case 32: return launch(cache_read_blocks<T, V, Code, 32>);
+        case 64: return launch(cache_read_blocks<T, V, Code, 64>);
+        case 96: return launch(cache_read_blocks<T, V, Code, 96>);
+        default: return launch(cache_read_blocks<T, V, Code, 128>);
+    }
+}
+
 template <typename T, typename Code>
 int read_of(const lattice_cache& c, const int32_t* lengths, void* k, void* v, hipStream_t stream) {
     constexpr int kMost = 16 / sizeof(T);
-    // Blocks of threads below 2^22 along x; the rest of the sequences follow in
-    // their loops.
-    const int together = static_cast<int>(std::max(1ll, std::min<long long>(c.sequences, (1ll << 22) / c.blocks)));
-    const dim3 grid(static_cast<unsigned>(together) * c.blocks, c.kv_heads, 2);
     T *keys = static_cast<T*>(k), *values = static_cast<T*>(v);
     if (row_vector<T>(c.dim, {k, v}, {}) == kMost) {
-        cache_read_blocks<T, kMost, Code><<<grid, kCacheThreads, 0, stream>>>(c, lengths, keys, values);
+        launch_read<T, kMost, Code>(c, lengths, keys, values, stream);
     } else {
-        cache_read_blocks<T, 1, Code><<<grid, kCacheThreads, 0, stream>>>(c, lengths, keys, values);
+        launch_read<T, 1, Code>(c, lengths, keys, values, stream);
     }
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
@@ -413,7 +472,7 @@ extern "C" int lattice_hip_cache_write(const lattice_cache* cache, int dtype, co
                     "cache row strides must be non-negative.");
     if (rows == 0 || cache->sequences == 0 || cache->blocks == 0) return LATTICE_OK;
     LATTICE_REQUIRE(k && v && offsets && lengths, "cache row pointers must be non-null.");
-    LATTICE_REQUIRE(write_blocks(*cache, rows) < 1ll << 37, "the cache has too many sequences and heads.");
+    LATTICE_REQUIRE(cache_fits(*cache, write_slots(*cache, rows)), "the cache has too many sequences and heads.");
     const CacheSource keys{k, k_row_stride, k_head_stride}, values{v, v_row_stride, v_head_stride};
     hipStream_t stream = as_stream(stream_ptr);
     if (cache->code == LATTICE_CODE_E4M3)
@@ -428,6 +487,8 @@ extern "C" int lattice_hip_cache_read(const lattice_cache* cache, int dtype, con
                     "cache rows must be float32, float16 or bfloat16.");
     if (cache->sequences == 0 || cache->blocks == 0) return LATTICE_OK;
     LATTICE_REQUIRE(k && v && lengths, "cache row pointers must be non-null.");
+    LATTICE_REQUIRE(cache_fits(*cache, 1ll * cache->sequences * cache->blocks),
+                    "the cache has too many sequences and heads.");
     hipStream_t stream = as_stream(stream_ptr);
     if (cache->code == LATTICE_CODE_E4M3) return read_code<CodeE4m3>(*cache, dtype, lengths, k, v, stream);
     return read_code<CodeInt8>(*cache, dtype, lengths, k, v, stream);
