@@ -288,32 +288,54 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
             post_b[k] = vector_or<T, V>(a.post_bias, c, channels, 0.0f);
         }
     }
-    for (long long start = static_cast<long long>(blockIdx.x) * per_block; start < a.rows;
-         start += static_cast<long long>(gridDim.x) * per_block) {
+    // A row's vectors are read while the one before is computed, where registers
+    // hold both.
+    constexpr bool kAhead = K == 1;
+    struct Held {
+        float4 stat;
+        Vec in[K], dy[K], dh[K], part[K];
+    };
+    const auto load = [&](long long row, Held& r) {
+        const bool live = row < active;
+        r.stat = live ? statistics[row] : float4{0.0f, 0.0f, 0.0f, 0.0f};
+        const long long at = row * channels;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = first + k * stride;
+            r.in[k] = r.dy[k] = r.dh[k] = r.part[k] = Vec{};
+            if (!live || c >= channels) continue;
+            r.in[k] = Vec::load(static_cast<const T*>(g.sum) + at + c);
+            if (g.grad_normed) r.dy[k] = Vec::load(static_cast<const T*>(g.grad_normed) + at + c);
+            if (g.grad_sum) r.dh[k] = Vec::load(static_cast<const T*>(g.grad_sum) + at + c);
+            if (reads_x) r.part[k] = Vec::load(static_cast<const T*>(a.x) + row * a.x_stride + c);
+        }
+    };
+    const long long step = static_cast<long long>(gridDim.x) * per_block;
+    Held next;
+    if constexpr (kAhead) load(static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / group, next);
+    for (long long start = static_cast<long long>(blockIdx.x) * per_block; start < a.rows; start += step) {
         const long long row = start + threadIdx.x / group;
         const bool live = row < active;
-        const float4 stat = live ? statistics[row] : float4{0.0f, 0.0f, 0.0f, 0.0f};
-        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+        Held held;
+        if constexpr (kAhead) {
+            held = next;
+            load(row + step, next);
+        } else {
+            load(row, held);
+        }
+        const float4 stat = held.stat;
         const long long at = row * channels;
         float n[K][V], slope[K][V], t[K][V], m[K][V];
         float2 along{0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = first + k * stride;
-            const bool here = live && c < channels;
-            Vec in, dy, dh, part;
-            if (here) {
-                in = Vec::load(static_cast<const T*>(g.sum) + at + c);
-                if (g.grad_normed) dy = Vec::load(static_cast<const T*>(g.grad_normed) + at + c);
-                if (g.grad_sum) dh = Vec::load(static_cast<const T*>(g.grad_sum) + at + c);
-                if (reads_x) part = Vec::load(x + c);
-            }
+            const bool here = live && first + k * stride < channels;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = here && g.grad_normed ? dy.at(j) : 0.0f;
-                n[k][j] = here ? (in.at(j) - stat.x) * stat.y : 0.0f;
-                t[k][j] = here && g.grad_sum ? dh.at(j) : 0.0f;
-                m[k][j] = here && reads_x ? part.at(j) : 0.0f;
+                const float d = held.dy[k].at(j);
+                n[k][j] = here ? (held.in[k].at(j) - stat.x) * stat.y : 0.0f;
+                t[k][j] = held.dh[k].at(j);
+                m[k][j] = held.part[k].at(j);
                 slope[k][j] = d * w[k].at(j);
                 sums[0][k][j] += d * n[k][j];
                 sums[1][k][j] += d;
