@@ -25,46 +25,58 @@ namespace lattice {
 namespace {
 
 constexpr int kJoinBlock = 256;
-constexpr int kJoinHeld = 4;         // most vectors of a row that a thread holds
+constexpr int kJoinWidest = 512;     // most threads a row
+constexpr int kJoinHeld = 2;         // most vectors of a row that a thread holds
 constexpr int kJoinPartials = 1024;  // most blocks that sum the vectors' gradients
-constexpr int kJoinSums = 5;         // weight, bias, gate, post weight, post bias
+constexpr int kJoinBlocks = 4096;    // most blocks that walk the rows otherwise
+constexpr int kfloats = 5;         // weight, bias, gate, post weight, post bias
 
 struct JoinGrads {
     const void *sum, *grad_sum, *grad_normed;
     void *grad_x, *grad_residual;
-    void* vectors[kJoinSums];  // NULL: not wanted
+    void* vectors[kfloats];  // NULL: not wanted
 };
 
-// The sum over a row's `group` threads: a power of two of a wave's lanes, or
-// the whole block.
-__device__ inline float row_sum(float v, int group, float* shared) {
-    for (int step = 1; step < min(group, kWave); step *= 2) v += __shfl_xor(v, step);
-    if (group <= kWave) return v;
-    __syncthreads();
-    if (lane_id() == 0) shared[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinBlock / kWave; ++w) total += shared[w];
-    return total;
+// The sum over `lanes` lanes, a power of two, next to each other.
+template <int CONTROL>
+__device__ inline float lane_moved(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CONTROL, 0xf, 0xf, true));
 }
-// Two sums at once.
-__device__ inline float2 row_sums(float2 v, int group, float2* shared) {
-    for (int step = 1; step < min(group, kWave); step *= 2) {
-        v.x += __shfl_xor(v.x, step);
-        v.y += __shfl_xor(v.y, step);
+__device__ inline float lanes_sum(float v, int lanes) {
+    if (lanes >= 2) v += lane_moved<0xb1>(v);    // of pairs: 1, 0, 3, 2
+    if (lanes >= 4) v += lane_moved<0x4e>(v);    // of fours: 2, 3, 0, 1
+    if (lanes >= 8) v += lane_moved<0x141>(v);   // eights mirrored: their fours are equal
+    if (lanes >= 16) v += lane_moved<0x140>(v);  // sixteens mirrored
+    if (lanes >= 32) {
+        const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
     }
+    if (lanes >= 64) {
+        const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+    }
+    return v;
+}
+
+// The sum over a row's `group` threads: a power of two of a wave's lanes, or of
+// a block's waves.
+__device__ inline float2 lanes_sum(float2 v, int lanes) { return {lanes_sum(v.x, lanes), lanes_sum(v.y, lanes)}; }
+__device__ inline void add_to(float& v, float more) { v += more; }
+__device__ inline void add_to(float2& v, float2 more) {
+    v.x += more.x;
+    v.y += more.y;
+}
+template <typename F>
+__device__ inline F row_sum(F v, int group, F* shared) {
+    v = lanes_sum(v, min(group, kWave));
     if (group <= kWave) return v;
+    const int wave = threadIdx.x / kWave, waves = group / kWave, from = wave & -waves;
     __syncthreads();
-    if (lane_id() == 0) shared[threadIdx.x / kWave] = v;
+    if (lane_id() == 0) shared[wave] = v;
     __syncthreads();
-    float2 total{0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kJoinBlock / kWave; ++w) {
-        total.x += shared[w].x;
-        total.y += shared[w].y;
-    }
-    return total;
+    v = shared[from];
+    for (int w = 1; w < waves; ++w) add_to(v, shared[from + w]);
+    return v;
 }
 
 __device__ inline int active_count(const lattice_residual_norm& a) {
@@ -113,15 +125,15 @@ __device__ inline RowStatistics row_statistics(const float (&v)[K][V], int chann
     return s;
 }
 
-template <typename T, int V, int K, bool POST>
-__global__ void __launch_bounds__(kJoinBlock)
+template <typename T, int V, int K, int BLOCK, bool POST>
+__global__ void __launch_bounds__(BLOCK)
 residual_norm_rows(lattice_residual_norm a, int group, T* __restrict__ sum, T* __restrict__ normed,
                    float4* __restrict__ statistics) {
     typedef RowVec<T, V> Vec;
-    __shared__ float shared[kJoinBlock / kWave];
+    __shared__ float shared[BLOCK / kWave];
     const int active = active_count(a), channels = a.channels;
     const int lane = threadIdx.x & (group - 1), first = lane * V, stride = group * V;
-    const int per_block = kJoinBlock / group;
+    const int per_block = BLOCK / group;
     Vec w[K], b[K], gate[K], post_w[K], post_b[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -134,26 +146,42 @@ residual_norm_rows(lattice_residual_norm a, int group, T* __restrict__ sum, T* _
             post_b[k] = vector_or<T, V>(a.post_bias, c, channels, 0.0f);
         }
     }
-    for (long long start = static_cast<long long>(blockIdx.x) * per_block; start < a.rows;
-         start += static_cast<long long>(gridDim.x) * per_block) {
-        const long long row = start + threadIdx.x / group;
-        const bool live = row < active;
-        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-        const T* residual = static_cast<const T*>(a.residual) + row * a.residual_stride;
-        float u[K][V], h[K][V];
+    // A row's vectors are read while the one before is computed, where registers
+    // hold both.
+    constexpr bool kAhead = K == 1;
+    struct Held {
+        Vec part[K], rest[K];
+    };
+    const auto load = [&](long long row, Held& r) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = first + k * stride;
-            const bool here = live && c < channels;
-            Vec part, rest;
-            if (here) {
-                part = Vec::load(x + c);
-                rest = Vec::load(residual + c);
-            }
+            r.part[k] = r.rest[k] = Vec{};
+            if (row >= active || c >= channels) continue;
+            r.part[k] = Vec::load(static_cast<const T*>(a.x) + row * a.x_stride + c);
+            r.rest[k] = Vec::load(static_cast<const T*>(a.residual) + row * a.residual_stride + c);
+        }
+    };
+    const long long step = static_cast<long long>(gridDim.x) * per_block;
+    Held next;
+    if constexpr (kAhead) load(static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / group, next);
+    for (long long start = static_cast<long long>(blockIdx.x) * per_block; start < a.rows; start += step) {
+        const long long row = start + threadIdx.x / group;
+        const bool live = row < active;
+        Held held;
+        if constexpr (kAhead) {
+            held = next;
+            load(row + step, next);
+        } else {
+            load(row, held);
+        }
+        float u[K][V], h[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                u[k][j] = here ? part.at(j) : 0.0f;
-                h[k][j] = here ? rest.at(j) : 0.0f;
+                u[k][j] = held.part[k].at(j);
+                h[k][j] = held.rest[k].at(j);
             }
         }
         RowStatistics post{0.0f, 0.0f, 0.0f};
@@ -262,18 +290,18 @@ residual_norm_wide(lattice_residual_norm a, T* sum, T* __restrict__ normed, floa
 }
 
 // grad_x and grad_residual, and this block's sums over its rows in
-// partials[block][kJoinSums][channels] (NULL: none are wanted).
-template <typename T, int V, int K, bool POST>
-__global__ void __launch_bounds__(kJoinBlock)
+// partials[block][kfloats][channels] (NULL: none are wanted).
+template <typename T, int V, int K, int BLOCK, bool POST>
+__global__ void __launch_bounds__(BLOCK)
 residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const float4* __restrict__ statistics,
                         float* __restrict__ partials) {
     typedef RowVec<T, V> Vec;
     constexpr int kSums = POST ? 5 : 3;
-    __shared__ float2 shared[kJoinBlock / kWave];
-    __shared__ float columns[V * kJoinBlock];
+    __shared__ float2 shared[BLOCK / kWave];
+    __shared__ float columns[V * BLOCK];
     const int active = active_count(a), channels = a.channels;
     const int lane = threadIdx.x & (group - 1), first = lane * V, stride = group * V;
-    const int per_block = kJoinBlock / group;
+    const int per_block = BLOCK / group;
     const float inv = 1.0f / static_cast<float>(channels);
     const bool reads_x = POST || g.vectors[2];
     Vec w[K], gate[K], post_w[K], post_b[K];
@@ -343,7 +371,7 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
                 along.y += slope[k][j] * n[k][j];
             }
         }
-        along = row_sums(along, group, shared);
+        along = row_sum(along, group, shared);
         if (a.rms) along.x = 0.0f;
         float2 back{0.0f, 0.0f};
 #pragma unroll
@@ -368,7 +396,7 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
             }
         }
         if constexpr (POST) {
-            back = row_sums(back, group, shared);
+            back = row_sum(back, group, shared);
             if (a.rms) back.x = 0.0f;
         }
         if (row >= a.rows) continue;
@@ -387,21 +415,21 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
         }
     }
     if (!partials) return;
-    float* mine = partials + static_cast<long long>(blockIdx.x) * kJoinSums * channels;
+    float* mine = partials + static_cast<long long>(blockIdx.x) * kfloats * channels;
 #pragma unroll
     for (int which = 0; which < kSums; ++which) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < V; ++j) columns[j * kJoinBlock + threadIdx.x] = sums[which][k][j];
+            for (int j = 0; j < V; ++j) columns[j * BLOCK + threadIdx.x] = sums[which][k][j];
             __syncthreads();
             // `columns` holds V rows of per_block groups.
-            for (int i = threadIdx.x; i < V * group; i += kJoinBlock) {
+            for (int i = threadIdx.x; i < V * group; i += BLOCK) {
                 const int j = i / group, owner = i & (group - 1), c = (owner + k * group) * V + j;
                 if (c >= channels) continue;
                 float sum = 0.0f;
-                for (int r = 0; r < per_block; ++r) sum += columns[j * kJoinBlock + r * group + owner];
+                for (int r = 0; r < per_block; ++r) sum += columns[j * BLOCK + r * group + owner];
                 mine[which * static_cast<long long>(channels) + c] = sum;
             }
         }
@@ -434,7 +462,7 @@ residual_norm_grad_wide(lattice_residual_norm a, JoinGrads g, const float4* __re
                 along.x += slope;
                 along.y += slope * ((static_cast<float>(h[c]) - stat.x) * stat.y);
             }
-            along = row_sums(along, kJoinBlock, shared);
+            along = row_sum(along, kJoinBlock, shared);
         }
         along = a.rms ? float2{0.0f, along.y * inv} : float2{along.x * inv, along.y * inv};
         if (means && threadIdx.x == 0) means[row] = along;
@@ -450,7 +478,7 @@ residual_norm_grad_wide(lattice_residual_norm a, JoinGrads g, const float4* __re
                 back.x += slope;
                 back.y += slope * ((static_cast<float>(x[c]) - post.x) * post.y);
             }
-            back = row_sums(back, kJoinBlock, shared);
+            back = row_sum(back, kJoinBlock, shared);
             back = a.rms ? float2{0.0f, back.y * inv} : float2{back.x * inv, back.y * inv};
         }
         for (int c = threadIdx.x; c < channels; c += kJoinBlock) {
@@ -476,7 +504,7 @@ residual_norm_grad_columns(lattice_residual_norm a, JoinGrads g, const float4* _
     if (c >= channels) return;
     const JoinChannel<T, POST> v(a, c);
     const bool reads_x = POST || g.vectors[2];
-    float sums[kJoinSums] = {};
+    float sums[kfloats] = {};
     for (long long row = blockIdx.y; row < active; row += gridDim.y) {
         const float4 stat = statistics[row];
         const float2 along = means[row];
@@ -493,12 +521,12 @@ residual_norm_grad_columns(lattice_residual_norm a, JoinGrads g, const float4* _
         sums[3] += POST ? du * ((x - stat.z) * stat.w) : 0.0f;
         sums[4] += POST ? du : 0.0f;
     }
-    float* mine = partials + static_cast<long long>(blockIdx.y) * kJoinSums * channels;
+    float* mine = partials + static_cast<long long>(blockIdx.y) * kfloats * channels;
 #pragma unroll
     for (int which = 0; which < (POST ? 5 : 3); ++which) mine[which * static_cast<long long>(channels) + c] = sums[which];
 }
 
-// partials [count][kJoinSums][channels] -> the vectors' gradients: 16 columns a
+// partials [count][kfloats][channels] -> the vectors' gradients: 16 columns a
 // block, 64 slices of the partials added in slice order.
 constexpr int kFinishBlock = 1024, kFinishSlices = kFinishBlock / 16;
 template <typename T>
@@ -508,7 +536,7 @@ residual_norm_grad_finish(const float* __restrict__ partials, int count, int cha
     const int at = threadIdx.x & 15, slice = threadIdx.x >> 4;
     T* out = static_cast<T*>(g.vectors[blockIdx.y]);
     if (!out) return;
-    const long long row = static_cast<long long>(kJoinSums) * channels;
+    const long long row = static_cast<long long>(kfloats) * channels;
     for (long long first = blockIdx.x * 16ll; first < channels; first += gridDim.x * 16ll) {
         const long long c = first + at;
         float sum = 0.0f;
@@ -534,17 +562,16 @@ residual_norm_grad_finish(const float* __restrict__ partials, int count, int cha
     }
 }
 
-// Threads and vectors a thread for rows of `vectors` vectors.
+// Threads a row and vectors a thread for rows of `vectors` vectors.
 struct JoinShape {
     int group, held;  // held 0: rows that no block holds
+    int block() const { return std::max(group, kJoinBlock); }
 };
 inline JoinShape join_shape(int vectors) {
-    if (vectors > kJoinBlock * kJoinHeld) return {kJoinBlock, 0};
+    if (vectors > kJoinWidest * kJoinHeld) return {kJoinBlock, 0};
     int group = 1;
-    while (group < vectors && group < kWave) group *= 2;
-    if (group < vectors) group = kJoinBlock;
-    const int held = (vectors + group - 1) / group;
-    return {group, held == 3 ? 4 : held};
+    while (group < vectors && group < kJoinWidest) group *= 2;
+    return {group, (vectors + group - 1) / group};
 }
 
 // Vectors of 16, 4 and one element's bytes are instantiated.
@@ -574,17 +601,15 @@ inline bool join_sums(const JoinGrads& g) {
 template <typename T, int V, bool POST>
 int launch_join(const lattice_residual_norm& a, T* sum, T* normed, float4* statistics, hipStream_t stream) {
     const JoinShape shape = join_shape(a.channels / V);
-#define LATTICE_JOIN_ROWS(K)                                                                                 \
-    residual_norm_rows<T, V, K, POST><<<grid_for(a.rows, kJoinBlock / shape.group, 4096), kJoinBlock, 0, stream>>>( \
-        a, shape.group, sum, normed, statistics)
-    switch (shape.held) {
-        case 1: LATTICE_JOIN_ROWS(1); break;
-        case 2: LATTICE_JOIN_ROWS(2); break;
-        case 4: LATTICE_JOIN_ROWS(4); break;
-        default:
-            residual_norm_wide<T, POST><<<grid_for(a.rows, 1, 4096), kJoinBlock, 0, stream>>>(a, sum, normed, statistics);
+    if (shape.held) {
+        const auto kernel = shape.held == 2               ? residual_norm_rows<T, V, 2, kJoinWidest, POST>
+                            : shape.group == kJoinWidest ? residual_norm_rows<T, V, 1, kJoinWidest, POST>
+                                                         : residual_norm_rows<T, V, 1, kJoinBlock, POST>;
+        kernel<<<grid_for(a.rows, shape.block() / shape.group, kJoinBlocks), shape.block(), 0, stream>>>(
+            a, shape.group, sum, normed, statistics);
+    } else {
+        residual_norm_wide<T, POST><<<grid_for(a.rows, 1, 4096), kJoinBlock, 0, stream>>>(a, sum, normed, statistics);
     }
-#undef LATTICE_JOIN_ROWS
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
 }
@@ -593,30 +618,27 @@ template <typename T, int V, bool POST>
 int launch_join_grad(const lattice_residual_norm& a, const JoinGrads& g, const float4* statistics, float* partials,
                      float2* means, hipStream_t stream) {
     const JoinShape shape = join_shape(a.channels / V);
-    const int per_block = shape.held ? kJoinBlock / shape.group : 1;
+    const int per_block = shape.held ? shape.block() / shape.group : 1;
     const int blocks = join_partials(a.rows, a.channels, per_block);
-#define LATTICE_JOIN_ROWS(K)                                                                                  \
-    residual_norm_grad_rows<T, V, K, POST>                                                                    \
-        <<<partials ? blocks : grid_for(a.rows, per_block, 4096), kJoinBlock, 0, stream>>>(a, g, shape.group, \
-                                                                                           statistics, partials)
-    switch (shape.held) {
-        case 1: LATTICE_JOIN_ROWS(1); break;
-        case 2: LATTICE_JOIN_ROWS(2); break;
-        case 4: LATTICE_JOIN_ROWS(4); break;
-        default:
-            residual_norm_grad_wide<T, POST>
-                <<<grid_for(a.rows, 1, 4096), kJoinBlock, 0, stream>>>(a, g, statistics, partials ? means : nullptr);
-            if (partials) {
-                LATTICE_LAUNCH_CHECK();
-                residual_norm_grad_columns<T, POST>
-                    <<<dim3((a.channels + kJoinBlock - 1) / kJoinBlock, blocks), kJoinBlock, 0, stream>>>(
-                        a, g, statistics, means, partials);
-            }
+    if (shape.held) {
+        const auto kernel = shape.held == 2               ? residual_norm_grad_rows<T, V, 2, kJoinWidest, POST>
+                            : shape.group == kJoinWidest ? residual_norm_grad_rows<T, V, 1, kJoinWidest, POST>
+                                                         : residual_norm_grad_rows<T, V, 1, kJoinBlock, POST>;
+        kernel<<<partials ? blocks : grid_for(a.rows, per_block, kJoinBlocks), shape.block(), 0, stream>>>(
+            a, g, shape.group, statistics, partials);
+    } else {
+        residual_norm_grad_wide<T, POST>
+            <<<grid_for(a.rows, 1, 4096), kJoinBlock, 0, stream>>>(a, g, statistics, partials ? means : nullptr);
+        if (partials) {
+            LATTICE_LAUNCH_CHECK();
+            residual_norm_grad_columns<T, POST>
+                <<<dim3((a.channels + kJoinBlock - 1) / kJoinBlock, blocks), kJoinBlock, 0, stream>>>(
+                    a, g, statistics, means, partials);
+        }
     }
-#undef LATTICE_JOIN_ROWS
     LATTICE_LAUNCH_CHECK();
     if (partials) {
-        residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kJoinSums), kFinishBlock, 0, stream>>>(
+        residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kfloats), kFinishBlock, 0, stream>>>(
             partials, blocks, a.channels, a.scale, g);
         LATTICE_LAUNCH_CHECK();
     }
@@ -677,7 +699,7 @@ const char* join_fault(const lattice_residual_norm* a) {
 // No rows: the vectors' gradients are zero.
 template <typename T>
 int join_grad_empty(const lattice_residual_norm& a, const JoinGrads& g, hipStream_t stream) {
-    residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kJoinSums), kFinishBlock, 0, stream>>>(
+    residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kfloats), kFinishBlock, 0, stream>>>(
         nullptr, 0, a.channels, 0.0f, g);
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
@@ -710,7 +732,7 @@ extern "C" int lattice_hip_residual_norm(const lattice_residual_norm* args, void
 extern "C" size_t lattice_hip_residual_norm_grad_workspace_bytes(int rows, int channels) {
     if (rows <= 0 || channels <= 0) return 0;
     // The most blocks any vector width gives: one row a block.
-    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1)) * kJoinSums * channels * sizeof(float)) +
+    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1)) * kfloats * channels * sizeof(float)) +
            aligned_bytes(static_cast<size_t>(rows) * sizeof(float2));
 }
 
@@ -737,7 +759,7 @@ extern "C" int lattice_hip_residual_norm_grad(const lattice_residual_norm* args,
     float2* means = nullptr;
     if (join_sums(g)) {
         Workspace ws{static_cast<char*>(workspace), workspace ? workspace_bytes : 0};
-        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1)) * kJoinSums *
+        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1)) * kfloats *
                                   args->channels);
         means = ws.take<float2>(args->rows);
         LATTICE_REQUIRE(partials && means, "residual norm gradient workspace is too small.");
