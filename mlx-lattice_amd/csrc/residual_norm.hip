@@ -27,6 +27,7 @@ namespace {
 constexpr int kJoinBlock = 256;
 constexpr int kJoinWidest = 512;     // most threads a row
 constexpr int kJoinHeld = 2;         // most vectors of a row that a thread holds
+constexpr int kJoinMost = 16 / 2 * kJoinWidest * kJoinHeld;  // most channels that a block holds
 constexpr int kJoinPartials = 1024;  // most blocks that sum the vectors' gradients
 constexpr int kJoinBlocks = 4096;    // most blocks that walk the rows otherwise
 constexpr int kfloats = 5;         // weight, bias, gate, post weight, post bias
@@ -584,11 +585,17 @@ int join_vector(const lattice_residual_norm& a, std::initializer_list<const void
     return v == most ? v : v >= word ? word : 1;
 }
 
-// Blocks that sum the vectors' gradients, of `per_block` rows at a time.
-inline int join_partials(int rows, int channels, int per_block) {
+// Blocks of `threads` that sum the vectors' gradients, of `per_block` rows at a
+// time: what is resident, more while their partial rows stay under half a
+// million sums.  1024 channels in float32 take 121 us with 512 blocks and 126
+// with 1024 (25000 rows), 2048 in float16 134 with 512 and 216 with 256.  Rows
+// that no block holds: two million sums, or 32 rows of them.
+inline int join_partials(int rows, int channels, int per_block, int threads) {
     const long long blocks = (static_cast<long long>(rows) + per_block - 1) / per_block;
-    // Wide rows: no more partials than two million sums, or 32 of them.
-    const long long cap = std::max<long long>(32, std::min<long long>(kJoinPartials, (1ll << 21) / channels));
+    const long long cap = channels > kJoinMost
+                              ? std::max(32, (1 << 21) / channels)
+                              : std::max(kJoinPartials / 2 * kJoinBlock / threads,
+                                         std::min(kJoinPartials, (1 << 19) / channels));
     return static_cast<int>(std::max<long long>(1, std::min(blocks, cap)));
 }
 
@@ -619,7 +626,7 @@ int launch_join_grad(const lattice_residual_norm& a, const JoinGrads& g, const f
                      float2* means, hipStream_t stream) {
     const JoinShape shape = join_shape(a.channels / V);
     const int per_block = shape.held ? shape.block() / shape.group : 1;
-    const int blocks = join_partials(a.rows, a.channels, per_block);
+    const int blocks = join_partials(a.rows, a.channels, per_block, shape.held ? shape.block() : kJoinBlock);
     if (shape.held) {
         const auto kernel = shape.held == 2               ? residual_norm_grad_rows<T, V, 2, kJoinWidest, POST>
                             : shape.group == kJoinWidest ? residual_norm_grad_rows<T, V, 1, kJoinWidest, POST>
@@ -732,7 +739,7 @@ extern "C" int lattice_hip_residual_norm(const lattice_residual_norm* args, void
 extern "C" size_t lattice_hip_residual_norm_grad_workspace_bytes(int rows, int channels) {
     if (rows <= 0 || channels <= 0) return 0;
     // The most blocks any vector width gives: one row a block.
-    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1)) * kfloats * channels * sizeof(float)) +
+    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1, kJoinBlock)) * kfloats * channels * sizeof(float)) +
            aligned_bytes(static_cast<size_t>(rows) * sizeof(float2));
 }
 
@@ -759,7 +766,7 @@ extern "C" int lattice_hip_residual_norm_grad(const lattice_residual_norm* args,
     float2* means = nullptr;
     if (join_sums(g)) {
         Workspace ws{static_cast<char*>(workspace), workspace ? workspace_bytes : 0};
-        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1)) * kfloats *
+        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1, kJoinBlock)) * kfloats *
                                   args->channels);
         means = ws.take<float2>(args->rows);
         LATTICE_REQUIRE(partials && means, "residual norm gradient workspace is too small.");
