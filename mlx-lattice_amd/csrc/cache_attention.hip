@@ -58,21 +58,32 @@ CacheLayout cache_layout(const CacheCall& call) {
         l.share = false;
         l.tiles = 2;
     } else {
-        // The largest tiles that are mostly filled and, their tokens split, give
-        // every unit its blocks.
+        // Tiles that share the codes' reads and widening, if the chip stays full.
+        // Queries of 8 heads over 2 key heads in bfloat16, us with one, two and the
+        // most tiles: 4 x 512 over 4096 tokens 27, 28, 33 at 32 channels, 43, 40, 44
+        // at 96; 4 x 333 of 8 key heads in a window of 1024 12, 14, 16 at 32 and 30,
+        // 25 at 128; 2 x 2048 of 16 heads over 16384 tokens 548, 362, 323 at 64.
+        // 128 queries over 8192 tokens, split in its best way, 14.5 and 15.0 at 32,
+        // 30 and 24 at 128.
+        const int most = f32 ? cache_most_tiles<float>(width) : cache_most_tiles<_Float16>(width);
+        const int pair_blocks = f32 || width <= 64 ? kUnits : kUnits / 4;
         const long long seen = std::min<long long>(
             static_cast<long long>(a.left) + a.right + a.sinks + std::min(a.queries, 16),
             static_cast<long long>(c.blocks) * kCacheBlock);
-        const int most = f32 ? cache_most_tiles<float>(width) : cache_most_tiles<_Float16>(width);
-        for (int tiles : {most, 2, 1}) {
-            const long long own = blocks(16 * tiles), parts = std::min<long long>(64, seen / (tiles > 1 ? 2048 : 512));
-            if (tiles > 1 && (!filled(16 * tiles) || own * std::max(1ll, parts) < kUnits / 2)) continue;
-            l.tiles = tiles;
-            if (own < kUnits) {
-                const long long wanted = (tiles > 1 ? 2 : 4) * kUnits;
-                l.splits = static_cast<int>(std::max(1ll, std::min(parts, (wanted + own - 1) / own)));
-            }
-            break;
+        const auto parts = [&](int tiles) { return std::max(1ll, std::min<long long>(64, seen / (tiles > 1 ? 2048 : 1024))); };
+        if (most > 2 && filled(16 * most) && blocks(16 * most) >= kUnits) {
+            l.tiles = most;
+        } else if (filled(32) && blocks(32) * parts(2) >= pair_blocks) {
+            l.tiles = 2;
+        }
+        // Parts of 1024 tokens or more, 256 a wave, since each is joined in a
+        // launch of its own.  One query of 16 heads over 4 key heads of 32 caches,
+        // us in 1, 4, 8 and 16 parts: 8000 tokens of 64 channels 27, 24, 25, 26,
+        // 32768 of 128 -, 192, 169, 165.
+        const long long own = blocks(16 * l.tiles);
+        if (own < kUnits) {
+            const long long wanted = (l.tiles > 1 ? 2 : 4) * kUnits;
+            l.splits = static_cast<int>(std::min(parts(l.tiles), (wanted + own - 1) / own));
         }
     }
     l.slots = pairs / l.rows() + c.sequences + 2;

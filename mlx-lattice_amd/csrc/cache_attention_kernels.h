@@ -463,19 +463,12 @@ __device__ inline void cache_queries(CacheTerms<T> (&q)[R][DP / 32], const Cache
     }
 }
 
-// How positions p_low .. p_high see a block of tokens from j0 on.
+// Whether positions p_low .. p_high see all of a block of tokens from j0 on.
 struct CacheView {
-    int all_to, all_from, all_first;      // all of it
-    int some_to, some_from, some_first;  // some of it
+    int to, from, first;
     __device__ CacheView(const lattice_cache_attention& a, int nk, int p_low, int p_high)
-        : all_to(min(nk, p_low + a.right + 1) - kCacheBlock),
-          all_from(p_high - a.left),
-          all_first(a.sinks - kCacheBlock),
-          some_to(min(nk, p_high + a.right + 1) - 1),
-          some_from(p_low - a.left - kCacheBlock + 1),
-          some_first(a.sinks - 1) {}
-    __device__ bool all(int j0) const { return j0 <= all_to && (j0 >= all_from || j0 <= all_first); }
-    __device__ bool some(int j0) const { return j0 <= some_to && (j0 >= some_from || j0 <= some_first); }
+        : to(min(nk, p_low + a.right + 1) - kCacheBlock), from(p_high - a.left), first(a.sinks - kCacheBlock) {}
+    __device__ bool all(int j0) const { return j0 <= to && (j0 >= from || j0 <= first); }
 };
 
 // The factor of a block's scores, positive, so that -inf stays -inf.
@@ -680,9 +673,8 @@ struct CacheStage {
     typedef typename CacheOperand<O>::Frag Frag;
     static constexpr int kFrags = DP / 16;
     static constexpr int kBytes = kFrags * kWave * 16;
-    // Operands that a wave makes; where they do not go around, the last waves
-    // have one less.
-    static constexpr int kMine = (kFrags + kAttnWaves - 1) / kAttnWaves;
+    static_assert(kFrags % kAttnWaves == 0);
+    static constexpr int kMine = kFrags / kAttnWaves;  // operands that a wave makes
     struct Codes {
         uint2 w[kMine];
     };
@@ -696,7 +688,7 @@ struct CacheStage {
         const int n = lane_id() & 15, g = lane_id() >> 4;
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
-            const int f = min(wave + kAttnWaves * k, kFrags - 1);
+            const int f = wave + kAttnWaves * k;
             place[k] = values ? (16 * f + n) * kCacheBlock + 8 * g
                               : key_token(f / (DP / 32), n) * DP + key_channel<DP, false>(f % (DP / 32), g);
         }
@@ -717,9 +709,8 @@ struct CacheStage {
     __device__ static void write(char* to, const Codes& from, int wave) {
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
-            // The last ones twice, with the same bytes.
-            const int f = min(wave + kAttnWaves * k, kFrags - 1);
-            *reinterpret_cast<Frag*>(to + (f * kWave + lane_id()) * 16) = widen<Code, O>(from.w[k]);
+            *reinterpret_cast<Frag*>(to + ((wave + kAttnWaves * k) * kWave + lane_id()) * 16) =
+                widen<Code, O>(from.w[k]);
         }
     }
     __device__ static Frag operand(const char* from, int f) {
