@@ -473,7 +473,7 @@ struct CacheView {
 
 // The factor of a block's scores, positive, so that -inf stays -inf.
 __device__ inline float cache_factor(float scale, int key_exponent) {
-    return fmaxf(scale * power_of_two(max(key_exponent, kCacheLeast)), FLT_MIN);
+    return fmaxf(scale * power_of_two(max(key_exponent, kCacheLeast)), 0x1p-149f);
 }
 
 // Sums over the four lanes of a pair, and products in units of one.

@@ -67,7 +67,9 @@ def cache_attention(q: torch.Tensor, cache: QuantizedCache, *,
     are clamped to the rows there are.
 
     A query that sees nothing gives zeros, as do rows in no sequence; what a
-    query does not see never reaches it.  Without gradient.
+    query does not see never reaches it.  Products of queries and codes are
+    summed before the blocks' powers of two go in, and overflow float32 from
+    queries of ``2 ** 112`` on.  Without gradient.
     """
     left, right = (_ALL if b is None else int(b) for b in (left, right))
     if scale is None:

@@ -32,8 +32,8 @@ def residual_norm(x: SparseTensor | torch.Tensor,
     where ``norm`` is over the channels of a row, ``(z - mean) / sqrt(var +
     eps)``, or ``z / sqrt(mean(z ** 2) + eps)`` with ``rms``.  ``sum`` is
     rounded to the rows' dtype first, and ``normed`` is of what it holds, as an
-    addition and :func:`layer_norm` give it.  The vectors have shape ``(C,)`` and the rows' dtype (``None``: 1 for weights and gate, 0 for
-    biases).  Rows at and past the device count ``active_rows`` (a sparse
+    addition and :func:`layer_norm` give it.  The vectors have shape ``(C,)``
+    and the rows' dtype (``None``: 1 for weights and gate, 0 for biases).  Rows at and past the device count ``active_rows`` (a sparse
     tensor's own) become zeros and take no part in the gradients.  Statistics
     and sums are float32; float32, float16 and bfloat16 rows.
     """

@@ -189,6 +189,24 @@ def test_infinities_and_nan(value, code):
 
 
 @pytest.mark.parametrize('code', CODES)
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', (32, 33))
+def test_infinities_under_far_exponents(dim, dtype, code):
+    """Rows that hold nothing finite, whose exponent is the least, and rows
+    behind earlier tokens beyond their type's range."""
+    gen = torch.Generator(device='cuda').manual_seed(17)
+    cache = random_cache(gen, code, 3, 64, 1, dim)
+    cache.key_exponents[1] = 110
+    cache.value_exponents[1] = -126
+    k, v = (t.clone() for t in _rows(gen, dtype, 9, 1, dim))
+    k[:3], v[:3] = math.inf, -math.inf
+    for rows in (k, v):
+        rows[4, 0, 3], rows[5, 0, dim - 1] = -math.inf, math.nan
+        rows[8] = math.nan
+    _check(cache, k, v, (3, 3, 3), (3, 40, 34))
+
+
+@pytest.mark.parametrize('code', CODES)
 def test_zeros_and_values_at_the_ends_of_float32(code):
     gen = torch.Generator(device='cuda').manual_seed(8)
     cache = random_cache(gen, code, 4, 32, 1, 32)

@@ -309,6 +309,26 @@ def test_scales(scale, dtype):
         _check(-q, cache, (20, 1), (160, 50), 60, 0, 3, -scale)
 
 
+@pytest.mark.parametrize('dtype', (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize('heads, rows', ((4, 3), (64, 600)))
+def test_keys_next_to_nothing_under_large_queries(heads, rows, dtype):
+    """The factor of the scores, 0.05 log2(e) 2^-126, is below the normal
+    numbers; the scores are some 0.005."""
+    gen = torch.Generator(device='cuda').manual_seed(16)
+    cache = random_cache(gen, torch.int8, 1, 704, 2, 128)
+    cache.key_exponents.fill_(-126)
+    q = _queries(gen, dtype, rows, heads, 128, 2.0 ** 114)
+    got = _ops().cache_attention(q, cache, offsets=_ints(0, rows),
+                                 lengths=_ints(700), right=0, scale=0.05)
+    want, bound = _reference(q, cache, (rows,), (700,), None, 0, 0, 0.05,
+                             device='cuda')
+    # The factor is over 2^-130 and a multiple of 2^-149: off by at most 2^-20
+    # of it.  That much of the scores (below 1) goes into the shares, on either
+    # side of the quotient.
+    values = decoded(cache)[1].abs().max()
+    assert_within(got, want, bound.cpu() + values * 2 * 2.0 ** -20)
+
+
 def test_long_tail_under_one_large_score():
     """A token with 2^13 times the share of each of 16,000 others, whose
     values the result is made of, in half precision."""
