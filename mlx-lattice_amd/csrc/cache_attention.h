@@ -21,11 +21,16 @@ struct CacheLayout {
     int rows() const { return 16 * tiles * (share ? 1 : kAttnWaves); }
 };
 
-// Most tiles of pairs that fit a wave's registers.
+// Most tiles of pairs that fit a wave's registers.  2 x 2048 queries of 16 heads
+// in float32 over 8192 tokens, us with one and two: 469 and 409 at 64 channels, 786
+// and 671 at 128, where some 70 bytes a lane no longer fit.
 template <typename T> constexpr int cache_most_tiles(int width) {
     return sizeof(T) == 4 ? (width == 32 ? 4 : 2) : width <= 64 ? 4 : width == 96 ? 3 : 2;
 }
-// Where widening a block's codes once for four waves, by way of LDS, is faster.
+// Where widening a block's codes once for four waves, by way of LDS, is faster: 2
+// x 2048 queries of 16 heads over 16384 tokens take 619 us against 700 with two
+// tiles that widen their own in bfloat16, 638 against 735 from int8 in half
+// precision.  Narrower heads have three or four tiles to a widening.
 template <typename T> constexpr bool cache_many(int width) { return width == 128 && sizeof(T) == 2; }
 
 // Both structures, with bounds that keep positions inside 32 bits.

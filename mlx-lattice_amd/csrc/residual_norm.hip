@@ -12,12 +12,21 @@
 //
 // Bound by memory: the forward pass reads two arrays and writes two, the
 // gradients read four (three where neither gate nor first norm need x) and
-// write two.  A group of lanes, or a whole block for rows of more vectors than
-// a wave has lanes, holds a row in registers; the vectors' sums stay in the
-// registers of the lanes that own the channels over all rows a block walks,
-// then go to one partial row a block, and a second launch adds those in a fixed
-// order.  Rows wider than a block holds are read again from the caches, and
-// their vectors' sums take a pass of their own.
+// write two.  A power of two of threads, of a wave's lanes or of a block's waves,
+// holds a row in registers, 16 bytes a thread, and reads the next row while it
+// computes one: 160 us without that, 125 with, for the gradients below.  Sums go
+// across lanes without LDS (102 us with, 86 without, for the forward pass of
+// 400000 rows of 128 channels in bfloat16 with the first norm).  The vectors'
+// sums stay in the registers of the lanes that own the channels over all rows a
+// block walks, then go to one partial row a block, and a second launch adds those
+// in a fixed order.  Rows wider than a block holds are read again from the
+// caches, and their vectors' sums take a pass of their own.
+//
+// 400000 rows of 128 channels, half precision, with a gate: forward 76 us (5.4
+// TB/s), gradients 125 us (4.9 TB/s) and 4 for the vectors' sums.  25013 rows of
+// 1000 channels, float32, both norms: 74 us (5.4), 140 (4.3) and 5.  6250 rows of
+// 8192 channels, half precision: 162 and 371 us, as rows that no block holds 406
+// and 763.
 
 #include "rows.h"
 
