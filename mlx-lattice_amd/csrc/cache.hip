@@ -160,19 +160,18 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     const uint32_t slot = cache_place(groups);
     const int task = blockIdx.x % groups * (kCacheThreads / kWave) + threadIdx.x / kWave;
     const RowPartition partition{offsets, c.sequences, rows};
-    const int e = partition.find(slot, write_slot);
-    if (!partition.real(e) || task >= 2 * c.kv_heads) return;
+    const CacheSequence s = find_cache_sequence(partition, lengths, c.blocks * kCacheBlock, slot, write_slot);
+    if (!s.real || task >= 2 * c.kv_heads) return;
     const bool values = task & 1;
     const int head = task >> 1;
-    const CacheSequence s = cache_sequence(partition, lengths, c.blocks * kCacheBlock, e);
     const int first = max(s.shift(), 0);
-    const long long block = first / kCacheBlock + static_cast<long long>(slot - write_slot(s.q0, e));
+    const long long block = first / kCacheBlock + static_cast<long long>(slot - write_slot(s.q0, s.index));
     if (block >= c.blocks) return;
     const int lo = static_cast<int>(block) * kCacheBlock;
     const int begin = max(first, lo) - lo, end = min(s.nk - lo, kCacheBlock);
     if (begin >= end) return;
 
-    const long long at = (static_cast<long long>(e - 1) * c.kv_heads + head) * c.blocks + block;
+    const long long at = (static_cast<long long>(s.index - 1) * c.kv_heads + head) * c.blocks + block;
     uint8_t* codes = static_cast<uint8_t*>(values ? c.values : c.keys) + at * kCacheBlock * DP;
     int8_t* exponent = (values ? c.value_exponents : c.key_exponents) + at;
     const CacheSource& source = values ? vals : keys;

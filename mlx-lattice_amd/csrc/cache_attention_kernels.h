@@ -570,16 +570,15 @@ cache_attend_few(CacheCall call, int splits, CachePart part, T* __restrict__ out
     const RowPartition partition{a.offsets, c.sequences, a.queries};
     const auto slot_of = [group](int start, int e) { return start * group / kRows + e; };
     const uint32_t slot = block_slot(splits);
-    const int e = partition.find(slot, slot_of);
-    const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
+    const CacheSequence s = find_cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, slot, slot_of);
     const uint32_t count = s.nq * group;
-    const uint32_t first = slot_first<kRows>(slot, slot_of(s.q0, e), count);
+    const uint32_t first = slot_first<kRows>(slot, slot_of(s.q0, s.index), count);
     if (first >= count) return;
 
     const int p_low = static_cast<int>(first / group) + s.shift();
     const int p_high = static_cast<int>((min(first + kRows, count) - 1) / group) + s.shift();
-    const AttnTiles blocks = partition.real(e) ? cache_blocks(a, s.nk, p_low, p_high) : AttnTiles{0, 0, 0};
-    const CacheReader<DP> reader(c, e - 1, kv);
+    const AttnTiles blocks = s.real ? cache_blocks(a, s.nk, p_low, p_high) : AttnTiles{0, 0, 0};
+    const CacheReader<DP> reader(c, s.index - 1, kv);
     const int parts = splits * kAttnWaves, mine = split * kAttnWaves + wave;
     const int from = static_cast<int>(static_cast<long long>(blocks.count) * mine / parts);
     const int to = static_cast<int>(static_cast<long long>(blocks.count) * (mine + 1) / parts);
@@ -660,7 +659,7 @@ cache_attend_few(CacheCall call, int splits, CachePart part, T* __restrict__ out
     }
     if (wave != 0) return;
     if (splits == 1) {
-        write_pairs<T, Code, DP, R>(call, s, e - 1, rows, state, out, &scratch);
+        write_pairs<T, Code, DP, R>(call, s, s.index - 1, rows, state, out, &scratch);
         return;
     }
     const long long items = static_cast<long long>(a.queries) * a.heads;
@@ -751,10 +750,9 @@ cache_attend_many(CacheCall call, T* __restrict__ out) {
     const RowPartition partition{a.offsets, c.sequences, a.queries};
     const auto slot_of = [group](int start, int e) { return start * group / kSlot + e; };
     const uint32_t slot = block_slot(1);
-    const int e = partition.find(slot, slot_of);
-    const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
+    const CacheSequence s = find_cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, slot, slot_of);
     const uint32_t count = s.nq * group;
-    const uint32_t start = slot_first<kSlot>(slot, slot_of(s.q0, e), count);
+    const uint32_t start = slot_first<kSlot>(slot, slot_of(s.q0, s.index), count);
     if (start >= count) return;
     // A wave behind the last pair repeats it, unwritten.
     const uint32_t first = start + wave * kRows, mine = min(first, count - 1);
@@ -768,12 +766,12 @@ cache_attend_many(CacheCall call, T* __restrict__ out) {
     const int p_high = static_cast<int>((min(mine + kRows, count) - 1) / group) + s.shift();
     CacheState<T, DP, R> state;
     state.clear();
-    const AttnTiles blocks = partition.real(e)
+    const AttnTiles blocks = s.real
                                  ? cache_blocks(a, s.nk, static_cast<int>(start / group) + s.shift(),
                                                 static_cast<int>((min(start + kSlot, count) - 1) / group) + s.shift())
                                  : AttnTiles{0, 0, 0};
     if (blocks.count > 0) {
-        const long long at = (static_cast<long long>(e - 1) * c.kv_heads + kv) * c.blocks;
+        const long long at = (static_cast<long long>(s.index - 1) * c.kv_heads + kv) * c.blocks;
         const Stage keys(c.keys, at, false, wave), values(c.values, at, true, wave);
         const int8_t *key_exponents = c.key_exponents + at, *value_exponents = c.value_exponents + at;
         const CacheView view(a, s.nk, p_low, p_high);
@@ -845,7 +843,7 @@ cache_attend_many(CacheCall call, T* __restrict__ out) {
         }
     }
     close_state<T, DP, R>(state);
-    write_pairs<T, Code, DP, R>(call, s, e - 1, rows, state, out, &scratch[wave]);
+    write_pairs<T, Code, DP, R>(call, s, s.index - 1, rows, state, out, &scratch[wave]);
 }
 
 // Joins the parts (at most 64) of a pair: a wave a (query, head).
@@ -884,9 +882,10 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
     if (__any(!finite)) {
         const int row = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
         const RowPartition partition{a.offsets, c.sequences, a.queries};
-        const int e = partition.find(row, [](int start, int) { return static_cast<uint32_t>(start); });
-        const CacheSequence s = cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, e);
-        attend_pair<T, Code>(call, s, e - 1, row - s.q0, head, out, &scratch[wave]);
+        const CacheSequence s =
+            find_cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, row,
+                                [](int start, int) { return static_cast<uint32_t>(start); });
+        attend_pair<T, Code>(call, s, s.index - 1, row - s.q0, head, out, &scratch[wave]);
         return;
     }
     if (half == 0 && d < c.dim) {
