@@ -53,8 +53,8 @@ def residual_norm(x: SparseTensor | torch.Tensor,
         raise ValueError('a sparse residual needs a sparse tensor.')
     vectors = (weight, bias, gate, post_weight, post_bias)
     how = (vectors, scale, post_norm, rms, eps, active_rows)
-    if torch.is_grad_enabled() and (
-            x.requires_grad or residual.requires_grad
-            or any(v is not None and v.requires_grad for v in vectors)):
-        return ext.residual_norm_node(x, residual, *how)
+    if torch.is_grad_enabled():
+        for t in (x, residual, *vectors):
+            if t is not None and t.requires_grad:
+                return ext.residual_norm_node(x, residual, *how)
     return ext.residual_norm(x, residual, *how, False)[:2]
