@@ -428,6 +428,7 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
     float* mine = partials + static_cast<long long>(blockIdx.x) * kfloats * channels;
 #pragma unroll
     for (int which = 0; which < kSums; ++which) {
+        if (!g.vectors[which]) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             __syncthreads();
@@ -533,7 +534,8 @@ residual_norm_grad_columns(lattice_residual_norm a, JoinGrads g, const float4* _
     }
     float* mine = partials + static_cast<long long>(blockIdx.y) * kfloats * channels;
 #pragma unroll
-    for (int which = 0; which < (POST ? 5 : 3); ++which) mine[which * static_cast<long long>(channels) + c] = sums[which];
+    for (int which = 0; which < (POST ? 5 : 3); ++which)
+        if (g.vectors[which]) mine[which * static_cast<long long>(channels) + c] = sums[which];
 }
 
 // partials [count][kfloats][channels] -> the vectors' gradients: 16 columns a
