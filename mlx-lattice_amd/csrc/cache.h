@@ -124,6 +124,16 @@ __device__ inline CacheSequence find_cache_sequence(const RowPartition& rows, co
     return cache_sequence(rows, capacity, e, rows.start(e), rows.start(e + 1), rows.real(e) ? lengths[e - 1] : 0);
 }
 
+// Places, slots or blocks of tokens, of `groups` blocks of threads each, next to
+// each other; those past 2^22 blocks of threads go on along z, above `parts`.
+inline dim3 cache_grid(long long places, uint32_t groups, int parts) {
+    const long long x = std::min<long long>(places, (1 << 22) / groups);
+    return dim3(static_cast<unsigned>(x) * groups, 1, static_cast<unsigned>((places + x - 1) / x * parts));
+}
+__device__ inline uint32_t cache_place(uint32_t groups, uint32_t parts) {
+    return blockIdx.x / groups + gridDim.x / groups * (parts == 1 ? blockIdx.z : blockIdx.z / parts);
+}
+
 __host__ __device__ inline int cache_width(const lattice_cache& c) { return (c.dim + 31) / 32 * 32; }
 
 // What every entry checks; NULL, or what is wrong.

@@ -66,15 +66,6 @@ __host__ __device__ inline uint32_t head_groups(int kv_heads) {
     return (2u * kv_heads + kCacheThreads / kWave - 1) / (kCacheThreads / kWave);
 }
 
-// Places, slots or blocks of tokens, of `groups` blocks of threads each; those
-// past 2^22 blocks of threads go on along z.
-inline dim3 cache_grid(long long places, uint32_t groups) {
-    const long long x = std::min<long long>(places, (1 << 22) / groups);
-    return dim3(static_cast<unsigned>(x) * groups, 1, static_cast<unsigned>((places + x - 1) / x));
-}
-__device__ inline uint32_t cache_place(uint32_t groups) {
-    return blockIdx.x / groups + gridDim.x / groups * blockIdx.z;
-}
 inline bool cache_fits(const lattice_cache& c, long long places) {
     return places < 1ll << 31 && places * head_groups(c.kv_heads) < 1ll << 36;
 }
@@ -157,7 +148,7 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     constexpr int kTokens = Hold::kTokens, kGroups = Hold::kGroups;
     // The heads of a slot next to each other, as they lie in its rows.
     const uint32_t groups = head_groups(c.kv_heads);
-    const uint32_t slot = cache_place(groups);
+    const uint32_t slot = cache_place(groups, 1);
     const int task = blockIdx.x % groups * (kCacheThreads / kWave) + threadIdx.x / kWave;
     const RowPartition partition{offsets, c.sequences, rows};
     const CacheSequence s = find_cache_sequence(partition, lengths, c.blocks * kCacheBlock, slot, write_slot);
@@ -323,7 +314,7 @@ cache_read_blocks(lattice_cache c, const int32_t* __restrict__ lengths, T* __res
     constexpr int kTokens = Hold::kTokens, kGroups = Hold::kGroups;
     // The heads of a block next to each other, as they lie in its rows.
     const uint32_t groups = head_groups(c.kv_heads);
-    const uint32_t place = cache_place(groups);
+    const uint32_t place = cache_place(groups, 1);
     const int task = blockIdx.x % groups * (kCacheThreads / kWave) + threadIdx.x / kWave;
     const long long s = place / c.blocks;
     const int block = place % c.blocks;
@@ -398,7 +389,7 @@ long long write_slots(const lattice_cache& c, int rows) {
 template <typename T, int V, typename Code>
 void launch_write(const lattice_cache& c, const CacheSource& k, const CacheSource& v, int rows,
                   const int32_t* offsets, const int32_t* lengths, hipStream_t stream) {
-    const dim3 grid = cache_grid(write_slots(c, rows), head_groups(c.kv_heads));
+    const dim3 grid = cache_grid(write_slots(c, rows), head_groups(c.kv_heads), 1);
     const auto launch = [&](auto kernel) {
         kernel<<<grid, kCacheThreads, 0, stream>>>(c, k, v, rows, offsets, lengths);
     };
@@ -427,7 +418,7 @@ int write_of(const lattice_cache& c, const CacheSource& k, const CacheSource& v,
 
 template <typename T, int V, typename Code>
 void launch_read(const lattice_cache& c, const int32_t* lengths, T* k, T* v, hipStream_t stream) {
-    const dim3 grid = cache_grid(1ll * c.sequences * c.blocks, head_groups(c.kv_heads));
+    const dim3 grid = cache_grid(1ll * c.sequences * c.blocks, head_groups(c.kv_heads), 1);
     const auto launch = [&](auto kernel) { kernel<<<grid, kCacheThreads, 0, stream>>>(c, lengths, k, v); };
     switch (cache_width(c)) {
         case 32: return launch(cache_read_blocks<T, V, Code, 32>);

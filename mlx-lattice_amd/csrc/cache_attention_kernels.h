@@ -26,10 +26,10 @@
 // Single tokens are bound by memory: a byte a value is read, once.  One query of
 // 16 heads over 4 key heads of 128 channels, 32 caches of 32768 tokens, some 24
 // thousand filled, in half precision: 164 us, 5.07 TB/s, where a copy reaches
-// 5.23.  Small calls are bound by latency: 6.0 us for 4 caches in a window of
+// 5.23.  Small calls are bound by latency: 5.9 us for 4 caches in a window of
 // 512.  Chunks are bound by the matrix cores and the exponentials and widenings
 // beside them: 2 x 2048 causal queries of 16 heads of 128 channels over 16384
-// tokens in bfloat16 take 552 us, 904 TFLOP/s, where a product of 8192 x 8192 x
+// tokens in bfloat16 take 537 us, 929 TFLOP/s, where a product of 8192 x 8192 x
 // 8192 reaches 1207; the matrix cores work 0.35 of the time, the vector units
 // 0.47.
 #pragma once
@@ -566,10 +566,10 @@ cache_attend_few(CacheCall call, int splits, CachePart part, T* __restrict__ out
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
     const int n = lane & 15, g = lane >> 4;
     const uint32_t group = a.heads / c.kv_heads;
-    const int kv = blockIdx.y, split = block_part(splits);
+    const int kv = blockIdx.x % c.kv_heads, split = block_part(splits);
     const RowPartition partition{a.offsets, c.sequences, a.queries};
     const auto slot_of = [group](int start, int e) { return start * group / kRows + e; };
-    const uint32_t slot = block_slot(splits);
+    const uint32_t slot = cache_place(c.kv_heads, splits);
     const CacheSequence s = find_cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, slot, slot_of);
     const uint32_t count = s.nq * group;
     const uint32_t first = slot_first<kRows>(slot, slot_of(s.q0, s.index), count);
@@ -745,11 +745,11 @@ cache_attend_many(CacheCall call, T* __restrict__ out) {
     const lattice_cache_attention& a = call.args;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t group = a.heads / c.kv_heads;
-    const int kv = blockIdx.y;
+    const int kv = blockIdx.x % c.kv_heads;
     constexpr int kSlot = kRows * kAttnWaves;
     const RowPartition partition{a.offsets, c.sequences, a.queries};
     const auto slot_of = [group](int start, int e) { return start * group / kSlot + e; };
-    const uint32_t slot = block_slot(1);
+    const uint32_t slot = cache_place(c.kv_heads, 1);
     const CacheSequence s = find_cache_sequence(partition, a.lengths, c.blocks * kCacheBlock, slot, slot_of);
     const uint32_t count = s.nq * group;
     const uint32_t start = slot_first<kSlot>(slot, slot_of(s.q0, s.index), count);
@@ -899,7 +899,9 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
 template <typename T, typename Code, int DP>
 int launch_cache_attend(const CacheCall& call, const CacheLayout& l, const CachePart& part, T* out,
                         hipStream_t stream) {
-    const dim3 grid = slot_grid(l.slots, call.cache.kv_heads, l.splits);
+    // Key heads next to each other: a die's L2 has few of them, and the blocks of
+    // a unit are of unequal sequences (537 us, 550 slot by slot, for the chunks above).
+    const dim3 grid = cache_grid(l.slots, call.cache.kv_heads, l.splits);
     const auto few = [&](auto kernel) { kernel<<<grid, kAttnBlock, 0, stream>>>(call, l.splits, part, out); };
     if (!l.share) {
         if constexpr (cache_many<T>(DP)) cache_attend_many<T, Code, DP, 2><<<grid, kAttnBlock, 0, stream>>>(call, out);
