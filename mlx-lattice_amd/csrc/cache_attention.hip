@@ -114,6 +114,7 @@ extern "C" int lattice_hip_cache_attention(const lattice_cache* cache, const lat
     LATTICE_REQUIRE(out, "attention pointers must be non-null.");
     const CacheCall call = cache_call(*cache, *args);
     const CacheLayout l = cache_layout(call);
+    LATTICE_REQUIRE(l.slots * cache->kv_heads * l.splits < 1ll << 36, "the cache has too many sequences and heads.");
     CachePart part{nullptr, nullptr};
     if (l.splits > 1) {
         Workspace ws{static_cast<char*>(workspace), workspace ? workspace_bytes : 0};

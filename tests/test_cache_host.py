@@ -149,6 +149,24 @@ def test_attention_refusals(changes, message):
         ctypes.byref(cache), ctypes.byref(args)) == 0
 
 
+def test_more_blocks_than_a_launch_has():
+    lib = _library()
+    message = b'too many sequences and heads'
+    cache = _cache(sequences=1 << 23, kv_heads=(1 << 16) - 1)
+    assert lib.lattice_hip_cache_write(
+        ctypes.byref(cache), 1, void(4096), long_(128), long_(64), void(4096),
+        long_(128), long_(64), 8, void(4096), void(4096), None) == 1
+    assert message in lib.lattice_hip_last_error()
+    assert lib.lattice_hip_cache_read(ctypes.byref(cache), 1, void(4096),
+                                      void(4096), void(4096), None) == 1
+    assert message in lib.lattice_hip_last_error()
+    args = _attention(queries=1, heads=(1 << 16) - 1)
+    assert lib.lattice_hip_cache_attention(
+        ctypes.byref(cache), ctypes.byref(args), void(4096), None,
+        ctypes.c_size_t(0), None) == 1
+    assert message in lib.lattice_hip_last_error()
+
+
 def test_attention_workspaces():
     lib = _library()
     cache = _cache(dim=60)

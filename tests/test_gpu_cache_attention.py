@@ -138,6 +138,36 @@ def test_many_short_sequences(dtype):
            1, 2, device='cuda')
 
 
+# On either side of what one read of the offsets finds, written and attended.
+@pytest.mark.parametrize('first', (0, 5))
+@pytest.mark.parametrize('batches', (1, 60, 61, 62, 63, 64, 65, 130))
+def test_numbers_of_sequences(batches, first):
+    gen = torch.Generator(device='cuda').manual_seed(17)
+    counts = [(3 * s + 1) % 5 for s in range(batches)]
+    lengths = [c + s % 50 for s, c in enumerate(counts)]
+    cache = random_cache(gen, torch.int8, batches, 64, 1, 32)
+    rows = first + sum(counts) + 4
+    q = _queries(gen, torch.float16, rows, 2, 32)
+    k, v = (torch.randn((rows, 1, 32), generator=gen, device='cuda')
+            for _ in range(2))
+    before = decoded(cache)
+    at = _offsets(counts, first)
+    _ops().write_cache(cache, k, v, offsets=at, lengths=_ints(*lengths))
+    for got, then, new in zip(decoded(cache), before, (k, v)):
+        place = first
+        for s, (count, length) in enumerate(zip(counts, lengths)):
+            # Magnitudes are below 7.9 = 127 2^-4: half a step is 2^-5.
+            wanted = new[place:place + count, 0].cpu().double()
+            place += count
+            start = length - count
+            now, was = got[s, :length, 0], then[s, :start, 0]
+            assert ((now[start:] - wanted).abs() <= 2.0 ** -5).all()
+            assert ((now[:start] - was).abs() <= 2.0 ** -5).all()
+    got = _check(q, cache, counts, lengths, 20, 1, 2, first=first,
+                 device='cuda')
+    assert not got[:first].any() and not got[-4:].any()
+
+
 @pytest.mark.parametrize('code', CODES)
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('heads, count', ((4, 1), (4, 9), (64, 70)))
