@@ -30,8 +30,8 @@
 // 512.  Chunks are bound by the matrix cores and the exponentials and widenings
 // beside them: 2 x 2048 causal queries of 16 heads of 128 channels over 16384
 // tokens in bfloat16 take 537 us, 929 TFLOP/s, where a product of 8192 x 8192 x
-// 8192 reaches 1207; the matrix cores work 0.35 of the time, the vector units
-// 0.47.
+// 8192 reaches 1207; the matrix cores work 0.37 of the time, the vector units
+// 0.49.
 #pragma once
 
 #include "cache_attention.h"
