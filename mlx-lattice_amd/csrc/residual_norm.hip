@@ -39,12 +39,12 @@ constexpr int kJoinHeld = 2;         // most vectors of a row that a thread hold
 constexpr int kJoinMost = 16 / 2 * kJoinWidest * kJoinHeld;  // most channels that a block holds
 constexpr int kJoinPartials = 1024;  // most blocks that sum the vectors' gradients
 constexpr int kJoinBlocks = 4096;    // most blocks that walk the rows otherwise
-constexpr int kfloats = 5;         // weight, bias, gate, post weight, post bias
+constexpr int kJoinSums = 5;         // weight, bias, gate, post weight, post bias
 
 struct JoinGrads {
     const void *sum, *grad_sum, *grad_normed;
     void *grad_x, *grad_residual;
-    void* vectors[kfloats];  // NULL: not wanted
+    void* vectors[kJoinSums];  // NULL: not wanted
 };
 
 // The sum over `lanes` lanes, a power of two, next to each other.
@@ -300,7 +300,7 @@ residual_norm_wide(lattice_residual_norm a, T* sum, T* __restrict__ normed, floa
 }
 
 // grad_x and grad_residual, and this block's sums over its rows in
-// partials[block][kfloats][channels] (NULL: none are wanted).
+// partials[block][kJoinSums][channels] (NULL: none are wanted).
 template <typename T, int V, int K, int BLOCK, bool POST>
 __global__ void __launch_bounds__(BLOCK)
 residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const float4* __restrict__ statistics,
@@ -425,7 +425,7 @@ residual_norm_grad_rows(lattice_residual_norm a, JoinGrads g, int group, const f
         }
     }
     if (!partials) return;
-    float* mine = partials + static_cast<long long>(blockIdx.x) * kfloats * channels;
+    float* mine = partials + static_cast<long long>(blockIdx.x) * kJoinSums * channels;
 #pragma unroll
     for (int which = 0; which < kSums; ++which) {
         if (!g.vectors[which]) continue;
@@ -515,7 +515,7 @@ residual_norm_grad_columns(lattice_residual_norm a, JoinGrads g, const float4* _
     if (c >= channels) return;
     const JoinChannel<T, POST> v(a, c);
     const bool reads_x = POST || g.vectors[2];
-    float sums[kfloats] = {};
+    float sums[kJoinSums] = {};
     for (long long row = blockIdx.y; row < active; row += gridDim.y) {
         const float4 stat = statistics[row];
         const float2 along = means[row];
@@ -532,13 +532,13 @@ residual_norm_grad_columns(lattice_residual_norm a, JoinGrads g, const float4* _
         sums[3] += POST ? du * ((x - stat.z) * stat.w) : 0.0f;
         sums[4] += POST ? du : 0.0f;
     }
-    float* mine = partials + static_cast<long long>(blockIdx.y) * kfloats * channels;
+    float* mine = partials + static_cast<long long>(blockIdx.y) * kJoinSums * channels;
 #pragma unroll
     for (int which = 0; which < (POST ? 5 : 3); ++which)
         if (g.vectors[which]) mine[which * static_cast<long long>(channels) + c] = sums[which];
 }
 
-// partials [count][kfloats][channels] -> the vectors' gradients: 16 columns a
+// partials [count][kJoinSums][channels] -> the vectors' gradients: 16 columns a
 // block, 64 slices of the partials added in slice order.
 constexpr int kFinishBlock = 1024, kFinishSlices = kFinishBlock / 16;
 template <typename T>
@@ -548,7 +548,7 @@ residual_norm_grad_finish(const float* __restrict__ partials, int count, int cha
     const int at = threadIdx.x & 15, slice = threadIdx.x >> 4;
     T* out = static_cast<T*>(g.vectors[blockIdx.y]);
     if (!out) return;
-    const long long row = static_cast<long long>(kfloats) * channels;
+    const long long row = static_cast<long long>(kJoinSums) * channels;
     for (long long first = blockIdx.x * 16ll; first < channels; first += gridDim.x * 16ll) {
         const long long c = first + at;
         float sum = 0.0f;
@@ -656,7 +656,7 @@ int launch_join_grad(const lattice_residual_norm& a, const JoinGrads& g, const f
     }
     LATTICE_LAUNCH_CHECK();
     if (partials) {
-        residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kfloats), kFinishBlock, 0, stream>>>(
+        residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kJoinSums), kFinishBlock, 0, stream>>>(
             partials, blocks, a.channels, a.scale, g);
         LATTICE_LAUNCH_CHECK();
     }
@@ -717,7 +717,7 @@ const char* join_fault(const lattice_residual_norm* a) {
 // No rows: the vectors' gradients are zero.
 template <typename T>
 int join_grad_empty(const lattice_residual_norm& a, const JoinGrads& g, hipStream_t stream) {
-    residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kfloats), kFinishBlock, 0, stream>>>(
+    residual_norm_grad_finish<T><<<dim3(grid_for(a.channels, 16, 1u << 16), kJoinSums), kFinishBlock, 0, stream>>>(
         nullptr, 0, a.channels, 0.0f, g);
     LATTICE_LAUNCH_CHECK();
     return LATTICE_OK;
@@ -741,6 +741,8 @@ extern "C" int lattice_hip_residual_norm(const lattice_residual_norm* args, void
     LATTICE_REQUIRE_JOIN(args);
     if (args->rows == 0) return LATTICE_OK;
     LATTICE_REQUIRE(sum && normed, "residual norm pointers must be non-null.");
+    LATTICE_REQUIRE(reinterpret_cast<uintptr_t>(statistics) % 16 == 0,
+                    "residual norm statistics must lie on 16-byte boundaries.");
     hipStream_t stream = as_stream(stream_ptr);
     if (args->dtype == LATTICE_F32) return join_of<float>(*args, sum, normed, statistics, stream);
     if (args->dtype == LATTICE_F16) return join_of<_Float16>(*args, sum, normed, statistics, stream);
@@ -750,7 +752,7 @@ extern "C" int lattice_hip_residual_norm(const lattice_residual_norm* args, void
 extern "C" size_t lattice_hip_residual_norm_grad_workspace_bytes(int rows, int channels) {
     if (rows <= 0 || channels <= 0) return 0;
     // The most blocks any vector width gives: one row a block.
-    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1, kJoinBlock)) * kfloats * channels * sizeof(float)) +
+    return aligned_bytes(static_cast<size_t>(join_partials(rows, channels, 1, kJoinBlock)) * kJoinSums * channels * sizeof(float)) +
            aligned_bytes(static_cast<size_t>(rows) * sizeof(float2));
 }
 
@@ -764,6 +766,8 @@ extern "C" int lattice_hip_residual_norm_grad(const lattice_residual_norm* args,
                       {grad_weight, grad_bias, grad_gate, grad_post_weight, grad_post_bias}};
     LATTICE_REQUIRE(args->rows == 0 || (sum && statistics && grad_x && grad_residual),
                     "residual norm pointers must be non-null.");
+    LATTICE_REQUIRE(reinterpret_cast<uintptr_t>(statistics) % 16 == 0,
+                    "residual norm statistics must lie on 16-byte boundaries.");
     LATTICE_REQUIRE(args->post_norm || (!grad_post_weight && !grad_post_bias),
                     "without post_norm there are no gradients of its vectors.");
     hipStream_t stream = as_stream(stream_ptr);
@@ -777,7 +781,7 @@ extern "C" int lattice_hip_residual_norm_grad(const lattice_residual_norm* args,
     float2* means = nullptr;
     if (join_sums(g)) {
         Workspace ws{static_cast<char*>(workspace), workspace ? workspace_bytes : 0};
-        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1, kJoinBlock)) * kfloats *
+        partials = ws.take<float>(static_cast<size_t>(join_partials(args->rows, args->channels, 1, kJoinBlock)) * kJoinSums *
                                   args->channels);
         means = ws.take<float2>(args->rows);
         LATTICE_REQUIRE(partials && means, "residual norm gradient workspace is too small.");

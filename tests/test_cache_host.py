@@ -253,6 +253,19 @@ def test_junction_workspaces_and_results():
                                          None) == 0
 
 
+def test_junction_statistics_off_their_boundaries():
+    lib = _library()
+    args = _junction()
+    for rc in (lib.lattice_hip_residual_norm(
+            ctypes.byref(args), void(4096), void(4096), void(4104), None),
+            lib.lattice_hip_residual_norm_grad(
+                ctypes.byref(args), void(4096), void(4104),
+                *[void(4096)] * 4, *[None] * 5, None, ctypes.c_size_t(0),
+                None)):
+        assert rc == 1
+        assert b'16-byte boundaries' in lib.lattice_hip_last_error()
+
+
 def test_cache_shapes():
     from mlx_lattice_amd import QuantizedCache
 
