@@ -382,6 +382,39 @@ def test_captured_graph_replays(channels):
             assert torch.equal(got, eager)
 
 
+@pytest.mark.parametrize('channels', (96, 2048))
+def test_captured_training_step(channels):
+    """A differentiated call in a captured graph, each pass with leaves of its
+    own over the same memory."""
+    given, cotangents = _inputs(300, channels, torch.bfloat16)
+
+    def step():
+        leaves = {k: t.detach().requires_grad_() for k, t in given.items()}
+        out = _ops().residual_norm(**leaves, scale=0.5, post_norm=True)
+        return [*(t.detach() for t in out), *torch.autograd.grad(
+            out, list(leaves.values()), cotangents)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        fresh, slopes = _inputs(300, channels, torch.bfloat16, seed=seed + 9)
+        for name, t in given.items():
+            t.data.copy_(fresh[name])
+        for t, new in zip(cotangents, slopes):
+            t.copy_(new)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, eager in zip(captured, want):
+            assert torch.equal(got, eager)
+
+
 def test_only_the_gradients_asked_for():
     given, cotangents = _inputs(20, 32, torch.float32)
     for names in itertools.chain(itertools.combinations(given, 1),
