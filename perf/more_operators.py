@@ -26,7 +26,6 @@ each block of 32 tokens and key head, keys ``(32, width)`` and values ``(width,
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -45,9 +44,7 @@ _SCALE = 0.5  # of a junction's gated part
 _LOW = -126  # the least exponent of a block
 
 
-@functools.cache
 def _package():
-    """The library, which a user's program has imported before it calls."""
     package = str(Path(__file__).resolve().parent.parent / 'mlx-lattice_amd')
     if package not in sys.path:
         sys.path.insert(0, package)
