@@ -6,7 +6,7 @@
 namespace lattice {
 
 // A part of a row's softmax, over some of its tokens: the largest score (log2),
-// the sum of exp2(score - top), and the sum of that times v.
+// the sum of exp2(score - top), and the average of v by those shares.
 struct CachePart {
     float* values;   // [splits][queries * heads][dim]
     float2* states;  // [splits][queries * heads]: (top, sum)

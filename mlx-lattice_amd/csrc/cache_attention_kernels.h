@@ -198,7 +198,7 @@ template <typename T, int DP, int R>
 struct CacheState {
     f32x4_attn acc[R][DP / 16];
     float top[R], sum[R];
-    int unit[R];  // sums are in units of 2^top, acc in units of 2^(top + unit)
+    int unit[R];  // sums are in units of 2^top, acc in units of 2^(top + unit); once closed, acc is their quotient
 
     __device__ void clear() {
 #pragma unroll
@@ -390,10 +390,13 @@ __device__ inline void attend_pair(const CacheCall& call, const CacheSequence& s
         const float old = top == next ? 1.0f : exp2f(top - next);
         // Of -inf before any other score, no share (alone, 0 / 0 in the end).
         const float share = x != -INFINITY ? exp2f(x - next) : 0.0f;
+        // Averages, as close_state has them.
+        const float before = sum * old;
         top = next;
-        sum = sum * old + wave_sum(share);
+        sum = before + wave_sum(share);
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f, kept = before * inv;
         wave_fence();
-        scratch->p[lane] = share;
+        scratch->p[lane] = share * inv;
         wave_fence();
 #pragma unroll
         for (int b = 0; b < kAttnMaxDim / kWave; ++b) {
@@ -405,15 +408,15 @@ __device__ inline void attend_pair(const CacheCall& call, const CacheSequence& s
                 const uint8_t code =
                     values[(static_cast<long long>(block) * width + d) * kCacheBlock + j % kCacheBlock];
                 const int e = c.value_exponents[at + block];
-                add += scratch->p[t] * (Code::value(code) * power_of_two(max(e, kCacheLeast)));
+                add += scratch->p[t] * Code::value(code) * power_of_two(max(e, kCacheLeast));
             }
-            acc[b] = acc[b] * old + add;
+            acc[b] = acc[b] * kept + add;
         }
     }
 #pragma unroll
     for (int b = 0; b < kAttnMaxDim / kWave; ++b) {
         const int d = lane + b * kWave;
-        if (d < c.dim) out[(row * a.heads + head) * c.dim + d] = static_cast<T>(total ? acc[b] / sum : 0.0f);
+        if (d < c.dim) out[(row * a.heads + head) * c.dim + d] = static_cast<T>(total && sum == 0.0f ? NAN : acc[b]);
     }
 }
 
@@ -489,12 +492,15 @@ __device__ inline float cache_factor(float scale, int key_exponent) {
     return fmaxf(scale * power_of_two(max(key_exponent, kCacheLeast)), 0x1p-149f);
 }
 
-// Sums over the four lanes of a pair, and products in units of one.
+// Sums over the four lanes of a pair, and averages of the values: divided before
+// the power of two comes back, since a sum of values near the type's end is past
+// it where their average is not.  What sees nothing has zeros.
 template <typename T, int DP, int R>
 __device__ inline void close_state(CacheState<T, DP, R>& state) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         state.sum[r] = pair_sum(state.sum[r]);
+        state.rescale(r, state.sum[r] != 0.0f ? 1.0f / state.sum[r] : 0.0f);
         // In two steps of normal numbers.
         const int unit = state.unit[r] - CacheRange<T>::kFill;
         state.rescale(r, bounded_power(unit / 2));
@@ -515,16 +521,13 @@ __device__ inline void write_pairs(const CacheCall& call, const CacheSequence& s
     for (int r = 0; r < R; ++r) {
         const long long at = (static_cast<long long>(s.q0) + rows[r].i) * a.heads + rows[r].head;
         const bool sees = rows[r].hi >= max(0, rows[r].lo) || (a.sinks > 0 && rows[r].hi >= 0);
-        const float inv = sees ? 1.0f / state.sum[r] : 0.0f;
-        uint32_t largest = 0;
+        // Without any share, all scores are -inf.
+        uint32_t largest = sees && state.sum[r] == 0.0f ? 0x7f800000u : 0;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
+            // The bits of magnitudes are ordered, NaN above infinity.
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                state.acc[r][t][i] *= inv;
-                // The bits of magnitudes are ordered, NaN above infinity.
-                largest = max(largest, __float_as_uint(state.acc[r][t][i]) & 0x7fffffffu);
-            }
+            for (int i = 0; i < 4; ++i) largest = max(largest, __float_as_uint(state.acc[r][t][i]) & 0x7fffffffu);
         }
         const uint64_t spoilt = ballot(rows[r].valid && largest >= 0x7f800000u);
         uint32_t again = static_cast<uint32_t>(spoilt | spoilt >> 16 | spoilt >> 32 | spoilt >> 48) & 0xffffu;
@@ -630,7 +633,8 @@ cache_attend_few(CacheCall call, int splits, CachePart part, T* __restrict__ out
             const float2 other = states[w * kRows + 16 * r + n];
             sum += other.y * __builtin_amdgcn_exp2f(other.x - top);
         }
-        state.rescale(r, __builtin_amdgcn_exp2f(state.top[r] - top));
+        const float mine = state.sum[r] * __builtin_amdgcn_exp2f(state.top[r] - top);
+        state.rescale(r, sum != 0.0f ? mine / sum : 0.0f);
         state.top[r] = top;
         state.sum[r] = sum;
     }
@@ -859,8 +863,8 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
     if (at >= items) return;
     const float2 state = lane < splits ? part.states[lane * items + at] : float2{kCacheFloor, 0.0f};
     const float top = wave_max(state.x);
-    const float factor = __builtin_amdgcn_exp2f(state.x - top);
-    const float sum = wave_sum(state.y * factor);
+    const float mine = state.y * __builtin_amdgcn_exp2f(state.x - top);
+    const float sum = wave_sum(mine), factor = sum != 0.0f ? mine / sum : 0.0f;
     // Each half of the wave has every second part, a lane four channels.
     const int half = lane >> 5, d = (lane & 31) * 4;
     const float* values = part.values + at * c.dim + min(d, c.dim - 4);
@@ -875,7 +879,7 @@ cache_join(CacheCall call, int splits, CachePart part, T* __restrict__ out) {
     bool finite = sum > 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        acc[i] = (acc[i] + __shfl_xor(acc[i], 32)) / sum;
+        acc[i] += __shfl_xor(acc[i], 32);
         finite = finite && fabsf(acc[i]) < INFINITY;
     }
     // Rows that see nothing, and those that are not finite.
