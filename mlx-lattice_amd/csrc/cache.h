@@ -7,11 +7,15 @@
 namespace lattice {
 
 constexpr int kCacheBlock = 32;        // tokens that share an exponent
-constexpr int kCacheLeast = -126;      // the least exponent: 2^e and 2^-e are normal numbers
+constexpr int kCacheLeast = -126;      // the least exponent: 2^e is a normal number
 constexpr int kCacheLongest = 1 << 29;  // lengths are clamped to it, so that positions stay inside 32 bits
 
 // 2^e for e in -126 .. 127.
 __device__ inline float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// 2^-e for e in -126 .. 127, the last of which is below the normal numbers.
+__device__ inline float inverse_power(int e) {
+    return __uint_as_float(e < 127 ? static_cast<uint32_t>(127 - e) << 23 : 1u << 22);
+}
 
 typedef __bf16 bf16x2_cache __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_cache __attribute__((ext_vector_type(2)));

@@ -228,7 +228,7 @@ cache_write_blocks(lattice_cache c, CacheSource keys, CacheSource vals, int rows
     int next = block_exponent<Code>(wave_max(most));
     if (begin > 0) next = max(next, before);
     const bool moves = begin > 0 && next != before;
-    const float factor = power_of_two(-next), moved = power_of_two(max(before - next, kCacheLeast));
+    const float factor = inverse_power(next), moved = power_of_two(max(before - next, kCacheLeast));
     if (lane == 0) *exponent = static_cast<int8_t>(next);
     if (!values) {
 #pragma unroll

@@ -1,11 +1,20 @@
-"""Attention over an 8-bit cache of values near the end of float32's range:
-sums of them leave it, their averages do not."""
+"""An 8-bit cache at the end of float32's range: attention over values whose
+sums leave it and whose averages do not, and rows behind the largest
+exponents."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
-from cache_reference import decoded, random_cache
+from cache_reference import (
+    appended,
+    codes_of,
+    decoded,
+    random_cache,
+    same_values,
+)
 from transformer_reference import assert_within, attention_f64
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +108,45 @@ def test_many_equal_shares(dtype):
     cache.value_exponents.fill_(106)  # 416 * 2 ** 106 is 3.4e34
     _check(torch.zeros((1, 1, 32), dtype=dtype, device='cuda'), cache, (1,),
            (12000,))
+
+
+@pytest.mark.parametrize('code', CODES)
+@pytest.mark.parametrize('dtype', (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize('dim', (32, 33))
+@pytest.mark.parametrize('exponent', (125, 126, 127))
+def test_rows_behind_the_largest_exponents(exponent, dim, dtype, code):
+    """Exponents that no row asks for but a cache may hold: the new rows'
+    codes are what is left of them."""
+    import mlx_lattice_amd.ops as ops
+
+    gen = torch.Generator(device='cuda').manual_seed(3)
+    cache = random_cache(gen, code, 2, 64, 2, dim)
+    cache.key_exponents.fill_(exponent)
+    cache.value_exponents.fill_(exponent)
+    size = torch.finfo(torch.bfloat16).max
+    # Some on the border between two codes.
+    rows = torch.rand((8, 4, dim), generator=gen, device='cuda') * 2 - 1
+    rows *= size
+    rows[1] = 2.0 ** exponent
+    rows[2] = -1.5 * 2.0 ** min(exponent, 126)
+    rows[3] = 2.0 ** 100
+    rows[5, :, ::3], rows[5, :, 1::3] = math.inf, -math.inf
+    rows[6, :, ::7] = math.nan
+    rows = rows.to(dtype)
+    k, v = rows[:, :2], rows[:, 2:]
+    want = [codes_of(cache)[0], codes_of(cache)[1],
+            cache.key_exponents.cpu().clone(),
+            cache.value_exponents.cpu().clone()]
+    for s, (at, before) in enumerate(((slice(0, 4), 7), (slice(4, 8), 40))):
+        for which, part in enumerate((k, v)):
+            for head in range(2):
+                want[which][s, head], want[2 + which][s, head] = appended(
+                    want[which][s, head], want[2 + which][s, head],
+                    part[at, head].cpu().double(), code, before, before + 4,
+                    64)
+    assert (want[2] == exponent).all()
+    ops.write_cache(cache, k, v, offsets=_ints(0, 4, 8),
+                    lengths=_ints(11, 44))
+    for got, ref in zip((*codes_of(cache), cache.key_exponents.cpu(),
+                         cache.value_exponents.cpu()), want):
+        assert same_values(got, ref)
