@@ -794,7 +794,8 @@ int lattice_hip_residual_norm(const lattice_residual_norm* args, void* sum,
  * inactive rows), and, unless NULL, the vectors' [channels], summed over the
  * active rows in an order fixed by the shape.  sum and statistics as the
  * forward call gave them; the cotangents grad_sum and grad_normed are
- * contiguous (NULL: zero). */
+ * contiguous (NULL: zero).  The values of args->residual and bias are not read,
+ * those of x only with post_norm or for grad_gate. */
 size_t lattice_hip_residual_norm_grad_workspace_bytes(int rows, int channels);
 int lattice_hip_residual_norm_grad(
     const lattice_residual_norm* args, const void* sum,

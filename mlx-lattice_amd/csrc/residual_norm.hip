@@ -692,7 +692,16 @@ int join_grad_of(const lattice_residual_norm& a, const JoinGrads& g, const float
                  float2* means, hipStream_t stream) {
     const float4* stats = reinterpret_cast<const float4*>(statistics);
     constexpr int kMost = 16 / sizeof(T), kWord = 4 / sizeof(T);
-    const int v = join_vector<T>(a, {g.sum, g.grad_sum, g.grad_normed, g.grad_x, g.grad_residual});
+    // What is not read does not count: not the residual nor the bias, x with the
+    // first norm or for the gate.
+    lattice_residual_norm read = a;
+    read.residual = read.bias = nullptr;
+    read.residual_stride = 0;
+    if (!a.post_norm && !g.vectors[2]) {
+        read.x = nullptr;
+        read.x_stride = 0;
+    }
+    const int v = join_vector<T>(read, {g.sum, g.grad_sum, g.grad_normed, g.grad_x, g.grad_residual});
     if (v == kMost) return join_grad_post<T, kMost>(a, g, stats, partials, means, stream);
     if constexpr (kWord > 1) {
         if (v == kWord) return join_grad_post<T, kWord>(a, g, stats, partials, means, stream);

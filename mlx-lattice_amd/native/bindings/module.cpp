@@ -442,10 +442,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("keep_statistics"),
           "The junction of two parts of a block: (sum, normed, statistics); vectors are (weight, bias, gate, "
           "post_weight, post_bias).");
-    m.def("residual_norm_grad", &ln::residual_norm_grad, py::arg("grad_sum"), py::arg("grad_normed"), py::arg("sum"),
+    m.def("residual_norm_grad",
+          [](const c10::optional<at::Tensor>& grad_sum, const c10::optional<at::Tensor>& grad_normed,
+             const at::Tensor& sum, const at::Tensor& statistics, const c10::optional<at::Tensor>& x,
+             const c10::optional<at::Tensor>&, const ln::JoinVectors& vectors, double scale, bool post_norm, bool rms,
+             double eps, const c10::optional<at::Tensor>& active_rows, const std::array<bool, 5>& wanted) {
+              return ln::residual_norm_grad(grad_sum, grad_normed, sum, statistics, x, vectors, scale, post_norm, rms,
+                                            eps, active_rows, wanted);
+          },
+          py::arg("grad_sum"), py::arg("grad_normed"), py::arg("sum"),
           py::arg("statistics"), py::arg("x"), py::arg("residual"), py::arg("vectors"), py::arg("scale"),
           py::arg("post_norm"), py::arg("rms"), py::arg("eps"), py::arg("active_rows"), py::arg("wanted"),
-          "Gradients of the junction: of x, residual and the wanted vectors.");
+          "Gradients of the junction: of x, residual and the wanted vectors.  The residual's values are not read (it may "
+          "be None), x's only with post_norm or for the gate.");
     m.def("residual_norm_node", &ln::residual_norm_node, py::arg("x"), py::arg("residual"), py::arg("vectors"),
           py::arg("scale"), py::arg("post_norm"), py::arg("rms"), py::arg("eps"), py::arg("active_rows"),
           "residual_norm as a differentiable node: (sum, normed).");

@@ -53,13 +53,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm(const at::Tensor& x
                                                              const c10::optional<at::Tensor>& active_rows,
                                                              bool keep_statistics);
 // The gradients of x, residual and the vectors; a vector's is undefined (None)
-// unless wanted.
+// unless wanted.  x is read with post_norm or where the gate's gradient is
+// wanted, and may be undefined otherwise; so may the bias, and the post bias
+// where the gate's gradient is not wanted.
 std::vector<at::Tensor> residual_norm_grad(const c10::optional<at::Tensor>& grad_sum,
                                            const c10::optional<at::Tensor>& grad_normed, const at::Tensor& sum,
-                                           const at::Tensor& statistics, const at::Tensor& x,
-                                           const at::Tensor& residual, const JoinVectors& vectors, double scale,
-                                           bool post_norm, bool rms, double eps,
-                                           const c10::optional<at::Tensor>& active_rows,
+                                           const at::Tensor& statistics, const c10::optional<at::Tensor>& x,
+                                           const JoinVectors& vectors, double scale, bool post_norm, bool rms,
+                                           double eps, const c10::optional<at::Tensor>& active_rows,
                                            const std::array<bool, 5>& wanted);
 
 // keys, values, key exponents and value exponents of a cache.

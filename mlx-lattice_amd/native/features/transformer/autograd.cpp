@@ -133,13 +133,12 @@ struct ResidualNorm : Function<ResidualNorm> {
         const JoinVectors vectors{weight, bias, gate, post_weight, post_bias};
         auto [sum, normed, statistics] = residual_norm(x, residual, vectors, scale, post_norm, rms, eps, active_rows,
                                                        true);
-        variable_list saved{x, residual, sum, statistics, or_undefined(active_rows)};
         std::vector<bool> wanted;
-        for (const MaybeTensor& v : vectors) {
-            saved.push_back(or_undefined(v));
-            wanted.push_back(wants_grad(v));
-        }
-        ctx->save_for_backward(saved);
+        for (const MaybeTensor& v : vectors) wanted.push_back(wants_grad(v));
+        // What the gradients read: neither the residual nor the bias.
+        ctx->save_for_backward({post_norm || wanted[2] ? x : at::Tensor(), sum, statistics, or_undefined(active_rows),
+                                or_undefined(weight), or_undefined(gate), or_undefined(post_weight),
+                                wanted[2] ? or_undefined(post_bias) : at::Tensor()});
         ctx->saved_data["wanted"] = c10::List<bool>({wanted[0], wanted[1], wanted[2], wanted[3], wanted[4]});
         ctx->saved_data["x"] = wants_grad(x);
         ctx->saved_data["residual"] = wants_grad(residual);
@@ -155,15 +154,15 @@ struct ResidualNorm : Function<ResidualNorm> {
         if (!grads[0].defined() && !grads[1].defined()) return out;
         const auto saved = ctx->get_saved_variables();
         auto& data = ctx->saved_data;
-        const JoinVectors vectors{or_none(saved[5]), or_none(saved[6]), or_none(saved[7]), or_none(saved[8]),
-                                  or_none(saved[9])};
+        const JoinVectors vectors{or_none(saved[4]), c10::nullopt, or_none(saved[5]), or_none(saved[6]),
+                                  or_none(saved[7])};
         const auto list = data["wanted"].toBoolList();
         std::array<bool, 5> wanted;
         for (int i = 0; i < 5; ++i) wanted[i] = list.get(i);
         variable_list made = residual_norm_grad(
-            or_none(grads[0]), or_none(grads[1]), saved[2], saved[3], saved[0], saved[1], vectors,
+            or_none(grads[0]), or_none(grads[1]), saved[1], saved[2], or_none(saved[0]), vectors,
             data["scale"].toDouble(), data["post_norm"].toBool(), data["rms"].toBool(), data["eps"].toDouble(),
-            or_none(saved[4]), wanted);
+            or_none(saved[3]), wanted);
         if (!data["x"].toBool()) made[0] = at::Tensor();
         if (!data["residual"].toBool()) made[1] = at::Tensor();
         made = once(std::move(made));

@@ -80,14 +80,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_norm(const at::Tensor& x
 
 std::vector<at::Tensor> residual_norm_grad(const c10::optional<at::Tensor>& grad_sum_in,
                                            const c10::optional<at::Tensor>& grad_normed_in, const at::Tensor& sum,
-                                           const at::Tensor& statistics, const at::Tensor& x,
-                                           const at::Tensor& residual, const JoinVectors& vectors, double scale,
-                                           bool post_norm, bool rms, double eps,
-                                           const c10::optional<at::Tensor>& active_rows,
+                                           const at::Tensor& statistics, const c10::optional<at::Tensor>& x_in,
+                                           const JoinVectors& vectors, double scale, bool post_norm, bool rms,
+                                           double eps, const c10::optional<at::Tensor>& active_rows,
                                            const std::array<bool, 5>& wanted) {
-    refuse_tangents({x, residual, or_undefined(grad_sum_in), or_undefined(grad_normed_in)});
+    const bool reads_x = post_norm || wanted[2];
+    if (reads_x && (!x_in || !x_in->defined())) {
+        throw std::invalid_argument("x is needed by post_norm and by the gate's gradient.");
+    }
+    // The sum stands in for rows that are not read.
+    const at::Tensor& x = reads_x ? *x_in : sum;
+    refuse_tangents({x, or_undefined(grad_sum_in), or_undefined(grad_normed_in)});
     const auto guard = guard_of(x);
-    const Join j = join_of(x, residual, vectors, scale, post_norm, rms, eps, active_rows);
+    require_same(sum, x, "sum");
+    if (sum.sizes() != x.sizes() || !sum.is_contiguous()) {
+        throw std::invalid_argument("sum must be that of the forward call.");
+    }
+    const Join j = join_of(x, sum, vectors, scale, post_norm, rms, eps, active_rows);
     at::Tensor cotangents[2];
     const c10::optional<at::Tensor>* given[2] = {&grad_sum_in, &grad_normed_in};
     for (int i = 0; i < 2; ++i) {
@@ -97,10 +106,6 @@ std::vector<at::Tensor> residual_norm_grad(const c10::optional<at::Tensor>& grad
             throw std::invalid_argument("the cotangent must match the output shape.");
         }
         cotangents[i] = (*given[i])->contiguous();
-    }
-    require_same(sum, x, "sum");
-    if (sum.sizes() != x.sizes() || !sum.is_contiguous()) {
-        throw std::invalid_argument("sum must be that of the forward call.");
     }
     if (statistics.dim() != 2 || statistics.size(0) != x.size(0) || statistics.size(1) != 4 ||
         statistics.scalar_type() != at::kFloat || !statistics.is_contiguous() || statistics.device() != x.device()) {

@@ -465,3 +465,70 @@ def test_refusals():
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         refused('forward-mode', dual, x, error=RuntimeError)
+
+
+@pytest.mark.parametrize('channels', (48, 9000))
+@pytest.mark.parametrize('rms', (False, True))
+def test_what_no_gradient_reads_may_change(rms, channels):
+    """The residual and the bias are not read by the backward pass, nor is x
+    without the first norm and a gradient of the gate, or the first norm's bias
+    without the latter: changing them in place between the passes is fine."""
+    for post in (False, True):
+        given, cotangents = _inputs(40, channels, torch.float32)
+        if not post:
+            del given['post_weight'], given['post_bias']
+        for wanted, changed in (
+                ([n for n in given if n != 'gate'],
+                 ['residual', 'bias'] + (['post_bias'] if post else ['x'])),
+                (list(given), ['residual', 'bias'])):
+            grads = []
+            for change in (False, True):
+                # Leaves are multiplied first, so that what the call takes may
+                # be changed.
+                leaves = {k: t.detach().clone().requires_grad_(k in wanted)
+                          for k, t in given.items()}
+                inputs = {k: t * 1 for k, t in leaves.items()}
+                out = _ops().residual_norm(**inputs, scale=0.5, rms=rms,
+                                           post_norm=post)
+                if change:
+                    with torch.no_grad():
+                        for name in changed:
+                            inputs[name].add_(100.0)
+                grads.append(torch.autograd.grad(
+                    out, [leaves[n] for n in wanted], cotangents))
+            for a, b in zip(*grads):
+                assert torch.equal(a, b)
+
+
+def test_what_a_gradient_reads_may_not_change():
+    given, cotangents = _inputs(40, 48, torch.float32)
+    for name in ('x', 'weight', 'gate', 'post_weight', 'post_bias'):
+        leaves = {k: t.detach().clone().requires_grad_()
+                  for k, t in given.items()}
+        inputs = {k: t * 1 for k, t in leaves.items()}
+        out = _ops().residual_norm(**inputs, post_norm=True)
+        with torch.no_grad():
+            inputs[name].add_(100.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace'):
+            torch.autograd.grad(out, list(leaves.values()), cotangents)
+
+
+def test_gradient_without_x():
+    from mlx_lattice_amd._native import ext
+
+    given, (dh, dy) = _inputs(30, 40, torch.float16)
+    vectors = [given['weight'], None, given['gate'], None, None]
+    total, _, stats = ext.residual_norm(
+        given['x'], given['residual'], vectors, 0.5, False, False, 1e-5, None,
+        True)
+
+    def grad(x, wanted, post=False):
+        return ext.residual_norm_grad(dh, dy, total, stats, x, None, vectors,
+                                      0.5, post, False, 1e-5, None, wanted)
+
+    some = [True, True, False, False, False]
+    for a, b in zip(grad(None, some), grad(given['x'], some)):
+        assert a is None and b is None or torch.equal(a, b)
+    for wanted, post in (([True] * 3 + [False] * 2, False), (some, True)):
+        with pytest.raises(ValueError, match='x is needed'):
+            grad(None, wanted, post)
