@@ -940,6 +940,13 @@ typedef struct lattice_cache_attention {
 } lattice_cache_attention;
 size_t lattice_hip_cache_attention_workspace_bytes(
     const lattice_cache* cache, const lattice_cache_attention* args);
+/* The kernel that a call's sizes choose.  *share: the waves of a block have the
+ * same rows of heads and split the tokens (1), or have rows of their own (0);
+ * *tiles: tiles of 16 rows a wave; *splits: parts that the tokens are split into
+ * over blocks of threads, joined by a second launch. */
+int lattice_hip_cache_attention_layout(const lattice_cache* cache,
+                                       const lattice_cache_attention* args,
+                                       int* share, int* tiles, int* splits);
 int lattice_hip_cache_attention(const lattice_cache* cache,
                                 const lattice_cache_attention* args, void* out,
                                 void* workspace, size_t workspace_bytes,

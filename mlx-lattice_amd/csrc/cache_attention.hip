@@ -104,6 +104,20 @@ extern "C" size_t lattice_hip_cache_attention_workspace_bytes(const lattice_cach
     return aligned_bytes(rows * cache->dim * sizeof(float)) + aligned_bytes(rows * sizeof(float2));
 }
 
+extern "C" int lattice_hip_cache_attention_layout(const lattice_cache* cache, const lattice_cache_attention* args,
+                                                  int* share, int* tiles, int* splits) {
+    if (const char* fault = cache_attention_fault(cache, args)) {
+        set_error(fault);
+        return LATTICE_ERROR_INVALID_ARGUMENT;
+    }
+    LATTICE_REQUIRE(share && tiles && splits, "attention pointers must be non-null.");
+    const CacheLayout l = cache_layout(cache_call(*cache, *args));
+    *share = l.share;
+    *tiles = l.tiles;
+    *splits = l.splits;
+    return LATTICE_OK;
+}
+
 extern "C" int lattice_hip_cache_attention(const lattice_cache* cache, const lattice_cache_attention* args, void* out,
                                            void* workspace, size_t workspace_bytes, void* stream_ptr) {
     if (const char* fault = cache_attention_fault(cache, args)) {
