@@ -18,7 +18,7 @@
 //
 // 30001 rows of 8 key heads of 128 channels, keys and values: 61 us from float32
 // (5.0 TB/s), 47 from half precision to int8 (3.9 TB/s; 120004 rows 4.5).  8-byte
-// loads, with more tokens a lane, take 61 us.  One token of 32 sequences: 6.0 us,
+// loads, with more tokens a lane, take 61 us.  One token of 32 sequences: 6.2 us,
 // the launch and four reads that wait for each other.  Reading 65536 tokens of 4
 // key heads of 128 channels to bfloat16: 31 us (5.9 TB/s, codes partly from the
 // last cache), 41 with nothing cached; heads of 32 channels at the same rate.

@@ -28,9 +28,9 @@ template <typename T> constexpr int cache_most_tiles(int width) {
     return sizeof(T) == 4 ? (width == 32 ? 4 : 2) : width <= 64 ? 4 : width == 96 ? 3 : 2;
 }
 // Where widening a block's codes once for four waves, by way of LDS, is faster: 2
-// x 2048 queries of 16 heads over 16384 tokens take 619 us against 700 with two
-// tiles that widen their own in bfloat16, 638 against 735 from int8 in half
-// precision.  Narrower heads have three or four tiles to a widening.
+// x 2048 queries of 16 heads over 16384 tokens take 588 us against 679 with two
+// tiles that widen their own in bfloat16, 4096 queries 597 against 680 from int8
+// in half precision.  Narrower heads have three or four tiles to a widening.
 template <typename T> constexpr bool cache_many(int width) { return width == 128 && sizeof(T) == 2; }
 
 // Both structures, with bounds that keep positions inside 32 bits.

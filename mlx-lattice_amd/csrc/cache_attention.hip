@@ -52,6 +52,12 @@ CacheLayout cache_layout(const CacheCall& call) {
     };
     const auto filled = [&](int rows) { return 2 * pairs > static_cast<long long>(rows) * sequences; };
     CacheLayout l{true, 1, 1, 0};
+    // Rows of their own for the waves where that fills the chip.  One sequence of
+    // 16 heads over 4 key heads in bfloat16 over 16384 tokens, us with and without,
+    // by blocks of 128 pairs: 64 404 and 122, 128 407 and 197, 256 408 and 355, 352
+    // 542 and 502, 512 564 and 636, 752 808 and 886, 1024 950 and 1098.  In a window
+    // of 1024: 128 36 and 23, 256 37 and 43, 512 55 and 81; prompts that see only
+    // themselves, whose last rows are the longest: 256 59 and 45, 512 133 and 125.
     const bool f32 = a.dtype == LATTICE_F32;
     if ((f32 ? cache_many<float>(width) : cache_many<_Float16>(width)) && filled(32 * kAttnWaves) &&
         blocks(32 * kAttnWaves) >= kUnits) {
